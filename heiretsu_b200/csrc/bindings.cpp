@@ -46,6 +46,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("B"), py::arg("T"), py::arg("nh"), py::arg("dvec"), py::arg("dq_acc"), py::arg("dqkv"),
         py::arg("drop_seed") = py::none(), py::arg("drop_site") = 0, py::arg("drop_p") = 0.0, py::arg("h0") = 0,
         py::arg("nh_total") = 0, py::arg("head_dim") = 64);
+  m.def("token_logprobs", &hb::token_logprobs);
+  m.def("policy_loss", &hb::policy_loss);
+  m.def("preference_loss", &hb::preference_loss);
+  m.def("act8_pack", &hb::act8_pack);
+  m.def("act8_unpack", &hb::act8_unpack);
+  m.def("layernorm_fwd_act8", &hb::layernorm_fwd_act8);
+  m.def("layernorm_bwd_act8_scratch_rows", &hb::layernorm_bwd_act8_scratch_rows);
+  m.def("layernorm_bwd_act8", &hb::layernorm_bwd_act8);
   m.def("raw_malloc", &hb::raw_malloc);
   m.def("raw_free", &hb::raw_free);
   m.def("tensor_from_ptr", &hb::tensor_from_ptr);
