@@ -15,7 +15,8 @@
 
 namespace hb {
 
-long policy_scratch_doubles(int M);
+long logit_row_limit(int type);
+long policy_scratch_doubles();
 long preference_scratch_doubles(int P);
 void token_logprobs_launch(const LogitRows& a, cudaStream_t s);
 void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratch, float* loss, float* stats,
@@ -66,7 +67,9 @@ LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targ
   a.type = logit_type(logits, op);
   const int64_t M = logits.size(0);
   TORCH_CHECK(V >= 1 && V <= logits.size(1), op, ": V must be in [1, row width]");
-  TORCH_CHECK(M <= kIntMax && logits.size(1) <= kIntMax - 4096, op, ": too many rows or columns");
+  TORCH_CHECK(M <= kIntMax, op, ": too many rows");
+  const int64_t widest = logit_row_limit(a.type);  // what the shared memory of one cluster holds
+  TORCH_CHECK(V <= widest, op, ": V must be at most ", std::to_string(widest), " for this dtype");
   TORCH_CHECK(logits.stride(0) >= 0, op, ": logits need a row stride that is not negative");
   const at::Device dev = logits.device();
   check_vec(targets, at::kLong, M, dev, op, "targets");
@@ -87,7 +90,8 @@ LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targ
     TORCH_CHECK(g.device() == dev && g.scalar_type() == logits.scalar_type() && g.dim() == 2 && g.size(0) == M &&
                     (g.size(1) <= 1 || g.stride(1) == 1),
                 op, ": grad must be a matrix with contiguous rows like logits, of its dtype, rows and device");
-    TORCH_CHECK(g.size(1) >= V && g.size(1) <= kIntMax - 4096, op, ": grad must be at least V wide");
+    TORCH_CHECK(g.size(1) >= V && g.size(1) <= widest, op, ": grad must be at least V wide and at most ",
+                std::to_string(widest));
     TORCH_CHECK(M <= 1 || g.stride(0) >= g.size(1), op, ": grad rows must not overlap");
     const bool same = g.data_ptr() == logits.data_ptr() && (M <= 1 || g.stride(0) == logits.stride(0));
     const auto x = extent(logits), y = extent(g);
@@ -152,7 +156,7 @@ void policy_loss(const at::Tensor& logits, int64_t V, const at::Tensor& targets,
   p.clip_lo = static_cast<float>(1.0 - clip_low);
   p.clip_hi = static_cast<float>(1.0 + clip_high);
   p.kl_coef = static_cast<float>(kl_coef);
-  at::Tensor scratch = at::empty({policy_scratch_doubles(a.M)}, logits.options().dtype(at::kDouble));
+  at::Tensor scratch = at::empty({policy_scratch_doubles()}, logits.options().dtype(at::kDouble));
   policy_loss_launch(a, p, scratch.data_ptr<double>(), loss.data_ptr<float>(), stats.data_ptr<float>(),
                      at::cuda::getCurrentCUDAStream());
 }

@@ -13,10 +13,13 @@ def logprobs(logits, V, targets, ignore=IGNORE):
     """(logp, lse, unit gradient [M, V]) in 64 bits; zeros in ignored rows."""
     x = logits[:, :V].double()
     live = targets != ignore
-    lse = torch.logsumexp(x, 1)
+    top = x.amax(1, keepdim=True)
+    y = x - top  # first: next to a mask of the type's lowest value, log of the sum would vanish even in 64 bits
+    rest = torch.logsumexp(y, 1)
+    lse = top[:, 0] + rest
     at = torch.arange(x.shape[0], device=x.device), targets.clamp(0, V - 1)
-    logp = x[at] - lse
-    g = -torch.exp(x - lse[:, None])
+    logp = y[at] - rest
+    g = -torch.exp(y - rest[:, None])
     g[at] += 1
     zero = torch.zeros((), dtype=torch.float64, device=x.device)
     return torch.where(live, logp, zero), torch.where(live, lse, zero), torch.where(live[:, None], g, zero)
