@@ -20,7 +20,7 @@ struct LogitRows {
   float* lse;              // [M] log-sum-exp of the row (0 for ignored rows), or nullptr
   void* grad;              // [M, W], row stride gld, the logits' type; may be x itself; nullptr: none
   long gld;
-  int W;
+  int W;                   // without a gradient: the logits' width
   int* status;
 };
 

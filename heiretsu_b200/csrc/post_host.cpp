@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <string>
@@ -100,6 +101,8 @@ LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targ
     a.grad = g.data_ptr();
     a.gld = g.stride(0);
     a.W = static_cast<int>(g.size(1));
+  } else {
+    a.W = static_cast<int>(std::max(V, std::min(widest, logits.size(1))));  // rows are dealt out as with a gradient
   }
   a.status = device_status_ptr(logits.get_device());
   return a;

@@ -25,7 +25,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCtasPerSm = 2;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -39,17 +39,17 @@ struct Piece {
   static constexpr int kElems = TYPE == kLogitF32 ? 4 : 8;
   static constexpr int kBytes = 16 / kElems;
   static constexpr bool kF16 = TYPE == kLogitF16;
-  // elements at and behind `n` become -inf
-  static __device__ __forceinline__ void mask(uint4& r, int n) {
+  static constexpr uint32_t kMinusInf = TYPE == kLogitF32 ? 0xFF800000u : kF16 ? 0xFC00u : 0xFF80u;
+  // elements at and behind `n` become `bits`
+  static __device__ __forceinline__ void fill(uint4& r, int n, uint32_t bits) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (TYPE == kLogitF32) {
-        if (i >= n) w[i] = 0xFF800000u;
+        if (i >= n) w[i] = bits;
       } else {
-        constexpr uint32_t kInf = kF16 ? 0xFC00u : 0xFF80u;
-        if (2 * i >= n) w[i] = kInf | (kInf << 16);
-        else if (2 * i + 1 >= n) w[i] = (w[i] & 0xFFFFu) | (kInf << 16);
+        if (2 * i >= n) w[i] = bits | (bits << 16);
+        else if (2 * i + 1 >= n) w[i] = (w[i] & 0xFFFFu) | (bits << 16);
       }
     }
   }
@@ -65,10 +65,12 @@ struct Piece {
       }
     }
   }
-  static __device__ __forceinline__ float at(const uint4& r, int e) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
-    if constexpr (TYPE == kLogitF32) return __uint_as_float(w[e]);
-    else return e & 1 ? hi16<kF16>(w[e >> 1]) : lo16<kF16>(w[e >> 1]);
+  // element e (known at run time) of a piece to element i of a row
+  static __device__ __forceinline__ void store_at(const uint4& r, int e, void* base, long i) {
+    const int k = TYPE == kLogitF32 ? e : e >> 1;
+    const uint32_t w = k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w;
+    if constexpr (TYPE == kLogitF32) static_cast<uint32_t*>(base)[i] = w;
+    else static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(e & 1 ? w >> 16 : w);
   }
   static __device__ __forceinline__ uint4 narrow(const float (&v)[kElems]) {
     uint4 r;
@@ -93,8 +95,17 @@ __device__ __forceinline__ void store1(void* base, long i, float v) {
   else static_cast<uint16_t*>(base)[i] = from_f32<TYPE == kLogitF16>(v);
 }
 
-__device__ __forceinline__ void copy_piece(void* smem, const void* gmem, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(bytes) : "memory");
+// Asynchronous copy of one piece; the bytes behind `bytes` become 0.
+__device__ __forceinline__ void copy_piece(uint32_t smem, const void* gmem, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_piece(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ uint4 read_piece(uint32_t smem) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(smem) : "memory");
+  return r;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -102,38 +113,17 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Running sum of exp(x - m) against a reference m. The reference moves only when a value exceeds it by more
-// than 6 (a term is then at most e^6, so 2^31 of them stay far below overflow), so almost no piece pays for a rescale.
-// x - m is taken before the factor log2 e: the product alone would overflow for masks of the type's lowest
-// value. An empty sum (nothing, or only -inf) has s = 0 and any m; NaN and +inf make s NaN.
+// Running sum of exp(x - m) under the largest value so far; nothing, or only -inf, is s = 0 with any m; NaN and
+// +inf make s NaN. x - m is taken before the factor log2 e, which alone would overflow for masks of the
+// type's lowest value.
 struct Sum {
-  float m = 0.f, limit = -INFINITY, s = 0.f;
-  __device__ __forceinline__ void move(float to) {
-    if (s != 0.f) s *= ex2((m - to) * kLog2e);
-    m = to;
-    limit = to + 6.f;
-  }
-  template <int N>
-  __device__ __forceinline__ void add(const float (&v)[N]) {
-    float top = max3f(v[0], v[1], v[2]);
-    if constexpr (N == 8) top = max3f(max3f(top, v[4], v[5]), v[6], v[7]);
-    top = fmaxf(top, v[3]);
-    if (top > limit) move(top);
-    const uint64_t l2 = f2_pack(kLog2e, kLog2e), neg = f2_pack(-m, -m);
-    uint64_t acc = f2_pack(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      float a, b;
-      f2_unpack(f2_mul(f2_add(f2_pack(v[i], v[i + 1]), neg), l2), a, b);
-      acc = f2_add(acc, f2_pack(ex2(a), ex2(b)));
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    if (v > m) {
+      if (s != 0.f) s *= ex2((m - v) * kLog2e);
+      m = v;
     }
-    float a, b;
-    f2_unpack(acc, a, b);
-    s += a + b;
-  }
-  __device__ __forceinline__ void add1(float v) {
-    if (v > limit) move(v);
-    s += ex2((v - m) * kLog2e);
+    if (v != -INFINITY) s += ex2((v - m) * kLog2e);
   }
 };
 
@@ -180,6 +170,7 @@ enum Mode : int { kLogp = 0, kUnit = 1, kPolicy = 2 };
 // How the rows are dealt out: clusters of `split` CTAs, each CTA holding `pieces` 16-byte pieces of a row.
 struct Deal {
   int split, pieces, clusters;
+  bool aligned;    // every row of the logits starts on a 16-byte boundary
   bool vec_store;  // rows of grad start at the same offset from a 16-byte boundary as those of the logits
 };
 
@@ -189,10 +180,14 @@ constexpr int kStages = 4;  // copy groups of one row
 // [c pieces, (c + 1) pieces) of the row in shared memory. Every thread copies, reads and refills its own 16-byte
 // slots (asynchronous copies, waited for in four groups), so the copies need no barrier, and the next row's copies
 // are issued slot by slot as the current row's gradient leaves: the memory pipe never drains.
-//   pass 1 (while the copies arrive): per-thread running (m, s); joined over the warp, the CTA (one barrier) and,
-//          where split > 1, the cluster (each CTA writes its (m, s, x_t) into every other's shared memory;
-//          one cluster barrier);
-//   pass 2 (gradient): coef ([j == t] - exp(x_j - lse)) from the slots, stored in 16-byte pieces.
+//   pass 1 (while the copies arrive): S = sum_j exp(x_j - x_t). The target's own logit is the reference of every
+//          sum: its term is exactly 1, so S >= 1 cannot vanish, no running maximum is needed, sums of threads, CTAs
+//          (one barrier) and the cluster (one exchange through shared memory) just add, and logp = -log S. Rows
+//          where S passes 2^120 (a target more than 83 below the largest logit, or at -inf; NaN) are summed again
+//          under a maximum.
+//   pass 2 (gradient): coef ([j == t] - exp(x_j - x_t) / S) from the slots, in 16-byte pieces.
+// The difference x_j - x_t is taken before the factor log2 e: it is exact or nearly so wherever the term matters,
+// also for logits far from 0, and finite for masks of the type's lowest value.
 // So a row crosses DRAM once each way. Rows may start at any element: the columns before the first 16-byte
 // boundary (`head`, fewer than one piece) are read by single threads of the first CTA.
 template <int TYPE, int MODE>
@@ -201,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   using P = Piece<TYPE>;
   constexpr int E = P::kElems;
   extern __shared__ uint4 slots[];
-  __shared__ float sm_m[2][kWarps], sm_s[2][kWarps], sm_x[2], xch[2][8][3];
+  __shared__ float sm_s[2][kWarps], xch[2][8], slow_m[kWarps], slow_s[kWarps], slow_x[8][2];
   __shared__ int sm_n[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = d.split > 1 ? static_cast<int>(blockIdx.x) % d.split : 0;
@@ -210,28 +205,58 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const int iters = (d.pieces + kThreads - 1) / kThreads;
   if (d.split > 1) cooperative_groups::this_cluster().sync();  // every CTA runs before its shared memory is written
 
-  const auto row_ptr = [&](int row) { return static_cast<const char*>(a.x) + (long)row * a.ld * P::kBytes; };
-  // columns of a row before its first 16-byte boundary
-  const auto head_of = [&](int row) {
-    return static_cast<int>((16u - (reinterpret_cast<uintptr_t>(row_ptr(row)) & 15u)) & 15u) / P::kBytes;
+  // A row as this CTA sees it: its address, the columns before the first 16-byte boundary, and how many of this
+  // CTA's pieces lie wholly inside the V columns; `rest` elements more are in piece `full`.
+  struct Row {
+    const char* base;
+    const char* body;  // address of this thread's first piece
+    int head, full, rest;
   };
-  const auto copy_slot = [&](const char* base, int head, int i) {
-    const int n = a.V - head - (piece0 + i) * E;  // columns from here to the end
-    if (i < d.pieces && n > 0) copy_piece(&slots[i], base + (head + (long)(piece0 + i) * E) * P::kBytes, min(n, E) * P::kBytes);
+  const auto row_of = [&](int row) {
+    Row r;
+    r.base = static_cast<const char*>(a.x) + (long)row * a.ld * P::kBytes;
+    r.head = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(r.base) & 15u)) & 15u) / P::kBytes;
+    const int cols = a.V - r.head - piece0 * E;  // from this CTA's first piece to the end of the row
+    r.full = min(max(cols, 0) / E, d.pieces);
+    r.rest = r.full < d.pieces ? max(cols, 0) - r.full * E : 0;
+    r.body = r.base + (r.head + (long)piece0 * E) * P::kBytes + tid * 16;
+    return r;
+  };
+  constexpr int kStep = kThreads * 16;  // bytes from one of a thread's slots to its next
+  const uint32_t mine = smem_u32(slots) + tid * 16;
+  // Iterations in which every thread has a whole piece, whatever the row's head: the same for all rows, so a slot
+  // belongs to the same stage in all of them. Stage g ends with iteration min((g + 1) per_stage, even); the uneven
+  // rest (fewer pieces than threads, the last of them partial) goes with the last stage.
+  const int even = min(max(a.V - (d.aligned ? 0 : E - 1) - piece0 * E, 0) / E, d.pieces) / kThreads;
+  const uint32_t even_end = mine + even * kStep;
+  const uint32_t stage_step = (even + kStages - 1) / kStages * kStep;
+  const auto stage_end = [&](int g) { return min(mine + (g + 1) * stage_step, even_end); };
+  const auto copy_rest = [&](const Row& r) {
+#pragma unroll 1
+    for (int k = even; k < iters; ++k) {
+      const int i = k * kThreads + tid;
+      const int n = i < r.full ? 16 : i == r.full ? r.rest * P::kBytes : 0;
+      if (n > 0) copy_piece(mine + k * kStep, r.body + (long)k * kStep, n);
+    }
+  };
+  const auto copy_row = [&](const Row& r) {
+    const char* src = r.body;
+    uint32_t to = mine;
+    for (int g = 0; g < kStages; ++g) {
+      for (; to < stage_end(g); to += kStep, src += kStep) copy_piece(to, src);
+      if (g == kStages - 1) copy_rest(r);
+      copies_commit();
+    }
+  };
+  const auto commit_row = [&] {
+    for (int g = 0; g < kStages; ++g) copies_commit();
   };
 
   int64_t t = a.ignore_index;
+  Row cur = row_of(first < a.M ? first : 0);
   if (first < a.M) t = a.targets[first];
-  if (first < a.M && t != a.ignore_index) {
-    const char* base = row_ptr(first);
-    const int head = head_of(first);
-    for (int g = 0, k = 0; g < kStages; ++g) {
-      for (; k < iters * (g + 1) / kStages; ++k) copy_slot(base, head, k * kThreads + tid);
-      copies_commit();
-    }
-  } else {
-    for (int g = 0; g < kStages; ++g) copies_commit();
-  }
+  if (t != a.ignore_index) copy_row(cur);
+  else commit_row();
 
   float unit_w = 0.f;
   double sum_loss = 0.0, sum_kl = 0.0, sum_clip = 0.0;
@@ -253,109 +278,129 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   for (int row = first; row < a.M; row += d.clusters) {
     const int next = row + d.clusters;
     const int64_t t_next = next < a.M ? a.targets[next] : a.ignore_index;
-    const bool more = t_next != a.ignore_index;
-    const char* next_base = row_ptr(more ? next : row);
-    const int next_head = head_of(more ? next : row);
+    const Row nxt = row_of(next < a.M ? next : row);
+    const bool more = t_next != a.ignore_index;  // there are copies to make
     const bool counted = t != a.ignore_index;
     const bool bad = counted && (t < 0 || t >= a.V);
-    const char* base = row_ptr(row);
-    const int head = head_of(row);
-    float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w;
-    if constexpr (MODE == kPolicy) {  // read here, used after pass 1
-      if (counted) {
+    const int tc = bad || !counted ? -1 : static_cast<int>(t);
+    const bool head_col = rank == 0 && tid < min(cur.head, a.V);
+    float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w, xt = 0.f, xh = 0.f;
+    if (counted) {  // read here, used after pass 1
+      if (!bad) xt = load1<TYPE>(cur.base, tc);
+      if (head_col) xh = load1<TYPE>(cur.base, tid);
+      if constexpr (MODE == kPolicy) {
         old = p.old_logp[row];
-        adv = p.adv[row / p.adv_rows];
+        adv = p.adv[p.adv_rows == 1 ? row : row / p.adv_rows];
         if (p.ref_logp) ref = p.ref_logp[row];
         if (p.weights) w = p.weights[row];
       }
     }
-    // the piece (of this CTA) and element that hold the target; head columns have piece -1
-    const int tc = bad || !counted ? -1 : static_cast<int>(t);
-    const bool head_col = rank == 0 && tid < min(head, a.V);
-    float xh = 0.f;
-    float logp = 0.f, lse = 0.f, m = 0.f, log2s = 0.f;
+    // p_j = 2^((x_j - m) log2 e - log2s) with m = xt (or the row's maximum, `slow`)
+    float logp = 0.f, lse = 0.f, log2s = 0.f, m = 0.f;
+    bool slow = false;
     if (counted) {
-      if (head_col) xh = load1<TYPE>(base, tid);
-      Sum sum;
+      float s0 = 0.f, s1 = 0.f;
+      const auto add_piece = [&](const uint4& r) {
+        float v[E];
+        P::widen(r, v);
 #pragma unroll
-      for (int g = 0, k = 0; g < kStages; ++g) {
+        for (int e = 0; e < E; e += 2) {
+          s0 += ex2((v[e] - xt) * kLog2e);
+          s1 += ex2((v[e + 1] - xt) * kLog2e);
+        }
+      };
+      uint32_t at = mine;
+      const char* src = nxt.body;
+#pragma unroll 1
+      for (int g = 0; g < kStages; ++g) {
         copies_wait<kStages - 1>();
-        for (; k < iters * (g + 1) / kStages; ++k) {
-          const int i = k * kThreads + tid;
-          const int c0 = head + (piece0 + i) * E;
-          if (i < d.pieces && c0 < a.V) {
-            uint4 r = slots[i];
-            if (c0 + E > a.V) P::mask(r, a.V - c0);
-            float v[E];
-            P::widen(r, v);
-            if (static_cast<unsigned>(tc - c0) < static_cast<unsigned>(E)) {
-              float x = v[0];
-#pragma unroll
-              for (int e = 1; e < E; ++e) x = e == tc - c0 ? v[e] : x;
-              sm_x[parity] = x;
-            }
-            sum.add(v);
-          }
-          if constexpr (MODE == kLogp) {
-            if (more) copy_slot(next_base, next_head, i);
+        const uint32_t end = stage_end(g);
+#pragma unroll 1
+        for (; at < end; at += kStep) {
+          add_piece(read_piece(at));
+          if constexpr (MODE == kLogp) {  // the slot is free: the next row's piece
+            if (more) copy_piece(at, src);
+            src += kStep;
           }
         }
-        // pass 1 of a gradient row leaves its slots in place: an empty group keeps the count of groups
-        copies_commit();
+        if (g == kStages - 1) {
+#pragma unroll 1
+          for (int k = even; k < iters; ++k) {
+            const int i = k * kThreads + tid;
+            const int n = i < cur.full ? E : i == cur.full ? cur.rest : 0;
+            if (n > 0) {
+              uint4 r = read_piece(mine + k * kStep);
+              if (n < E) P::fill(r, n, P::kMinusInf);
+              add_piece(r);
+            }
+          }
+          if (MODE == kLogp && more) copy_rest(nxt);
+        }
+        copies_commit();  // empty where the row's pieces stay for its gradient: it keeps the count of groups
       }
-      if (head_col) {
-        sum.add1(xh);
-        if (tid == tc) sm_x[parity] = xh;
-      }
-      float s = sum.s;
-      m = sum.m;
-      join_lanes<32>(m, s);
-      if (lane == 0) {
-        sm_m[parity][warp] = m;
-        sm_s[parity][warp] = s;
-      }
+      float s = s0 + s1;
+      if (head_col) s += ex2((xh - xt) * kLog2e);
+      s = warp_sum(s);
+      if (lane == 0) sm_s[parity][warp] = s;
       __syncthreads();
-      m = sm_m[parity][lane % kWarps];
       s = sm_s[parity][lane % kWarps];
-      join_lanes<kWarps>(m, s);
-      float xt = 0.f;
-      const bool mine = tc >= 0 && (tc < head ? rank == 0 : (tc - head) / E / d.pieces == rank);
-      if (mine) xt = sm_x[parity];
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (d.split > 1) {
         auto cl = cooperative_groups::this_cluster();
-        if (tid < d.split) {
-          float* to = cl.map_shared_rank(&xch[parity][rank][0], tid);
-          to[0] = m;
-          to[1] = s;
-          to[2] = mine ? xt : -INFINITY;
-        }
+        if (tid < d.split) *cl.map_shared_rank(&xch[parity][rank], tid) = s;
         cl.sync();
-        float top = -INFINITY;
-        for (int c = 0; c < d.split; ++c)
-          if (xch[parity][c][1] != 0.f) top = fmaxf(top, xch[parity][c][0]);
         s = 0.f;
-        xt = -INFINITY;
-        for (int c = 0; c < d.split; ++c) {
-          const float sc = xch[parity][c][1], xc = xch[parity][c][2];
-          if (sc != 0.f) s += sc * ex2((xch[parity][c][0] - top) * kLog2e);
-          if (xc != -INFINITY) xt = xc;  // only the owner's is not -inf (NaN included)
-        }
-        m = top;
+        for (int c = 0; c < d.split; ++c) s += xch[parity][c];
       }
       parity ^= 1;
-      const float ln = logf(s);
-      log2s = log2f(s);
-      lse = m + ln;
-      logp = bad ? NAN : (xt - m) - ln;
-    } else {
-#pragma unroll
-      for (int g = 0, k = 0; g < kStages; ++g) {
-        if constexpr (MODE == kLogp) {
-          if (more)
-            for (; k < iters * (g + 1) / kStages; ++k) copy_slot(next_base, next_head, k * kThreads + tid);
+      slow = bad || !(s < 1.329227995784916e36f);  // 2^120; also NaN
+      if (!slow) {
+        m = xt;
+        const float ln = logf(s);
+        log2s = ln * kLog2e;
+        logp = -ln;
+        lse = xt + ln;
+      } else {
+        // the same sum under a maximum, from global memory, one column at a time
+        Sum z;
+        const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
+        const int hi = min(a.V, cur.head + (piece0 + d.pieces) * E);
+        for (int j = lo + tid; j < hi; j += kThreads) z.add(load1<TYPE>(cur.base, j));
+        m = z.m;
+        s = z.s;
+        join_lanes<32>(m, s);
+        if (lane == 0) {
+          slow_m[warp] = m;
+          slow_s[warp] = s;
         }
-        copies_commit();
+        __syncthreads();
+        m = slow_m[lane % kWarps];
+        s = slow_s[lane % kWarps];
+        join_lanes<kWarps>(m, s);
+        if (d.split > 1) {
+          auto cl = cooperative_groups::this_cluster();
+          if (tid < d.split) {
+            float* to = cl.map_shared_rank(&slow_x[rank][0], tid);
+            to[0] = m;
+            to[1] = s;
+          }
+          cl.sync();
+          m = slow_x[lane % d.split][0];
+          s = lane < d.split ? slow_x[lane][1] : 0.f;
+          join_lanes<32>(m, s);
+          cl.sync();  // read before the next slow row writes it
+        } else {
+          __syncthreads();
+        }
+        log2s = log2f(s);
+        const float ln = logf(s);
+        lse = m + ln;
+        logp = bad ? NAN : (xt - m) - ln;
       }
+    } else {
+      if (MODE == kLogp && more) copy_row(nxt);
+      else commit_row();
     }
     if (rank == 0 && tid == 0) {
       a.logp[row] = logp;
@@ -368,63 +413,97 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (counted) {
           const RowTerm r = policy_term(p, logp, old, adv, ref, w);
           coef = r.coef * (p.grad_scale ? *p.grad_scale : 1.f);
-          sum_loss += r.loss;
-          sum_kl += r.kl;
-          sum_clip += r.clipped;
+          if (tid == 0) {
+            sum_loss += r.loss;
+            sum_kl += r.kl;
+            sum_clip += r.clipped;
+          }
         }
       }
       if (bad) coef = NAN;
-      const bool zero = coef == 0.f;  // ignored rows and clipped tokens: nothing to evaluate
       char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
-      if (rank == 0 && tid < min(head, a.W)) {
-        const float g = head_col && !zero ? coef * ((tid == tc ? 1.f : 0.f) - ex2(fmaf(xh - m, kLog2e, -log2s))) : 0.f;
-        store1<TYPE>(out, tid, g);
-      }
-      const uint64_t l2 = f2_pack(kLog2e, kLog2e), neg = f2_pack(-m, -m), nl = f2_pack(-log2s, -log2s);
-      const uint64_t nc = f2_pack(-coef, -coef);
+      char* out_body = out + (cur.head + (long)piece0 * E) * P::kBytes;
+      char* out_mine = out_body + tid * 16;
+      const bool zero = coef == 0.f;  // ignored rows and clipped tokens: nothing to evaluate
+      const bool fast = d.vec_store && !slow;
+      const auto grad_piece = [&](const uint4& r, float (&v)[E]) {
+        P::widen(r, v);
 #pragma unroll
-      for (int g = 0, k = 0; g < kStages; ++g) {
-        for (; k < iters * (g + 1) / kStages; ++k) {
-          const int i = k * kThreads + tid;
-          const int c0 = head + (piece0 + i) * E;
-          if (i < d.pieces && c0 < a.W) {
-            float v[E];
-            if (zero || c0 >= a.V) {
-#pragma unroll
-              for (int e = 0; e < E; ++e) v[e] = 0.f;
-            } else {
-              P::widen(slots[i], v);
-#pragma unroll
-              for (int e = 0; e < E; e += 2) {
-                float q0, q1;
-                f2_unpack(f2_fma(f2_add(f2_pack(v[e], v[e + 1]), neg), l2, nl), q0, q1);
-                f2_unpack(f2_mul(f2_pack(ex2(q0), ex2(q1)), nc), v[e], v[e + 1]);
-              }
-              if (static_cast<unsigned>(tc - c0) < static_cast<unsigned>(E)) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                  if (e == tc - c0) v[e] = fmaf(ex2(fmaf(P::at(slots[i], e) - m, kLog2e, -log2s)), -coef, coef);
-              }
-              if (c0 + E > a.V) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                  if (c0 + e >= a.V) v[e] = 0.f;
-              }
+        for (int e = 0; e < E; ++e) v[e] = -coef * ex2(fmaf(v[e] - xt, kLog2e, -log2s));
+      };
+      if (fast) {
+        uint32_t at = mine;
+        const char* src = nxt.body;
+#pragma unroll 1
+        for (int g = 0; g < kStages; ++g) {
+          const uint32_t end = stage_end(g);
+#pragma unroll 1
+          for (; at < end; at += kStep) {
+            uint4 o = make_uint4(0u, 0u, 0u, 0u);
+            if (!zero) {
+              float v[E];
+              grad_piece(read_piece(at), v);
+              o = P::narrow(v);
             }
-            if (d.vec_store && c0 + E <= a.W) {
-              *reinterpret_cast<uint4*>(out + (long)c0 * P::kBytes) = P::narrow(v);
-            } else {
-#pragma unroll
-              for (int e = 0; e < E; ++e)
-                if (c0 + e < a.W) store1<TYPE>(out, c0 + e, v[e]);
-            }
+            *reinterpret_cast<uint4*>(out_mine) = o;
+            if (more) copy_piece(at, src);  // the slot is free: the next row's piece
+            out_mine += kStep;
+            src += kStep;
           }
-          if (more) copy_slot(next_base, next_head, i);
+          if (g < kStages - 1) copies_commit();
         }
+      }
+      // the uneven rest, the columns behind V, and rows that take single stores
+      if (!slow) {
+#pragma unroll 1
+        for (int k = fast ? even : 0; k < iters; ++k) {
+          const int i = k * kThreads + tid;
+          const int c0 = cur.head + (piece0 + i) * E;
+          if (i >= d.pieces || c0 >= a.W) break;
+          const int n = zero ? 0 : i < cur.full ? E : i == cur.full ? cur.rest : 0;  // elements to evaluate
+          float v[E];
+          uint4 r = make_uint4(0u, 0u, 0u, 0u);
+          if (n > 0) {
+            grad_piece(read_piece(mine + k * kStep), v);
+            r = P::narrow(v);
+            if (n < E) P::fill(r, n, 0u);
+          }
+          if (fast && c0 + E <= a.W) {
+            *reinterpret_cast<uint4*>(out_body + (long)i * 16) = r;
+          } else {
+#pragma unroll 1
+            for (int e = 0; e < E && c0 + e < a.W; ++e) P::store_at(r, e, out_body, (long)i * E + e);
+          }
+        }
+      }
+      if (!more) {
+        if (fast) copies_commit();
+        else commit_row();
+      } else if (fast) {
+        copy_rest(nxt);
         copies_commit();
+      } else {
+        copy_row(nxt);
+      }
+      if (rank == 0 && tid < min(cur.head, a.W) && !slow)
+        store1<TYPE>(out, tid, head_col && !zero ? -coef * ex2(fmaf(xh - xt, kLog2e, -log2s)) : 0.f);
+      if (slow) {
+        const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
+        const int hi = min(a.W, cur.head + (piece0 + d.pieces) * E);
+        for (int j = lo + tid; j < hi; j += kThreads) {
+          const float g = j < a.V ? coef * ((j == tc ? 1.f : 0.f) - ex2(fmaf(load1<TYPE>(cur.base, j) - m, kLog2e, -log2s))) : 0.f;
+          store1<TYPE>(out, j, g);
+        }
+      } else if (tc >= 0 && !zero) {
+        // the target's element, by the thread that has just stored its piece (or head column)
+        const int i = tc < cur.head ? -1 : (tc - cur.head) / E - piece0;
+        const bool owner = i < 0 ? tc < cur.head && rank == 0 && tid == tc : i < d.pieces && tid == i % kThreads;
+        // (1 - p_t from logp itself, which keeps its digits where p_t is near 1)
+        if (owner) store1<TYPE>(out, tc, -coef * expm1f(logp));
       }
     }
     t = t_next;
+    cur = row_of(next < a.M ? next : row);
   }
   if constexpr (MODE == kPolicy) {
     if (rank == 0 && tid == 0) {
@@ -511,9 +590,11 @@ constexpr int kMaxPiecesShared = (228 * 1024 / kCtasPerSm - 2048) / 16;  // kCta
 constexpr int kMaxSplit = 8;
 
 // Deals M rows of `row_pieces` pieces to clusters of 1, 2, 4 or 8 CTAs: the split with the least estimated
-// time, rounds * (fixed cost of a row + its bytes at an SM's share of the memory rate).
-Deal deal_rows(int M, long row_pieces, int dirs, int sms) {
-  Deal best{0, 0, 0, true};
+// time, rounds * (fixed cost of a row + its bytes, both ways, at an SM's share of the memory rate). It goes by the
+// logits alone, with or without a gradient, so equal logits give equal bits in all three losses (the order of a
+// row's sum goes by the split): a policy step on the tokens it has just scored starts at ratios of exactly 1.
+Deal deal_rows(int M, long row_pieces, int sms) {
+  Deal best{};
   double least = 0.0;
   for (int c = 1; c <= kMaxSplit; c *= 2) {
     const long pieces = (row_pieces + c - 1) / c;
@@ -522,7 +603,7 @@ Deal deal_rows(int M, long row_pieces, int dirs, int sms) {
     const int most = sms * resident / c;
     const int clusters = M < most ? M : most;
     const int rounds = (M + most - 1) / most;
-    const double ns = rounds * ((c > 1 ? 2200.0 : 1500.0) + 16.0 * pieces * dirs * resident / 43.0);
+    const double ns = rounds * ((c > 1 ? 2200.0 : 1500.0) + 32.0 * pieces * resident / 43.0);
     if (best.split == 0 || ns < least) {
       least = ns;
       best.split = c;
@@ -566,9 +647,10 @@ void launch_rows(const LogitRows& a, const PolicyTerms& p, const Deal& d, double
 
 Deal deal_of(const LogitRows& a) {
   const int elems = a.type == kLogitF32 ? 4 : 8, bytes = 16 / elems;
-  const long width = a.grad && a.W > a.V ? a.W : a.V;
-  Deal d = deal_rows(a.M, (width + elems - 1) / elems, a.grad ? 2 : 1, num_sms(current_device()));
+  const long width = a.W > a.V ? a.W : a.V;
+  Deal d = deal_rows(a.M, (width + elems - 1) / elems, num_sms(current_device()));
   if (d.split == 0) throw std::runtime_error("logit rows are too wide");  // the torch-facing checks refuse them first
+  d.aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.M <= 1 || a.ld * bytes % 16 == 0);
   d.vec_store = a.grad && reinterpret_cast<uintptr_t>(a.x) % 16 == reinterpret_cast<uintptr_t>(a.grad) % 16 &&
                 (a.M <= 1 || (a.ld - a.gld) * bytes % 16 == 0);
   return d;

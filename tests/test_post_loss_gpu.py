@@ -131,6 +131,42 @@ def test_masked_logits():
             assert ((grad[r].double() - g64[r]).abs() <= EPS[dt] * g64[r].abs() + 2e-5 + 2.0 ** -25).all(), r
 
 
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("V,W,off", [(5003, 5008, 0), (70001, 70001, 3)])
+def test_unlikely_targets(V, W, off, dt):
+    """Targets far below the largest logit (80 to 1000), at -inf, or far above the rest; logits around 1e4."""
+    M = 24
+    x, t, _ = make(M, V, W, dt, seed=21, off=off, ignored=0.0)
+    at = torch.arange(M, device="cuda")
+    for r, low in enumerate((60, 80, 83, 85, 90, 120, 500, 1000)):
+        x[r, t[r]] = -low
+        x[r, (t[r] + 1) % V] = 2.0
+    x[8, t[8]] = float("-inf")
+    x[9, t[9]] = 60000.0 if dt == FP16 else 1e30
+    x[10, :V] += 10000.0
+    x[11, :V] -= 10000.0
+    x[12, t[12]] = 200.0
+    t[13] = IGNORE
+    grad = torch.full_like(x, 3.0)
+    logp, lse = K().token_logprobs(x, V, t, grad=grad)
+    only, _ = K().token_logprobs(x, V, t)
+    status_ok()
+    assert torch.equal(only, logp)
+    assert logp[8] == float("-inf") and torch.isfinite(lse).all()
+    lp64, lse64, g64 = logprobs(x, V, t)
+    ok = at != 8
+    # the sum's own error, and roundings of log-probabilities of this size (fp32 x - lse at 1e4: 2^-24 of x, too)
+    big = torch.where(torch.isfinite(x[at, t.clamp_min(0)]), x[at, t.clamp_min(0)].double().abs(), 0)
+    tol = lse_bound(torch.zeros_like(lse64), V) + 8 * 2.0 ** -24 * lp64.abs() + 2.0 ** -24 * big
+    assert ((logp.double() - lp64).abs() <= tol)[ok].all()
+    assert ((lse.double() - lse64).abs() <= tol + 4 * 2.0 ** -24 * lse64.abs())[ok].all()
+    assert (grad[13] == 0).all() and (grad[:, V:] == 0).all()
+    rel = 2.0 ** -20 + tol[:, None]  # exponentials of arguments up to ~25 that matter, and the sum's error
+    p = -g64
+    p[at, t.clamp_min(0)] += 1.0     # p's error is the gradient's: 1 - p_t keeps no relative accuracy at p_t = 1
+    assert ((grad[:, :V].double() - g64).abs() <= EPS[dt] * g64.abs() + rel * (p.abs() + 2.0 ** -24) + 2.0 ** -25).all()
+
+
 def test_rows_without_any_value():
     """A counted row of -inf only, or with NaN or +inf, gives NaN (as a log-softmax does) and leaves the others alone."""
     M, V = 6, 777
@@ -179,6 +215,22 @@ def test_other_ignore_index_and_no_rows():
     loss, stats, _, grad = K().policy_loss(e, 64, t[:0], lp, lp)
     assert loss.item() == 0 and grad.shape == (0, 64)
     status_ok()
+
+
+@pytest.mark.parametrize("M,V,W", [(3, 50257, 50304), (61, 50257, 50304), (400, 5000, 5000)])
+def test_scoring_and_losses_agree_bit_for_bit(M, V, W):
+    """The same logits give the same log-probabilities with and without a gradient and in the policy loss, so the
+    first policy step on freshly scored tokens has ratios of exactly 1: loss = -mean(A), nothing clipped, KL 0."""
+    x, t, g = make(M, V, W, BF16, seed=M)
+    score, _ = K().token_logprobs(x, V, t)
+    again, _ = K().token_logprobs(x, V, t, grad=torch.empty_like(x))
+    adv = torch.randn(M, device="cuda", generator=g)
+    loss, stats, logp, _ = K().policy_loss(x, V, t, score, adv, ref_logp=score, kl_coef=0.5)
+    status_ok()
+    assert torch.equal(score, again) and torch.equal(score, logp)
+    live = (t != IGNORE).double()
+    want = -(live * adv.double()).sum() / live.sum()
+    assert (stats == 0).all() and (loss.double() - want).abs() <= 2.0 ** -22 * (adv.abs().mean() + want.abs())
 
 
 def policy_inputs(x, V, t, g, ref=True):
@@ -251,6 +303,23 @@ def test_policy_advantage_per_sequence():
         b = K().policy_loss(x, 333, t, old, adv[:n].repeat_interleave(24 // n), ref_logp=ref, kl_coef=0.1)
         for p, q in zip(a, b):
             assert torch.equal(p, q)
+
+
+def test_policy_with_broken_inputs():
+    """NaN or infinite log-probabilities and advantages reach their own row's gradient only, never the padding."""
+    M, V, W = 10, 1001, 1024
+    x, t, g = make(M, V, W, BF16, seed=14, ignored=0.0)
+    old, adv, ref = policy_inputs(x, V, t, g)
+    clean = K().policy_loss(x, V, t, old, adv, ref_logp=ref, kl_coef=0.1)
+    old[1], adv[2], adv[3], ref[4] = float("nan"), float("inf"), float("nan"), float("inf")
+    old[5] = float("inf")          # ratio 0: gradient 0 but for the KL term
+    loss, stats, logp, grad = K().policy_loss(x, V, t, old, adv, ref_logp=ref, kl_coef=0.1)
+    status_ok()
+    assert not torch.isfinite(loss) and torch.equal(logp, clean[2])
+    assert (grad[:, V:] == 0).all()
+    for r in (0, 6, 7, 8, 9):
+        assert torch.equal(grad[r], clean[3][r])
+    assert not torch.isfinite(grad[1:5, :V]).all(1).any() and torch.isfinite(grad[5]).all()
 
 
 def test_policy_gradient_against_differences():
