@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -22,9 +23,10 @@ namespace hb {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCtasPerSm = 2;
+constexpr int kUnroll = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -107,11 +109,8 @@ __device__ __forceinline__ uint4 read_piece(uint32_t smem) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(smem) : "memory");
   return r;
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// Waits for all of this thread's copies.
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Running sum of exp(x - m) under the largest value so far; nothing, or only -inf, is s = 0 with any m; NaN and
 // +inf make s NaN. x - m is taken before the factor log2 e, which alone would overflow for masks of the
@@ -170,17 +169,18 @@ enum Mode : int { kLogp = 0, kUnit = 1, kPolicy = 2 };
 // How the rows are dealt out: clusters of `split` CTAs, each CTA holding `pieces` 16-byte pieces of a row.
 struct Deal {
   int split, pieces, clusters;
+  int window, list;  // rows scanned at a time, and the entries of the list of a cluster's rows among them
   bool aligned;    // every row of the logits starts on a 16-byte boundary
   bool vec_store;  // rows of grad start at the same offset from a 16-byte boundary as those of the logits
 };
 
-constexpr int kStages = 4;  // copy groups of one row
-
-// Row kernel. A cluster of `split` CTAs takes rows cluster, cluster + clusters, ...; CTA c holds pieces
+// Row kernel. Clusters of `split` CTAs deal the counted rows, and apart from them the ignored ones, among themselves in
+// turn (every CTA scans the targets and lists its own: equal work wherever the ignored rows are). CTA c holds pieces
 // [c pieces, (c + 1) pieces) of the row in shared memory. Every thread copies, reads and refills its own 16-byte
-// slots (asynchronous copies, waited for in four groups), so the copies need no barrier, and the next row's copies
-// are issued slot by slot as the current row's gradient leaves: the memory pipe never drains.
-//   pass 1 (while the copies arrive): S = sum_j exp(x_j - x_t). The target's own logit is the reference of every
+// slots (asynchronous copies), so the copies need no barrier, and the next row's are issued slot by slot as the current
+// row's gradient leaves (without a gradient: as its pieces are read), so they arrive during this row's arithmetic and
+// that of the SM's other CTA.
+//   pass 1: S = sum_j exp(x_j - x_t). The target's own logit is the reference of every
 //          sum: its term is exactly 1, so S >= 1 cannot vanish, no running maximum is needed, sums of threads, CTAs
 //          (one barrier) and the cluster (one exchange through shared memory) just add, and logp = -log S. Rows
 //          where S passes 2^120 (a target more than 83 below the largest logit, or at -inf; NaN) are summed again
@@ -198,11 +198,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   extern __shared__ uint4 slots[];
   __shared__ float sm_s[2][kWarps], xch[2][8], slow_m[kWarps], slow_s[kWarps], slow_x[8][2];
   __shared__ int sm_n[kWarps];
+  int* const list = reinterpret_cast<int*>(slots + d.pieces);  // counted rows from the front, ignored from the back
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = d.split > 1 ? static_cast<int>(blockIdx.x) % d.split : 0;
   const int first = blockIdx.x / d.split;
   const int piece0 = rank * d.pieces;
   const int iters = (d.pieces + kThreads - 1) / kThreads;
+  if constexpr (MODE == kPolicy) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (d.split > 1) cooperative_groups::this_cluster().sync();  // every CTA runs before its shared memory is written
 
   // A row as this CTA sees it: its address, the columns before the first 16-byte boundary, and how many of this
@@ -224,13 +226,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   };
   constexpr int kStep = kThreads * 16;  // bytes from one of a thread's slots to its next
   const uint32_t mine = smem_u32(slots) + tid * 16;
-  // Iterations in which every thread has a whole piece, whatever the row's head: the same for all rows, so a slot
-  // belongs to the same stage in all of them. Stage g ends with iteration min((g + 1) per_stage, even); the uneven
-  // rest (fewer pieces than threads, the last of them partial) goes with the last stage.
+  // Iterations in which every thread has a whole piece, whatever the row's head; the uneven rest (fewer pieces than
+  // threads, the last of them partial) is kept out of their loops.
   const int even = min(max(a.V - (d.aligned ? 0 : E - 1) - piece0 * E, 0) / E, d.pieces) / kThreads;
-  const uint32_t even_end = mine + even * kStep;
-  const uint32_t stage_step = (even + kStages - 1) / kStages * kStep;
-  const auto stage_end = [&](int g) { return min(mine + (g + 1) * stage_step, even_end); };
   const auto copy_rest = [&](const Row& r) {
 #pragma unroll 1
     for (int k = even; k < iters; ++k) {
@@ -241,64 +239,112 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   };
   const auto copy_row = [&](const Row& r) {
     const char* src = r.body;
-    uint32_t to = mine;
-    for (int g = 0; g < kStages; ++g) {
-      for (; to < stage_end(g); to += kStep, src += kStep) copy_piece(to, src);
-      if (g == kStages - 1) copy_rest(r);
-      copies_commit();
-    }
-  };
-  const auto commit_row = [&] {
-    for (int g = 0; g < kStages; ++g) copies_commit();
+#pragma unroll 4
+    for (int k = 0; k < even; ++k) copy_piece(mine + k * kStep, src + (long)k * kStep);
+    copy_rest(r);
   };
 
-  int64_t t = a.ignore_index;
-  Row cur = row_of(first < a.M ? first : 0);
-  if (first < a.M) t = a.targets[first];
-  if (t != a.ignore_index) copy_row(cur);
-  else commit_row();
+  // An ignored row: log-probability 0 and, with a gradient, zeros in this CTA's share of its columns.
+  const auto zero_row = [&](int row) {
+    if (rank == 0 && tid == 0) {
+      a.logp[row] = 0.f;
+      if (a.lse) a.lse[row] = 0.f;
+    }
+    if constexpr (MODE != kLogp) {
+      char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
+      const int lo = min(piece0 * E, a.W), hi = min((piece0 + d.pieces) * E, a.W);
+      const int lead = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(out + (long)lo * P::kBytes) & 15u)) & 15u) / P::kBytes;
+      const int body = min(lo + lead, hi), n = (hi - body) / E;
+      if (tid < body - lo) store1<TYPE>(out, lo + tid, 0.f);
+      uint4* to = reinterpret_cast<uint4*>(out + (long)body * P::kBytes);
+#pragma unroll 4
+      for (int i = tid; i < n; i += kThreads) to[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (tid < hi - body - n * E) store1<TYPE>(out, body + n * E + tid, 0.f);
+    }
+  };
 
   float unit_w = 0.f;
   double sum_loss = 0.0, sum_kl = 0.0, sum_clip = 0.0;
-  if constexpr (MODE == kPolicy) {
-    if (!p.weights) {  // 1 / (counted rows): every CTA counts, while its first copies are in flight
-      int n = 0;
-#pragma unroll 4
-      for (int i = tid; i < a.M; i += kThreads) n += a.targets[i] != a.ignore_index;
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0) sm_n[warp] = n;
-      __syncthreads();
-      n = 0;
-      for (int w = 0; w < kWarps; ++w) n += sm_n[w];
-      unit_w = 1.f / static_cast<float>(max(n, 1));
-    }
-  }
-
   int parity = 0;
-  for (int row = first; row < a.M; row += d.clusters) {
-    const int next = row + d.clusters;
-    const int64_t t_next = next < a.M ? a.targets[next] : a.ignore_index;
-    const Row nxt = row_of(next < a.M ? next : row);
-    const bool more = t_next != a.ignore_index;  // there are copies to make
-    const bool counted = t != a.ignore_index;
-    const bool bad = counted && (t < 0 || t >= a.V);
-    const int tc = bad || !counted ? -1 : static_cast<int>(t);
-    const bool head_col = rank == 0 && tid < min(cur.head, a.V);
-    float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w, xt = 0.f, xh = 0.f;
-    if (counted) {  // read here, used after pass 1
-      if (!bad) xt = load1<TYPE>(cur.base, tc);
-      if (head_col) xh = load1<TYPE>(cur.base, tid);
-      if constexpr (MODE == kPolicy) {
-        old = p.old_logp[row];
-        adv = p.adv[p.adv_rows == 1 ? row : row / p.adv_rows];
-        if (p.ref_logp) ref = p.ref_logp[row];
-        if (p.weights) w = p.weights[row];
+  // Lists this cluster's rows of [w0, w0 + n): rank r of the counted (ignored) rows goes to cluster r % clusters.
+  int mine_counted = 0, mine_ignored = 0;
+  const auto scan = [&](int w0, int n) {
+    constexpr int kBatch = 8;  // loads in flight
+    const int seg = (n + kThreads * kBatch - 1) / (kThreads * kBatch) * (32 * kBatch);  // rows of one warp
+    const int lo = min(warp * seg, n), hi = min(lo + seg, n);
+    int c = 0;
+    for (int i = lo; i < hi; i += 32 * kBatch) {
+      int64_t t[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) t[k] = i + 32 * k + lane < hi ? a.targets[w0 + i + 32 * k + lane] : a.ignore_index;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) c += t[k] != a.ignore_index;
+    }
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();  // the list's and sm_n's last readers are done
+    if (lane == 0) sm_n[warp] = c;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sm_n[w];
+      all += sm_n[w];
+    }
+    int counted = before, ignored = lo - before;
+    for (int i = lo; i < hi; i += 32 * kBatch) {
+      int64_t t[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) t[k] = i + 32 * k + lane < hi ? a.targets[w0 + i + 32 * k + lane] : a.ignore_index;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int at = i + 32 * k + lane;
+        const bool in = at < hi, yes = in && t[k] != a.ignore_index, no = in && !yes;
+        const uint32_t set = __ballot_sync(0xffffffffu, yes), out = __ballot_sync(0xffffffffu, no);
+        const uint32_t below = (1u << lane) - 1u;
+        const uint32_t r = yes ? counted + __popc(set & below) : ignored + __popc(out & below);
+        const uint32_t q = r / static_cast<uint32_t>(d.clusters);
+        if (in && r - q * d.clusters == static_cast<uint32_t>(first)) list[yes ? q : d.list - 1 - q] = w0 + at;
+        counted += __popc(set);
+        ignored += __popc(out);
       }
+    }
+    __syncthreads();
+    mine_counted = (all - first + d.clusters - 1) / d.clusters;  // first < clusters: not negative
+    mine_ignored = (n - all - first + d.clusters - 1) / d.clusters;
+    return all;
+  };
+  const int window = min(a.M, d.window);
+  int all = 0;
+  if (MODE == kPolicy && !p.weights && window < a.M) {  // 1 / (counted rows) of several windows
+    for (int w0 = 0; w0 < a.M; w0 += window) all += scan(w0, min(window, a.M - w0));
+    unit_w = 1.f / static_cast<float>(max(all, 1));
+  }
+  for (int w0 = 0; w0 < a.M; w0 += window) {
+  all = scan(w0, min(window, a.M - w0));
+  if (MODE == kPolicy && window == a.M) unit_w = 1.f / static_cast<float>(max(all, 1));
+  int zeros = 0;  // ignored rows done
+  Row cur = row_of(mine_counted > 0 ? list[0] : 0);
+  if (mine_counted > 0) copy_row(cur);
+  for (int j = 0; j < mine_counted; ++j) {
+    const int row = list[j];
+    const bool more = j + 1 < mine_counted;  // there are copies to make
+    const Row nxt = row_of(more ? list[j + 1] : row);
+    const int64_t t = a.targets[row];
+    const bool bad = t < 0 || t >= a.V;
+    const int tc = bad ? -1 : static_cast<int>(t);
+    const bool head_col = rank == 0 && tid < min(cur.head, a.V);
+    // read here, used after pass 1
+    const float xt = bad ? 0.f : load1<TYPE>(cur.base, tc), xh = head_col ? load1<TYPE>(cur.base, tid) : 0.f;
+    float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w;
+    if constexpr (MODE == kPolicy) {
+      old = p.old_logp[row];
+      adv = p.adv[p.adv_rows == 1 ? row : row / p.adv_rows];
+      if (p.ref_logp) ref = p.ref_logp[row];
+      if (p.weights) w = p.weights[row];
     }
     // p_j = 2^((x_j - m) log2 e - log2s) with m = xt (or the row's maximum, `slow`)
     float logp = 0.f, lse = 0.f, log2s = 0.f, m = 0.f;
     bool slow = false;
-    if (counted) {
+    {
       float s0 = 0.f, s1 = 0.f;
       const auto add_piece = [&](const uint4& r) {
         float v[E];
@@ -309,35 +355,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           s1 += ex2((v[e + 1] - xt) * kLog2e);
         }
       };
-      uint32_t at = mine;
-      const char* src = nxt.body;
-#pragma unroll 1
-      for (int g = 0; g < kStages; ++g) {
-        copies_wait<kStages - 1>();
-        const uint32_t end = stage_end(g);
-#pragma unroll 1
-        for (; at < end; at += kStep) {
+      copies_wait();
+      {
+        uint32_t at = mine;
+        const char* src = nxt.body;
+#pragma unroll kUnroll
+        for (int k = 0; k < even; ++k, at += kStep, src += kStep) {
           add_piece(read_piece(at));
-          if constexpr (MODE == kLogp) {  // the slot is free: the next row's piece
-            if (more) copy_piece(at, src);
-            src += kStep;
-          }
+          if (MODE == kLogp && more) copy_piece(at, src);  // the slot is free: the next row's piece
         }
-        if (g == kStages - 1) {
-#pragma unroll 1
-          for (int k = even; k < iters; ++k) {
-            const int i = k * kThreads + tid;
-            const int n = i < cur.full ? E : i == cur.full ? cur.rest : 0;
-            if (n > 0) {
-              uint4 r = read_piece(mine + k * kStep);
-              if (n < E) P::fill(r, n, P::kMinusInf);
-              add_piece(r);
-            }
-          }
-          if (MODE == kLogp && more) copy_rest(nxt);
-        }
-        copies_commit();  // empty where the row's pieces stay for its gradient: it keeps the count of groups
       }
+#pragma unroll 1
+      for (int k = even; k < iters; ++k) {
+        const int i = k * kThreads + tid;
+        const int n = i < cur.full ? E : i == cur.full ? cur.rest : 0;
+        if (n > 0) {
+          uint4 r = read_piece(mine + k * kStep);
+          if (n < E) P::fill(r, n, P::kMinusInf);
+          add_piece(r);
+        }
+      }
+      if (MODE == kLogp && more) copy_rest(nxt);
       float s = s0 + s1;
       if (head_col) s += ex2((xh - xt) * kLog2e);
       s = warp_sum(s);
@@ -398,9 +436,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         lse = m + ln;
         logp = bad ? NAN : (xt - m) - ln;
       }
-    } else {
-      if (MODE == kLogp && more) copy_row(nxt);
-      else commit_row();
     }
     if (rank == 0 && tid == 0) {
       a.logp[row] = logp;
@@ -408,23 +443,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (bad) record_error(a.status, kBadArg, 410);
     }
     if constexpr (MODE != kLogp) {
-      float coef = counted ? 1.f : 0.f;
+      float coef = 1.f;
       if constexpr (MODE == kPolicy) {
-        if (counted) {
-          const RowTerm r = policy_term(p, logp, old, adv, ref, w);
-          coef = r.coef * (p.grad_scale ? *p.grad_scale : 1.f);
-          if (tid == 0) {
-            sum_loss += r.loss;
-            sum_kl += r.kl;
-            sum_clip += r.clipped;
-          }
+        const RowTerm r = policy_term(p, logp, old, adv, ref, w);
+        coef = r.coef * (p.grad_scale ? *p.grad_scale : 1.f);
+        if (tid == 0) {
+          sum_loss += r.loss;
+          sum_kl += r.kl;
+          sum_clip += r.clipped;
         }
       }
       if (bad) coef = NAN;
       char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
       char* out_body = out + (cur.head + (long)piece0 * E) * P::kBytes;
       char* out_mine = out_body + tid * 16;
-      const bool zero = coef == 0.f;  // ignored rows and clipped tokens: nothing to evaluate
+      const bool zero = coef == 0.f;  // clipped tokens: nothing to evaluate
       const bool fast = d.vec_store && !slow;
       const auto grad_piece = [&](const uint4& r, float (&v)[E]) {
         P::widen(r, v);
@@ -434,23 +467,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (fast) {
         uint32_t at = mine;
         const char* src = nxt.body;
-#pragma unroll 1
-        for (int g = 0; g < kStages; ++g) {
-          const uint32_t end = stage_end(g);
-#pragma unroll 1
-          for (; at < end; at += kStep) {
-            uint4 o = make_uint4(0u, 0u, 0u, 0u);
-            if (!zero) {
-              float v[E];
-              grad_piece(read_piece(at), v);
-              o = P::narrow(v);
-            }
-            *reinterpret_cast<uint4*>(out_mine) = o;
+        if (!zero) {
+#pragma unroll kUnroll
+          for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
+            float v[E];
+            grad_piece(read_piece(at), v);
+            *reinterpret_cast<uint4*>(out_mine) = P::narrow(v);
             if (more) copy_piece(at, src);  // the slot is free: the next row's piece
-            out_mine += kStep;
-            src += kStep;
           }
-          if (g < kStages - 1) copies_commit();
+        } else {
+#pragma unroll 4
+          for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
+            *reinterpret_cast<uint4*>(out_mine) = make_uint4(0u, 0u, 0u, 0u);
+            if (more) copy_piece(at, src);
+          }
         }
       }
       // the uneven rest, the columns behind V, and rows that take single stores
@@ -476,14 +506,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           }
         }
       }
-      if (!more) {
-        if (fast) copies_commit();
-        else commit_row();
-      } else if (fast) {
-        copy_rest(nxt);
-        copies_commit();
-      } else {
-        copy_row(nxt);
+      if (more) {
+        if (fast) copy_rest(nxt);
+        else copy_row(nxt);
       }
       if (rank == 0 && tid < min(cur.head, a.W) && !slow)
         store1<TYPE>(out, tid, head_col && !zero ? -coef * ex2(fmaf(xh - xt, kLog2e, -log2s)) : 0.f);
@@ -502,8 +527,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (owner) store1<TYPE>(out, tc, -coef * expm1f(logp));
       }
     }
-    t = t_next;
-    cur = row_of(next < a.M ? next : row);
+    cur = nxt;
+    // the ignored rows, spread over the counted ones: their stores go beside the next row's arithmetic
+    for (; (long)zeros * mine_counted < (long)mine_ignored * (j + 1); ++zeros) zero_row(list[d.list - 1 - zeros]);
+  }
+  for (; zeros < mine_ignored; ++zeros) zero_row(list[d.list - 1 - zeros]);
   }
   if constexpr (MODE == kPolicy) {
     if (rank == 0 && tid == 0) {
@@ -512,7 +540,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       part[3L * first + 2] = sum_clip;
     }
   }
-  copies_wait<0>();
 }
 
 __device__ __forceinline__ double block_sum(double v, double* sh) {
@@ -526,18 +553,28 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// loss and statistics: the rows' terms added in a fixed order, in 64 bits.
-__global__ void __launch_bounds__(1024) policy_sum_kernel(const double* __restrict__ part, int n,
-                                                          float* __restrict__ loss, float* __restrict__ stats) {
-  __shared__ double sh[32];
+// loss and statistics: the clusters' partial sums added in a fixed order, in 64 bits. Launched beside the row kernel
+// (programmatic dependent launch), so that only its own few hundred nanoseconds follow the last row.
+constexpr int kSumThreads = 128;
+__global__ void __launch_bounds__(kSumThreads) policy_sum_kernel(const double* __restrict__ part, int n,
+                                                                 float* __restrict__ loss, float* __restrict__ stats) {
+  __shared__ double sh[kSumThreads / 32][3];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double s[3] = {0.0, 0.0, 0.0};
-  for (int i = threadIdx.x; i < n; i += 1024)
-    for (int k = 0; k < 3; ++k) s[k] += part[3L * i + k];
-  for (int k = 0; k < 3; ++k) s[k] = block_sum(s[k], sh);
-  if (threadIdx.x == 0) {
-    loss[0] = (float)s[0];
-    stats[0] = (float)s[1];
-    stats[1] = (float)s[2];
+  for (int i = threadIdx.x; i < n; i += kSumThreads)
+    for (int k = 0; k < 3; ++k) s[k] += __ldcg(part + 3L * i + k);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5][k] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    double v = 0.0;
+    for (int w = 0; w < kSumThreads / 32; ++w) v += sh[w][threadIdx.x];
+    if (threadIdx.x == 0) loss[0] = static_cast<float>(v);
+    else stats[threadIdx.x - 1] = static_cast<float>(v);
   }
 }
 
@@ -585,8 +622,10 @@ __global__ void __launch_bounds__(256) preference_sum_kernel(const double* __res
 
 // Shared memory: 228 KB an SM, 227 KB a CTA; each CTA also takes 1 KB for the system and under 1 KB for the
 // kernel's own arrays.
-constexpr int kMaxPieces = (227 * 1024 - 1024) / 16;                  // one CTA on the SM
-constexpr int kMaxPiecesShared = (228 * 1024 / kCtasPerSm - 2048) / 16;  // kCtasPerSm of them
+constexpr int kListRows = 510;  // rows of one window that a cluster takes, at most
+constexpr int kListBytes = (kListRows + 2) * 4;
+constexpr int kMaxPieces = (227 * 1024 - 1024 - kListBytes) / 16;                     // one CTA on the SM
+constexpr int kMaxPiecesShared = (228 * 1024 / kCtasPerSm - 2048 - kListBytes) / 16;  // kCtasPerSm of them
 constexpr int kMaxSplit = 8;
 
 // Deals M rows of `row_pieces` pieces to clusters of 1, 2, 4 or 8 CTAs: the split with the least estimated
@@ -601,7 +640,7 @@ Deal deal_rows(int M, long row_pieces, int sms) {
     if (pieces > kMaxPieces) continue;
     const int resident = pieces <= kMaxPiecesShared ? kCtasPerSm : 1;
     const int most = sms * resident / c;
-    const int clusters = M < most ? M : most;
+    const int clusters = std::max(1, std::min(M, most));
     const int rounds = (M + most - 1) / most;
     const double ns = rounds * ((c > 1 ? 2200.0 : 1500.0) + 32.0 * pieces * resident / 43.0);
     if (best.split == 0 || ns < least) {
@@ -609,6 +648,9 @@ Deal deal_rows(int M, long row_pieces, int sms) {
       best.split = c;
       best.pieces = static_cast<int>(pieces);
       best.clusters = clusters;
+      best.window = static_cast<int>(std::min<long>(M, (long)clusters * kListRows));
+      // ceil(counted / clusters) + ceil(ignored / clusters) entries at most
+      best.list = (best.window + clusters - 1) / clusters + 1;
     }
   }
   return best;
@@ -620,13 +662,13 @@ void launch_typed(const LogitRows& a, const PolicyTerms& p, const Deal& d, doubl
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
   const int dev = current_device();
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    HB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPieces * 16));
+    HB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPieces * 16 + kListBytes));
     ready.fetch_or(uint64_t{1} << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(d.clusters * d.split));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(d.pieces) * 16;
+  cfg.dynamicSmemBytes = static_cast<size_t>(d.pieces) * 16 + static_cast<size_t>(d.list) * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -672,8 +714,17 @@ void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratc
                         cudaStream_t s) {
   const Deal d = deal_of(a);
   launch_rows<kPolicy>(a, p, d, scratch, s);
-  policy_sum_kernel<<<1, 1024, 0, s>>>(scratch, d.clusters, loss, stats);
-  HB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kSumThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.M > 0 ? 1 : 0;
+  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, policy_sum_kernel, static_cast<const double*>(scratch), a.M > 0 ? d.clusters : 0,
+                                   loss, stats));
 }
 
 void preference_loss_launch(const float* logp, const float* ref, const int64_t* targets, int64_t ignore_index, int P,
