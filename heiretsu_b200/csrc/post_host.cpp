@@ -18,7 +18,7 @@ namespace hb {
 
 long logit_row_limit(int type);
 long policy_scratch_doubles();
-long preference_scratch_doubles(int P);
+long preference_scratch_doubles(long tokens);
 void token_logprobs_launch(const LogitRows& a, cudaStream_t s);
 void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratch, float* loss, float* stats,
                         cudaStream_t s);
@@ -68,7 +68,7 @@ LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targ
   a.type = logit_type(logits, op);
   const int64_t M = logits.size(0);
   TORCH_CHECK(V >= 1 && V <= logits.size(1), op, ": V must be in [1, row width]");
-  TORCH_CHECK(M <= kIntMax, op, ": too many rows");
+  TORCH_CHECK(M <= kIntMax / 2, op, ": too many rows");
   const int64_t widest = logit_row_limit(a.type);  // what the shared memory of one cluster holds
   TORCH_CHECK(V <= widest, op, ": V must be at most ", std::to_string(widest), " for this dtype");
   TORCH_CHECK(logits.stride(0) >= 0, op, ": logits need a row stride that is not negative");
@@ -172,7 +172,7 @@ void preference_loss(const at::Tensor& logp, const at::Tensor& targets, int64_t 
   TORCH_CHECK(logp.dim() == 2 && logp.size(0) % 2 == 0, op,
               ": logp must be [2 * pairs, T], the chosen sequences before the rejected ones");
   const int64_t n = logp.numel(), P = logp.size(0) / 2, T = logp.size(1);
-  TORCH_CHECK(P <= kIntMax && T <= kIntMax, op, ": too many pairs or tokens");
+  TORCH_CHECK(P <= kIntMax / 2 && T <= kIntMax / 2, op, ": too many pairs or tokens");
   TORCH_CHECK(std::isfinite(beta), op, ": beta must be finite");
   TORCH_CHECK(label_smoothing >= 0 && label_smoothing <= 1, op, ": label_smoothing must be in [0, 1]");
   c10::cuda::CUDAGuard g(logp.device());
@@ -183,11 +183,13 @@ void preference_loss(const at::Tensor& logp, const at::Tensor& targets, int64_t 
   check_vec(rewards, at::kFloat, 2 * P, dev, op, "rewards");
   check_vec(dlogp, at::kFloat, n, dev, op, "dlogp");
   if (given(ref_logp)) check_vec(*ref_logp, at::kFloat, n, dev, op, "ref_logp");
-  at::Tensor scratch = at::empty({preference_scratch_doubles(static_cast<int>(P))}, logp.options().dtype(at::kDouble));
+  const long doubles = preference_scratch_doubles(n);
+  at::Tensor scratch;
+  if (doubles > 0) scratch = at::empty({doubles}, logp.options().dtype(at::kDouble));
   preference_loss_launch(logp.data_ptr<float>(), given(ref_logp) ? ref_logp->data_ptr<float>() : nullptr,
                          targets.data_ptr<int64_t>(), ignore_index, static_cast<int>(P), static_cast<int>(T),
                          beta, label_smoothing, loss.data_ptr<float>(),
-                         rewards.data_ptr<float>(), dlogp.data_ptr<float>(), scratch.data_ptr<double>(),
+                         rewards.data_ptr<float>(), dlogp.data_ptr<float>(), doubles > 0 ? scratch.data_ptr<double>() : nullptr,
                          at::cuda::getCurrentCUDAStream());
 }
 

@@ -312,6 +312,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     mine_ignored = (n - all - first + d.clusters - 1) / d.clusters;
     return all;
   };
+  // As many clusters as rows (`one_each`): nothing to list, and the row's copies need not wait for its target (an
+  // ignored row is then read in vain, one per cluster).
+  const bool one_each = a.M <= d.clusters;
+  if (one_each) copy_row(row_of(first));
+  const auto scan_one = [&] {
+    if (tid == 0) list[0] = first;
+    mine_counted = a.targets[first] != a.ignore_index;
+    mine_ignored = 1 - mine_counted;
+    int c = 0;
+    if (MODE == kPolicy && !p.weights) {
+      for (int i = tid; i < a.M; i += kThreads) c += a.targets[i] != a.ignore_index;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (lane == 0) sm_n[warp] = c;
+    }
+    __syncthreads();
+    if (MODE == kPolicy && !p.weights) {
+      c = 0;
+      for (int w = 0; w < kWarps; ++w) c += sm_n[w];
+    }
+    return c;
+  };
   const int window = min(a.M, d.window);
   int all = 0;
   if (MODE == kPolicy && !p.weights && window < a.M) {  // 1 / (counted rows) of several windows
@@ -319,220 +340,221 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     unit_w = 1.f / static_cast<float>(max(all, 1));
   }
   for (int w0 = 0; w0 < a.M; w0 += window) {
-  all = scan(w0, min(window, a.M - w0));
-  if (MODE == kPolicy && window == a.M) unit_w = 1.f / static_cast<float>(max(all, 1));
-  int zeros = 0;  // ignored rows done
-  Row cur = row_of(mine_counted > 0 ? list[0] : 0);
-  if (mine_counted > 0) copy_row(cur);
-  for (int j = 0; j < mine_counted; ++j) {
-    const int row = list[j];
-    const bool more = j + 1 < mine_counted;  // there are copies to make
-    const Row nxt = row_of(more ? list[j + 1] : row);
-    const int64_t t = a.targets[row];
-    const bool bad = t < 0 || t >= a.V;
-    const int tc = bad ? -1 : static_cast<int>(t);
-    const bool head_col = rank == 0 && tid < min(cur.head, a.V);
-    // read here, used after pass 1
-    const float xt = bad ? 0.f : load1<TYPE>(cur.base, tc), xh = head_col ? load1<TYPE>(cur.base, tid) : 0.f;
-    float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w;
-    if constexpr (MODE == kPolicy) {
-      old = p.old_logp[row];
-      adv = p.adv[p.adv_rows == 1 ? row : row / p.adv_rows];
-      if (p.ref_logp) ref = p.ref_logp[row];
-      if (p.weights) w = p.weights[row];
-    }
-    // p_j = 2^((x_j - m) log2 e - log2s) with m = xt (or the row's maximum, `slow`)
-    float logp = 0.f, lse = 0.f, log2s = 0.f, m = 0.f;
-    bool slow = false;
-    {
-      float s0 = 0.f, s1 = 0.f;
-      const auto add_piece = [&](const uint4& r) {
-        float v[E];
-        P::widen(r, v);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          s0 += ex2((v[e] - xt) * kLog2e);
-          s1 += ex2((v[e + 1] - xt) * kLog2e);
-        }
-      };
-      copies_wait();
+    all = one_each ? scan_one() : scan(w0, min(window, a.M - w0));
+    if (MODE == kPolicy && window == a.M) unit_w = 1.f / static_cast<float>(max(all, 1));
+    int zeros = 0;  // ignored rows done
+    Row cur = row_of(mine_counted > 0 ? list[0] : 0);
+    if (mine_counted > 0 && !one_each) copy_row(cur);
+    for (int j = 0; j < mine_counted; ++j) {
+      const int row = list[j];
+      const bool more = j + 1 < mine_counted;  // there are copies to make
+      const Row nxt = row_of(more ? list[j + 1] : row);
+      const int64_t t = a.targets[row];
+      const bool bad = t < 0 || t >= a.V;
+      const int tc = bad ? -1 : static_cast<int>(t);
+      const bool head_col = rank == 0 && tid < min(cur.head, a.V);
+      // read here, used after pass 1
+      const float xt = bad ? 0.f : load1<TYPE>(cur.base, tc), xh = head_col ? load1<TYPE>(cur.base, tid) : 0.f;
+      float old = 0.f, adv = 0.f, ref = 0.f, w = unit_w;
+      if constexpr (MODE == kPolicy) {
+        old = p.old_logp[row];
+        adv = p.adv[p.adv_rows == 1 ? row : row / p.adv_rows];
+        if (p.ref_logp) ref = p.ref_logp[row];
+        if (p.weights) w = p.weights[row];
+      }
+      // p_j = 2^((x_j - m) log2 e - log2s) with m = xt (or the row's maximum, `slow`)
+      float logp = 0.f, lse = 0.f, log2s = 0.f, m = 0.f;
+      bool slow = false;
       {
-        uint32_t at = mine;
-        const char* src = nxt.body;
-#pragma unroll kUnroll
-        for (int k = 0; k < even; ++k, at += kStep, src += kStep) {
-          add_piece(read_piece(at));
-          if (MODE == kLogp && more) copy_piece(at, src);  // the slot is free: the next row's piece
-        }
-      }
-#pragma unroll 1
-      for (int k = even; k < iters; ++k) {
-        const int i = k * kThreads + tid;
-        const int n = i < cur.full ? E : i == cur.full ? cur.rest : 0;
-        if (n > 0) {
-          uint4 r = read_piece(mine + k * kStep);
-          if (n < E) P::fill(r, n, P::kMinusInf);
-          add_piece(r);
-        }
-      }
-      if (MODE == kLogp && more) copy_rest(nxt);
-      float s = s0 + s1;
-      if (head_col) s += ex2((xh - xt) * kLog2e);
-      s = warp_sum(s);
-      if (lane == 0) sm_s[parity][warp] = s;
-      __syncthreads();
-      s = sm_s[parity][lane % kWarps];
+        float s0 = 0.f, s1 = 0.f;
+        const auto add_piece = [&](const uint4& r) {
+          float v[E];
+          P::widen(r, v);
 #pragma unroll
-      for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (d.split > 1) {
-        auto cl = cooperative_groups::this_cluster();
-        if (tid < d.split) *cl.map_shared_rank(&xch[parity][rank], tid) = s;
-        cl.sync();
-        s = 0.f;
-        for (int c = 0; c < d.split; ++c) s += xch[parity][c];
-      }
-      parity ^= 1;
-      slow = bad || !(s < 1.329227995784916e36f);  // 2^120; also NaN
-      if (!slow) {
-        m = xt;
-        const float ln = logf(s);
-        log2s = ln * kLog2e;
-        logp = -ln;
-        lse = xt + ln;
-      } else {
-        // the same sum under a maximum, from global memory, one column at a time
-        Sum z;
-        const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
-        const int hi = min(a.V, cur.head + (piece0 + d.pieces) * E);
-        for (int j = lo + tid; j < hi; j += kThreads) z.add(load1<TYPE>(cur.base, j));
-        m = z.m;
-        s = z.s;
-        join_lanes<32>(m, s);
-        if (lane == 0) {
-          slow_m[warp] = m;
-          slow_s[warp] = s;
+          for (int e = 0; e < E; e += 2) {
+            s0 += ex2((v[e] - xt) * kLog2e);
+            s1 += ex2((v[e + 1] - xt) * kLog2e);
+          }
+        };
+        copies_wait();
+        {
+          uint32_t at = mine;
+          const char* src = nxt.body;
+#pragma unroll kUnroll
+          for (int k = 0; k < even; ++k, at += kStep, src += kStep) {
+            add_piece(read_piece(at));
+            if (MODE == kLogp && more) copy_piece(at, src);  // the slot is free: the next row's piece
+          }
         }
+#pragma unroll 1
+        for (int k = even; k < iters; ++k) {
+          const int i = k * kThreads + tid;
+          const int n = i < cur.full ? E : i == cur.full ? cur.rest : 0;
+          if (n > 0) {
+            uint4 r = read_piece(mine + k * kStep);
+            if (n < E) P::fill(r, n, P::kMinusInf);
+            add_piece(r);
+          }
+        }
+        if (MODE == kLogp && more) copy_rest(nxt);
+        float s = s0 + s1;
+        if (head_col) s += ex2((xh - xt) * kLog2e);
+        s = warp_sum(s);
+        if (lane == 0) sm_s[parity][warp] = s;
         __syncthreads();
-        m = slow_m[lane % kWarps];
-        s = slow_s[lane % kWarps];
-        join_lanes<kWarps>(m, s);
+        s = sm_s[parity][lane % kWarps];
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (d.split > 1) {
           auto cl = cooperative_groups::this_cluster();
-          if (tid < d.split) {
-            float* to = cl.map_shared_rank(&slow_x[rank][0], tid);
-            to[0] = m;
-            to[1] = s;
-          }
+          if (tid < d.split) *cl.map_shared_rank(&xch[parity][rank], tid) = s;
           cl.sync();
-          m = slow_x[lane % d.split][0];
-          s = lane < d.split ? slow_x[lane][1] : 0.f;
+          s = 0.f;
+          for (int c = 0; c < d.split; ++c) s += xch[parity][c];
+        }
+        parity ^= 1;
+        slow = bad || !(s < 1.329227995784916e36f);  // 2^120; also NaN
+        if (!slow) {
+          m = xt;
+          const float ln = logf(s);
+          log2s = ln * kLog2e;
+          logp = -ln;
+          lse = xt + ln;
+        } else {
+          // the same sum under a maximum, from global memory, one column at a time
+          Sum z;
+          const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
+          const int hi = min(a.V, cur.head + (piece0 + d.pieces) * E);
+          for (int j = lo + tid; j < hi; j += kThreads) z.add(load1<TYPE>(cur.base, j));
+          m = z.m;
+          s = z.s;
           join_lanes<32>(m, s);
-          cl.sync();  // read before the next slow row writes it
-        } else {
+          if (lane == 0) {
+            slow_m[warp] = m;
+            slow_s[warp] = s;
+          }
           __syncthreads();
-        }
-        log2s = log2f(s);
-        const float ln = logf(s);
-        lse = m + ln;
-        logp = bad ? NAN : (xt - m) - ln;
-      }
-    }
-    if (rank == 0 && tid == 0) {
-      a.logp[row] = logp;
-      if (a.lse) a.lse[row] = lse;
-      if (bad) record_error(a.status, kBadArg, 410);
-    }
-    if constexpr (MODE != kLogp) {
-      float coef = 1.f;
-      if constexpr (MODE == kPolicy) {
-        const RowTerm r = policy_term(p, logp, old, adv, ref, w);
-        coef = r.coef * (p.grad_scale ? *p.grad_scale : 1.f);
-        if (tid == 0) {
-          sum_loss += r.loss;
-          sum_kl += r.kl;
-          sum_clip += r.clipped;
-        }
-      }
-      if (bad) coef = NAN;
-      char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
-      char* out_body = out + (cur.head + (long)piece0 * E) * P::kBytes;
-      char* out_mine = out_body + tid * 16;
-      const bool zero = coef == 0.f;  // clipped tokens: nothing to evaluate
-      const bool fast = d.vec_store && !slow;
-      const auto grad_piece = [&](const uint4& r, float (&v)[E]) {
-        P::widen(r, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = -coef * ex2(fmaf(v[e] - xt, kLog2e, -log2s));
-      };
-      if (fast) {
-        uint32_t at = mine;
-        const char* src = nxt.body;
-        if (!zero) {
-#pragma unroll kUnroll
-          for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
-            float v[E];
-            grad_piece(read_piece(at), v);
-            *reinterpret_cast<uint4*>(out_mine) = P::narrow(v);
-            if (more) copy_piece(at, src);  // the slot is free: the next row's piece
-          }
-        } else {
-#pragma unroll 4
-          for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
-            *reinterpret_cast<uint4*>(out_mine) = make_uint4(0u, 0u, 0u, 0u);
-            if (more) copy_piece(at, src);
-          }
-        }
-      }
-      // the uneven rest, the columns behind V, and rows that take single stores
-      if (!slow) {
-#pragma unroll 1
-        for (int k = fast ? even : 0; k < iters; ++k) {
-          const int i = k * kThreads + tid;
-          const int c0 = cur.head + (piece0 + i) * E;
-          if (i >= d.pieces || c0 >= a.W) break;
-          const int n = zero ? 0 : i < cur.full ? E : i == cur.full ? cur.rest : 0;  // elements to evaluate
-          float v[E];
-          uint4 r = make_uint4(0u, 0u, 0u, 0u);
-          if (n > 0) {
-            grad_piece(read_piece(mine + k * kStep), v);
-            r = P::narrow(v);
-            if (n < E) P::fill(r, n, 0u);
-          }
-          if (fast && c0 + E <= a.W) {
-            *reinterpret_cast<uint4*>(out_body + (long)i * 16) = r;
+          m = slow_m[lane % kWarps];
+          s = slow_s[lane % kWarps];
+          join_lanes<kWarps>(m, s);
+          if (d.split > 1) {
+            auto cl = cooperative_groups::this_cluster();
+            if (tid < d.split) {
+              float* to = cl.map_shared_rank(&slow_x[rank][0], tid);
+              to[0] = m;
+              to[1] = s;
+            }
+            cl.sync();
+            m = slow_x[lane % d.split][0];
+            s = lane < d.split ? slow_x[lane][1] : 0.f;
+            join_lanes<32>(m, s);
+            cl.sync();  // read before the next slow row writes it
           } else {
-#pragma unroll 1
-            for (int e = 0; e < E && c0 + e < a.W; ++e) P::store_at(r, e, out_body, (long)i * E + e);
+            __syncthreads();
+          }
+          log2s = log2f(s);
+          const float ln = logf(s);
+          lse = m + ln;
+          logp = bad ? NAN : (xt - m) - ln;
+        }
+      }
+      if (rank == 0 && tid == 0) {
+        a.logp[row] = logp;
+        if (a.lse) a.lse[row] = lse;
+        if (bad) record_error(a.status, kBadArg, 410);
+      }
+      if constexpr (MODE != kLogp) {
+        float coef = 1.f;
+        if constexpr (MODE == kPolicy) {
+          const RowTerm r = policy_term(p, logp, old, adv, ref, w);
+          coef = r.coef * (p.grad_scale ? *p.grad_scale : 1.f);
+          if (tid == 0) {
+            sum_loss += r.loss;
+            sum_kl += r.kl;
+            sum_clip += r.clipped;
           }
         }
-      }
-      if (more) {
-        if (fast) copy_rest(nxt);
-        else copy_row(nxt);
-      }
-      if (rank == 0 && tid < min(cur.head, a.W) && !slow)
-        store1<TYPE>(out, tid, head_col && !zero ? -coef * ex2(fmaf(xh - xt, kLog2e, -log2s)) : 0.f);
-      if (slow) {
-        const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
-        const int hi = min(a.W, cur.head + (piece0 + d.pieces) * E);
-        for (int j = lo + tid; j < hi; j += kThreads) {
-          const float g = j < a.V ? coef * ((j == tc ? 1.f : 0.f) - ex2(fmaf(load1<TYPE>(cur.base, j) - m, kLog2e, -log2s))) : 0.f;
-          store1<TYPE>(out, j, g);
+        if (bad) coef = NAN;
+        char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
+        char* out_body = out + (cur.head + (long)piece0 * E) * P::kBytes;
+        char* out_mine = out_body + tid * 16;
+        const bool zero = coef == 0.f;  // clipped tokens: nothing to evaluate
+        const bool fast = d.vec_store && !slow;
+        const auto grad_piece = [&](const uint4& r, float (&v)[E]) {
+          P::widen(r, v);
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = -coef * ex2(fmaf(v[e] - xt, kLog2e, -log2s));
+        };
+        if (fast) {
+          uint32_t at = mine;
+          const char* src = nxt.body;
+          if (!zero) {
+#pragma unroll kUnroll
+            for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
+              float v[E];
+              grad_piece(read_piece(at), v);
+              *reinterpret_cast<uint4*>(out_mine) = P::narrow(v);
+              if (more) copy_piece(at, src);  // the slot is free: the next row's piece
+            }
+          } else {
+#pragma unroll 4
+            for (int k = 0; k < even; ++k, at += kStep, src += kStep, out_mine += kStep) {
+              *reinterpret_cast<uint4*>(out_mine) = make_uint4(0u, 0u, 0u, 0u);
+              if (more) copy_piece(at, src);
+            }
+          }
         }
-      } else if (tc >= 0 && !zero) {
-        // the target's element, by the thread that has just stored its piece (or head column)
-        const int i = tc < cur.head ? -1 : (tc - cur.head) / E - piece0;
-        const bool owner = i < 0 ? tc < cur.head && rank == 0 && tid == tc : i < d.pieces && tid == i % kThreads;
-        // (1 - p_t from logp itself, which keeps its digits where p_t is near 1)
-        if (owner) store1<TYPE>(out, tc, -coef * expm1f(logp));
+        // the uneven rest, the columns behind V, and rows that take single stores
+        if (!slow) {
+#pragma unroll 1
+          for (int k = fast ? even : 0; k < iters; ++k) {
+            const int i = k * kThreads + tid;
+            const int c0 = cur.head + (piece0 + i) * E;
+            if (i >= d.pieces || c0 >= a.W) break;
+            const int n = zero ? 0 : i < cur.full ? E : i == cur.full ? cur.rest : 0;  // elements to evaluate
+            float v[E];
+            uint4 r = make_uint4(0u, 0u, 0u, 0u);
+            if (n > 0) {
+              grad_piece(read_piece(mine + k * kStep), v);
+              r = P::narrow(v);
+              if (n < E) P::fill(r, n, 0u);
+            }
+            if (fast && c0 + E <= a.W) {
+              *reinterpret_cast<uint4*>(out_body + (long)i * 16) = r;
+            } else {
+#pragma unroll 1
+              for (int e = 0; e < E && c0 + e < a.W; ++e) P::store_at(r, e, out_body, (long)i * E + e);
+            }
+          }
+        }
+        if (more) {
+          if (fast) copy_rest(nxt);
+          else copy_row(nxt);
+        }
+        if (rank == 0 && tid < min(cur.head, a.W) && !slow)
+          store1<TYPE>(out, tid, head_col && !zero ? -coef * ex2(fmaf(xh - xt, kLog2e, -log2s)) : 0.f);
+        if (slow) {
+          const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
+          const int hi = min(a.W, cur.head + (piece0 + d.pieces) * E);
+          for (int j = lo + tid; j < hi; j += kThreads) {
+            const float g = j < a.V ? coef * ((j == tc ? 1.f : 0.f) - ex2(fmaf(load1<TYPE>(cur.base, j) - m, kLog2e, -log2s))) : 0.f;
+            store1<TYPE>(out, j, g);
+          }
+        } else if (tc >= 0 && !zero) {
+          // the target's element, by the thread that has just stored its piece (or head column)
+          const int i = tc < cur.head ? -1 : (tc - cur.head) / E - piece0;
+          const bool owner = i < 0 ? tc < cur.head && rank == 0 && tid == tc : i < d.pieces && tid == i % kThreads;
+          // (1 - p_t from logp itself, which keeps its digits where p_t is near 1)
+          if (owner) store1<TYPE>(out, tc, -coef * expm1f(logp));
+        }
       }
+      cur = nxt;
+      // the ignored rows, spread over the counted ones: their stores go beside the next row's arithmetic
+      for (; (long)zeros * mine_counted < (long)mine_ignored * (j + 1); ++zeros) zero_row(list[d.list - 1 - zeros]);
     }
-    cur = nxt;
-    // the ignored rows, spread over the counted ones: their stores go beside the next row's arithmetic
-    for (; (long)zeros * mine_counted < (long)mine_ignored * (j + 1); ++zeros) zero_row(list[d.list - 1 - zeros]);
+    for (; zeros < mine_ignored; ++zeros) zero_row(one_each ? first : list[d.list - 1 - zeros]);
   }
-  for (; zeros < mine_ignored; ++zeros) zero_row(list[d.list - 1 - zeros]);
-  }
+  copies_wait();  // of a row read in vain
   if constexpr (MODE == kPolicy) {
     if (rank == 0 && tid == 0) {
       part[3L * first] = sum_loss;
@@ -540,17 +562,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       part[3L * first + 2] = sum_clip;
     }
   }
-}
-
-__device__ __forceinline__ double block_sum(double v, double* sh) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) v += sh[w];
-  __syncthreads();
-  return v;
 }
 
 // loss and statistics: the clusters' partial sums added in a fixed order, in 64 bits. Launched beside the row kernel
@@ -578,46 +589,131 @@ __global__ void __launch_bounds__(kSumThreads) policy_sum_kernel(const double* _
   }
 }
 
-// log(1 + e^t) without overflow.
-__device__ __forceinline__ double softplus(double t) { return fmax(t, 0.0) + log1p(exp(-fabs(t))); }
+// Preference loss. A group of G warps takes a pair: the sums of both sequences in 64 bits, the pair's loss and
+// factor, then both gradient rows (the targets are read again, from cache). CLUSTER: one cluster of 8 CTAs does
+// all pairs and adds their losses through shared memory: one launch, which is what small batches are bound by
+// (2^17 tokens are 2.6 MB). Larger batches spread over the SMs and leave their sums to preference_sum_kernel. Either
+// way the order of every sum is fixed.
+constexpr int kPrefThreads = 1024;
+constexpr int kPrefWarps = kPrefThreads / 32;
+constexpr int kPrefCluster = 8;
+constexpr long kPrefClusterTokens = 1L << 18;
+constexpr int kPrefMaxCtas = 1024;
 
-// One CTA per pair: sums both sequences, then writes both gradient rows.
-__global__ void __launch_bounds__(256) preference_kernel(const float* __restrict__ logp, const float* __restrict__ ref,
-                                                         const int64_t* __restrict__ targets, int64_t ignore_index,
-                                                         int P, int T, double beta, double smoothing,
-                                                         float* __restrict__ rewards, float* __restrict__ dlogp,
-                                                         double* __restrict__ part) {
-  __shared__ double sh[32];
-  const int i = blockIdx.x;
-  double sum[2];
-  for (int h = 0; h < 2; ++h) {
-    const long base = (long)(i + h * P) * T;
+struct Preference {
+  const float *logp, *ref;  // ref may be nullptr
+  const int64_t* targets;
+  int64_t ignore_index;
+  int P, T, G;
+  double beta, smoothing;
+  float *loss, *rewards, *dlogp;
+  double* part;  // [gridDim.x] without a cluster
+};
+
+template <bool CLUSTER>
+__global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preference a) {
+  __shared__ double sums[2][kPrefWarps][2], losses[kPrefWarps], total[kPrefCluster];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per_cta = kPrefWarps / a.G, groups = per_cta * gridDim.x;
+  const int group = blockIdx.x * per_cta + warp / a.G;
+  const int gl = threadIdx.x % (a.G * 32), gn = a.G * 32;  // thread within its group
+  if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();
+  double loss = 0.0;
+  int parity = 0;
+  for (int p0 = 0; p0 < a.P; p0 += groups) {  // the same rounds for every thread of the CTA
+    const int pair = p0 + group;
+    const bool in = pair < a.P;
+    double s[2] = {0.0, 0.0};
+    if (in) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long base = ((long)pair + (long)h * a.P) * a.T;
+        constexpr int kBatch = 8;  // loads in flight
+        for (int j0 = gl; j0 < a.T; j0 += kBatch * gn) {
+          int64_t t[kBatch];
+          float v[kBatch], r[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const int j = j0 + k * gn;
+            const bool at = j < a.T;
+            t[k] = at ? a.targets[base + j] : a.ignore_index;
+            v[k] = at ? a.logp[base + j] : 0.f;
+            r[k] = at && a.ref ? a.ref[base + j] : 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+            if (t[k] != a.ignore_index) s[h] += static_cast<double>(v[k]) - static_cast<double>(r[k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      s[1] += __shfl_xor_sync(0xffffffffu, s[1], o);
+    }
+    if (a.G > 1) {
+      if (lane == 0) {
+        sums[parity][warp][0] = s[0];
+        sums[parity][warp][1] = s[1];
+      }
+      __syncthreads();
+      s[0] = s[1] = 0.0;
+      const int w0 = warp / a.G * a.G;
+      for (int w = w0; w < w0 + a.G; ++w) {
+        s[0] += sums[parity][w][0];
+        s[1] += sums[parity][w][1];
+      }
+      parity ^= 1;
+    }
+    if (in) {
+      const double good = a.beta * s[0], poor = a.beta * s[1], z = good - poor;
+      // sigmoid(z), sigmoid(-z) and log(1 + e^-z), log(1 + e^z) from e = e^-|z|, which cannot overflow
+      const double e = exp(-fabs(z)), big = 1.0 / (1.0 + e), small = e * big, l = log1p(e);
+      const double sig = z >= 0.0 ? big : small, sig_neg = z >= 0.0 ? small : big;
+      const float c = static_cast<float>(z != z ? z : a.beta / a.P * (a.smoothing * sig - (1.0 - a.smoothing) * sig_neg));
+      if (gl == 0) {
+        a.rewards[pair] = static_cast<float>(good);
+        a.rewards[a.P + pair] = static_cast<float>(poor);
+        loss += (1.0 - a.smoothing) * (fmax(-z, 0.0) + l) + a.smoothing * (fmax(z, 0.0) + l);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long base = ((long)pair + (long)h * a.P) * a.T;
+        const float g = h ? -c : c;
+#pragma unroll 8
+        for (int j = gl; j < a.T; j += gn) a.dlogp[base + j] = a.targets[base + j] != a.ignore_index ? g : 0.f;
+      }
+    }
+  }
+  if (gl == 0) losses[warp] = loss;  // the first warp of each group holds its pairs' sum
+  __syncthreads();
+  if constexpr (CLUSTER) {
+    auto cl = cooperative_groups::this_cluster();
+    if (threadIdx.x == 0) {
+      double v = 0.0;
+      for (int w = 0; w < kPrefWarps; w += a.G) v += losses[w];
+      *cl.map_shared_rank(&total[blockIdx.x], 0) = v;
+    }
+    cl.sync();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      double v = 0.0;
+      for (int c = 0; c < kPrefCluster; ++c) v += total[c];
+      a.loss[0] = a.P > 0 ? static_cast<float>(v / a.P) : 0.f;
+    }
+  } else if (threadIdx.x == 0) {
     double v = 0.0;
-    for (int j = threadIdx.x; j < T; j += blockDim.x)
-      if (targets[base + j] != ignore_index) v += (double)logp[base + j] - (ref ? (double)ref[base + j] : 0.0);
-    sum[h] = beta * block_sum(v, sh);
-  }
-  const double z = sum[0] - sum[1];
-  const double c = beta / P * (smoothing / (1.0 + exp(-z)) - (1.0 - smoothing) / (1.0 + exp(z)));
-  if (threadIdx.x == 0) {
-    rewards[i] = (float)sum[0];
-    rewards[P + i] = (float)sum[1];
-    part[i] = (1.0 - smoothing) * softplus(-z) + smoothing * softplus(z);
-  }
-  for (int h = 0; h < 2; ++h) {
-    const long base = (long)(i + h * P) * T;
-    const float g = (float)(h ? -c : c);
-    for (int j = threadIdx.x; j < T; j += blockDim.x) dlogp[base + j] = targets[base + j] != ignore_index ? g : 0.f;
+    for (int w = 0; w < kPrefWarps; w += a.G) v += losses[w];
+    a.part[blockIdx.x] = v;
   }
 }
 
-__global__ void __launch_bounds__(256) preference_sum_kernel(const double* __restrict__ part, int P,
-                                                             float* __restrict__ loss) {
-  __shared__ double sh[32];
+__global__ void __launch_bounds__(32) preference_sum_kernel(const double* __restrict__ part, int n, int P,
+                                                            float* __restrict__ loss) {
   double v = 0.0;
-  for (int i = threadIdx.x; i < P; i += 256) v += part[i];
-  v = block_sum(v, sh);
-  if (threadIdx.x == 0) loss[0] = P > 0 ? (float)(v / P) : 0.f;
+  for (int i = threadIdx.x; i < n; i += 32) v += part[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (threadIdx.x == 0) loss[0] = static_cast<float>(v / P);
 }
 
 // Shared memory: 228 KB an SM, 227 KB a CTA; each CTA also takes 1 KB for the system and under 1 KB for the
@@ -702,7 +798,7 @@ Deal deal_of(const LogitRows& a) {
 
 long logit_row_limit(int type) { return static_cast<long>(kMaxPieces) * kMaxSplit * (type == kLogitF32 ? 4 : 8); }
 long policy_scratch_doubles() { return 3L * kCtasPerSm * num_sms(current_device()); }
-long preference_scratch_doubles(int P) { return P; }
+long preference_scratch_doubles(long tokens) { return tokens <= kPrefClusterTokens ? 0 : kPrefMaxCtas; }
 
 void token_logprobs_launch(const LogitRows& a, cudaStream_t s) {
   const PolicyTerms none{};
@@ -730,12 +826,29 @@ void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratc
 void preference_loss_launch(const float* logp, const float* ref, const int64_t* targets, int64_t ignore_index, int P,
                             int T, double beta, double smoothing, float* loss, float* rewards, float* dlogp,
                             double* scratch, cudaStream_t s) {
-  if (P > 0) {
-    preference_kernel<<<P, 256, 0, s>>>(logp, ref, targets, ignore_index, P, T, beta, smoothing, rewards, dlogp,
-                                        scratch);
-    HB_CUDA_CHECK(cudaGetLastError());
+  Preference a{logp, ref, targets, ignore_index, P, T, 1, beta, smoothing, loss, rewards, dlogp, scratch};
+  if (2L * P * T <= kPrefClusterTokens) {
+    const int n = std::max(1, (P + kPrefCluster - 1) / kPrefCluster);  // pairs of one CTA
+    while (a.G * 2 * n <= kPrefWarps) a.G *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kPrefCluster);
+    cfg.blockDim = dim3(kPrefThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kPrefCluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, preference_kernel<true>, static_cast<const Preference>(a)));
+    return;
   }
-  preference_sum_kernel<<<1, 256, 0, s>>>(scratch, P, loss);
+  while (a.G < kPrefWarps && a.G * 256 < T) a.G *= 2;  // 8 tokens of a sequence a thread
+  const int per_cta = kPrefWarps / a.G;
+  const int ctas = std::min((P + per_cta - 1) / per_cta, kPrefMaxCtas);
+  preference_kernel<false><<<ctas, kPrefThreads, 0, s>>>(a);
+  HB_CUDA_CHECK(cudaGetLastError());
+  preference_sum_kernel<<<1, 32, 0, s>>>(scratch, ctas, P, loss);
   HB_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -73,6 +73,7 @@ SHAPES = [  # M, V, W (row width), off (elements the rows are shifted by), ld
     (700, 2049, 2056, 0, None),   # more rows than CTAs that run at once
     (2, 131071, 131071, 0, None),
     (1, 300001, 300001, 1, None),
+    (160001, 33, 40, 0, None),    # more rows than one scan of the targets lists
 ]
 
 
@@ -352,7 +353,8 @@ def pairs(P, T, seed, ref=True, empty=False):
 
 
 @pytest.mark.parametrize("ref", [True, False])
-@pytest.mark.parametrize("P,T", [(1, 1), (1, 57), (2, 128), (3, 1023), (5, 4097), (64, 33), (300, 7), (1, 20001), (1030, 2)])
+@pytest.mark.parametrize("P,T", [(1, 1), (1, 57), (2, 128), (3, 1023), (5, 4097), (64, 33), (300, 7), (1, 20001), (1030, 2),
+                                 (131, 1031), (1, 200001), (40000, 5)])
 def test_preference_loss(P, T, ref):
     for beta, eps, empty in ((0.1, 0.0, False), (0.7, 0.1, True), (-0.2, 1.0, False)):
         lp, t, r = pairs(P, T, P + T, ref, empty)
