@@ -33,13 +33,23 @@ __device__ __forceinline__ float act8_inv_scale(uint32_t byte) {
 __device__ __forceinline__ float act8_scale(uint32_t byte) {
   return byte == kAct8Nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
 }
-// Rounding by adding 1.5 * 2^23: the sum's low byte is the code in two's complement (|x 2^-e| <= 127). A NaN
-// or infinity times 0 is NaN; its code is never used (the byte says NaN).
-__device__ __forceinline__ uint32_t act8_code(float x, float inv) {
-  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)) & 0xFFu;
+// Four codes, the first in the low byte. Rounding by adding 1.5 * 2^23: the sum's low byte is the code in two's
+// complement (|x 2^-e| <= 127). Blocks with byte 255 get codes 0 (an infinity or NaN times 0 is NaN).
+__device__ __forceinline__ uint32_t act8_codes(const float (&x)[4], uint32_t byte) {
+  const float inv = act8_inv_scale(byte);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+  const uint32_t all = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  return byte == kAct8Nan ? 0u : all;
 }
-__device__ __forceinline__ float act8_value(uint32_t code, float scale) {
-  return static_cast<float>(static_cast<int8_t>(code)) * scale;
+// Their values. A byte, with its sign bit flipped, is code + 128; put under the exponent of 2^23 it reads as the
+// number 2^23 + 128 + code, so one byte permutation and one subtraction give the code as a float.
+__device__ __forceinline__ void act8_values(uint32_t codes, float scale, float (&v)[4]) {
+  const uint32_t flipped = codes ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = (__uint_as_float(__byte_perm(flipped, 0x4B000000u, 0x7650u + i)) - 8388736.f) * scale;
 }
 
 }  // namespace hb

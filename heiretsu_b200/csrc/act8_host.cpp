@@ -17,7 +17,7 @@ void act8_pack_launch(const void* x, long ld, int type, int8_t* q, uint8_t* e, l
 void act8_unpack_launch(const int8_t* q, const uint8_t* e, int type, void* x, void* h, long M, int N, cudaStream_t s);
 void ln_fwd_act8_launch(const float* x, const float* w, const float* b, void* y, int8_t* q, uint8_t* e, float* rstd,
                         int M, int H, float eps, bool f16, cudaStream_t s);
-int ln_bwd_act8_ctas(int M, int device);
+int ln_bwd_act8_ctas(int M, int H, int device);
 void ln_bwd_act8_launch(const float* dy, const int8_t* q, const uint8_t* e, const float* rstd, const float* w,
                         const float* b, const float* dres_in, float* dres, void* dres16, void* y, float* part, int ctas,
                         float* dgamma, float* dbeta, int M, int H, bool f16, cudaStream_t s);
@@ -52,7 +52,9 @@ void check_codes(const at::Tensor& q, const at::Tensor& e, const char* op) {
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   TORCH_CHECK(q.dim() == 2 && q.size(1) <= kIntMax - kBlock, op, ": q must be [rows, columns]");
   check_mat(q, at::kChar, q.size(0), q.size(1), q.device(), op, "q");
-  check_mat(e, at::kByte, q.size(0), (q.size(1) + kBlock - 1) / kBlock, q.device(), op, "e");
+  const int64_t nb = (q.size(1) + kBlock - 1) / kBlock;
+  check_mat(e, at::kByte, q.size(0), nb, q.device(), op, "e");
+  TORCH_CHECK(q.size(0) == 0 || nb <= (kIntMax - 64) / q.size(0), op, ": too many blocks");
 }
 
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -115,7 +117,8 @@ void layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w, const at::Tens
 
 int64_t layernorm_bwd_act8_scratch_rows(const at::Tensor& q) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.size(0) <= kIntMax, "layernorm_bwd_act8: q must be a CUDA matrix");
-  return ln_bwd_act8_ctas(static_cast<int>(q.size(0)), q.get_device());
+  check_width(q.size(0), q.size(1), "layernorm_bwd_act8");
+  return ln_bwd_act8_ctas(static_cast<int>(q.size(0)), static_cast<int>(q.size(1)), q.get_device());
 }
 
 void layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
@@ -138,7 +141,7 @@ void layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Ten
   check_mat(y, dres16.scalar_type(), M, H, dev, op, "y");
   check_vec(dgamma, H, dev, op, "dgamma");
   check_vec(dbeta, H, dev, op, "dbeta");
-  const int ctas = ln_bwd_act8_ctas(static_cast<int>(M), q.get_device());
+  const int ctas = ln_bwd_act8_ctas(static_cast<int>(M), static_cast<int>(H), q.get_device());
   TORCH_CHECK(scratch.device() == dev && scratch.scalar_type() == at::kFloat && scratch.is_contiguous() &&
                   scratch.numel() >= (int64_t)ctas * 2 * H,
               op, ": scratch too small");

@@ -482,12 +482,6 @@ void ln_bwd_launch(const float* dy, const float* x, const float* mean, const flo
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
-// dgamma / dbeta += the column sums of `rows` partial rows [2, H] (also used by the 8-bit LayerNorm, act8.cu).
-void ln_reduce_partials_launch(const float* part, int rows, int H, float* dgamma, float* dbeta, cudaStream_t s) {
-  reduce_rows_kernel<<<(2 * H + 31) / 32, kReduceRowsThreads, 0, s>>>(part, rows, 2 * H, dgamma, dbeta, H);
-  HB_CUDA_CHECK(cudaGetLastError());
-}
-
 // out = 16-bit(g * mask): 4 elements (2 mask pairs) per thread.
 template <bool F16>
 __global__ void dropout_bf16_kernel(const float* __restrict__ g, __nv_bfloat16* __restrict__ out, long M, int H,
