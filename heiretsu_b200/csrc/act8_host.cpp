@@ -66,34 +66,49 @@ void check_width(int64_t M, int64_t H, const char* op) {
   TORCH_CHECK(M <= kIntMax, op, ": too many rows");
 }
 
+// Empty codes and exponent bytes of an [M, N] activation.
+std::pair<at::Tensor, at::Tensor> codes_like(const at::Tensor& x) {
+  const auto opts = x.options();
+  return {at::empty(x.sizes(), opts.dtype(at::kChar)),
+          at::empty({x.size(0), (x.size(1) + kBlock - 1) / kBlock}, opts.dtype(at::kByte))};
+}
+void check_out_type(at::ScalarType dt, const char* op) {
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, op, ": dtype must be bf16, fp16 or fp32");
+}
+
 }  // namespace
 
-void act8_pack(const at::Tensor& x, at::Tensor& q, at::Tensor& e) {
+std::tuple<at::Tensor, at::Tensor> act8_pack(const at::Tensor& x) {
   const char* op = "act8_pack";
   TORCH_CHECK(x.is_cuda(), op, ": x must be a CUDA tensor");
   TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1) && x.stride(0) >= 0, op,
               ": x must be 2-D with contiguous rows");
-  c10::cuda::CUDAGuard g(x.device());
-  check_codes(q, e, op);
-  TORCH_CHECK(q.sizes() == x.sizes() && q.device() == x.device(), op, ": q must be like x");
-  act8_pack_launch(x.data_ptr(), x.stride(0), act_type(x, op, "x"), q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(),
-                   x.size(0), static_cast<int>(x.size(1)), at::cuda::getCurrentCUDAStream());
-}
-
-void act8_unpack(const at::Tensor& q, const at::Tensor& e, at::Tensor& x, const c10::optional<at::Tensor>& h) {
-  const char* op = "act8_unpack";
-  check_codes(q, e, op);
-  c10::cuda::CUDAGuard g(q.device());
   const int type = act_type(x, op, "x");
-  check_mat(x, x.scalar_type(), q.size(0), q.size(1), q.device(), op, "x");
-  const bool gelu = h && h->defined();
-  if (gelu) check_mat(*h, x.scalar_type(), q.size(0), q.size(1), q.device(), op, "h");
-  act8_unpack_launch(q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), type, x.data_ptr(), gelu ? h->data_ptr() : nullptr,
-                     q.size(0), static_cast<int>(q.size(1)), at::cuda::getCurrentCUDAStream());
+  c10::cuda::CUDAGuard g(x.device());
+  auto [q, e] = codes_like(x);
+  check_codes(q, e, op);
+  act8_pack_launch(x.data_ptr(), x.stride(0), type, q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), x.size(0),
+                   static_cast<int>(x.size(1)), at::cuda::getCurrentCUDAStream());
+  return {q, e};
 }
 
-void layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, at::Tensor& y, at::Tensor& q,
-                        at::Tensor& e, at::Tensor& rstd, double eps) {
+std::tuple<at::Tensor, at::Tensor> act8_unpack(const at::Tensor& q, const at::Tensor& e, at::ScalarType dtype,
+                                               bool gelu) {
+  const char* op = gelu ? "act8_unpack_gelu" : "act8_unpack";
+  check_codes(q, e, op);
+  check_out_type(dtype, op);
+  c10::cuda::CUDAGuard g(q.device());
+  at::Tensor x = at::empty(q.sizes(), q.options().dtype(dtype)), h;
+  if (gelu) h = at::empty_like(x);
+  act8_unpack_launch(q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), act_type(x, op, "x"), x.data_ptr(),
+                     gelu ? h.data_ptr() : nullptr, q.size(0), static_cast<int>(q.size(1)),
+                     at::cuda::getCurrentCUDAStream());
+  return {x, h};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w,
+                                                                              const at::Tensor& b, double eps,
+                                                                              at::ScalarType dtype) {
   const char* op = "layernorm_fwd_act8";
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, op, ": x must be a CUDA matrix");
   c10::cuda::CUDAGuard g(x.device());
@@ -103,27 +118,19 @@ void layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w, const at::Tens
   check_mat(x, at::kFloat, M, H, dev, op, "x");
   check_vec(w, H, dev, op, "w");
   check_vec(b, H, dev, op, "b");
-  TORCH_CHECK(act_type(y, op, "y") != 2, op, ": y must be bf16 or fp16");
-  check_mat(y, y.scalar_type(), M, H, dev, op, "y");
-  check_codes(q, e, op);
-  TORCH_CHECK(q.sizes() == x.sizes() && q.device() == dev, op, ": q must be like x");
-  check_vec(rstd, M, dev, op, "rstd");
-  TORCH_CHECK(aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y) && aligned16(q), op,
-              ": x, w, b, y and q must start on 16-byte boundaries");
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, op, ": dtype must be bf16 or fp16");
+  TORCH_CHECK(aligned16(x) && aligned16(w) && aligned16(b), op, ": x, w and b must start on 16-byte boundaries");
+  auto [q, e] = codes_like(x);
+  at::Tensor y = at::empty({M, H}, x.options().dtype(dtype)), rstd = at::empty({M}, x.options());
   ln_fwd_act8_launch(x.data_ptr<float>(), w.data_ptr<float>(), b.data_ptr<float>(), y.data_ptr(), q.data_ptr<int8_t>(),
                      e.data_ptr<uint8_t>(), rstd.data_ptr<float>(), static_cast<int>(M), static_cast<int>(H),
-                     static_cast<float>(eps), y.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
+                     static_cast<float>(eps), dtype == at::kHalf, at::cuda::getCurrentCUDAStream());
+  return {y, q, e, rstd};
 }
 
-int64_t layernorm_bwd_act8_scratch_rows(const at::Tensor& q) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.size(0) <= kIntMax, "layernorm_bwd_act8: q must be a CUDA matrix");
-  check_width(q.size(0), q.size(1), "layernorm_bwd_act8");
-  return ln_bwd_act8_ctas(static_cast<int>(q.size(0)), static_cast<int>(q.size(1)), q.get_device());
-}
-
-void layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
-                        const at::Tensor& w, const at::Tensor& b, const at::Tensor& dres_in, at::Tensor& dres,
-                        at::Tensor& dres16, at::Tensor& y, at::Tensor& scratch, at::Tensor& dgamma, at::Tensor& dbeta) {
+at::Tensor layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
+                              const at::Tensor& w, const at::Tensor& b, const at::Tensor& dres_in, at::Tensor& dres,
+                              at::Tensor& dres16, at::Tensor& dgamma, at::Tensor& dbeta) {
   const char* op = "layernorm_bwd_act8";
   check_codes(q, e, op);
   c10::cuda::CUDAGuard g(q.device());
@@ -138,21 +145,19 @@ void layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Ten
   check_mat(dres, at::kFloat, M, H, dev, op, "dres");
   TORCH_CHECK(act_type(dres16, op, "dres16") != 2, op, ": dres16 must be bf16 or fp16");
   check_mat(dres16, dres16.scalar_type(), M, H, dev, op, "dres16");
-  check_mat(y, dres16.scalar_type(), M, H, dev, op, "y");
   check_vec(dgamma, H, dev, op, "dgamma");
   check_vec(dbeta, H, dev, op, "dbeta");
   const int ctas = ln_bwd_act8_ctas(static_cast<int>(M), static_cast<int>(H), q.get_device());
-  TORCH_CHECK(scratch.device() == dev && scratch.scalar_type() == at::kFloat && scratch.is_contiguous() &&
-                  scratch.numel() >= (int64_t)ctas * 2 * H,
-              op, ": scratch too small");
   TORCH_CHECK(aligned16(dy) && aligned16(q) && aligned16(w) && aligned16(b) && aligned16(dres_in) && aligned16(dres) &&
-                  aligned16(dres16) && aligned16(y) && aligned16(scratch),
+                  aligned16(dres16),
               op, ": every matrix must start on a 16-byte boundary");
+  at::Tensor y = at::empty({M, H}, dres16.options()), scratch = at::empty({ctas * 2 * H}, dy.options());
   ln_bwd_act8_launch(dy.data_ptr<float>(), q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), rstd.data_ptr<float>(),
                      w.data_ptr<float>(), b.data_ptr<float>(), dres_in.data_ptr<float>(), dres.data_ptr<float>(),
                      dres16.data_ptr(), y.data_ptr(), scratch.data_ptr<float>(), ctas, dgamma.data_ptr<float>(),
                      dbeta.data_ptr<float>(), static_cast<int>(M), static_cast<int>(H),
                      dres16.scalar_type() == at::kHalf, at::cuda::getCurrentCUDAStream());
+  return y;
 }
 
 }  // namespace hb

@@ -52,7 +52,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_pack", &hb::act8_pack);
   m.def("act8_unpack", &hb::act8_unpack);
   m.def("layernorm_fwd_act8", &hb::layernorm_fwd_act8);
-  m.def("layernorm_bwd_act8_scratch_rows", &hb::layernorm_bwd_act8_scratch_rows);
   m.def("layernorm_bwd_act8", &hb::layernorm_bwd_act8);
   m.def("raw_malloc", &hb::raw_malloc);
   m.def("raw_free", &hb::raw_free);

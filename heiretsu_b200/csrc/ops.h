@@ -54,24 +54,24 @@ void attention_bwd(const at::Tensor& qkv, const at::Tensor& out, const at::Tenso
                    int64_t B, int64_t T, int64_t nh, at::Tensor& dvec, at::Tensor& dq_acc, at::Tensor& dqkv,
                    const c10::optional<at::Tensor>& drop_seed, int64_t drop_site, double drop_p, int64_t h0,
                    int64_t nh_total, int64_t head_dim);
-void token_logprobs(const at::Tensor& logits, int64_t V, const at::Tensor& targets, int64_t ignore_index,
-                    at::Tensor& logp, at::Tensor& lse, const c10::optional<at::Tensor>& grad);
-void policy_loss(const at::Tensor& logits, int64_t V, const at::Tensor& targets, int64_t ignore_index,
-                 const at::Tensor& old_logp, const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp,
-                 const c10::optional<at::Tensor>& weights, const c10::optional<at::Tensor>& grad_scale,
-                 double clip_low, double clip_high, double kl_coef, at::Tensor& loss, at::Tensor& stats,
-                 at::Tensor& logp, at::Tensor& grad);
-void preference_loss(const at::Tensor& logp, const at::Tensor& targets, int64_t ignore_index,
-                     const c10::optional<at::Tensor>& ref_logp, double beta, double label_smoothing, at::Tensor& loss,
-                     at::Tensor& rewards, at::Tensor& dlogp);
-void act8_pack(const at::Tensor& x, at::Tensor& q, at::Tensor& e);
-void act8_unpack(const at::Tensor& q, const at::Tensor& e, at::Tensor& x, const c10::optional<at::Tensor>& h);
-void layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, at::Tensor& y, at::Tensor& q,
-                        at::Tensor& e, at::Tensor& rstd, double eps);
-int64_t layernorm_bwd_act8_scratch_rows(const at::Tensor& q);
-void layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
-                        const at::Tensor& w, const at::Tensor& b, const at::Tensor& dres_in, at::Tensor& dres,
-                        at::Tensor& dres16, at::Tensor& y, at::Tensor& scratch, at::Tensor& dgamma, at::Tensor& dbeta);
+std::tuple<at::Tensor, at::Tensor> token_logprobs(const at::Tensor& logits, int64_t V, const at::Tensor& targets,
+                                                  int64_t ignore_index, const c10::optional<at::Tensor>& grad);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss(
+    const at::Tensor& logits, int64_t V, const at::Tensor& targets, const at::Tensor& old_logp,
+    const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp, const c10::optional<at::Tensor>& weights,
+    double clip_low, double clip_high, double kl_coef, const c10::optional<at::Tensor>& grad_scale,
+    int64_t ignore_index, const c10::optional<at::Tensor>& grad_out);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> preference_loss(const at::Tensor& logp, const at::Tensor& targets,
+                                                               const c10::optional<at::Tensor>& ref_logp, double beta,
+                                                               double label_smoothing, int64_t ignore_index);
+std::tuple<at::Tensor, at::Tensor> act8_pack(const at::Tensor& x);
+std::tuple<at::Tensor, at::Tensor> act8_unpack(const at::Tensor& q, const at::Tensor& e, at::ScalarType dtype, bool gelu);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layernorm_fwd_act8(const at::Tensor& x, const at::Tensor& w,
+                                                                              const at::Tensor& b, double eps,
+                                                                              at::ScalarType dtype);
+at::Tensor layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
+                              const at::Tensor& w, const at::Tensor& b, const at::Tensor& dres_in, at::Tensor& dres,
+                              at::Tensor& dres16, at::Tensor& dgamma, at::Tensor& dbeta);
 uint64_t raw_malloc(int64_t bytes);
 void raw_free(uint64_t ptr);
 at::Tensor tensor_from_ptr(uint64_t ptr, int64_t numel, at::ScalarType dtype, int64_t device);

@@ -61,7 +61,6 @@ std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
 LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targets, int64_t ignore_index,
                      const at::Tensor& logp, const c10::optional<at::Tensor>& lse,
                      const c10::optional<at::Tensor>& grad, const char* op) {
-  TORCH_CHECK(logits.is_cuda(), op, ": logits must be a CUDA tensor");
   TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1), op,
               ": logits must be 2-D with contiguous rows");
   LogitRows a{};
@@ -110,34 +109,38 @@ LogitRows logit_rows(const at::Tensor& logits, int64_t V, const at::Tensor& targ
 
 }  // namespace
 
-void token_logprobs(const at::Tensor& logits, int64_t V, const at::Tensor& targets, int64_t ignore_index,
-                    at::Tensor& logp, at::Tensor& lse, const c10::optional<at::Tensor>& grad) {
+std::tuple<at::Tensor, at::Tensor> token_logprobs(const at::Tensor& logits, int64_t V, const at::Tensor& targets,
+                                                  int64_t ignore_index, const c10::optional<at::Tensor>& grad) {
   const char* op = "token_logprobs";
-  TORCH_CHECK(logits.is_cuda(), op, ": logits must be a CUDA tensor");
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, op, ": logits must be a CUDA matrix");
   c10::cuda::CUDAGuard g(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor logp = at::empty({logits.size(0)}, f32), lse = at::empty({logits.size(0)}, f32);
   const LogitRows a = logit_rows(logits, V, targets, ignore_index, logp, lse, grad, op);
   token_logprobs_launch(a, at::cuda::getCurrentCUDAStream());
+  return {logp, lse};
 }
 
-void policy_loss(const at::Tensor& logits, int64_t V, const at::Tensor& targets, int64_t ignore_index,
-                 const at::Tensor& old_logp, const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp,
-                 const c10::optional<at::Tensor>& weights, const c10::optional<at::Tensor>& grad_scale,
-                 double clip_low, double clip_high, double kl_coef, at::Tensor& loss, at::Tensor& stats,
-                 at::Tensor& logp, at::Tensor& grad) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> policy_loss(
+    const at::Tensor& logits, int64_t V, const at::Tensor& targets, const at::Tensor& old_logp,
+    const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp, const c10::optional<at::Tensor>& weights,
+    double clip_low, double clip_high, double kl_coef, const c10::optional<at::Tensor>& grad_scale,
+    int64_t ignore_index, const c10::optional<at::Tensor>& grad_out) {
   const char* op = "policy_loss";
-  TORCH_CHECK(logits.is_cuda(), op, ": logits must be a CUDA tensor");
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, op, ": logits must be a CUDA matrix");
   c10::cuda::CUDAGuard g(logits.device());
-  const LogitRows a = logit_rows(logits, V, targets, ignore_index, logp, c10::nullopt, grad, op);
-  TORCH_CHECK(a.grad != nullptr || a.M == 0, op, ": a gradient buffer is needed");
   const at::Device dev = logits.device();
-  const int64_t M = a.M;
+  const int64_t M = logits.size(0);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor logp = at::empty({M}, f32), loss = at::empty({}, f32), stats = at::empty({2}, f32);
+  at::Tensor grad = given(grad_out) ? *grad_out : at::empty_like(logits);
+  const LogitRows a = logit_rows(logits, V, targets, ignore_index, logp, c10::nullopt, grad, op);
   PolicyTerms p{};
   check_vec(old_logp, at::kFloat, M, dev, op, "old_logp");
   const int64_t n_adv = advantages.numel();
-  TORCH_CHECK(M == 0 || (n_adv >= 1 && M % n_adv == 0), op, ": advantages must hold one value per row or per equal run of rows");
+  TORCH_CHECK(M == 0 || (n_adv >= 1 && M % n_adv == 0), op,
+              ": advantages must hold one value per row or per equal run of rows");
   check_vec(advantages, at::kFloat, n_adv, dev, op, "advantages");
-  check_vec(loss, at::kFloat, 1, dev, op, "loss");
-  check_vec(stats, at::kFloat, 2, dev, op, "stats");
   TORCH_CHECK(clip_low >= 0 && clip_low <= 1 && clip_high >= 0 && std::isfinite(clip_high), op,
               ": clip_low must be in [0, 1] and clip_high finite and not negative");
   TORCH_CHECK(std::isfinite(kl_coef), op, ": kl_coef must be finite");
@@ -162,11 +165,12 @@ void policy_loss(const at::Tensor& logits, int64_t V, const at::Tensor& targets,
   at::Tensor scratch = at::empty({policy_scratch_doubles()}, logits.options().dtype(at::kDouble));
   policy_loss_launch(a, p, scratch.data_ptr<double>(), loss.data_ptr<float>(), stats.data_ptr<float>(),
                      at::cuda::getCurrentCUDAStream());
+  return {loss, stats, logp, grad};
 }
 
-void preference_loss(const at::Tensor& logp, const at::Tensor& targets, int64_t ignore_index,
-                     const c10::optional<at::Tensor>& ref_logp, double beta, double label_smoothing, at::Tensor& loss,
-                     at::Tensor& rewards, at::Tensor& dlogp) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> preference_loss(const at::Tensor& logp, const at::Tensor& targets,
+                                                               const c10::optional<at::Tensor>& ref_logp, double beta,
+                                                               double label_smoothing, int64_t ignore_index) {
   const char* op = "preference_loss";
   TORCH_CHECK(logp.is_cuda(), op, ": logp must be a CUDA tensor");
   TORCH_CHECK(logp.dim() == 2 && logp.size(0) % 2 == 0, op,
@@ -179,18 +183,17 @@ void preference_loss(const at::Tensor& logp, const at::Tensor& targets, int64_t 
   const at::Device dev = logp.device();
   check_vec(logp, at::kFloat, n, dev, op, "logp");
   check_vec(targets, at::kLong, n, dev, op, "targets");
-  check_vec(loss, at::kFloat, 1, dev, op, "loss");
-  check_vec(rewards, at::kFloat, 2 * P, dev, op, "rewards");
-  check_vec(dlogp, at::kFloat, n, dev, op, "dlogp");
   if (given(ref_logp)) check_vec(*ref_logp, at::kFloat, n, dev, op, "ref_logp");
+  const auto f32 = logp.options();
+  at::Tensor loss = at::empty({}, f32), rewards = at::empty({2, P}, f32), dlogp = at::empty(logp.sizes(), f32);
   const long doubles = preference_scratch_doubles(n);
   at::Tensor scratch;
-  if (doubles > 0) scratch = at::empty({doubles}, logp.options().dtype(at::kDouble));
+  if (doubles > 0) scratch = at::empty({doubles}, f32.dtype(at::kDouble));
   preference_loss_launch(logp.data_ptr<float>(), given(ref_logp) ? ref_logp->data_ptr<float>() : nullptr,
-                         targets.data_ptr<int64_t>(), ignore_index, static_cast<int>(P), static_cast<int>(T),
-                         beta, label_smoothing, loss.data_ptr<float>(),
-                         rewards.data_ptr<float>(), dlogp.data_ptr<float>(), doubles > 0 ? scratch.data_ptr<double>() : nullptr,
-                         at::cuda::getCurrentCUDAStream());
+                         targets.data_ptr<int64_t>(), ignore_index, static_cast<int>(P), static_cast<int>(T), beta,
+                         label_smoothing, loss.data_ptr<float>(), rewards.data_ptr<float>(), dlogp.data_ptr<float>(),
+                         doubles > 0 ? scratch.data_ptr<double>() : nullptr, at::cuda::getCurrentCUDAStream());
+  return {loss, rewards, dlogp};
 }
 
 }  // namespace hb

@@ -589,16 +589,14 @@ __global__ void __launch_bounds__(kSumThreads) policy_sum_kernel(const double* _
   }
 }
 
-// Preference loss. A group of G warps takes a pair: the sums of both sequences in 64 bits, the pair's loss and
-// factor, then both gradient rows (the targets are read again, from cache). CLUSTER: one cluster of 8 CTAs does
-// all pairs and adds their losses through shared memory: one launch, which is what small batches are bound by
-// (2^17 tokens are 2.6 MB). Larger batches spread over the SMs and leave their sums to preference_sum_kernel. Either
-// way the order of every sum is fixed.
-constexpr int kPrefThreads = 1024;
+// Preference loss. A group of G warps takes a pair: the sums of both sequences in 64 bits, the pair's factor, both
+// gradient rows, and last the pair's loss (its logarithm is off the gradient's path). Small batches, which latency
+// bounds, run in one CTA that also adds the losses; others spread over the SMs and leave each CTA's sum to
+// preference_sum_kernel, launched beside them. The order of every sum is fixed.
+constexpr int kPrefThreads = 512;
 constexpr int kPrefWarps = kPrefThreads / 32;
-constexpr int kPrefCluster = 8;
-constexpr long kPrefClusterTokens = 1L << 18;
 constexpr int kPrefMaxCtas = 1024;
+constexpr long kPrefOneCta = 8192;  // tokens of a batch that one CTA takes
 
 struct Preference {
   const float *logp, *ref;  // ref may be nullptr
@@ -607,29 +605,29 @@ struct Preference {
   int P, T, G;
   double beta, smoothing;
   float *loss, *rewards, *dlogp;
-  double* part;  // [gridDim.x] without a cluster
+  double* part;  // [gridDim.x]; nullptr: one CTA, which writes the loss
 };
 
-template <bool CLUSTER>
 __global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preference a) {
-  __shared__ double sums[2][kPrefWarps][2], losses[kPrefWarps], total[kPrefCluster];
+  __shared__ double sums[2][kPrefWarps][2], losses[kPrefWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per_cta = kPrefWarps / a.G, groups = per_cta * gridDim.x;
   const int group = blockIdx.x * per_cta + warp / a.G;
-  const int gl = threadIdx.x % (a.G * 32), gn = a.G * 32;  // thread within its group
-  if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();
+  const int gn = a.G * 32, gl = threadIdx.x & (gn - 1);  // threads of a group (a power of two), this one
   double loss = 0.0;
   int parity = 0;
   for (int p0 = 0; p0 < a.P; p0 += groups) {  // the same rounds for every thread of the CTA
     const int pair = p0 + group;
     const bool in = pair < a.P;
     double s[2] = {0.0, 0.0};
+    uint32_t counted[2] = {0u, 0u};  // of this thread's first 32 tokens
     if (in) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const long base = ((long)pair + (long)h * a.P) * a.T;
         constexpr int kBatch = 8;  // loads in flight
-        for (int j0 = gl; j0 < a.T; j0 += kBatch * gn) {
+        for (int j0 = gl, n = 0; j0 < a.T; j0 += kBatch * gn, n += kBatch) {
           int64_t t[kBatch];
           float v[kBatch], r[kBatch];
 #pragma unroll
@@ -641,8 +639,12 @@ __global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preferen
             r[k] = at && a.ref ? a.ref[base + j] : 0.f;
           }
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k)
-            if (t[k] != a.ignore_index) s[h] += static_cast<double>(v[k]) - static_cast<double>(r[k]);
+          for (int k = 0; k < kBatch; ++k) {
+            if (t[k] != a.ignore_index) {
+              s[h] += static_cast<double>(v[k]) - static_cast<double>(r[k]);
+              if (n + k < 32) counted[h] |= 1u << (n + k);
+            }
+          }
         }
       }
     }
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preferen
       }
       __syncthreads();
       s[0] = s[1] = 0.0;
-      const int w0 = warp / a.G * a.G;
+      const int w0 = warp & ~(a.G - 1);
       for (int w = w0; w < w0 + a.G; ++w) {
         s[0] += sums[parity][w][0];
         s[1] += sums[parity][w][1];
@@ -667,53 +669,62 @@ __global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preferen
     }
     if (in) {
       const double good = a.beta * s[0], poor = a.beta * s[1], z = good - poor;
-      // sigmoid(z), sigmoid(-z) and log(1 + e^-z), log(1 + e^z) from e = e^-|z|, which cannot overflow
-      const double e = exp(-fabs(z)), big = 1.0 / (1.0 + e), small = e * big, l = log1p(e);
+      // sigmoid(|z|) and sigmoid(-|z|) from e = e^-|z|, which cannot overflow
+      const double e = exp(-fabs(z)), big = 1.0 / (1.0 + e), small = e * big;
       const double sig = z >= 0.0 ? big : small, sig_neg = z >= 0.0 ? small : big;
       const float c = static_cast<float>(z != z ? z : a.beta / a.P * (a.smoothing * sig - (1.0 - a.smoothing) * sig_neg));
-      if (gl == 0) {
-        a.rewards[pair] = static_cast<float>(good);
-        a.rewards[a.P + pair] = static_cast<float>(poor);
-        loss += (1.0 - a.smoothing) * (fmax(-z, 0.0) + l) + a.smoothing * (fmax(z, 0.0) + l);
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const long base = ((long)pair + (long)h * a.P) * a.T;
         const float g = h ? -c : c;
-#pragma unroll 8
-        for (int j = gl; j < a.T; j += gn) a.dlogp[base + j] = a.targets[base + j] != a.ignore_index ? g : 0.f;
+#pragma unroll 4
+        for (int j = gl, n = 0; j < a.T; j += gn, ++n) {
+          const bool yes = n < 32 ? (counted[h] >> n & 1u) != 0u : a.targets[base + j] != a.ignore_index;
+          a.dlogp[base + j] = yes ? g : 0.f;
+        }
+      }
+      if (gl == 0) {
+        a.rewards[pair] = static_cast<float>(good);
+        a.rewards[a.P + pair] = static_cast<float>(poor);
+        const double l = log1p(e);  // log(1 + e^-z) = max(-z, 0) + l, log(1 + e^z) = max(z, 0) + l
+        loss += z != z ? z : (1.0 - a.smoothing) * (fmax(-z, 0.0) + l) + a.smoothing * (fmax(z, 0.0) + l);
       }
     }
   }
   if (gl == 0) losses[warp] = loss;  // the first warp of each group holds its pairs' sum
   __syncthreads();
-  if constexpr (CLUSTER) {
-    auto cl = cooperative_groups::this_cluster();
-    if (threadIdx.x == 0) {
-      double v = 0.0;
-      for (int w = 0; w < kPrefWarps; w += a.G) v += losses[w];
-      *cl.map_shared_rank(&total[blockIdx.x], 0) = v;
-    }
-    cl.sync();
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      double v = 0.0;
-      for (int c = 0; c < kPrefCluster; ++c) v += total[c];
-      a.loss[0] = a.P > 0 ? static_cast<float>(v / a.P) : 0.f;
-    }
-  } else if (threadIdx.x == 0) {
+  if (threadIdx.x == 0) {
     double v = 0.0;
     for (int w = 0; w < kPrefWarps; w += a.G) v += losses[w];
-    a.part[blockIdx.x] = v;
+    if (a.part) a.part[blockIdx.x] = v;
+    else a.loss[0] = a.P > 0 ? static_cast<float>(v / a.P) : 0.f;
   }
 }
 
 __global__ void __launch_bounds__(32) preference_sum_kernel(const double* __restrict__ part, int n, int P,
                                                             float* __restrict__ loss) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += 32) v += part[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 32) v += __ldcg(part + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (threadIdx.x == 0) loss[0] = static_cast<float>(v / P);
+}
+
+// Launch of a kernel that starts with griddepcontrol.wait, beside the one before it on the stream.
+template <class... Params, class... Args>
+void launch_beside(void (*k)(Params...), int ctas, int threads, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, static_cast<Params>(args)...));
 }
 
 // Shared memory: 228 KB an SM, 227 KB a CTA; each CTA also takes 1 KB for the system and under 1 KB for the
@@ -798,7 +809,7 @@ Deal deal_of(const LogitRows& a) {
 
 long logit_row_limit(int type) { return static_cast<long>(kMaxPieces) * kMaxSplit * (type == kLogitF32 ? 4 : 8); }
 long policy_scratch_doubles() { return 3L * kCtasPerSm * num_sms(current_device()); }
-long preference_scratch_doubles(long tokens) { return tokens <= kPrefClusterTokens ? 0 : kPrefMaxCtas; }
+long preference_scratch_doubles(long tokens) { return tokens <= kPrefOneCta ? 0 : kPrefMaxCtas; }
 
 void token_logprobs_launch(const LogitRows& a, cudaStream_t s) {
   const PolicyTerms none{};
@@ -810,46 +821,21 @@ void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratc
                         cudaStream_t s) {
   const Deal d = deal_of(a);
   launch_rows<kPolicy>(a, p, d, scratch, s);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(1);
-  cfg.blockDim = dim3(kSumThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = a.M > 0 ? 1 : 0;
-  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, policy_sum_kernel, static_cast<const double*>(scratch), a.M > 0 ? d.clusters : 0,
-                                   loss, stats));
+  launch_beside(policy_sum_kernel, 1, kSumThreads, s, scratch, a.M > 0 ? d.clusters : 0, loss, stats);
 }
 
 void preference_loss_launch(const float* logp, const float* ref, const int64_t* targets, int64_t ignore_index, int P,
                             int T, double beta, double smoothing, float* loss, float* rewards, float* dlogp,
                             double* scratch, cudaStream_t s) {
-  Preference a{logp, ref, targets, ignore_index, P, T, 1, beta, smoothing, loss, rewards, dlogp, scratch};
-  if (2L * P * T <= kPrefClusterTokens) {
-    const int n = std::max(1, (P + kPrefCluster - 1) / kPrefCluster);  // pairs of one CTA
-    while (a.G * 2 * n <= kPrefWarps) a.G *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kPrefCluster);
-    cfg.blockDim = dim3(kPrefThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = kPrefCluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, preference_kernel<true>, static_cast<const Preference>(a)));
-    return;
-  }
-  while (a.G < kPrefWarps && a.G * 256 < T) a.G *= 2;  // 8 tokens of a sequence a thread
+  Preference a{logp, ref, targets, ignore_index, P, T, 1, beta, smoothing, loss, rewards, dlogp, nullptr};
+  while (a.G < kPrefWarps && a.G * 128 < T) a.G *= 2;  // 4 tokens of a sequence a thread
   const int per_cta = kPrefWarps / a.G;
-  const int ctas = std::min((P + per_cta - 1) / per_cta, kPrefMaxCtas);
-  preference_kernel<false><<<ctas, kPrefThreads, 0, s>>>(a);
+  const bool one = preference_scratch_doubles(2L * P * T) == 0;
+  const int ctas = one ? 1 : std::min((P + per_cta - 1) / per_cta, kPrefMaxCtas);
+  if (!one) a.part = scratch;
+  preference_kernel<<<ctas, kPrefThreads, 0, s>>>(a);
   HB_CUDA_CHECK(cudaGetLastError());
-  preference_sum_kernel<<<1, 32, 0, s>>>(scratch, ctas, P, loss);
-  HB_CUDA_CHECK(cudaGetLastError());
+  if (!one) launch_beside(preference_sum_kernel, 1, 32, s, scratch, ctas, P, loss);
 }
 
 }  // namespace hb

@@ -93,7 +93,8 @@ def cross_entropy_bwd_(logits, V, targets, lse, scale: Optional[torch.Tensor], s
 
 
 # ---------------------------------------------------------------------------
-# Post-training losses
+# Post-training losses (the outputs of these and of the 8-bit activations are allocated by
+# the extension: that halves the host's share of a short call)
 # ---------------------------------------------------------------------------
 def token_logprobs(logits: torch.Tensor, V: int, targets: torch.Tensor, ignore_index: int = -100,
                    grad: Optional[torch.Tensor] = None):
@@ -104,11 +105,7 @@ def token_logprobs(logits: torch.Tensor, V: int, targets: torch.Tensor, ignore_i
     NaN and the bad-argument status. ``grad`` (a buffer like ``logits``, or ``logits`` itself: in place) receives
     the gradient of each row's log-probability, onehot - softmax, zero in ignored rows and in columns >= V: the
     gradient of any loss of the log-probabilities is this with row i times dloss/dlogp[i]."""
-    M = logits.shape[0]
-    out = torch.empty(2, M, device=logits.device, dtype=torch.float32)
-    logp, lse = out[0], out[1]
-    _ext().token_logprobs(logits, int(V), targets, int(ignore_index), logp, lse, grad)
-    return logp, lse
+    return _ext().token_logprobs(logits, V, targets, ignore_index, grad)
 
 
 def policy_loss(logits: torch.Tensor, V: int, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
@@ -124,14 +121,8 @@ def policy_loss(logits: torch.Tensor, V: int, targets: torch.Tensor, old_logp: t
     clipped rows), logp [M], grad): ``grad`` (a new tensor like ``logits``, the given buffer, or ``logits`` itself)
     is the loss's gradient times the device scalar ``grad_scale`` (fp32 [1], default 1). Without ``ref_logp``
     there is no KL term and its statistic is 0."""
-    M = logits.shape[0]
-    if grad is None:
-        grad = torch.empty_like(logits)
-    out = torch.empty(M + 3, device=logits.device, dtype=torch.float32)
-    logp, loss, stats = out[:M], out[M], out[M + 1:]
-    _ext().policy_loss(logits, int(V), targets, int(ignore_index), old_logp, advantages, ref_logp, weights, grad_scale,
-                       float(clip_low), float(clip_high), float(kl_coef), loss, stats, logp, grad)
-    return loss, stats, logp, grad
+    return _ext().policy_loss(logits, V, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef,
+                              grad_scale, ignore_index, grad)
 
 
 def preference_loss(logp: torch.Tensor, targets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None,
@@ -142,51 +133,30 @@ def preference_loss(logp: torch.Tensor, targets: torch.Tensor, ref_logp: Optiona
     take no part (a sequence without any counts 0). With S = sum over a sequence of logp - ref_logp (``ref_logp``
     like ``logp``; none: 0), rewards = beta S and z = beta (S_chosen - S_rejected), the loss is the mean over pairs of
     -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z); sums run in 64 bits."""
-    P = logp.shape[0] // 2
-    out = torch.empty(2 * P + 1, device=logp.device, dtype=torch.float32)
-    rewards, loss = out[:2 * P].view(2, P), out[2 * P]
-    dlogp = torch.empty_like(logp)
-    _ext().preference_loss(logp, targets, int(ignore_index), ref_logp, float(beta), float(label_smoothing), loss,
-                           rewards, dlogp)
-    return loss, rewards, dlogp
+    return _ext().preference_loss(logp, targets, ref_logp, beta, label_smoothing, ignore_index)
 
 
 # ---------------------------------------------------------------------------
 # Activations in 8 bits (format: csrc/act8.cuh)
 # ---------------------------------------------------------------------------
-ACT8_BLOCK = 128  # columns that share one exponent byte
-
-
-def _act8_like(x: torch.Tensor):
-    M, N = x.shape
-    return (torch.empty(M, N, device=x.device, dtype=torch.int8),
-            torch.empty(M, (N + ACT8_BLOCK - 1) // ACT8_BLOCK, device=x.device, dtype=torch.uint8))
-
-
 def act8_pack(x: torch.Tensor):
     """x [M, N] (bf16, fp16 or fp32, contiguous rows) -> (q int8 [M, N], e uint8 [M, ceil(N / 128)]).
 
     A block of 128 columns keeps 2^(e - 127), the least power of two >= max|x| / 127 (and >= 2^-126), and codes
     x / 2^(e - 127) rounded to nearest even: each value is off by at most max|x| / 127 of its block. A block with an
     infinity or NaN comes back as NaN."""
-    q, e = _act8_like(x)
-    _ext().act8_pack(x, q, e)
-    return q, e
+    return _ext().act8_pack(x)
 
 
 def act8_unpack(q: torch.Tensor, e: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of ``act8_pack``'s codes in bf16, fp16 or fp32 (clamped to the type's largest finite value)."""
-    x = torch.empty(q.shape, device=q.device, dtype=dtype)
-    _ext().act8_unpack(q, e, x, None)
-    return x
+    return _ext().act8_unpack(q, e, dtype, False)[0]
 
 
 def act8_unpack_gelu(q: torch.Tensor, e: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
     """(GELU(x), x) with x = ``act8_unpack(q, e, dtype)``: both operands of the MLP's backward from its kept
     pre-activation (tanh form of GELU, evaluated on the unrounded value)."""
-    x = torch.empty(q.shape, device=q.device, dtype=dtype)
-    h = torch.empty_like(x)
-    _ext().act8_unpack(q, e, x, h)
+    x, h = _ext().act8_unpack(q, e, dtype, True)
     return h, x
 
 
@@ -194,23 +164,14 @@ def layernorm_fwd_act8(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor, eps: f
                        dtype: torch.dtype = torch.bfloat16):
     """``layernorm_fwd`` that keeps xh = (x - mean) rstd in 8 bits instead of x, mean and y for the backward:
     fp32 x [M, H] -> (y in the 16-bit ``dtype``, q, e, rstd [M])."""
-    q, e = _act8_like(x)
-    y = torch.empty(x.shape, device=x.device, dtype=dtype)
-    rstd = torch.empty(x.shape[0], device=x.device, dtype=torch.float32)
-    _ext().layernorm_fwd_act8(x, w, b, y, q, e, rstd, eps)
-    return y, q, e, rstd
+    return _ext().layernorm_fwd_act8(x, w, b, eps, dtype)
 
 
-def layernorm_bwd_act8(dy, q, e, rstd, w, b, dres_in, dres, dres16, dgamma, dbeta, scratch=None) -> torch.Tensor:
+def layernorm_bwd_act8(dy, q, e, rstd, w, b, dres_in, dres, dres16, dgamma, dbeta) -> torch.Tensor:
     """``layernorm_bwd`` from the kept codes: dres = dres_in + dLN/dx(dy) (``dres`` may be ``dres_in``), dres16 =
     16-bit(dres), dgamma / dbeta (fp32) += their sums. Returns y = xh w + b of the kept xh in dres16's format: the
     operand of the next weight gradient."""
-    if scratch is None:
-        scratch = torch.empty(_ext().layernorm_bwd_act8_scratch_rows(q) * 2 * q.shape[1], device=q.device,
-                              dtype=torch.float32)
-    y = torch.empty(q.shape, device=q.device, dtype=dres16.dtype)
-    _ext().layernorm_bwd_act8(dy, q, e, rstd, w, b, dres_in, dres, dres16, y, scratch, dgamma, dbeta)
-    return y
+    return _ext().layernorm_bwd_act8(dy, q, e, rstd, w, b, dres_in, dres, dres16, dgamma, dbeta)
 
 
 # ---------------------------------------------------------------------------

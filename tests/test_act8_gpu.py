@@ -261,7 +261,7 @@ def test_refusals():
             lambda: ln(x[:, :128], w[:128], w[:128]), lambda: ln(x, w.half(), w),
             lambda: bw(x, q, e, r[:3], w, w, x, x, x16, w, w), lambda: bw(x16, q, e, r, w, w, x, x, x16, w, w),
             lambda: bw(x, q, e, r, w, w, x, x, x, w, w), lambda: bw(x[:3], q, e, r, w, w, x, x, x16, w, w),
-            lambda: bw(x, q, e, r, w, w, x, x, x16, w, w, scratch=w[:1]),
+            lambda: bw(x, q, e, r, w, w, x, x, x16, w, w.half()), lambda: bw(x, q, e, r, w, w, x, x[:, 1:], x16, w, w),
             lambda: bw(x, q, e, r, w, w, x, x, x16, w[:128], w),
     ):
         with pytest.raises(RuntimeError):
