@@ -51,6 +51,17 @@ __device__ __forceinline__ void store4(void* p, long i, const float (&v)[4]) {
         make_uint2(pack16<TYPE == kActF16>(v[0], v[1]), pack16<TYPE == kActF16>(v[2], v[3]));
   }
 }
+// 16 bytes of an activation.
+template <int TYPE, int E>
+__device__ __forceinline__ void store_share(void* p, long i, const float (&v)[E]) {
+  if constexpr (TYPE == kActF32) {
+    store4<TYPE>(p, i, v);
+  } else {
+    constexpr bool F16 = TYPE == kActF16;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+        make_uint4(pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3]), pack16<F16>(v[4], v[5]), pack16<F16>(v[6], v[7]));
+  }
+}
 template <int TYPE>
 __device__ __forceinline__ void store1(void* p, long i, float v) {
   if constexpr (TYPE == kActF32) static_cast<float*>(p)[i] = v;
@@ -85,101 +96,145 @@ __device__ __forceinline__ float gelu_full(float x) {
   return x * r;
 }
 
-constexpr int kPackBlocks = 4;  // consecutive blocks of one warp: their loads are in flight together
+// One lane's share of a step of pack or unpack: 16 bytes of the activation, so 4 (fp32) or 8 consecutive columns, and
+// a warp covers 1 or 2 blocks of 128 columns a step.
+template <int TYPE>
+struct Share {
+  static constexpr int kElems = TYPE == kActF32 ? 4 : 8;
+  static constexpr int kLanes = kAct8Block / kElems;  // lanes of a block
+  static constexpr int kBlocks = 32 / kLanes;         // blocks of a step
+};
+template <int STEP>
+__device__ __forceinline__ void next_block(uint32_t& row, uint32_t& k, uint32_t nb) {
+  k += STEP;
+#pragma unroll
+  for (int i = 0; i < STEP; ++i)
+    if (k >= nb) k -= nb, ++row;
+}
+constexpr int kPackSteps = 4;  // steps of one warp: their loads are in flight together
 
-// One warp per kPackBlocks blocks; a lane holds 4 consecutive columns of a block (VEC: N and the row stride are
-// multiples of 4 and every row starts on a boundary of 4 elements), else columns lane + 32 k. Bound by memory: one
-// load and one store of each value.
+// Each warp takes kPackSteps * kBlocks consecutive blocks. VEC: N and the row stride are multiples of the share and
+// rows start on 16-byte boundaries; else the lane's columns are kLanes apart and move one by one. Bound by memory:
+// each value is loaded and stored once.
 template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(256) act8_pack_kernel(const void* __restrict__ x, long ld, uint8_t* __restrict__ q,
                                                         uint8_t* __restrict__ e, uint32_t blocks, int N, uint32_t nb) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t b0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kPackBlocks;
-  if (b0 >= blocks) return;
-  long row[kPackBlocks];
-  int col[kPackBlocks];
-  float v[kPackBlocks][4];
-  uint32_t r0 = b0 / nb, k0 = b0 - r0 * nb;
+  using S = Share<TYPE>;
+  constexpr int E = S::kElems;
+  const int lane = threadIdx.x & 31, part = lane / S::kLanes, sub = lane % S::kLanes;
+  const uint32_t first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kPackSteps * S::kBlocks);
+  uint32_t r = (first + part) / nb, k = first + part - r * nb;  // row, and block of the row
+  long row[kPackSteps];
+  int col[kPackSteps];  // first column of the lane's share; N: none
+  float v[kPackSteps][E];
 #pragma unroll
-  for (int u = 0; u < kPackBlocks; ++u) {
-    row[u] = r0;
-    col[u] = b0 + u < blocks ? static_cast<int>(k0) * kAct8Block + (VEC ? 4 * lane : lane) : N;
-    if (++k0 == nb) k0 = 0, ++r0;
+  for (int u = 0; u < kPackSteps; ++u) {
+    row[u] = r;
+    col[u] = first + part + u * S::kBlocks < blocks ? static_cast<int>(k) * kAct8Block + (VEC ? E * sub : sub) : N;
+    next_block<S::kBlocks>(r, k, nb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
+    for (int i = 0; i < E; ++i) v[u][i] = 0.f;
     if constexpr (VEC) {
-      if (col[u] < N) load4<TYPE>(x, row[u] * ld + col[u], v[u]);
+      if (col[u] < N) {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) load4<TYPE>(x, row[u] * ld + col[u] + i, *reinterpret_cast<float(*)[4]>(&v[u][i]));
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col[u] + 32 * i < N) v[u][i] = load1<TYPE>(x, row[u] * ld + col[u] + 32 * i);
+      for (int i = 0; i < E; ++i)
+        if (col[u] + S::kLanes * i < N) v[u][i] = load1<TYPE>(x, row[u] * ld + col[u] + S::kLanes * i);
     }
   }
-  uint32_t mine = 0;  // lane u keeps the byte of block u
+  uint32_t mine = 0;  // lane i keeps the byte of block i
 #pragma unroll
-  for (int u = 0; u < kPackBlocks; ++u) {
+  for (int u = 0; u < kPackSteps; ++u) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
-    const uint32_t byte = act8_byte(__reduce_max_sync(0xffffffffu, top));
-    if (lane == u) mine = byte;
-    const uint32_t codes = act8_codes(v[u], byte);
+    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
+    if constexpr (S::kBlocks == 1) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == u) mine = top;
+    } else {
+      const uint32_t t0 = __reduce_max_sync(0xffffffffu, part == 0 ? top : 0u);
+      const uint32_t t1 = __reduce_max_sync(0xffffffffu, part == 1 ? top : 0u);
+      top = part == 0 ? t0 : t1;
+      if (lane / 2 == u) mine = lane & 1 ? t1 : t0;
+    }
+    const uint32_t byte = act8_byte(top);
+    uint32_t codes[E / 4];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) codes[i] = act8_codes(*reinterpret_cast<float(*)[4]>(&v[u][4 * i]), byte);
+    uint8_t* to = q + row[u] * N + col[u];
     if constexpr (VEC) {
-      if (col[u] < N) *reinterpret_cast<uint32_t*>(q + row[u] * N + col[u]) = codes;
+      if (col[u] < N) {
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+        else *reinterpret_cast<uint32_t*>(to) = codes[0];
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col[u] + 32 * i < N) q[row[u] * N + col[u] + 32 * i] = static_cast<uint8_t>(codes >> (8 * i));
+      for (int i = 0; i < E; ++i)
+        if (col[u] + S::kLanes * i < N) to[S::kLanes * i] = static_cast<uint8_t>(codes[i / 4] >> (8 * (i & 3)));
     }
   }
-  if (lane < kPackBlocks && b0 + lane < blocks) e[b0 + lane] = static_cast<uint8_t>(mine);
+  if (lane < kPackSteps * S::kBlocks && first + lane < blocks) e[first + lane] = static_cast<uint8_t>(act8_byte(mine));
 }
 
 template <int TYPE, bool GELU, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ e,
                                                           void* __restrict__ x, void* __restrict__ h, uint32_t blocks,
                                                           int N, uint32_t nb) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t b0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kPackBlocks;
-  if (b0 >= blocks) return;
-  long at[kPackBlocks];
-  int col[kPackBlocks];
-  uint32_t codes[kPackBlocks], byte[kPackBlocks];
-  uint32_t r0 = b0 / nb, k0 = b0 - r0 * nb;
+  using S = Share<TYPE>;
+  constexpr int E = S::kElems;
+  const int lane = threadIdx.x & 31, part = lane / S::kLanes, sub = lane % S::kLanes;
+  const uint32_t first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kPackSteps * S::kBlocks) + part;
+  uint32_t r = first / nb, k = first - r * nb;
+  long at[kPackSteps];
+  int col[kPackSteps];
+  uint32_t codes[kPackSteps][E / 4], byte[kPackSteps];
 #pragma unroll
-  for (int u = 0; u < kPackBlocks; ++u) {
-    col[u] = b0 + u < blocks ? static_cast<int>(k0) * kAct8Block + (VEC ? 4 * lane : lane) : N;
-    at[u] = static_cast<long>(r0) * N + col[u];
-    if (++k0 == nb) k0 = 0, ++r0;
-    byte[u] = b0 + u < blocks ? e[b0 + u] : 0;
-    codes[u] = 0;
-    if constexpr (VEC) {
-      if (col[u] < N) codes[u] = *reinterpret_cast<const uint32_t*>(q + at[u]);
-    } else {
+  for (int u = 0; u < kPackSteps; ++u) {
+    const uint32_t blk = first + u * S::kBlocks;
+    col[u] = blk < blocks ? static_cast<int>(k) * kAct8Block + (VEC ? E * sub : sub) : N;
+    at[u] = static_cast<long>(r) * N + col[u];
+    byte[u] = blk < blocks ? e[blk] : 0;
+    next_block<S::kBlocks>(r, k, nb);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col[u] + 32 * i < N) codes[u] |= static_cast<uint32_t>(q[at[u] + 32 * i]) << (8 * i);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kPackBlocks; ++u) {
-    float v[4], g[4];
-    decode4<TYPE>(codes[u], byte[u], v);
-    if constexpr (GELU) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = gelu_full(v[i]);
-    }
+    for (int i = 0; i < E / 4; ++i) codes[u][i] = 0;
     if constexpr (VEC) {
       if (col[u] < N) {
-        store4<TYPE>(x, at[u], v);
-        if constexpr (GELU) store4<TYPE>(h, at[u], g);
+        if constexpr (E == 8) {
+          const uint2 c = *reinterpret_cast<const uint2*>(q + at[u]);
+          codes[u][0] = c.x, codes[u][1] = c.y;
+        } else {
+          codes[u][0] = *reinterpret_cast<const uint32_t*>(q + at[u]);
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (col[u] + 32 * i < N) {
-          store1<TYPE>(x, at[u] + 32 * i, v[i]);
-          if constexpr (GELU) store1<TYPE>(h, at[u] + 32 * i, g[i]);
+      for (int i = 0; i < E; ++i)
+        if (col[u] + S::kLanes * i < N) codes[u][i / 4] |= static_cast<uint32_t>(q[at[u] + S::kLanes * i]) << (8 * (i & 3));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPackSteps; ++u) {
+    float v[E], g[E];
+#pragma unroll
+    for (int i = 0; i < E; i += 4) decode4<TYPE>(codes[u][i / 4], byte[u], *reinterpret_cast<float(*)[4]>(&v[i]));
+    if constexpr (GELU) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) g[i] = gelu_full(v[i]);
+    }
+    if constexpr (VEC) {
+      if (col[u] < N) {
+        store_share<TYPE>(x, at[u], v);
+        if constexpr (GELU) store_share<TYPE>(h, at[u], g);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (col[u] + S::kLanes * i < N) {
+          store1<TYPE>(x, at[u] + S::kLanes * i, v[i]);
+          if constexpr (GELU) store1<TYPE>(h, at[u] + S::kLanes * i, g[i]);
         }
       }
     }
@@ -246,48 +301,119 @@ __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restric
   if (lane == 0) rstd_out[row] = rstd;
 }
 
-// LayerNorm backward: warps stride over rows; a lane keeps the row's codes (4 to a register, decoded twice: that is
-// cheaper than four registers each) and dy, and its columns' dgamma / dbeta sums. All loads of a row are issued
-// before its arithmetic, the incoming residual gradient before the first store (dres may be dres_in). Each CTA adds
-// its warps' sums in a fixed order and leaves one partial row.
+// LayerNorm backward: groups of WPR warps stride over rows, each warp with V4 of the row's blocks of 128 columns (at
+// most 6, so that 16 warps fit an SM's registers; they join their two sums through shared memory, one barrier of the
+// group a row). Every lane copies its own columns of a row (dy, codes, the incoming residual
+// gradient) into shared memory of its own with asynchronous copies, the next row's dy and codes as soon as this row's
+// are in registers and its residual gradient once this row's is used, so copies are in flight all the time and need
+// no barrier (with plain loads the few warps that the registers allow waited for memory: 40 us at 8192 x 1280). The
+// column sums of dgamma and dbeta stay in registers; codes are decoded twice, which is cheaper than four registers
+// each. Each CTA adds its groups' sums in a fixed order and leaves one partial row. dres may be dres_in: a row's
+// residual gradient is read before its outputs are stored, by the same lane.
 constexpr int kLnWarps = 8;
-constexpr int ln_ctas_per_sm(int v4) { return v4 <= 4 ? 2 : 1; }  // 17 V4 registers and about 20 more a thread
+constexpr int kLnCtasPerSm = 2;
+constexpr int ln_slot_bytes(int v4) { return v4 * 32 * 36; }      // of one warp: 16 + 16 + 4 bytes a lane and block
 
-template <int V4, bool F16>
-__global__ void __launch_bounds__(256, ln_ctas_per_sm(V4))
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits for all but the newest group.
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void read16(uint32_t from, float (&v)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+               : "r"(from)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t read4(uint32_t from) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+  return v;
+}
+
+template <int V4, int WPR, bool F16>
+__global__ void __launch_bounds__(256, kLnCtasPerSm)
     ln_bwd_act8_kernel(const float* __restrict__ dy, const uint8_t* __restrict__ q, const uint8_t* __restrict__ e,
                        const float* __restrict__ rstd, const float* __restrict__ w, const float* __restrict__ b,
                        const float* dres_in, float* dres, uint16_t* __restrict__ dres16, uint16_t* __restrict__ y,
                        float* __restrict__ part, int M, int H, int nb) {
   constexpr int kOut = F16 ? kActF16 : kActBf16;
-  extern __shared__ float sums[];  // [kLnWarps][2][H]
+  constexpr int kGroups = kLnWarps / WPR;
+  extern __shared__ __align__(16) float sums[];  // the warps' slots; after the rows, [kGroups][2][H]
+  __shared__ float joint[2][kLnWarps][2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp / WPR;
+  const int blk0 = warp % WPR * V4, col0 = kAct8Block * blk0 + 4 * lane;  // this warp's blocks, this lane's first column
+  // this lane's slots of block i: dy, residual gradient, codes
+  const uint32_t slot = smem_u32(sums) + warp * ln_slot_bytes(V4) + lane * 16;
+  const uint32_t slot_in = slot + V4 * 512, slot_q = slot + V4 * 1024 - lane * 12;
+  const int stride = gridDim.x * kGroups;
+  const auto copy_dy = [&](int r) {
+    const long base = static_cast<long>(r) * H + col0;
+#pragma unroll
+    for (int i = 0; i < V4; ++i) {
+      if (kAct8Block * i + col0 < H) {
+        copy16(slot + 512 * i, dy + base + kAct8Block * i);
+        copy4(slot_q + 128 * i, q + base + kAct8Block * i);
+      }
+    }
+  };
+  const auto copy_in = [&](int r) {
+    const long base = static_cast<long>(r) * H + col0;
+#pragma unroll
+    for (int i = 0; i < V4; ++i)
+      if (kAct8Block * i + col0 < H) copy16(slot_in + 512 * i, dres_in + base + kAct8Block * i);
+  };
   float ga[V4][4], ba[V4][4];
 #pragma unroll
   for (int i = 0; i < V4; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) ga[i][k] = ba[i][k] = 0.f;
+  int r = blockIdx.x * kGroups + group, parity = 0;
+  uint32_t bytes = 0;
+  float rs = 0.f;
+  if (r < M) {
+    copy_dy(r);
+    copies_commit();
+    copy_in(r);
+    copies_commit();
+    bytes = lane < nb ? e[static_cast<long>(r) * nb + lane] : 0u;
+    rs = rstd[r];
+  }
 #pragma unroll 1
-  for (int r = blockIdx.x * kLnWarps + warp; r < M; r += gridDim.x * kLnWarps) {
+  for (; r < M; r += stride) {
     const long base = static_cast<long>(r) * H;
+    const int next = r + stride;
     uint32_t codes[V4];
     float d[V4][4];
+    copies_wait();  // dy and codes; the residual gradient may be on its way
 #pragma unroll
     for (int i = 0; i < V4; ++i) {
-      const int j = kAct8Block * i + 4 * lane;
-      codes[i] = j < H ? *reinterpret_cast<const uint32_t*>(q + base + j) : 0u;
+      codes[i] = 0u;
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[i][k] = 0.f;
-      if (j < H) load4<kActF32>(dy, base + j, d[i]);
+      if (kAct8Block * i + col0 < H) {
+        read16(slot + 512 * i, d[i]);
+        codes[i] = read4(slot_q + 128 * i);
+      }
     }
-    const uint32_t bytes = lane < nb ? e[static_cast<long>(r) * nb + lane] : 0u;
-    const float rs = rstd[r];
+    uint32_t next_bytes = 0;
+    float next_rs = 0.f;
+    if (next < M) {
+      copy_dy(next);
+      next_bytes = lane < nb ? e[static_cast<long>(next) * nb + lane] : 0u;
+      next_rs = rstd[next];
+    }
+    copies_commit();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < V4; ++i) {
-      const int j = kAct8Block * i + 4 * lane;
-      const float scale = act8_scale(__shfl_sync(0xffffffffu, bytes, i));
+      const int j = kAct8Block * i + col0;
+      const float scale = act8_scale(__shfl_sync(0xffffffffu, bytes, blk0 + i));
       if (j < H) {
         float xh[4], ww[4], bb[4], o[4];
         act8_values(codes[i], scale, xh);
@@ -305,31 +431,48 @@ __global__ void __launch_bounds__(256, ln_ctas_per_sm(V4))
         store4<kOut>(y, base + j, o);
       }
     }
-    const float m1 = warp_sum(s1) / H, m2 = warp_sum(s2) / H;
-    float in[V4][4];
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if constexpr (WPR > 1) {
+      if (lane == 0) {
+        joint[parity][warp][0] = s1;
+        joint[parity][warp][1] = s2;
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * WPR) : "memory");
+      s1 = s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < V4; ++i) {
-      const int j = kAct8Block * i + 4 * lane;
-      if (j < H) load4<kActF32>(dres_in, base + j, in[i]);
+      for (int k = 0; k < WPR; ++k) {
+        s1 += joint[parity][group * WPR + k][0];
+        s2 += joint[parity][group * WPR + k][1];
+      }
+      parity ^= 1;  // the next row writes the other half: no second barrier
     }
+    const float m1 = s1 / H, m2 = s2 / H;
+    copies_wait();  // the residual gradient; the next row's dy may be on its way
 #pragma unroll
     for (int i = 0; i < V4; ++i) {
-      const int j = kAct8Block * i + 4 * lane;
-      const float scale = act8_scale(__shfl_sync(0xffffffffu, bytes, i));
+      const int j = kAct8Block * i + col0;
+      const float scale = act8_scale(__shfl_sync(0xffffffffu, bytes, blk0 + i));
       if (j < H) {
-        float xh[4], o[4];
+        float xh[4], in[4], o[4];
         act8_values(codes[i], scale, xh);
+        read16(slot_in + 512 * i, in);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = fmaf(rs, d[i][k] - m1 - xh[k] * m2, in[i][k]);
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(rs, d[i][k] - m1 - xh[k] * m2, in[k]);
         store4<kActF32>(dres, base + j, o);
         store4<kOut>(dres16, base + j, o);
       }
     }
+    if (next < M) copy_in(next);
+    copies_commit();
+    bytes = next_bytes;
+    rs = next_rs;
   }
-  float* to = sums + static_cast<long>(warp) * 2 * H;
+  __syncthreads();  // the slots become the sums
+  float* to = sums + static_cast<long>(group) * 2 * H;
 #pragma unroll
   for (int i = 0; i < V4; ++i) {
-    const int j = kAct8Block * i + 4 * lane;
+    const int j = kAct8Block * i + col0;
     if (j < H) {
       store4<kActF32>(to, j, ga[i]);
       store4<kActF32>(to, H + j, ba[i]);
@@ -339,7 +482,7 @@ __global__ void __launch_bounds__(256, ln_ctas_per_sm(V4))
   for (int c = threadIdx.x; c < 2 * H; c += 256) {
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < kLnWarps; ++k) v += sums[static_cast<long>(k) * 2 * H + c];
+    for (int k = 0; k < kGroups; ++k) v += sums[static_cast<long>(k) * 2 * H + c];
     part[static_cast<long>(blockIdx.x) * 2 * H + c] = v;
   }
 }
@@ -372,7 +515,10 @@ int blocks_of(long N) { return static_cast<int>((N + kAct8Block - 1) / kAct8Bloc
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // CTAs of a pack or unpack launch over `blocks` blocks.
-unsigned pack_ctas(long blocks) { return static_cast<unsigned>((blocks + 8 * kPackBlocks - 1) / (8 * kPackBlocks)); }
+unsigned pack_ctas(long blocks, int type) {
+  const long per_cta = 8L * kPackSteps * (type == kActF32 ? 1 : 2);
+  return static_cast<unsigned>((blocks + per_cta - 1) / per_cta);
+}
 
 // Row widths in float4 a lane that kernels are built for.
 #define HB_ACT8_WIDTHS(V4, ...)                                  \
@@ -397,27 +543,27 @@ int width_v4(int H) {
 
 void act8_pack_launch(const void* x, long ld, int type, int8_t* q, uint8_t* e, long M, int N, cudaStream_t s) {
   if (M == 0 || N == 0) return;
-  const int nb = blocks_of(N), bytes = type == kActF32 ? 4 : 2;
+  const int nb = blocks_of(N), share = type == kActF32 ? 4 : 8;
   const long blocks = M * nb;
-  const bool vec = N % 4 == 0 && (M == 1 || ld % 4 == 0) && aligned(x, 4 * bytes) && aligned(q, 4);
+  const bool vec = N % share == 0 && (M == 1 || ld % share == 0) && aligned(x, 16) && aligned(q, share);
 #define HB_PACK(T) (vec ? act8_pack_kernel<T, true> : act8_pack_kernel<T, false>)
   auto* k = type == kActF32 ? HB_PACK(kActF32) : type == kActF16 ? HB_PACK(kActF16) : HB_PACK(kActBf16);
 #undef HB_PACK
-  k<<<pack_ctas(blocks), 256, 0, s>>>(x, ld, reinterpret_cast<uint8_t*>(q), e, static_cast<uint32_t>(blocks), N, nb);
+  k<<<pack_ctas(blocks, type), 256, 0, s>>>(x, ld, reinterpret_cast<uint8_t*>(q), e, static_cast<uint32_t>(blocks), N, nb);
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
 void act8_unpack_launch(const int8_t* q, const uint8_t* e, int type, void* x, void* h, long M, int N, cudaStream_t s) {
   if (M == 0 || N == 0) return;
-  const int nb = blocks_of(N), bytes = type == kActF32 ? 4 : 2;
+  const int nb = blocks_of(N), share = type == kActF32 ? 4 : 8;
   const long blocks = M * nb;
-  const bool vec = N % 4 == 0 && aligned(q, 4) && aligned(x, 4 * bytes) && (!h || aligned(h, 4 * bytes));
+  const bool vec = N % share == 0 && aligned(q, share) && aligned(x, 16) && (!h || aligned(h, 16));
 #define HB_UNPACK(T)                                                                      \
   (h ? (vec ? act8_unpack_kernel<T, true, true> : act8_unpack_kernel<T, true, false>)     \
      : (vec ? act8_unpack_kernel<T, false, true> : act8_unpack_kernel<T, false, false>))
   auto* k = type == kActF32 ? HB_UNPACK(kActF32) : type == kActF16 ? HB_UNPACK(kActF16) : HB_UNPACK(kActBf16);
 #undef HB_UNPACK
-  k<<<pack_ctas(blocks), 256, 0, s>>>(reinterpret_cast<const uint8_t*>(q), e, x, h, static_cast<uint32_t>(blocks), N, nb);
+  k<<<pack_ctas(blocks, type), 256, 0, s>>>(reinterpret_cast<const uint8_t*>(q), e, x, h, static_cast<uint32_t>(blocks), N, nb);
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
@@ -430,28 +576,33 @@ void ln_fwd_act8_launch(const float* x, const float* w, const float* b, void* y,
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
+// Warps that share a row of the backward, and the blocks each of them takes: at most 6.
+static int ln_bwd_warps(int H) { return width_v4(H) <= 6 ? 1 : width_v4(H) <= 12 ? 2 : 4; }
+
 int ln_bwd_act8_ctas(int M, int H, int device) {
-  const int full = ln_ctas_per_sm(width_v4(H)) * num_sms(device), need = (M + kLnWarps - 1) / kLnWarps;
-  return std::max(1, std::min(need, full));
+  const int groups = kLnWarps / ln_bwd_warps(H);
+  return std::max(1, std::min((M + groups - 1) / groups, kLnCtasPerSm * num_sms(device)));
 }
 
 void ln_bwd_act8_launch(const float* dy, const int8_t* q, const uint8_t* e, const float* rstd, const float* w,
                         const float* b, const float* dres_in, float* dres, void* dres16, void* y, float* part, int ctas,
                         float* dgamma, float* dbeta, int M, int H, bool f16, cudaStream_t s) {
   if (M == 0) return;
-  const size_t smem = static_cast<size_t>(kLnWarps) * 2 * H * sizeof(float);  // 128 KB at most
   HB_ACT8_WIDTHS(width_v4(H), {
-    auto* k = f16 ? ln_bwd_act8_kernel<kV, true> : ln_bwd_act8_kernel<kV, false>;
-    if (smem > 48 * 1024) {
+    constexpr int kWpr = kV <= 6 ? 1 : kV <= 12 ? 2 : 4;
+    constexpr int kSmem = kLnWarps * ln_slot_bytes(kV / kWpr);  // the sums, 8 / kWpr * 2 H floats, need less
+    static_assert(kLnWarps / kWpr * 2 * kV * kAct8Block * 4 <= kSmem, "the sums take the place of the slots");
+    auto* k = f16 ? ln_bwd_act8_kernel<kV / kWpr, kWpr, true> : ln_bwd_act8_kernel<kV / kWpr, kWpr, false>;
+    if (kSmem > 48 * 1024) {
       static std::atomic<uint64_t> ready[2];  // devices whose shared-memory limit is raised
       const uint64_t bit = uint64_t{1} << current_device();
       if (!(ready[f16].load(std::memory_order_relaxed) & bit)) {
-        HB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kV * kLnWarps * 1024));
+        HB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         ready[f16].fetch_or(bit, std::memory_order_relaxed);
       }
     }
-    k<<<ctas, 256, smem, s>>>(dy, reinterpret_cast<const uint8_t*>(q), e, rstd, w, b, dres_in, dres,
-                              static_cast<uint16_t*>(dres16), static_cast<uint16_t*>(y), part, M, H, blocks_of(H));
+    k<<<ctas, 256, kSmem, s>>>(dy, reinterpret_cast<const uint8_t*>(q), e, rstd, w, b, dres_in, dres,
+                               static_cast<uint16_t*>(dres16), static_cast<uint16_t*>(y), part, M, H, blocks_of(H));
   });
   HB_CUDA_CHECK(cudaGetLastError());
   cudaLaunchConfig_t cfg{};
