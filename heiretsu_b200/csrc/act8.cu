@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
 }
 
 // LayerNorm forward: one warp per row, the row in registers (V4 float4 a lane; float4 i of the 32 lanes is block i),
-// statistics in two passes over the registers. One read of x, one write of y and of the codes.
+// statistics in two passes over the registers, in the order of ln_fwd_kernel (norm.cu): y has the same bits, so keeping
+// activations in 8 bits leaves the forward pass as it is. One read of x, one write of y and of the codes.
 template <int V4, bool F16>
 __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                           const float* __restrict__ b, uint16_t* __restrict__ y,
@@ -261,17 +262,15 @@ __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restric
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[i][k] = 0.f;
     if (j < H) load4<kActF32>(x, base + j, v[i]);
-    s += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+    s += v[i][0] + v[i][1] + v[i][2] + v[i][3];
   }
   const float mu = warp_sum(s) / H;
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < V4; ++i) {
-    const bool in = kAct8Block * i + 4 * lane < H;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[i][k] = in ? v[i][k] - mu : 0.f;
-      ss = fmaf(v[i][k], v[i][k], ss);
+    if (kAct8Block * i + 4 * lane < H) {
+      const float a = v[i][0] - mu, c = v[i][1] - mu, d = v[i][2] - mu, f = v[i][3] - mu;
+      ss += a * a + c * c + d * d + f * f;
     }
   }
   const float rstd = rsqrtf(warp_sum(ss) / H + eps);
@@ -282,7 +281,7 @@ __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restric
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      v[i][k] *= rstd;
+      v[i][k] = j < H ? (v[i][k] - mu) * rstd : 0.f;
       top = max(top, __float_as_uint(v[i][k]) & 0x7FFFFFFFu);
     }
     const uint32_t byte = act8_byte(__reduce_max_sync(0xffffffffu, top));

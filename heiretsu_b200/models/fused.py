@@ -105,32 +105,62 @@ def _dropout_of(blk):
     return d if (d is not None and blk.training) else None
 
 
-def _attn_fwd(blk, x: torch.Tensor, B: int, T: int, keep: bool):
-    """Attention sub-layer: x fp32 [M, H] -> x1 = x + drop(c_proj(attn(c_attn(ln_1(x)))))."""
+# Activations kept in 8 bits (``act_bits`` 8): what backward needs of a sub-layer is kept as 8-bit codes with a
+# power-of-two scale per 128 columns (csrc/act8.cuh). A dense block keeps per token: the normalised input of both
+# LayerNorms (which gives both the LayerNorm backward and, times gamma plus beta, the operand of the weight gradient
+# behind it), Q/K/V, the attention output and the MLP pre-activation (GELU is evaluated again): about 10 H bytes
+# instead of 36 H, without re-running the forward. Backward restores each where it is used; the forward is exact.
+class _Act8:
+    """Saved state of a sub-layer in 8 bits."""
+
+    def __init__(self, norm, *rest):
+        self.norm, self.rest = norm, rest  # norm: (codes, exponents, rstd) of the LayerNorm
+
+
+def _norm_fwd(ln, x: torch.Tensor, dt: torch.dtype, act8: bool):
+    """LayerNorm forward: (y, what backward needs of it)."""
+    if act8:
+        y, q, e, rstd = K.layernorm_fwd_act8(x, ln.weight, ln.bias, LN_EPS, dtype=dt)
+        return y, (q, e, rstd)
+    y, mean, rstd = K.layernorm_fwd(x, ln.weight, ln.bias, LN_EPS, dtype=dt)
+    return y, (mean, rstd)
+
+
+def _attn_fwd(blk, x: torch.Tensor, B: int, T: int, keep: bool, act8: bool = False):
+    """Attention sub-layer: x fp32 [M, H] -> x1 = x + drop(c_proj(attn(c_attn(ln_1(x))))).
+    ``act8`` (with ``keep``): the state for backward is kept in 8 bits."""
     attn = blk.attn
     d = _dropout_of(blk)
-    xn, m1, r1 = K.layernorm_fwd(x, blk.ln_1.weight, blk.ln_1.bias, LN_EPS, dtype=_dt(blk))
+    act8 = act8 and keep
+    xn, norm = _norm_fwd(blk.ln_1, x, _dt(blk), act8)
     qkv = G.linear_fwd(xn, attn.c_attn.weight.w16, attn.c_attn.bias)
     adrop = (d[0], 4 * d[1], d[2], 0, attn.nh_tp) if d else None
     y, lse = K.attention_fwd(qkv, B, T, attn.nh_tp, drop=adrop, head_dim=attn.dh)
     x1 = G.linear_fwd_resid(y, attn.c_proj.weight.w16, attn.c_proj.bias, x,
                             drop=(d[0], 4 * d[1] + 1, d[2], 0) if d else None)
-    return x1, ((x, xn, m1, r1, qkv, y, lse, d) if keep else None)
+    if act8:
+        return x1, _Act8(norm, K.act8_pack(qkv), K.act8_pack(y), lse, d)
+    return x1, ((x, xn, *norm, qkv, y, lse, d) if keep else None)
 
 
-def _mlp_fwd(blk, x1: torch.Tensor, keep: bool):
+def _mlp_fwd(blk, x1: torch.Tensor, keep: bool, act8: bool = False):
     """Dense MLP sub-layer: x2 = x1 + drop(c_proj(gelu(c_fc(ln_2(x1)))))."""
     mlp = blk.mlp
     d = _dropout_of(blk)
-    xn2, m2, r2 = K.layernorm_fwd(x1, blk.ln_2.weight, blk.ln_2.bias, LN_EPS, dtype=_dt(blk))
+    act8 = act8 and keep
+    xn2, norm = _norm_fwd(blk.ln_2, x1, _dt(blk), act8)
     h, pre = G.linear_fwd_gelu(xn2, mlp.c_fc.weight.w16, mlp.c_fc.bias)
     x2 = G.linear_fwd_resid(h, mlp.c_proj.weight.w16, mlp.c_proj.bias, x1,
                             drop=(d[0], 4 * d[1] + 2, d[2], 0) if d else None)
-    return x2, ((x1, xn2, m2, r2, pre, h, d) if keep else None)
+    if act8:
+        return x2, _Act8(norm, K.act8_pack(pre), d)
+    return x2, ((x1, xn2, *norm, pre, h, d) if keep else None)
 
 
 def _mlp_bwd(blk, saved, dres: torch.Tensor, dres16: torch.Tensor, ws: dict):
     """In place: dres (fp32) / dres16 (16-bit) go from d(x2) to d(x1)."""
+    if isinstance(saved, _Act8):
+        return _mlp_bwd_act8(blk, saved, dres, dres16)
     mlp = blk.mlp
     x1, xn2, m2, r2, pre, h, d = saved
     # gradient at c_proj's output
@@ -147,8 +177,56 @@ def _mlp_bwd(blk, saved, dres: torch.Tensor, dres16: torch.Tensor, ws: dict):
                     blk.ln_2.bias.main_grad, scratch=ws["ln_scratch"])
 
 
+def _norm_bwd_act8(ln, norm, dxn: torch.Tensor, dres: torch.Tensor, dres16: torch.Tensor) -> torch.Tensor:
+    """``layernorm_bwd`` from the kept codes; returns the LayerNorm's output for the weight gradient behind it."""
+    q, e, rstd = norm
+    return K.layernorm_bwd_act8(dxn, q, e, rstd, ln.weight, ln.bias, dres, dres, dres16, ln.weight.main_grad,
+                                ln.bias.main_grad)
+
+
+def _mlp_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor):
+    """``_mlp_bwd`` from 8-bit state. The gradients of c_fc's weight come last: their operand leaves the LayerNorm backward."""
+    mlp = blk.mlp
+    pre8, d = saved.rest
+    dout16 = K.dropout_bf16(dres, d[0], 4 * d[1] + 2, d[2], dtype=dres16.dtype) if d else dres16
+    h, pre = K.act8_unpack_gelu(*pre8, dtype=dres16.dtype)
+    dpre = G.linear_dgrad(dout16, mlp.c_proj.weight.w16, gelu_pre=pre)
+    del pre
+    G.linear_wgrad(dout16, h, out=mlp.c_proj.weight.main_grad, accumulate=True)
+    K.colsum_bf16(dout16, mlp.c_proj.bias.main_grad)
+    del dout16, h
+    dxn2 = G.linear_dgrad(dpre, mlp.c_fc.weight.w16, f32=True)
+    xn2 = _norm_bwd_act8(blk.ln_2, saved.norm, dxn2, dres, dres16)
+    del dxn2
+    G.linear_wgrad(dpre, xn2, out=mlp.c_fc.weight.main_grad, accumulate=True)
+    K.colsum_bf16(dpre, mlp.c_fc.bias.main_grad)
+
+
+def _attn_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor, B: int, T: int):
+    """``_attn_bwd`` from 8-bit state."""
+    attn = blk.attn
+    qkv8, y8, lse, d = saved.rest
+    dout16 = K.dropout_bf16(dres, d[0], 4 * d[1] + 1, d[2], dtype=dres16.dtype) if d else dres16
+    dy = G.linear_dgrad(dout16, attn.c_proj.weight.w16)
+    y = K.act8_unpack(*y8, dtype=dres16.dtype)
+    G.linear_wgrad(dout16, y, out=attn.c_proj.weight.main_grad, accumulate=True)
+    K.colsum_bf16(dout16, attn.c_proj.bias.main_grad)
+    del dout16
+    qkv = K.act8_unpack(*qkv8, dtype=dres16.dtype)
+    adrop = (d[0], 4 * d[1], d[2], 0, attn.nh_tp) if d else None
+    dqkv = K.attention_bwd(qkv, y, dy, lse, B, T, attn.nh_tp, drop=adrop, head_dim=attn.dh)
+    del dy, y, qkv
+    dxn = G.linear_dgrad(dqkv, attn.c_attn.weight.w16, f32=True)
+    xn = _norm_bwd_act8(blk.ln_1, saved.norm, dxn, dres, dres16)
+    del dxn
+    G.linear_wgrad(dqkv, xn, out=attn.c_attn.weight.main_grad, accumulate=True)
+    K.colsum_bf16(dqkv, attn.c_attn.bias.main_grad)
+
+
 def _attn_bwd(blk, saved, dres: torch.Tensor, dres16: torch.Tensor, B: int, T: int, ws: dict):
     """In place: dres / dres16 go from d(x1) to d(x)."""
+    if isinstance(saved, _Act8):
+        return _attn_bwd_act8(blk, saved, dres, dres16, B, T)
     attn = blk.attn
     x, xn, m1, r1, qkv, y, lse, d = saved
     # gradient at c_proj's output
@@ -207,10 +285,15 @@ def _is_moe(blk) -> bool:
 
 class _Recompute:
     """Saved state of a dense block run without keeping its activations: the block's
-    input and the dropout snapshot its forward used (backward reruns the forward)."""
+    input (in 8 bits with ``act8``) and the dropout snapshot its forward used
+    (backward reruns the forward)."""
 
-    def __init__(self, x_in, drop_now):
-        self.x_in, self.drop_now = x_in, drop_now
+    def __init__(self, x_in, drop_now, act8: bool = False):
+        self.act8, self.drop_now = act8, drop_now
+        self.x_in = K.act8_pack(x_in) if act8 else x_in
+
+    def block_input(self) -> torch.Tensor:
+        return K.act8_unpack(*self.x_in, dtype=torch.float32) if self.act8 else self.x_in
 
 
 def _rerun_dense(blk, r: "_Recompute", B: int, T: int):
@@ -219,7 +302,7 @@ def _rerun_dense(blk, r: "_Recompute", B: int, T: int):
     prev = getattr(blk, "_hb_drop_now", None)
     blk._hb_drop_now = r.drop_now
     try:
-        x1, sa = _attn_fwd(blk, r.x_in, B, T, True)
+        x1, sa = _attn_fwd(blk, r.block_input(), B, T, True)
         _, sm = _mlp_fwd(blk, x1, True)
     finally:
         blk._hb_drop_now = prev
@@ -228,7 +311,7 @@ def _rerun_dense(blk, r: "_Recompute", B: int, T: int):
 
 class _Body(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, blocks, B, T, recompute=False):
+    def forward(ctx, x, blocks, B, T, recompute=False, act8=False):
         from .fused_moe import moe_sublayer_fwd
 
         keep = x.requires_grad
@@ -240,14 +323,14 @@ class _Body(torch.autograd.Function):
             rerun = keep and recompute and not _is_moe(blk)
             x_in = x
             with nvtx(f"block{i}.attn.fwd"):
-                x, sa = _attn_fwd(blk, x, B, T, keep and not rerun)
+                x, sa = _attn_fwd(blk, x, B, T, keep and not rerun, act8)
             with nvtx(f"block{i}.mlp.fwd"):
                 if _is_moe(blk):
                     x, aux, sm = moe_sublayer_fwd(blk, None, x, keep)
                     aux_total = aux_total + aux
                 else:
-                    x, sm = _mlp_fwd(blk, x, keep and not rerun)
-            saved.append(_Recompute(x_in, getattr(blk, "_hb_drop_now", None)) if rerun else (sa, sm))
+                    x, sm = _mlp_fwd(blk, x, keep and not rerun, act8)
+            saved.append(_Recompute(x_in, getattr(blk, "_hb_drop_now", None), act8) if rerun else (sa, sm))
         ctx.blocks, ctx.saved, ctx.B, ctx.T = blocks, saved, B, T
         return x, aux_total
 
@@ -278,17 +361,22 @@ class _Body(torch.autograd.Function):
             if _BLOCK_DONE_HOOK is not None:
                 _BLOCK_DONE_HOOK(blk)
         ctx.saved = None
-        return dres, None, None, None, None
+        return dres, None, None, None, None, None
 
 
-def blocks_fused(blocks, x: torch.Tensor, cfg, recompute: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+def blocks_fused(blocks, x: torch.Tensor, cfg, recompute: bool = False,
+                 act_bits: int = 16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Run a list of blocks (dense or MoE) on x [B, T, H]; returns (fp32 x, summed MoE aux loss).
-    ``recompute``: dense blocks keep only their input and rerun their forward in backward."""
+    ``recompute``: dense blocks keep only their input and rerun their forward in backward.
+    ``act_bits`` 8: what is kept for backward is kept in 8 bits (with ``recompute``, the blocks' inputs);
+    MoE sub-layers keep 16 bits."""
+    if act_bits not in (8, 16):
+        raise ValueError(f"activations are kept in 16 or 8 bits, got {act_bits}")
     B, T, H = x.shape
     x2 = x.reshape(B * T, H)
     if x2.dtype != torch.float32:
         x2 = x2.float()
-    out, aux = _Body.apply(x2.contiguous(), list(blocks), B, T, bool(recompute))
+    out, aux = _Body.apply(x2.contiguous(), list(blocks), B, T, bool(recompute), act_bits == 8)
     return out.view(B, T, H), aux
 
 
@@ -376,7 +464,8 @@ def gpt_forward_fused(model, idx: torch.Tensor, targets: Optional[torch.Tensor],
     if topo is not None and getattr(topo, "tp", 1) > 1:
         return _gpt_forward_fused_tp(model, idx, targets)
     x = embed_fused(model.tr.wte.weight, model.tr.wpe.weight, idx)
-    x, aux = blocks_fused(model.tr.h, x, cfg, recompute=getattr(model, "recompute", False))
+    x, aux = blocks_fused(model.tr.h, x, cfg, recompute=getattr(model, "recompute", False),
+                          act_bits=getattr(model, "act_bits", 16))
     logits, loss = head_fused(model.tr.ln_f, model.lm_head.weight, x, targets, cfg.vocab_size,
                               want_logits=return_logits, grad_hint=getattr(model, "loss_grad_hint", 1.0),
                               grad_scale=getattr(model, "loss_grad_scale", None))

@@ -277,6 +277,7 @@ class GPT(nn.Module):
         init_gpt_weights(self, cfg.n_layer)
         self.fused = False  # set by heiretsu_b200.models.fused.enable_fused
         self.recompute = False  # activation checkpointing of the plain path (run_blocks)
+        self.act_bits = 16  # 8: the fused blocks keep their activations in 8 bits (models/fused.py)
         self._head_pool: list = []  # logits buffers reused by head_cross_entropy
 
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = True):
@@ -297,6 +298,25 @@ class GPT(nn.Module):
         if targets is not None:
             loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1))
         return logits, loss, aux_total
+
+    # Post-training objectives (models/objectives.py); like forward, fused where the model is.
+    def token_logprobs(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        """Log-probability of ``targets`` [B, T] (0 where -100), differentiable: fp32 [B, T]."""
+        from .objectives import token_logprobs
+        return token_logprobs(self, idx, targets)
+
+    def policy_loss(self, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
+                    ref_logp: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                    clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0):
+        """Clipped policy loss with a KL term -> (loss, aux_loss, stats [2], logp [B, T])."""
+        from .objectives import policy_loss
+        return policy_loss(self, idx, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef)
+
+    def preference_loss(self, idx: torch.Tensor, targets: torch.Tensor, ref_logp: Optional[torch.Tensor] = None,
+                        beta: float = 0.1, label_smoothing: float = 0.0):
+        """Preference loss on P chosen sequences followed by their P rejected partners -> (loss, aux_loss, rewards [2, P])."""
+        from .objectives import preference_loss
+        return preference_loss(self, idx, targets, ref_logp, beta, label_smoothing)
 
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())

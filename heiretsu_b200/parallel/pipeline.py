@@ -141,6 +141,7 @@ class StageModule(nn.Module):
         init_gpt_weights(self, cfg.n_layer)
         self.fused = False
         self.recompute = False  # activation checkpointing of the plain path (models.gpt.run_blocks)
+        self.act_bits = 16  # 8: the fused blocks keep their activations in 8 bits
         self._head_pool: list = []  # logits buffers reused by head_cross_entropy
         self.topo = topo
 
@@ -184,7 +185,7 @@ class StageModule(nn.Module):
             return out.view(Bs, T, H), aux / self.tp  # shard aux losses / tp sum to the mean
         if self._fused_on(x):
             from ..models.fused import blocks_fused
-            return blocks_fused(self.blocks, x, self.cfg, recompute=self.recompute)
+            return blocks_fused(self.blocks, x, self.cfg, recompute=self.recompute, act_bits=self.act_bits)
         from ..models.gpt import run_blocks
         return run_blocks(self.blocks, x, self.recompute)
 

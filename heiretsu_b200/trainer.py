@@ -143,6 +143,10 @@ def build_argparser() -> argparse.ArgumentParser:
     p.add_argument("--activation_checkpointing", type=int, default=0, choices=[0, 1],
                    help="keep only each block's input and recompute the block in backward (plain engine; fused "
                         "engine without TP: dense blocks, not yet run on GPUs)")
+    p.add_argument("--activation_bits", type=int, default=16, choices=[8, 16],
+                   help="8: keep the activations that backward needs in 8 bits (fused engine without TP: about 10 "
+                        "instead of 36 bytes per token and channel in a dense block; with --activation_checkpointing "
+                        "the blocks' inputs)")
     p.add_argument("--fused_tp_dropout", type=int, default=1, choices=[0, 1],
                    help="run tp > 1 with dropout > 0 on the fused engine (masks applied around the in-kernel "
                         "reduce-scatter and all-gather; default); 0 = such runs use the plain engine")
@@ -412,6 +416,12 @@ class Engine:
                 raise ValueError("--activation_checkpointing: the fused tensor-parallel blocks keep their "
                                  "activations; use --engine plain or tp 1")
             self.module.recompute = True  # plain: torch.utils.checkpoint; fused: dense blocks rerun in backward
+        if getattr(args, "activation_bits", 16) == 8:
+            if not self.fused:
+                raise ValueError("--activation_bits 8 runs on the fused engine (--device cuda, --amp bf16 or fp16)")
+            if topo.tp > 1:
+                raise ValueError("--activation_bits 8: the fused tensor-parallel blocks keep 16-bit activations; use tp 1")
+            self.module.act_bits = 8
         self.dropout_seed = None
         if self.fused and cfg.dropout > 0:
             # Device seed of the fused dropout masks: different per DP / PP rank

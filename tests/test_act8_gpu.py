@@ -152,7 +152,7 @@ def test_layernorm_forward(M, H, f16):
     top.scatter_reduce_(1, block.expand(M, H), xh.abs(), "amax")
     full = 127 * torch.exp2(e.double() - 127)
     assert (top <= full * (1 + 1e-4)).all() and ((top > full / 2 * (1 - 1e-4)) | (e == 1)).all()
-    assert torch.allclose(rstd, rstd0, rtol=1e-5)
+    assert torch.equal(rstd, rstd0) and torch.equal(y, y0)  # the forward pass does not change
 
 
 @pytest.mark.parametrize("f16", [BF16, FP16])
