@@ -1,11 +1,21 @@
 """8-bit activations: the format against a 64-bit oracle (codes equal, values equal), and the LayerNorm that keeps
 its normalised input in it."""
+import gc
+
 import pytest
 import torch
 
 from post_oracle import EPS, TINY, act8_codes, act8_values, gelu
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _leave_no_garbage():
+    """Other tests count the memory held between two points: nothing of these may be freed in between."""
+    yield
+    gc.collect()
+
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 

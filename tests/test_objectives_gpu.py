@@ -1,10 +1,20 @@
 """Post-training objectives and 8-bit activations of the GPT model on the GPU: the fused path against the plain fp32
 path, and the pieces together as a training program uses them (score with a frozen reference, preference or policy
 step with 8-bit activations, AdamW, captured and replayed)."""
+import gc
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _leave_no_garbage():
+    """Other tests count the memory held between two points: nothing of these may be freed in between."""
+    yield
+    gc.collect()
+
 
 IGNORE = -100
 V, T = 1000, 256

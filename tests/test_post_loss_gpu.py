@@ -3,12 +3,22 @@
 Tolerances are derived in tests/post_oracle.py before any run: they count the roundings of the output, of the
 exponentials and of the sums.
 """
+import gc
+
 import pytest
 import torch
 
 from post_oracle import EPS, IGNORE, grad_bound, logprobs, lse_bound, policy, preference
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _leave_no_garbage():
+    """Other tests count the memory held between two points: nothing of these may be freed in between."""
+    yield
+    gc.collect()
+
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
