@@ -63,7 +63,7 @@ bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_
 void check_width(int64_t M, int64_t H, const char* op) {
   TORCH_CHECK(H >= 4 && H % 4 == 0 && H <= 2048, op, ": the width must be a multiple of 4 in [4, 2048], got ",
               std::to_string(H));
-  TORCH_CHECK(M <= kIntMax, op, ": too many rows");
+  TORCH_CHECK(M <= kIntMax / 2, op, ": too many rows");
 }
 
 // Empty codes and exponent bytes of an [M, N] activation.
@@ -143,6 +143,10 @@ at::Tensor layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const a
   check_vec(b, H, dev, op, "b");
   check_mat(dres_in, at::kFloat, M, H, dev, op, "dres_in");
   check_mat(dres, at::kFloat, M, H, dev, op, "dres");
+  const auto from = reinterpret_cast<uintptr_t>(dres_in.data_ptr()), to = reinterpret_cast<uintptr_t>(dres.data_ptr());
+  const auto bytes = static_cast<uintptr_t>(M * H * 4);
+  TORCH_CHECK(from == to || from + bytes <= to || to + bytes <= from, op,
+              ": dres must be dres_in itself or not overlap it");
   TORCH_CHECK(act_type(dres16, op, "dres16") != 2, op, ": dres16 must be bf16 or fp16");
   check_mat(dres16, dres16.scalar_type(), M, H, dev, op, "dres16");
   check_vec(dgamma, H, dev, op, "dgamma");

@@ -271,6 +271,9 @@ def test_refusals():
             lambda: ln(x[:, :128], w[:128], w[:128]), lambda: ln(x, w.half(), w),
             lambda: bw(x, q, e, r[:3], w, w, x, x, x16, w, w), lambda: bw(x16, q, e, r, w, w, x, x, x16, w, w),
             lambda: bw(x, q, e, r, w, w, x, x, x, w, w), lambda: bw(x[:3], q, e, r, w, w, x, x, x16, w, w),
+            lambda: bw(x, q, e, r, w, w, x, torch.zeros(2048, device="cuda")[:1024].view(4, 256).t().contiguous().t(), x16, w, w),
+            lambda: (lambda z: bw(x, q, e, r, w, w, z[:1024].view(4, 256), z[4:1028].view(4, 256), x16, w, w))(
+                torch.zeros(1100, device="cuda")),  # dres overlaps dres_in, shifted
             lambda: bw(x, q, e, r, w, w, x, x, x16, w, w.half()), lambda: bw(x, q, e, r, w, w, x, x[:, 1:], x16, w, w),
             lambda: bw(x, q, e, r, w, w, x, x, x16, w[:128], w),
     ):
