@@ -23,9 +23,8 @@ namespace hb {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kCtasPerSm = 2;
+constexpr int kThreadsPerSm = 512;  // of the row kernel: 128 registers each
+constexpr int kCtasPerSm = 2;  // where two CTAs' shares fit an SM's shared memory; else one has all the threads
 constexpr int kUnroll = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -106,7 +105,10 @@ __device__ __forceinline__ void copy_piece(uint32_t smem, const void* gmem) {
 }
 __device__ __forceinline__ uint4 read_piece(uint32_t smem) {
   uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(smem) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(smem)
+               : "memory");
   return r;
 }
 // Waits for all of this thread's copies.
@@ -168,7 +170,7 @@ enum Mode : int { kLogp = 0, kUnit = 1, kPolicy = 2 };
 
 // How the rows are dealt out: clusters of `split` CTAs, each CTA holding `pieces` 16-byte pieces of a row.
 struct Deal {
-  int split, pieces, clusters;
+  int split, pieces, clusters, threads;
   int window, list;  // rows scanned at a time, and the entries of the list of a cluster's rows among them
   bool aligned;    // every row of the logits starts on a 16-byte boundary
   bool vec_store;  // rows of grad start at the same offset from a 16-byte boundary as those of the logits
@@ -190,11 +192,14 @@ struct Deal {
 // also for logits far from 0, and finite for masks of the type's lowest value.
 // So a row crosses DRAM once each way. Rows may start at any element: the columns before the first 16-byte
 // boundary (`head`, fewer than one piece) are read by single threads of the first CTA.
-template <int TYPE, int MODE>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+// Measured: 8192 x 50257 bf16 with a quarter of the rows ignored, 258 us: 1.44 GB, 5.6 TB/s (a copy reaches 6.4);
+// without a gradient 115 us (5.4 TB/s). What is left is instruction issue: about 12 instructions an element and
+// pass, half of them arithmetic; the transcendental unit is half busy.
+template <int TYPE, int MODE, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreadsPerSm / kThreads)
     logit_rows_kernel(const LogitRows a, const PolicyTerms p, const Deal d, double* __restrict__ part) {
   using P = Piece<TYPE>;
-  constexpr int E = P::kElems;
+  constexpr int E = P::kElems, kWarps = kThreads / 32;
   extern __shared__ uint4 slots[];
   __shared__ float sm_s[2][kWarps], xch[2][8], slow_m[kWarps], slow_s[kWarps], slow_x[8][2];
   __shared__ int sm_n[kWarps];
@@ -253,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if constexpr (MODE != kLogp) {
       char* out = static_cast<char*>(a.grad) + (long)row * a.gld * P::kBytes;
       const int lo = min(piece0 * E, a.W), hi = min((piece0 + d.pieces) * E, a.W);
-      const int lead = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(out + (long)lo * P::kBytes) & 15u)) & 15u) / P::kBytes;
+      const auto start = reinterpret_cast<uintptr_t>(out + (long)lo * P::kBytes);
+      const int lead = static_cast<int>((16u - (start & 15u)) & 15u) / P::kBytes;
       const int body = min(lo + lead, hi), n = (hi - body) / E;
       if (tid < body - lo) store1<TYPE>(out, lo + tid, 0.f);
       uint4* to = reinterpret_cast<uint4*>(out + (long)body * P::kBytes);
@@ -276,7 +282,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     for (int i = lo; i < hi; i += 32 * kBatch) {
       int64_t t[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) t[k] = i + 32 * k + lane < hi ? a.targets[w0 + i + 32 * k + lane] : a.ignore_index;
+      for (int k = 0; k < kBatch; ++k) {
+        const int at = i + 32 * k + lane;
+        t[k] = at < hi ? a.targets[w0 + at] : a.ignore_index;
+      }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) c += t[k] != a.ignore_index;
     }
@@ -293,7 +302,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     for (int i = lo; i < hi; i += 32 * kBatch) {
       int64_t t[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) t[k] = i + 32 * k + lane < hi ? a.targets[w0 + i + 32 * k + lane] : a.ignore_index;
+      for (int k = 0; k < kBatch; ++k) {
+        const int at = i + 32 * k + lane;
+        t[k] = at < hi ? a.targets[w0 + at] : a.ignore_index;
+      }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int at = i + 32 * k + lane;
@@ -537,7 +549,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           const int lo = rank == 0 ? 0 : cur.head + piece0 * E;
           const int hi = min(a.W, cur.head + (piece0 + d.pieces) * E);
           for (int j = lo + tid; j < hi; j += kThreads) {
-            const float g = j < a.V ? coef * ((j == tc ? 1.f : 0.f) - ex2(fmaf(load1<TYPE>(cur.base, j) - m, kLog2e, -log2s))) : 0.f;
+            float g = 0.f;
+            if (j < a.V) {
+              const float pj = ex2(fmaf(load1<TYPE>(cur.base, j) - m, kLog2e, -log2s));
+              g = coef * ((j == tc ? 1.f : 0.f) - pj);
+            }
             store1<TYPE>(out, j, g);
           }
         } else if (tc >= 0 && !zero) {
@@ -672,7 +688,8 @@ __global__ void __launch_bounds__(kPrefThreads) preference_kernel(const Preferen
       // sigmoid(|z|) and sigmoid(-|z|) from e = e^-|z|, which cannot overflow
       const double e = exp(-fabs(z)), big = 1.0 / (1.0 + e), small = e * big;
       const double sig = z >= 0.0 ? big : small, sig_neg = z >= 0.0 ? small : big;
-      const float c = static_cast<float>(z != z ? z : a.beta / a.P * (a.smoothing * sig - (1.0 - a.smoothing) * sig_neg));
+      const double dz = a.smoothing * sig - (1.0 - a.smoothing) * sig_neg;  // dloss / dz
+      const float c = static_cast<float>(z != z ? z : a.beta / a.P * dz);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const long base = ((long)pair + (long)h * a.P) * a.T;
@@ -739,6 +756,9 @@ constexpr int kMaxSplit = 8;
 // time, rounds * (fixed cost of a row + its bytes, both ways, at an SM's share of the memory rate). It goes by the
 // logits alone, with or without a gradient, so equal logits give equal bits in all three losses (the order of a
 // row's sum goes by the split): a policy step on the tokens it has just scored starts at ratios of exactly 1.
+// Measured (policy loss, 50257 columns, bf16; split 1 / 2 / 4 / 8): 16 rows 12.7 / 10.7 / 10.0 / 8.7 us, 61 rows 12.6 /
+// 10.6 / 10.6 / 16.7, 500 rows 25 / 27 / 49 / 74, 4096 rows 135 / 156 / 354 / 571. A CTA that has an SM for itself gets the
+// threads of two: 131072 columns, 4096 rows 393 us with 512 threads, 412 with 256.
 Deal deal_rows(int M, long row_pieces, int sms) {
   Deal best{};
   double least = 0.0;
@@ -755,6 +775,7 @@ Deal deal_rows(int M, long row_pieces, int sms) {
       best.split = c;
       best.pieces = static_cast<int>(pieces);
       best.clusters = clusters;
+      best.threads = kThreadsPerSm / resident;
       best.window = static_cast<int>(std::min<long>(M, (long)clusters * kListRows));
       // ceil(counted / clusters) + ceil(ignored / clusters) entries at most
       best.list = (best.window + clusters - 1) / clusters + 1;
@@ -763,9 +784,9 @@ Deal deal_rows(int M, long row_pieces, int sms) {
   return best;
 }
 
-template <int TYPE, int MODE>
+template <int TYPE, int MODE, int THREADS>
 void launch_typed(const LogitRows& a, const PolicyTerms& p, const Deal& d, double* part, cudaStream_t s) {
-  auto* k = logit_rows_kernel<TYPE, MODE>;
+  auto* k = logit_rows_kernel<TYPE, MODE, THREADS>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
   const int dev = current_device();
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
@@ -774,7 +795,7 @@ void launch_typed(const LogitRows& a, const PolicyTerms& p, const Deal& d, doubl
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(d.clusters * d.split));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = static_cast<size_t>(d.pieces) * 16 + static_cast<size_t>(d.list) * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -789,9 +810,14 @@ void launch_typed(const LogitRows& a, const PolicyTerms& p, const Deal& d, doubl
 template <int MODE>
 void launch_rows(const LogitRows& a, const PolicyTerms& p, const Deal& d, double* part, cudaStream_t s) {
   if (a.M == 0) return;
-  if (a.type == kLogitF32) launch_typed<kLogitF32, MODE>(a, p, d, part, s);
-  else if (a.type == kLogitF16) launch_typed<kLogitF16, MODE>(a, p, d, part, s);
-  else launch_typed<kLogitBf16, MODE>(a, p, d, part, s);
+#define HB_ROWS(T)                                                      \
+  (d.threads == kThreadsPerSm ? launch_typed<T, MODE, kThreadsPerSm>    \
+                              : launch_typed<T, MODE, kThreadsPerSm / kCtasPerSm>)
+  auto* launch = a.type == kLogitF32   ? HB_ROWS(kLogitF32)
+                 : a.type == kLogitF16 ? HB_ROWS(kLogitF16)
+                                       : HB_ROWS(kLogitBf16);
+#undef HB_ROWS
+  launch(a, p, d, part, s);
 }
 
 Deal deal_of(const LogitRows& a) {

@@ -185,7 +185,8 @@ def _norm_bwd_act8(ln, norm, dxn: torch.Tensor, dres: torch.Tensor, dres16: torc
 
 
 def _mlp_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor):
-    """``_mlp_bwd`` from 8-bit state. The gradients of c_fc's weight come last: their operand leaves the LayerNorm backward."""
+    """``_mlp_bwd`` from 8-bit state. The gradient of c_fc's weight comes last: its operand leaves the LayerNorm
+    backward."""
     mlp = blk.mlp
     pre8, d = saved.rest
     dout16 = K.dropout_bf16(dres, d[0], 4 * d[1] + 2, d[2], dtype=dres16.dtype) if d else dres16

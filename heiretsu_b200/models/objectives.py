@@ -31,7 +31,8 @@ def _fused(model, idx: torch.Tensor) -> bool:
     if not (model.fused and idx.is_cuda):
         return False
     if getattr(getattr(model, "topo", None), "tp", 1) > 1:
-        raise ValueError("post-training objectives on the fused engine need tp 1 (tensor parallelism: the plain engine)")
+        raise ValueError("post-training objectives on the fused engine need tp 1 (the plain engine runs them with tensor "
+                         "parallelism)")
     return True
 
 
@@ -194,7 +195,7 @@ def preference_loss_plain(logp, targets, ref_logp, beta, label_smoothing):
 
 # ---- entry points ----------------------------------------------------------------------
 def token_logprobs(model, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """Log-probability of ``targets`` [B, T] at every position, fp32 [B, T], differentiable; 0 where the target is -100."""
+    """Log-probability of ``targets`` [B, T] at every position: fp32 [B, T], differentiable, 0 where the target is -100."""
     _check(idx, targets)
     fused = _fused(model, idx)
     x, _ = _trunk(model, idx, fused)
@@ -206,8 +207,9 @@ def token_logprobs(model, idx: torch.Tensor, targets: torch.Tensor) -> torch.Ten
 def policy_loss(model, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                 ref_logp: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_coef: float = 0.0):
-    """Clipped policy loss with a KL term (formula: ``ops.kernels.policy_loss``): (loss, aux loss, stats [2], logp [B, T]).
+    """Clipped policy loss with a KL term (formula: ``ops.kernels.policy_loss``).
 
+    Returns (loss, aux loss, stats [2], logp [B, T]).
     ``old_logp``, ``ref_logp`` and ``weights`` [B, T]; ``advantages`` [B, T], or [B]: one per sequence. Tokens whose
     target is -100 take no part. ``stats`` = (weighted KL to the reference, weighted share of clipped tokens)."""
     _check(idx, targets, old_logp=old_logp, ref_logp=ref_logp, weights=weights)
@@ -218,10 +220,12 @@ def policy_loss(model, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch
     if fused:
         loss, stats, logp = _HeadPolicy.apply(
             *_head_args(model, x, targets), _flat32(old_logp), _flat32(advantages), _flat32(ref_logp), _flat32(weights),
-            clip_low, clip_high, kl_coef, getattr(model, "loss_grad_hint", 1.0), getattr(model, "loss_grad_scale", None))
+            clip_low, clip_high, kl_coef, getattr(model, "loss_grad_hint", 1.0),
+            getattr(model, "loss_grad_scale", None))
         return loss, aux, stats, logp.view(idx.shape)
     logp = _logp_plain(model, x, targets)
-    loss, stats = policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef)
+    loss, stats = policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high,
+                                    kl_coef)
     return loss, aux, stats, logp.detach()
 
 

@@ -103,9 +103,10 @@ def token_logprobs(logits: torch.Tensor, V: int, targets: torch.Tensor, ignore_i
     ``logits`` [M, >= V] in bf16, fp16 or fp32 with contiguous rows (any row stride, any alignment), ``targets``
     int64 [M]. Rows whose target is ``ignore_index`` give 0 in both, whatever they hold; a target outside [0, V) gives
     NaN and the bad-argument status. V is limited by shared memory (about 920,000 in 16 bits, 460,000 in fp32).
-    Equal logits (and shapes) give equal bits here, with ``grad``, and in ``policy_loss``. ``grad`` (a buffer like ``logits``, or ``logits`` itself: in place) receives
-    the gradient of each row's log-probability, onehot - softmax, zero in ignored rows and in columns >= V: the
-    gradient of any loss of the log-probabilities is this with row i times dloss/dlogp[i]."""
+    Equal logits (and shapes) give equal bits here, with ``grad``, and in ``policy_loss``. ``grad`` (a buffer like
+    ``logits``, or ``logits`` itself: in place) receives the gradient of each row's log-probability, onehot - softmax,
+    zero in ignored rows and in columns >= V: the gradient of any loss of the log-probabilities is this with row i
+    times dloss/dlogp[i]."""
     return _ext().token_logprobs(logits, V, targets, ignore_index, grad)
 
 

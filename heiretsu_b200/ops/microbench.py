@@ -245,7 +245,66 @@ def bench_ce(flush):
                  gbs=2 * M * Vp * 2 / ts / 1e6)]
 
 
-EXTRA_BENCHES = {"attention": bench_attention, "norm": bench_norm, "ce": bench_ce}
+def bench_post(flush):
+    """Post-training losses on [M, 50304] bf16 logits (every row counted) and the preference loss on 64 pairs; gbs
+    counts the inputs read once and the outputs written once."""
+    from . import kernels as K
+    from ._C import check_status
+
+    rows = []
+    V, Vp = 50257, 50304
+    for M in (16, 2048):
+        logits = torch.zeros(M, Vp, device="cuda", dtype=torch.bfloat16)
+        logits[:, :V] = 2 * torch.randn(M, V, device="cuda")
+        t = torch.randint(0, V, (M,), device="cuda")
+        old, _ = K.token_logprobs(logits, V, t)
+        adv, grad = torch.randn(M, device="cuda"), torch.empty_like(logits)
+        for name, dirs, fn in (
+                ("logprobs", 1, lambda: K.token_logprobs(logits, V, t)),
+                ("logprobs+grad", 2, lambda: K.token_logprobs(logits, V, t, grad=grad)),
+                ("policy", 2, lambda: K.policy_loss(logits, V, t, old, adv, ref_logp=old, kl_coef=0.1, grad=grad))):
+            ms = time_fn(fn, flush=flush)
+            rows.append(dict(op="post", name=f"{name} {M}x{V}", ms=ms, gbs=dirs * M * V * 2 / ms / 1e6))
+    lp = -torch.rand(128, 1024, device="cuda")
+    t = torch.randint(0, V, (128, 1024), device="cuda")
+    ms = time_fn(lambda: K.preference_loss(lp, t, ref_logp=lp), flush=flush)
+    rows.append(dict(op="post", name="preference 64x1024", ms=ms, gbs=lp.numel() * 20 / ms / 1e6))
+    check_status()
+    return rows
+
+
+def bench_act8(flush):
+    """8-bit activations of [8192, 5120] bf16, and the 8-bit LayerNorm at [8192, 1280] against the 16-bit one (ref_ms)."""
+    from . import kernels as K
+    from ._C import check_status
+
+    M, H = 8192, 1280
+    x, dy, dres = (torch.randn(M, H, device="cuda") for _ in range(3))
+    w, b = torch.randn(H, device="cuda"), torch.randn(H, device="cuda")
+    d16 = torch.empty(M, H, device="cuda", dtype=torch.bfloat16)
+    dg, db = torch.zeros(2, H, device="cuda").unbind(0)
+    pre = torch.randn(M, 4 * H, device="cuda").bfloat16()
+    q, e = K.act8_pack(pre)
+    n = pre.numel()
+    rows = []
+    for name, nbytes, fn in (("pack", 3 * n, lambda: K.act8_pack(pre)), ("unpack", 3 * n, lambda: K.act8_unpack(q, e)),
+                             ("unpack+gelu", 5 * n, lambda: K.act8_unpack_gelu(q, e))):
+        ms = time_fn(fn, flush=flush)
+        rows.append(dict(op="act8", name=f"{name} {M}x{4 * H}", ms=ms, gbs=nbytes / ms / 1e6))
+    y, mean, rstd = K.layernorm_fwd(x, w, b)
+    _, qn, en, rn = K.layernorm_fwd_act8(x, w, b)
+    ms = time_fn(lambda: K.layernorm_fwd_act8(x, w, b), flush=flush)
+    ref = time_fn(lambda: K.layernorm_fwd(x, w, b), flush=flush)
+    rows.append(dict(op="act8", name=f"layernorm fwd {M}x{H}", ms=ms, ref_ms=ref, gbs=7 * M * H / ms / 1e6))
+    ms = time_fn(lambda: K.layernorm_bwd_act8(dy, qn, en, rn, w, b, dres, dres, d16, dg, db), flush=flush)
+    ref = time_fn(lambda: K.layernorm_bwd(dy, x, mean, rstd, w, dres, dres, d16, dg, db), flush=flush)
+    rows.append(dict(op="act8", name=f"layernorm bwd {M}x{H}", ms=ms, ref_ms=ref, gbs=17 * M * H / ms / 1e6))
+    check_status()
+    return rows
+
+
+EXTRA_BENCHES = {"attention": bench_attention, "norm": bench_norm, "ce": bench_ce, "post": bench_post,
+                 "act8": bench_act8}
 
 
 def main(argv=None):
