@@ -482,6 +482,8 @@ def _gpt_forward_fused_tp(model, idx, targets):
 
     cfg, topo = model.cfg, model.topo
     B, T = idx.shape
+    if getattr(model, "act_bits", 16) != 16:
+        raise ValueError("fused tensor parallelism keeps its activations in 16 bits")
     ok, why = tp_supported(cfg, topo, B, T)
     if not ok:
         raise ValueError(f"fused tensor parallelism: {why}")

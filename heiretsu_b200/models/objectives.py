@@ -159,9 +159,11 @@ def _head_args(model, x: torch.Tensor, targets: torch.Tensor):
 # ---- formulas in PyTorch -------------------------------------------------------------
 def _logp_plain(model, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     logits = model.lm_head(model.tr.ln_f(x))
-    counts = targets != IGNORE
-    logp = F.log_softmax(logits.float(), dim=-1).gather(-1, targets.clamp_min(0)[..., None])[..., 0]
-    return torch.where(counts, logp, torch.zeros_like(logp))
+    V = logits.shape[-1]
+    counts, known = targets != IGNORE, (targets >= 0) & (targets < V)
+    logp = F.log_softmax(logits.float(), dim=-1).gather(-1, targets.clamp(0, V - 1)[..., None])[..., 0]
+    # a target that is no token gives NaN, as the kernels do
+    return torch.where(known, logp, torch.where(counts, torch.full_like(logp, float("nan")), torch.zeros_like(logp)))
 
 
 def policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef):

@@ -136,6 +136,15 @@ def test_nothing_counts():
     assert abs(loss.item() - 0.6931472) < 1e-6 and (rewards == 0).all()
 
 
+def test_targets_that_are_no_tokens_give_nan():
+    m, b = plain(torch.float32), batch()
+    tgt = b[1].clone()
+    tgt[0, 40], tgt[1, 41], tgt[2, 42] = 200, -1, IGNORE
+    lp = m.token_logprobs(b[0], tgt)
+    assert torch.isnan(lp[0, 40]) and torch.isnan(lp[1, 41]) and lp[2, 42] == 0
+    assert torch.isnan(lp).sum() == 2
+
+
 def test_refusals():
     m, b = plain(torch.float32), batch(3)
     idx, tgt, old, ref, adv = b
