@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
 
 // LayerNorm forward: one warp per row, the row in registers (V4 float4 a lane; float4 i of the 32 lanes is block i),
 // statistics in two passes over the registers, in the order of ln_fwd_kernel (norm.cu): y has the same bits, so keeping
-// activations in 8 bits leaves the forward pass as it is. 8192 x 1280: 73 MB in 16.5 us. One read of x, one write of y and of the codes.
+// activations in 8 bits leaves the forward pass as it is. One read of x, one write of y and of the codes: 8192 x 1280,
+// 73 MB in 16.5 us.
 template <int V4, bool F16>
 __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                           const float* __restrict__ b, uint16_t* __restrict__ y,
