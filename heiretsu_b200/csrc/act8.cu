@@ -248,13 +248,30 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
 // LayerNorm forward: one warp per row, the row in registers (V4 float4 a lane; float4 i of the 32 lanes is block i),
 // statistics in two passes over the registers, in the order of ln_fwd_kernel (norm.cu): y has the same bits, so keeping
 // activations in 8 bits leaves the forward pass as it is. One read of x, one write of y and of the codes: 8192 x 1280,
-// 73 MB in 16.5 us.
+// 73 MB in 19.5 us.
+// xh in 32 bits is off by up to 3 units in its last place, 4e-5 of a step, so where it lies closer than 2^-14 to the
+// middle between two codes (one value in 8000) the four codes are taken again from x, with a mean and rstd to about
+// 1e-8: 0.1 to 0.2 codes of a million then differ from those of xh in 64 bits, without it 1.5 (and 16.5 us). The
+// second look kept for the end of the row takes 22.8 us (the row read again) or 38 us (held in registers, which spill).
+constexpr float kNearTie = 0.5f - 0x1p-14f;
+__device__ __forceinline__ uint32_t ln_act8_tie(const float* __restrict__ x, double mean, double scaled) {
+  float v[4];
+  load4<kActF32>(x, 0, v);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double t = fmin(fmax((v[k] - mean) * scaled, -127.0), 127.0);
+    codes |= (static_cast<uint32_t>(__double2int_rn(t)) & 0xFFu) << (8 * k);
+  }
+  return codes;
+}
+// CTAs an SM that the registers are held to (64 a thread and 4 CTAs at 1280 columns; 80 and 3 took 20.7 us).
+constexpr int ln_fwd_ctas(int v4) { return v4 <= 2 ? 8 : v4 <= 4 ? 6 : v4 <= 6 ? 5 : v4 <= 10 ? 4 : v4 <= 12 ? 3 : 2; }
 template <int V4, bool F16>
-__global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restrict__ x, const float* __restrict__ w,
-                                                          const float* __restrict__ b, uint16_t* __restrict__ y,
-                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ e,
-                                                          float* __restrict__ rstd_out, int M, int H, int nb,
-                                                          float eps) {
+__global__ void __launch_bounds__(256, ln_fwd_ctas(V4))
+    ln_fwd_act8_kernel(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                       uint16_t* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ e,
+                       float* __restrict__ rstd_out, int M, int H, int nb, float eps) {
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= M) return;
@@ -270,15 +287,24 @@ __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restric
     s += v[i][0] + v[i][1] + v[i][2] + v[i][3];
   }
   const float mu = warp_sum(s) / H;
-  float ss = 0.f;
+  float ss = 0.f, rest = 0.f;
+  double wide = 0.0;
 #pragma unroll
   for (int i = 0; i < V4; ++i) {
     if (kAct8Block * i + 4 * lane < H) {
       const float a = v[i][0] - mu, c = v[i][1] - mu, d = v[i][2] - mu, f = v[i][3] - mu;
-      ss += a * a + c * c + d * d + f * f;
+      const float sq = a * a + c * c + d * d + f * f;
+      ss += sq;
+      wide += sq;
+      rest += (a + c) + (d + f);
     }
   }
   const float rstd = rsqrtf(warp_sum(ss) / H + eps);
+  // for the ties: what the sum of x - mu leaves of the mean, and rstd by a Newton step on the squares' 64-bit sum
+  const double part = 1.0 / H, off = warp_sum(rest) * part, mean = mu + off;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
+  const double r = rstd, rstd_wide = r * (1.5 - 0.5 * (wide * part - off * off + eps) * r * r);
   uint32_t mine = 0;  // lane i keeps the byte of block i
 #pragma unroll
   for (int i = 0; i < V4; ++i) {
@@ -292,7 +318,10 @@ __global__ void __launch_bounds__(256) ln_fwd_act8_kernel(const float* __restric
     const uint32_t byte = act8_byte(__reduce_max_sync(0xffffffffu, top));
     if (lane == i) mine = byte;
     if (j < H) {
-      *reinterpret_cast<uint32_t*>(q + base + j) = act8_codes(v[i], byte);
+      uint32_t codes = act8_codes(v[i], byte);
+      if (byte != kAct8Nan && act8_off_code(v[i], byte) > kNearTie)
+        codes = ln_act8_tie(x + base + j, mean, rstd_wide * act8_inv_scale(byte));
+      *reinterpret_cast<uint32_t*>(q + base + j) = codes;
       float ww[4], bb[4], o[4];
       load4<kActF32>(w, j, ww);
       load4<kActF32>(b, j, bb);

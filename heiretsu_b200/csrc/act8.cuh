@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t act8_codes(const float (&x)[4], uint32_t byt
   const uint32_t all = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
   return byte == kAct8Nan ? 0u : all;
 }
+// The farthest, in steps, that one of four values lies from its code (at most 1/2).
+__device__ __forceinline__ float act8_off_code(const float (&x)[4], uint32_t byte) {
+  const float inv = act8_inv_scale(byte);
+  float off = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = __fmul_rn(x[i], inv);
+    off = fmaxf(off, fabsf(t - (__fadd_rn(t, 12582912.f) - 12582912.f)));
+  }
+  return off;
+}
 // Their values. A byte, with its sign bit flipped, is code + 128; put under the exponent of 2^23 it reads as the
 // number 2^23 + 128 + code, so one byte permutation and one subtraction give the code as a float.
 __device__ __forceinline__ void act8_values(uint32_t codes, float scale, float (&v)[4]) {
