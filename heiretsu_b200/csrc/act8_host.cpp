@@ -155,6 +155,8 @@ at::Tensor layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const a
   TORCH_CHECK(aligned16(dy) && aligned16(q) && aligned16(w) && aligned16(b) && aligned16(dres_in) && aligned16(dres) &&
                   aligned16(dres16),
               op, ": every matrix must start on a 16-byte boundary");
+  const auto gamma = reinterpret_cast<uintptr_t>(dgamma.data_ptr()), beta = reinterpret_cast<uintptr_t>(dbeta.data_ptr());
+  TORCH_CHECK(gamma + H * 4 <= beta || beta + H * 4 <= gamma, op, ": dgamma and dbeta must not overlap");
   at::Tensor y = at::empty({M, H}, dres16.options()), scratch = at::empty({ctas * 2 * H}, dy.options());
   ln_bwd_act8_launch(dy.data_ptr<float>(), q.data_ptr<int8_t>(), e.data_ptr<uint8_t>(), rstd.data_ptr<float>(),
                      w.data_ptr<float>(), b.data_ptr<float>(), dres_in.data_ptr<float>(), dres.data_ptr<float>(),

@@ -285,3 +285,14 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
     status_ok()
+
+
+def test_backward_refuses_one_buffer_for_both_parameter_gradients():
+    x, w, b, g = ln_inputs(4, 256)
+    _, q, e, r = K().layernorm_fwd_act8(x, w, b)
+    dres, d16, sums = torch.zeros_like(x), x.bfloat16(), torch.zeros(512, device="cuda")
+    for dg, db in ((sums[:256], sums[:256]), (sums[:256], sums[128:384]), (sums[200:456], sums[:256])):
+        with pytest.raises(RuntimeError, match="dgamma and dbeta"):
+            K().layernorm_bwd_act8(x, q, e, r, w, b, dres, dres, d16, dg, db)
+    K().layernorm_bwd_act8(x, q, e, r, w, b, dres, dres, d16, sums[256:], sums[:256])  # next to each other
+    status_ok()
