@@ -76,6 +76,24 @@ def test_strided_rows(dt):
     status_ok()
 
 
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("M,N", [(1, 128), (3, 128), (17, 384), (1001, 640), (64, 5120)])
+def test_contiguous_and_strided_rows_give_the_same_codes(M, N, dt):
+    """Whole blocks without a gap between rows are packed as one row; with a gap, or from an odd start, row by row."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    x = (torch.randn(M, N, device="cuda", generator=g) * torch.exp2(torch.randint(-12, 8, (M, 1), device="cuda", generator=g))).to(dt)
+    x[M // 2, N - 1] = float("nan")
+    x[M - 1, 0] = float("-inf")
+    q, e = K().act8_pack(x)
+    same_codes(x, q, e)
+    for off, ld in ((0, N + 8), (1, N + 3)):
+        wide = torch.full((M, ld), 1e4, device="cuda", dtype=dt)
+        wide[:, off:off + N] = x
+        q2, e2 = K().act8_pack(wide[:, off:off + N])
+        assert torch.equal(q, q2) and torch.equal(e, e2)
+    status_ok()
+
+
 def test_extreme_values():
     for dt in (BF16, FP16, FP32):
         fi = torch.finfo(dt)
