@@ -108,8 +108,9 @@ def _dropout_of(blk):
 # Activations kept in 8 bits (``act_bits`` 8): what backward needs of a sub-layer is kept as 8-bit codes with a
 # power-of-two scale per 128 columns (csrc/act8.cuh). A dense block keeps per token: the normalised input of both
 # LayerNorms (which gives both the LayerNorm backward and, times gamma plus beta, the operand of the weight gradient
-# behind it), Q/K/V, the attention output and the MLP pre-activation (GELU is evaluated again): about 10 H bytes
-# instead of 36 H, without re-running the forward. Backward restores each where it is used; the forward is exact.
+# behind it), Q/K/V (the attention, without its projections, runs again on the restored ones), the attention output and
+# the MLP pre-activation (GELU is evaluated again): about 10 H bytes instead of 36 H, without re-running the GEMMs.
+# Backward restores each where it is used; the forward is exact.
 class _Act8:
     """Saved state of a sub-layer in 8 bits."""
 
@@ -139,7 +140,7 @@ def _attn_fwd(blk, x: torch.Tensor, B: int, T: int, keep: bool, act8: bool = Fal
     x1 = G.linear_fwd_resid(y, attn.c_proj.weight.w16, attn.c_proj.bias, x,
                             drop=(d[0], 4 * d[1] + 1, d[2], 0) if d else None)
     if act8:
-        return x1, _Act8(norm, K.act8_pack(qkv), K.act8_pack(y), lse, d)
+        return x1, _Act8(norm, K.act8_pack(qkv), K.act8_pack(y), d)
     return x1, ((x, xn, *norm, qkv, y, lse, d) if keep else None)
 
 
@@ -204,9 +205,12 @@ def _mlp_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor):
 
 
 def _attn_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor, B: int, T: int):
-    """``_attn_bwd`` from 8-bit state."""
+    """``_attn_bwd`` from 8-bit state. The attention runs again on the restored Q/K/V: its backward evaluates
+    P = exp(s - lse) and D = dy.y, which is the softmax's derivative only when lse and y are those of the same scores.
+    With the forward's, a score off by ds would leave rows of P that sum to e^ds and rows of dS that do not sum to 0,
+    which an offset common to a K channel multiplies. The kept y is the operand of c_proj's weight gradient."""
     attn = blk.attn
-    qkv8, y8, lse, d = saved.rest
+    qkv8, y8, d = saved.rest
     dout16 = K.dropout_bf16(dres, d[0], 4 * d[1] + 1, d[2], dtype=dres16.dtype) if d else dres16
     dy = G.linear_dgrad(dout16, attn.c_proj.weight.w16)
     y = K.act8_unpack(*y8, dtype=dres16.dtype)
@@ -215,8 +219,9 @@ def _attn_bwd_act8(blk, saved: _Act8, dres: torch.Tensor, dres16: torch.Tensor, 
     del dout16
     qkv = K.act8_unpack(*qkv8, dtype=dres16.dtype)
     adrop = (d[0], 4 * d[1], d[2], 0, attn.nh_tp) if d else None
+    y, lse = K.attention_fwd(qkv, B, T, attn.nh_tp, out=y, drop=adrop, head_dim=attn.dh)
     dqkv = K.attention_bwd(qkv, y, dy, lse, B, T, attn.nh_tp, drop=adrop, head_dim=attn.dh)
-    del dy, y, qkv
+    del dy, y, lse, qkv
     dxn = G.linear_dgrad(dqkv, attn.c_attn.weight.w16, f32=True)
     xn = _norm_bwd_act8(blk.ln_1, saved.norm, dxn, dres, dres16)
     del dxn

@@ -114,3 +114,18 @@ def gelu(x):
     """0.5 x (1 + tanh u) as x sigmoid(2u): the sum 1 + tanh u keeps no digit in 64 bits below u = -18."""
     x = x.double()
     return x * torch.sigmoid(2 * 0.7978845608028654 * (x + 0.044715 * x ** 3))
+
+
+def attention_grad(qkv, dout, B, T, nh, dh, mask=None):
+    """Gradient [B T, 3 nh dh] of causal softmax attention in 64 bits, by the formula: with P the softmax and y = (m P) V,
+    dP = m dy V^T, dS = P (dP - sum P dP). ``mask`` [B, nh, T, T]: the dropout factors m."""
+    q, k, v = qkv.double().view(B, T, 3, nh, dh).permute(2, 0, 3, 1, 4).unbind(0)
+    do = dout.double().view(B, T, nh, dh).transpose(1, 2)
+    s = q @ k.transpose(-1, -2) / dh ** 0.5
+    s = s.masked_fill(torch.ones(T, T, dtype=torch.bool, device=s.device).triu(1), float("-inf"))
+    p = torch.softmax(s, -1)
+    m = torch.ones_like(p) if mask is None else mask.double()
+    dp = m * (do @ v.transpose(-1, -2))
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) / dh ** 0.5
+    d = torch.stack([ds @ k, ds.transpose(-1, -2) @ q, (m * p).transpose(-1, -2) @ do])
+    return d.permute(1, 3, 0, 2, 4).reshape(B * T, 3 * nh * dh)
