@@ -96,14 +96,17 @@ class _HeadLogp(torch.autograd.Function):
         xn, mean, rstd, logits = _logits(x, ln_w, ln_b, wte, V)
         logp, _ = K.token_logprobs(logits, V, targets, grad=logits if with_grad else None)
         if with_grad:
-            ctx.save_for_backward(x, xn, mean, rstd, logits)
+            ctx.save_for_backward(x, xn, mean, rstd, logits, targets)
             ctx.params, ctx.V = (ln_w, ln_b, wte), V
         return logp
 
     @staticmethod
     def backward(ctx, dlogp):
-        x, xn, mean, rstd, unit = ctx.saved_tensors
-        dx = _head_grads(unit, ctx.V, xn, x, mean, rstd, *ctx.params, rows=dlogp.float().contiguous())
+        x, xn, mean, rstd, unit, targets = ctx.saved_tensors
+        # an ignored row's log-probability is the constant 0, whatever comes for it: the derivative of sqrt(-logp) or
+        # log(-logp) is infinite there, and 0 times infinity would reach every parameter
+        rows = torch.where(targets != IGNORE, dlogp.float(), 0.0)
+        dx = _head_grads(unit, ctx.V, xn, x, mean, rstd, *ctx.params, rows=rows)
         return dx, None, None, None, None, None, None
 
 
