@@ -7,7 +7,9 @@ term, and a preference loss on pairs (the reference trains on next-token cross-e
 * log-probabilities with a gradient: one pass over the 16-bit logits writes logp and, in place, the unit gradient
   G = onehot - softmax. Whatever loss the caller builds, its gradient in the logits is diag(dlogp) G, and the factor
   goes to the small operands: d(hidden) = diag(dlogp) (G W) and dW = G^T (diag(dlogp) hidden), so the logits are not
-  read a third time. Scoring without a gradient (a reference model, sampled tokens) only reads them;
+  read a third time. In fp16, whose range does not hold G (a probability below 2^-25 is 0) nor dlogp times the hidden
+  states under a loss scale, the gradient is formed in backward, dlogp and with it the loss scale included. Scoring
+  without a gradient (a reference model, sampled tokens) only reads the logits;
 * the policy loss is a function of each token alone, so one pass writes the loss terms and the complete gradient;
 * the preference loss sums log-probabilities over sequences first and runs on them.
 
@@ -94,19 +96,25 @@ class _HeadLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ln_w, ln_b, wte, targets, V, with_grad):
         xn, mean, rstd, logits = _logits(x, ln_w, ln_b, wte, V)
-        logp, _ = K.token_logprobs(logits, V, targets, grad=logits if with_grad else None)
+        ctx.unit = logits.dtype != torch.float16
+        logp, _ = K.token_logprobs(logits, V, targets, grad=logits if with_grad and ctx.unit else None)
         if with_grad:
-            ctx.save_for_backward(x, xn, mean, rstd, logits, targets)
+            ctx.save_for_backward(x, xn, mean, rstd, logits, targets, logp)
             ctx.params, ctx.V = (ln_w, ln_b, wte), V
         return logp
 
     @staticmethod
     def backward(ctx, dlogp):
-        x, xn, mean, rstd, unit, targets = ctx.saved_tensors
+        x, xn, mean, rstd, dl, targets, logp = ctx.saved_tensors
         # an ignored row's log-probability is the constant 0, whatever comes for it: the derivative of sqrt(-logp) or
         # log(-logp) is infinite there, and 0 times infinity would reach every parameter
         rows = torch.where(targets != IGNORE, dlogp.float(), 0.0)
-        dx = _head_grads(unit, ctx.V, xn, x, mean, rstd, *ctx.params, rows=rows)
+        if not ctx.unit:
+            # the policy loss of the model against itself has ratios of exactly 1: its gradient at advantage 1 and
+            # weight -dlogp is that of sum dlogp logp
+            K.policy_loss(dl, ctx.V, targets, logp, torch.ones(1, device=dl.device), weights=-rows, grad=dl)
+            rows = None
+        dx = _head_grads(dl, ctx.V, xn, x, mean, rstd, *ctx.params, rows=rows)
         return dx, None, None, None, None, None, None
 
 

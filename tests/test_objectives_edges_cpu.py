@@ -34,3 +34,55 @@ def test_a_loss_of_the_square_root(monkeypatch):
     got = grads(m, loss[0])
     for n, q in p.named_parameters():
         assert (got[n] - q.grad).norm() <= 5e-2 * q.grad.norm() + 1e-8, n
+
+
+def _spread_head(device, amp, M=64, H=128, V=384):
+    """(arguments of the log-probability head, weight): half of the tokens' logits lie about 17 below the others', so that
+    their probabilities are 1e-10 to 1e-8."""
+    g = torch.Generator().manual_seed(2)
+    u = torch.randn(H, generator=g).sign()
+    w = 0.05 * torch.randn(V, H, generator=g)
+    w[V // 2:] -= 0.19 * u
+    w, x = w.to(device), (torch.randn(M, H, generator=g) + u).to(device).requires_grad_(True)
+    wte, ln_w, ln_b = (torch.nn.Parameter(t) for t in (w, torch.ones(H, device=device), torch.zeros(H, device=device)))
+    for p in (wte, ln_w, ln_b):
+        p.main_grad = torch.zeros_like(p)
+    wte.w16 = w.to(amp)
+    tgt = torch.randint(0, V // 2, (M,), generator=g).to(device)
+    tgt[::7] = IGNORE
+    return (x, ln_w, ln_b, wte, tgt, V, True), wte
+
+
+def fp16_range(device, amp):
+    """(gradient of the head's weight, that of the formula on the same 16-bit operands, loss scale, probabilities)."""
+    from heiretsu_b200.models.objectives import _HeadLogp
+
+    scale = 65536.0
+    args, wte = _spread_head(device, amp)
+    x, tgt, V = args[0], args[4], args[5]
+    logp = _HeadLogp.apply(*args)
+    rows = torch.where(tgt != IGNORE, 0.4, 0.0) * scale
+    logp.backward(rows)
+    xn = torch.nn.functional.layer_norm(x.detach(), x.shape[1:]).to(amp).double()
+    p = torch.softmax((xn @ wte.w16.double().t()).to(amp).double(), 1)
+    one = torch.nn.functional.one_hot(tgt.clamp_min(0), V)
+    return wte.main_grad.double() / scale, ((rows[:, None].double() * (one - p)).t() @ xn) / scale, p
+
+
+def check_fp16_range(got, want, p):
+    """Every token's row, those of probability 1e-9 too. Errors: half a step of the logits (2^-11 of up to 32, or two steps
+    where 32-bit sums and the 64-bit one round apart) in p; half a step of the products, 2^-25 absolute where they are
+    subnormal: next to 65536 * 0.4 * 1e-9 = 2.6e-5 that is 0.1%."""
+    assert torch.isfinite(got).all()
+    rare = p.amax(0) < 3e-8
+    assert rare.sum() > 20 and (p.amax(0)[rare] > 1e-11).any()
+    seen = p.amax(0) > 1e-9
+    rel = (got - want).norm(dim=1) / want.norm(dim=1)
+    assert (rel[seen] <= 3 * 32 * 2.0 ** -11 + 0.005).all(), rel[seen].max()
+
+
+def test_fp16_probabilities_keep_their_gradient(monkeypatch):
+    """fp16 with a loss scale: dlogp 26214 times hidden states of 3 passes the type's largest value, and
+    probabilities below 2^-25 its least one; neither may lose the gradient."""
+    post_emulation.emulate(monkeypatch)
+    check_fp16_range(*fp16_range("cpu", torch.float16))

@@ -27,3 +27,13 @@ def test_a_derivative_that_is_infinite_at_ignored_tokens():
     torch.cuda.synchronize()
     check_status()
     close(grads(fz), grads(plain), 5e-2)
+
+
+def test_fp16_probabilities_keep_their_gradient():
+    from heiretsu_b200.ops._C import check_status
+    from test_objectives_edges_cpu import check_fp16_range, fp16_range
+
+    out = fp16_range("cuda", torch.float16)
+    torch.cuda.synchronize()
+    check_status()
+    check_fp16_range(*out)
