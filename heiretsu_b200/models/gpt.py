@@ -300,10 +300,11 @@ class GPT(nn.Module):
         return logits, loss, aux_total
 
     # Post-training objectives (models/objectives.py); like forward, fused where the model is.
-    def token_logprobs(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        """Log-probability of ``targets`` [B, T] (0 where -100), differentiable: fp32 [B, T]."""
+    def token_logprobs(self, idx: torch.Tensor, targets: torch.Tensor, return_aux: bool = False):
+        """Log-probability of ``targets`` [B, T] (0 where -100), differentiable: fp32 [B, T]; with ``return_aux``
+        (log-probabilities, aux loss)."""
         from .objectives import token_logprobs
-        return token_logprobs(self, idx, targets)
+        return token_logprobs(self, idx, targets, return_aux)
 
     def policy_loss(self, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                     ref_logp: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,

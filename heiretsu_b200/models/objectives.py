@@ -207,14 +207,19 @@ def preference_loss_plain(logp, targets, ref_logp, beta, label_smoothing):
 
 
 # ---- entry points ----------------------------------------------------------------------
-def token_logprobs(model, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-    """Log-probability of ``targets`` [B, T] at every position: fp32 [B, T], differentiable, 0 where the target is -100."""
+def token_logprobs(model, idx: torch.Tensor, targets: torch.Tensor, return_aux: bool = False):
+    """Log-probability of ``targets`` [B, T] at every position: fp32 [B, T], differentiable, 0 where the target is -100.
+
+    ``return_aux``: (log-probabilities, aux loss). A mixture-of-experts model that trains on a loss built from them adds
+    the aux loss to it, as the other objectives' callers do: without it the routers' load is not balanced."""
     _check(idx, targets)
     fused = _fused(model, idx)
-    x, _ = _trunk(model, idx, fused)
+    x, aux = _trunk(model, idx, fused)
     if fused:
-        return _HeadLogp.apply(*_head_args(model, x, targets)).view(idx.shape)
-    return _logp_plain(model, x, targets)
+        logp = _HeadLogp.apply(*_head_args(model, x, targets)).view(idx.shape)
+    else:
+        logp = _logp_plain(model, x, targets)
+    return (logp, aux) if return_aux else logp
 
 
 def policy_loss(model, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,

@@ -86,3 +86,23 @@ def test_fp16_probabilities_keep_their_gradient(monkeypatch):
     probabilities below 2^-25 its least one; neither may lose the gradient."""
     post_emulation.emulate(monkeypatch)
     check_fp16_range(*fp16_range("cpu", torch.float16))
+
+
+@pytest.mark.parametrize("engine", ["plain", "fused"])
+def test_balance_loss_beside_the_log_probabilities(monkeypatch, engine):
+    """A mixture-of-experts model: the aux loss of ``forward`` and the other objectives, whose gradient reaches the router."""
+    idx, tgt, old, _, adv = batch()
+    if engine == "plain":
+        m = plain(torch.float32, moe=True)
+        want = m(idx, tgt.clamp_min(0))[2]
+    else:  # dense blocks on the stand-ins: no balance loss, the same form
+        post_emulation.emulate(monkeypatch)
+        m = fused()[0]
+        want = torch.zeros(())
+    lp, aux = m.token_logprobs(idx, tgt, return_aux=True)
+    assert torch.equal(lp, m.token_logprobs(idx, tgt)) and torch.equal(aux, want)
+    assert torch.equal(aux, m.policy_loss(idx, tgt, old, adv)[1])
+    if engine == "plain":
+        routers = [p for n, p in m.named_parameters() if "router" in n or "gate" in n]
+        assert routers and aux > 0
+        assert any(g is not None and g.abs().max() > 0 for g in torch.autograd.grad(aux, routers, allow_unused=True))
