@@ -149,20 +149,26 @@ __device__ __forceinline__ RowTerm policy_term(const PolicyTerms& p, float logp,
   RowTerm t{0.f, 0.f, 0.f, 0.f};
   const float r = expf(logp - old);
   const float c = fminf(fmaxf(r, p.clip_lo), p.clip_hi);
-  const bool clipped = c * adv < r * adv;  // false for a NaN ratio, which so reaches the loss and the gradient
-  t.loss = clipped ? -c * adv : -r * adv;
-  t.coef = clipped ? 0.f : -r * adv;
+  // A ratio of infinity has overflowed 32 bits (log-ratios from 89) and stands for a finite one: an advantage, weight or
+  // KL factor of 0 takes it out. NaN stays: nothing turns a NaN log-probability into a number.
+  const float free = adv == 0.f && r == INFINITY ? 0.f : r * adv;
+  const bool clipped = c * adv < free;  // false for a NaN ratio, which so reaches the loss and the gradient
+  t.loss = clipped ? -c * adv : -free;
+  t.coef = clipped ? 0.f : -free;
   t.clipped = clipped ? w : 0.f;
   if (p.ref_logp) {
     const float u = ref - logp;
     const float e = expm1f(u);
     t.kl = e - u;
-    t.loss = fmaf(p.kl_coef, t.kl, t.loss);
-    t.coef = fmaf(-p.kl_coef, e, t.coef);
+    if (p.kl_coef != 0.f) {
+      t.loss = fmaf(p.kl_coef, t.kl, t.loss);
+      t.coef = fmaf(-p.kl_coef, e, t.coef);
+    }
   }
-  t.loss *= w;
-  t.kl *= w;
-  t.coef *= w;
+  const auto weigh = [w](float v) { return w == 0.f && fabsf(v) == INFINITY ? 0.f : w * v; };
+  t.loss = weigh(t.loss);
+  t.kl = weigh(t.kl);
+  t.coef = weigh(t.coef);
   return t;
 }
 

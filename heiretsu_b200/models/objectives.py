@@ -183,15 +183,19 @@ def policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, cl
     zero = torch.zeros_like(logp)
     w = counts / counts.sum().clamp_min(1) if weights is None else torch.where(counts, weights.float(), zero)
     adv = advantages.float() if advantages.shape == logp.shape else advantages.float()[:, None].expand_as(logp)
-    ratio = torch.exp(torch.where(counts, logp - old_logp.float(), zero))
+    # a ratio past 32 bits (log-ratios from 89) stands for a finite number, which the clip range, an advantage or a weight
+    # of 0 takes out, as in the kernel; infinity would leave NaN, here or in the exponential's derivative
+    finite = lambda d, out: torch.where(counts, torch.where(out, d.clamp(max=80), d), zero)  # noqa: E731
+    ratio = torch.exp(finite(logp - old_logp.float(), (adv >= 0) | (w == 0)))
     free, kept = ratio * adv, ratio.clamp(1 - clip_low, 1 + clip_high) * adv
     clipped = kept < free
     per = -torch.where(clipped, kept.detach(), free)
     kl = zero
     if ref_logp is not None:
-        u = torch.where(counts, ref_logp.float() - logp, zero)
+        u = finite(ref_logp.float() - logp, w == 0)
         kl = torch.expm1(u) - u
-        per = per + kl_coef * kl
+        if kl_coef != 0:
+            per = per + kl_coef * kl
     per = torch.where(counts, per, zero)
     return (w * per).sum(), torch.stack([(w * kl).sum(), (w * clipped).sum()]).detach()
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import post_emulation
+import post_oracle as O
 from test_objectives_cpu import IGNORE, batch, fused, grads, plain
 
 
@@ -106,3 +107,34 @@ def test_balance_loss_beside_the_log_probabilities(monkeypatch, engine):
         routers = [p for n, p in m.named_parameters() if "router" in n or "gate" in n]
         assert routers and aux > 0
         assert any(g is not None and g.abs().max() > 0 for g in torch.autograd.grad(aux, routers, allow_unused=True))
+
+
+def overflowing(n=24, device="cpu"):
+    """(log-probabilities, old, advantages, reference, weights): ratios and KL terms that 32 bits cannot hold, wherever the
+    clip range, an advantage or a weight of 0 takes them out of the loss."""
+    logp = torch.linspace(-9, -0.1, n, device=device)
+    old, adv, ref, w = logp - 0.05, torch.linspace(-1, 1, n, device=device), logp + 0.1, torch.full((n,), 1 / n, device=device)
+    old[3:6], adv[3:6] = -300.0, 0.0                   # no advantage
+    old[6:9], adv[6:9] = -300.0, 2.0                   # past the clip range
+    old[9:12], adv[9:12], w[9:12] = -300.0, -2.0, 0.0  # no weight
+    ref[12:15], w[12:15] = 300.0, 0.0
+    return logp, old, adv, ref, w
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+def test_policy_terms_past_32_bits(kl):
+    """Loss, statistics and gradient of the plain form against 64 bits, which hold e^300."""
+    from heiretsu_b200.models.objectives import policy_loss_plain
+
+    logp, old, adv, ref, w = (t[None] for t in overflowing())
+    if kl == 0:
+        ref[0, 15] = 300.0  # counts, in the statistic alone
+    lp = logp.clone().requires_grad_(True)
+    loss, stats = policy_loss_plain(lp, torch.zeros_like(lp).long(), old, adv, ref, w, 0.2, 0.25, kl)
+    loss.backward()
+    want, wstats, d = O.policy(logp[0], torch.ones(24, dtype=torch.bool), old[0], adv[0], ref[0], w[0], 0.2, 0.25, kl)
+    # 24 terms of at most 2, a few roundings each
+    assert abs(loss.item() - want.item()) <= 24 * 2 * 8 * 2.0 ** -24 and stats[1] == wstats[1].float()
+    assert (lp.grad[0].double() - d).abs().max() <= 8 * 2.0 ** -24 * d.abs().max()
+    if kl:
+        assert abs(stats[0].item() - wstats[0].item()) <= 1e-6

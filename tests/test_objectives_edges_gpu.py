@@ -60,3 +60,36 @@ def test_balance_loss_beside_the_log_probabilities():
     assert aux > 0 and abs(aux.item() - want.item()) <= 2.0 ** -20 * want.item()
     routers = [n for n in out[0] if "router" in n or "gate" in n]
     assert routers and all((out[1][n] - out[0][n]).norm() > 0 for n in routers)
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+def test_policy_terms_past_32_bits(kl):
+    """The kernel on ratios and KL terms that overflow 32 bits but take no part, against 64 bits."""
+    from heiretsu_b200.ops import kernels as K
+    from heiretsu_b200.ops._C import check_status
+    from post_oracle import grad_bound, logprobs, lse_bound, policy
+    from test_objectives_edges_cpu import overflowing
+
+    V, n = 1000, 24
+    _, old, adv, ref, w = overflowing(n, "cuda")
+    if kl == 0:
+        ref[15] = 300.0  # counts, in the statistic alone
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(n, V, device="cuda", generator=g)
+    t = torch.randint(0, V, (n,), device="cuda", generator=g)
+    lp64, lse64, unit = logprobs(x, V, t)
+    near = (old + 300).abs() > 1  # the others' ratios go by the log-probability
+    old = torch.where(near, (lp64 - 0.05).float(), old)
+    ref = torch.where(ref < 100, (lp64 + 0.1).float(), ref)
+    loss, stats, logp, grad = K.policy_loss(x, V, t, old, adv, ref_logp=ref, weights=w, clip_high=0.25, kl_coef=kl)
+    torch.cuda.synchronize()
+    check_status()
+    live = torch.ones(n, dtype=torch.bool, device="cuda")
+    want, wstats, d = policy(lp64, live, old, adv, ref, w, 0.2, 0.25, kl)
+    slack = 2 * lse_bound(lse64, V).max().item() + 16 * 2.0 ** -24  # of a ratio, relative
+    assert abs(loss.item() - want.item()) <= 2 * 1.3 * slack
+    assert stats[1] == wstats[1].float()
+    assert (torch.isinf(stats[0]) if kl == 0 else abs(stats[0].item() - wstats[0].item()) <= slack)
+    assert torch.isfinite(grad).all() and (grad[9:15] == 0).all()  # weight 0; the others keep their KL term
+    tol = grad_bound(d[:, None] * unit, d, x, lse64, V, x.dtype) + slack * (d[:, None] * unit).abs()
+    assert ((grad.double() - d[:, None] * unit).abs() <= tol).all()
