@@ -178,7 +178,9 @@ def _logp_plain(model, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
 
 
 def policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef):
-    """(loss, stats) of ``ops.kernels.policy_loss`` from log-probabilities [B, T], by autograd."""
+    """(loss, stats) of ``ops.kernels.policy_loss`` from log-probabilities [B, T], by autograd in them alone."""
+    old_logp, advantages, ref_logp, weights = (None if t is None else t.detach()
+                                               for t in (old_logp, advantages, ref_logp, weights))
     counts = targets != IGNORE
     zero = torch.zeros_like(logp)
     w = counts / counts.sum().clamp_min(1) if weights is None else torch.where(counts, weights.float(), zero)
@@ -201,9 +203,9 @@ def policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, cl
 
 
 def preference_loss_plain(logp, targets, ref_logp, beta, label_smoothing):
-    """(loss, rewards) of ``ops.kernels.preference_loss`` from log-probabilities [2P, T], by autograd."""
+    """(loss, rewards) of ``ops.kernels.preference_loss`` from log-probabilities [2P, T], by autograd in them alone."""
     counts = targets != IGNORE
-    diff = logp if ref_logp is None else logp - ref_logp.float()
+    diff = logp if ref_logp is None else logp - ref_logp.detach().float()
     rewards = beta * torch.where(counts, diff, torch.zeros_like(diff)).sum(1, dtype=torch.float64).view(2, -1)
     z = rewards[0] - rewards[1]
     loss = -(1 - label_smoothing) * F.logsigmoid(z) - label_smoothing * F.logsigmoid(-z)
@@ -233,7 +235,8 @@ def policy_loss(model, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch
 
     Returns (loss, aux loss, stats [2], logp [B, T]).
     ``old_logp``, ``ref_logp`` and ``weights`` [B, T]; ``advantages`` [B, T], or [B]: one per sequence. Tokens whose
-    target is -100 take no part. ``stats`` = (weighted KL to the reference, weighted share of clipped tokens)."""
+    target is -100 take no part. ``stats`` = (weighted KL to the reference, weighted share of clipped tokens).
+    All but the model is constant: no gradient goes to ``old_logp``, ``advantages``, ``ref_logp`` or ``weights``."""
     _check(idx, targets, old_logp=old_logp, ref_logp=ref_logp, weights=weights)
     if advantages.shape != idx.shape and advantages.shape != idx.shape[:1]:
         raise ValueError(f"advantages must be [B, T] or [B], got {tuple(advantages.shape)}")
@@ -256,7 +259,7 @@ def preference_loss(model, idx: torch.Tensor, targets: torch.Tensor, ref_logp: O
     """Preference loss on pairs (formula: ``ops.kernels.preference_loss``): (loss, aux loss, rewards [2, P]).
 
     ``idx`` and ``targets`` [2P, T]: P chosen sequences, then their P rejected partners; ``ref_logp`` [2P, T]: the
-    reference model's ``token_logprobs`` on the same tokens (none: a reference-free loss)."""
+    reference model's ``token_logprobs`` on the same tokens, a constant (none: a reference-free loss)."""
     _check(idx, targets, ref_logp=ref_logp)
     if idx.shape[0] % 2:
         raise ValueError(f"a preference batch holds chosen and rejected halves, got {idx.shape[0]} sequences")

@@ -138,3 +138,24 @@ def test_policy_terms_past_32_bits(kl):
     assert (lp.grad[0].double() - d).abs().max() <= 8 * 2.0 ** -24 * d.abs().max()
     if kl:
         assert abs(stats[0].item() - wstats[0].item()) <= 1e-6
+
+
+@pytest.mark.parametrize("engine", ["plain", "fused"])
+def test_only_the_model_is_differentiated(monkeypatch, engine):
+    """The first policy step may score its own tokens without no_grad: old log-probabilities, reference, advantages and
+    weights are constants on either engine, so the gradients are those of detached ones, not 0."""
+    post_emulation.emulate(monkeypatch)
+    idx, tgt, _, _, adv = batch()
+    out = []
+    for constant in (True, False):
+        m = fused()[0] if engine == "fused" else plain(torch.float32)
+        old = m.token_logprobs(idx, tgt)
+        a, w = adv.clone().requires_grad_(True), torch.full_like(adv, 0.01).requires_grad_(True)
+        given = [t.detach() if constant else t for t in (old, a, old, w)]
+        loss = m.policy_loss(idx, tgt, given[0], given[1], ref_logp=given[2], weights=given[3], kl_coef=0.1)[0]
+        loss = loss + m.preference_loss(idx, tgt, ref_logp=given[2])[0]
+        loss.backward()
+        assert a.grad is None and w.grad is None
+        out.append({n: (p.main_grad if engine == "fused" else p.grad).clone() for n, p in m.named_parameters()})
+    for n in out[0]:
+        assert out[0][n].norm() > 0 and torch.equal(out[0][n], out[1][n]), n
