@@ -173,8 +173,8 @@ def _logp_plain(model, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     V = logits.shape[-1]
     counts, known = targets != IGNORE, (targets >= 0) & (targets < V)
     logp = F.log_softmax(logits.float(), dim=-1).gather(-1, targets.clamp(0, V - 1)[..., None])[..., 0]
-    # a target that is no token gives NaN, as the kernels do
-    return torch.where(known, logp, torch.where(counts, torch.full_like(logp, float("nan")), torch.zeros_like(logp)))
+    # a target that is no token gives NaN, and so does its gradient: as with the kernels, the step is skipped
+    return torch.where(counts, logp * torch.where(counts & ~known, float("nan"), 1.0), torch.zeros_like(logp))
 
 
 def policy_loss_plain(logp, targets, old_logp, advantages, ref_logp, weights, clip_low, clip_high, kl_coef):

@@ -159,3 +159,17 @@ def test_only_the_model_is_differentiated(monkeypatch, engine):
         out.append({n: (p.main_grad if engine == "fused" else p.grad).clone() for n, p in m.named_parameters()})
     for n in out[0]:
         assert out[0][n].norm() > 0 and torch.equal(out[0][n], out[1][n]), n
+
+
+@pytest.mark.parametrize("objective", ["logp", "policy", "preference"])
+def test_a_target_that_is_no_token_gives_gradients_of_nan(objective):
+    """The plain path as the kernels: a step on such a batch is skipped for its gradient norm, not taken without the token."""
+    idx, tgt, old, ref, adv = batch()
+    tgt[0, 40] = 200
+    m = plain(torch.float32)
+    if objective == "logp":
+        loss = (m.token_logprobs(idx, tgt) * adv).sum()
+    else:
+        loss = (m.policy_loss(idx, tgt, old, adv) if objective == "policy" else m.preference_loss(idx, tgt, ref_logp=ref))[0]
+    loss.backward()
+    assert torch.isnan(loss) and torch.isnan(m.lm_head.weight.grad).any()
