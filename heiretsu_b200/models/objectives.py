@@ -18,6 +18,7 @@ parallelism shards the tokens of a batch over ranks and is refused here: use ``-
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -59,6 +60,20 @@ def _check(idx: torch.Tensor, targets: torch.Tensor, **per_token) -> None:
     for name, t in per_token.items():
         if t is not None and t.shape != idx.shape:
             raise ValueError(f"{name} must be [B, T] like idx, got {tuple(t.shape)}")
+
+
+def _check_policy(clip_low: float, clip_high: float, kl_coef: float) -> None:
+    if not (0 <= clip_low <= 1 and 0 <= clip_high < math.inf):
+        raise ValueError(f"clip_low must be in [0, 1] and clip_high finite and not negative, got {clip_low}, {clip_high}")
+    if not math.isfinite(kl_coef):
+        raise ValueError(f"kl_coef must be finite, got {kl_coef}")
+
+
+def _check_preference(beta: float, label_smoothing: float) -> None:
+    if not math.isfinite(beta):
+        raise ValueError(f"beta must be finite, got {beta}")
+    if not 0 <= label_smoothing <= 1:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
 
 
 def _flat32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -238,6 +253,7 @@ def policy_loss(model, idx: torch.Tensor, targets: torch.Tensor, old_logp: torch
     target is -100 take no part. ``stats`` = (weighted KL to the reference, weighted share of clipped tokens).
     All but the model is constant: no gradient goes to ``old_logp``, ``advantages``, ``ref_logp`` or ``weights``."""
     _check(idx, targets, old_logp=old_logp, ref_logp=ref_logp, weights=weights)
+    _check_policy(clip_low, clip_high, kl_coef)
     if advantages.shape != idx.shape and advantages.shape != idx.shape[:1]:
         raise ValueError(f"advantages must be [B, T] or [B], got {tuple(advantages.shape)}")
     fused = _fused(model, idx)
@@ -261,6 +277,7 @@ def preference_loss(model, idx: torch.Tensor, targets: torch.Tensor, ref_logp: O
     ``idx`` and ``targets`` [2P, T]: P chosen sequences, then their P rejected partners; ``ref_logp`` [2P, T]: the
     reference model's ``token_logprobs`` on the same tokens, a constant (none: a reference-free loss)."""
     _check(idx, targets, ref_logp=ref_logp)
+    _check_preference(beta, label_smoothing)
     if idx.shape[0] % 2:
         raise ValueError(f"a preference batch holds chosen and rejected halves, got {idx.shape[0]} sequences")
     fused = _fused(model, idx)

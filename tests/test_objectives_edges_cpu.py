@@ -173,3 +173,16 @@ def test_a_target_that_is_no_token_gives_gradients_of_nan(objective):
         loss = (m.policy_loss(idx, tgt, old, adv) if objective == "policy" else m.preference_loss(idx, tgt, ref_logp=ref))[0]
     loss.backward()
     assert torch.isnan(loss) and torch.isnan(m.lm_head.weight.grad).any()
+
+
+@pytest.mark.parametrize("bad", [dict(clip_low=1.5), dict(clip_low=-0.1), dict(clip_high=-0.1), dict(clip_high=float("inf")),
+                                 dict(clip_low=float("nan")), dict(kl_coef=float("inf")), dict(beta=float("nan")),
+                                 dict(label_smoothing=1.5), dict(label_smoothing=-0.5)])
+def test_numbers_the_kernels_refuse_are_refused_on_the_plain_path(bad):
+    idx, tgt, old, ref, adv = batch()
+    m = plain(torch.float32)
+    with pytest.raises(ValueError, match=next(iter(bad))):
+        if "beta" in bad or "label_smoothing" in bad:
+            m.preference_loss(idx, tgt, ref_logp=ref, **bad)
+        else:
+            m.policy_loss(idx, tgt, old, adv, ref_logp=ref, **bad)
