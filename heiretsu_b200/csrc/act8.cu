@@ -316,11 +316,14 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
 // LayerNorm forward: one warp per row, the row in registers (V4 float4 a lane; float4 i of the 32 lanes is block i),
 // statistics in two passes over the registers, in the order of ln_fwd_kernel (norm.cu): y has the same bits, so keeping
 // activations in 8 bits leaves the forward pass as it is. One read of x, one write of y and of the codes: 8192 x 1280,
-// 73 MB in 19.5 us.
-// xh in 32 bits is off by up to 3 units in its last place, 4e-5 of a step, so where it lies closer than 2^-14 to the
-// middle between two codes (one value in 8000) the four codes are taken again from x, with a mean and rstd to about
-// 1e-8: 0.1 to 0.2 codes of a million then differ from those of xh in 64 bits, without it 1.5 (and 16.5 us). The
-// second look kept for the end of the row takes 22.8 us (the row read again) or 38 us (held in registers, which spill).
+// 73 MB in 17.6 us of a graph of such calls (the 16-bit LayerNorm, 63 MB: 11.2).
+// xh in 32 bits is off by up to 3 units in its last place, 4e-5 of a step, and by the rounding of the row's mean (5e-6 of
+// a standard deviation, 2e-4 of a step, where the mean is 100 of them). So where it lies closer to the middle between
+// two codes than 2^-14 and the mean's rounding (one value in 8000 of centred rows), the four codes are taken again from
+// x, with a mean and rstd to about 1e-8: 0.1 to 0.2 codes of a million then differ from those of xh in 64 bits, without
+// it 1.5 (and 3 us less), and without the mean's part of it 46 at a mean of 100 standard deviations (0.4 us less: a
+// register spills; the mean and rstd kept in fewer registers take 18.2 us, their conversions move in front of the rows).
+// The second look kept for the end of the row takes 3 us more (the row read again) or 19 (held in registers, which spill).
 constexpr float kNearTie = 0.5f - 0x1p-14f;
 __device__ __forceinline__ uint32_t ln_act8_tie(const float* __restrict__ x, double mean, double scaled) {
   float v[4];
@@ -373,6 +376,7 @@ __global__ void __launch_bounds__(256, ln_fwd_ctas(V4))
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
   const double r = rstd, rstd_wide = r * (1.5 - 0.5 * (wide * part - off * off + eps) * r * r);
+  const float lean = fabsf(static_cast<float>(off)) * rstd;  // what the mean's rounding moves every xh by
   uint32_t mine = 0;  // lane i keeps the byte of block i
 #pragma unroll
   for (int i = 0; i < V4; ++i) {
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(256, ln_fwd_ctas(V4))
     if (lane == i) mine = byte;
     if (j < H) {
       uint32_t codes = act8_codes(v[i], byte);
-      if (byte != kAct8Nan && act8_off_code(v[i], byte) > kNearTie)
+      if (byte != kAct8Nan && fmaf(lean, act8_inv_scale(byte), act8_off_code(v[i], byte)) > kNearTie)
         codes = ln_act8_tie(x + base + j, mean, rstd_wide * act8_inv_scale(byte));
       *reinterpret_cast<uint32_t*>(q + base + j) = codes;
       float ww[4], bb[4], o[4];
