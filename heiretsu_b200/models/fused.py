@@ -26,6 +26,7 @@ add / LN / residual in fp32).
 from __future__ import annotations
 
 import os
+import warnings
 from typing import List, Optional, Tuple
 
 import torch
@@ -111,6 +112,11 @@ def _dropout_of(blk):
 # behind it), Q/K/V (the attention, without its projections, runs again on the restored ones), the attention output and
 # the MLP pre-activation (GELU is evaluated again): about 10 H bytes instead of 36 H, without re-running the GEMMs.
 # Backward restores each where it is used; the forward is exact.
+#
+# One scale serves 128 channels, so the format holds channels of like sizes: each value is off by at most 1/254 to
+# 1/127 of the largest among the 128, about 1% of a standard deviation where they are alike. A channel
+# 50 times larger leaves its 127 neighbours off by 15%, one 300 times larger by 70 to 90%, and their part of the
+# gradients with it. Trained models can have such channels; the first training forward looks for them.
 class _Act8:
     """Saved state of a sub-layer in 8 bits."""
 
@@ -118,10 +124,47 @@ class _Act8:
         self.norm, self.rest = norm, rest  # norm: (codes, exponents, rstd) of the LayerNorm
 
 
-def _norm_fwd(ln, x: torch.Tensor, dt: torch.dtype, act8: bool):
+# Channels that are off by more than this share of their root mean square count as lost, and this many of one tensor are
+# reported: half of a scale's 128, whatever the width.
+ACT8_LOST, ACT8_LOST_CHANNELS = 0.25, 64
+_ACT8_WATCH: Optional[list] = None  # (tensor's name, lost channels) of the forward that looks for them
+
+
+def _act8_watch(what: str, blk, x, codes) -> None:
+    """Notes how many channels of ``x`` (fp32 or 16-bit [M, N]; up to 512 of its rows are looked at) the codes lose."""
+    if _ACT8_WATCH is None:
+        return
+    rows = slice(None, None, max(1, codes[0].shape[0] // 256))
+    x = x(rows) if callable(x) else x[rows].float()
+    off = K.act8_unpack(codes[0][rows].contiguous(), codes[1][rows].contiguous(), dtype=torch.float32) - x
+    lost = off.square().sum(0) > ACT8_LOST ** 2 * x.square().sum(0)
+    _ACT8_WATCH.append((what, id(blk), lost.sum()))
+
+
+def _act8_pack(what: str, blk, x: torch.Tensor):
+    codes = K.act8_pack(x)
+    _act8_watch(what, blk, x, codes)
+    return codes
+
+
+def _act8_report(blocks, seen: list) -> None:
+    index = {id(b): i for i, b in enumerate(blocks)}
+    counts = torch.stack([n for _, _, n in seen]).tolist() if seen else []
+    bad = [f"block {index[b]} {what}: {n}" for (what, b, _), n in zip(seen, counts) if n >= ACT8_LOST_CHANNELS]
+    if bad:
+        more = f" and {len(bad) - 4} more" if len(bad) > 4 else ""
+        warnings.warn("activations in 8 bits: channels much larger than the others of their 128 leave those without "
+                      f"digits (channels off by more than a quarter: {', '.join(bad[:4])}{more}), and the gradients "
+                      "without their part; keep 16 bits for this model (checkpointing in 16 bits saves memory without "
+                      "loss)", stacklevel=3)
+
+
+def _norm_fwd(blk, ln, x: torch.Tensor, dt: torch.dtype, act8: bool):
     """LayerNorm forward: (y, what backward needs of it)."""
     if act8:
         y, q, e, rstd = K.layernorm_fwd_act8(x, ln.weight, ln.bias, LN_EPS, dtype=dt)
+        normed = lambda rows: torch.nn.functional.layer_norm(x[rows], x.shape[1:], eps=LN_EPS)  # noqa: E731
+        _act8_watch("LayerNorm", blk, normed, (q, e))
         return y, (q, e, rstd)
     y, mean, rstd = K.layernorm_fwd(x, ln.weight, ln.bias, LN_EPS, dtype=dt)
     return y, (mean, rstd)
@@ -133,14 +176,14 @@ def _attn_fwd(blk, x: torch.Tensor, B: int, T: int, keep: bool, act8: bool = Fal
     attn = blk.attn
     d = _dropout_of(blk)
     act8 = act8 and keep
-    xn, norm = _norm_fwd(blk.ln_1, x, _dt(blk), act8)
+    xn, norm = _norm_fwd(blk, blk.ln_1, x, _dt(blk), act8)
     qkv = G.linear_fwd(xn, attn.c_attn.weight.w16, attn.c_attn.bias)
     adrop = (d[0], 4 * d[1], d[2], 0, attn.nh_tp) if d else None
     y, lse = K.attention_fwd(qkv, B, T, attn.nh_tp, drop=adrop, head_dim=attn.dh)
     x1 = G.linear_fwd_resid(y, attn.c_proj.weight.w16, attn.c_proj.bias, x,
                             drop=(d[0], 4 * d[1] + 1, d[2], 0) if d else None)
     if act8:
-        return x1, _Act8(norm, K.act8_pack(qkv), K.act8_pack(y), d)
+        return x1, _Act8(norm, _act8_pack("Q/K/V", blk, qkv), _act8_pack("attention output", blk, y), d)
     return x1, ((x, xn, *norm, qkv, y, lse, d) if keep else None)
 
 
@@ -149,12 +192,12 @@ def _mlp_fwd(blk, x1: torch.Tensor, keep: bool, act8: bool = False):
     mlp = blk.mlp
     d = _dropout_of(blk)
     act8 = act8 and keep
-    xn2, norm = _norm_fwd(blk.ln_2, x1, _dt(blk), act8)
+    xn2, norm = _norm_fwd(blk, blk.ln_2, x1, _dt(blk), act8)
     h, pre = G.linear_fwd_gelu(xn2, mlp.c_fc.weight.w16, mlp.c_fc.bias)
     x2 = G.linear_fwd_resid(h, mlp.c_proj.weight.w16, mlp.c_proj.bias, x1,
                             drop=(d[0], 4 * d[1] + 2, d[2], 0) if d else None)
     if act8:
-        return x2, _Act8(norm, K.act8_pack(pre), d)
+        return x2, _Act8(norm, _act8_pack("MLP pre-activation", blk, pre), d)
     return x2, ((x1, xn2, *norm, pre, h, d) if keep else None)
 
 
@@ -294,9 +337,9 @@ class _Recompute:
     input (in 8 bits with ``act8``) and the dropout snapshot its forward used
     (backward reruns the forward)."""
 
-    def __init__(self, x_in, drop_now, act8: bool = False):
+    def __init__(self, blk, x_in, drop_now, act8: bool = False):
         self.act8, self.drop_now = act8, drop_now
-        self.x_in = K.act8_pack(x_in) if act8 else x_in
+        self.x_in = _act8_pack("input", blk, x_in) if act8 else x_in
 
     def block_input(self) -> torch.Tensor:
         return K.act8_unpack(*self.x_in, dtype=torch.float32) if self.act8 else self.x_in
@@ -336,7 +379,7 @@ class _Body(torch.autograd.Function):
                     aux_total = aux_total + aux
                 else:
                     x, sm = _mlp_fwd(blk, x, keep and not rerun, act8)
-            saved.append(_Recompute(x_in, getattr(blk, "_hb_drop_now", None), act8) if rerun else (sa, sm))
+            saved.append(_Recompute(blk, x_in, getattr(blk, "_hb_drop_now", None), act8) if rerun else (sa, sm))
         ctx.blocks, ctx.saved, ctx.B, ctx.T = blocks, saved, B, T
         return x, aux_total
 
@@ -375,14 +418,27 @@ def blocks_fused(blocks, x: torch.Tensor, cfg, recompute: bool = False,
     """Run a list of blocks (dense or MoE) on x [B, T, H]; returns (fp32 x, summed MoE aux loss).
     ``recompute``: dense blocks keep only their input and rerun their forward in backward.
     ``act_bits`` 8: what is kept for backward is kept in 8 bits (with ``recompute``, the blocks' inputs);
-    MoE sub-layers keep 16 bits."""
+    MoE sub-layers keep 16 bits. The first training forward of these blocks outside a graph capture warns of activations
+    that 8 bits do not hold (one read of the counts by the host)."""
+    global _ACT8_WATCH
     if act_bits not in (8, 16):
         raise ValueError(f"activations are kept in 16 or 8 bits, got {act_bits}")
     B, T, H = x.shape
     x2 = x.reshape(B * T, H)
     if x2.dtype != torch.float32:
         x2 = x2.float()
-    out, aux = _Body.apply(x2.contiguous(), list(blocks), B, T, bool(recompute), act_bits == 8)
+    blocks = list(blocks)
+    look = (act_bits == 8 and blocks and torch.is_grad_enabled() and x2.requires_grad
+            and not getattr(blocks[0], "_act8_looked", False)
+            and not (x2.is_cuda and torch.cuda.is_current_stream_capturing()))
+    _ACT8_WATCH = seen = [] if look else None
+    try:
+        out, aux = _Body.apply(x2.contiguous(), blocks, B, T, bool(recompute), act_bits == 8)
+    finally:
+        _ACT8_WATCH = None
+    if look:
+        blocks[0]._act8_looked = True
+        _act8_report(blocks, seen)
     return out.view(B, T, H), aux
 
 

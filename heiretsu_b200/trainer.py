@@ -146,7 +146,8 @@ def build_argparser() -> argparse.ArgumentParser:
     p.add_argument("--activation_bits", type=int, default=16, choices=[8, 16],
                    help="8: keep the activations that backward needs in 8 bits (fused engine without TP: about 10 "
                         "instead of 36 bytes per token and channel in a dense block; with --activation_checkpointing "
-                        "the blocks' inputs)")
+                        "the blocks' inputs). One scale serves 128 channels: not for models with channels 50 times larger "
+                        "than others (the first step warns of them)")
     p.add_argument("--fused_tp_dropout", type=int, default=1, choices=[0, 1],
                    help="run tp > 1 with dropout > 0 on the fused engine (masks applied around the in-kernel "
                         "reduce-scatter and all-gather; default); 0 = such runs use the plain engine")

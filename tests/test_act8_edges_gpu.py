@@ -36,3 +36,38 @@ def test_layernorm_codes_of_rows_with_an_offset(mean):
     block = torch.arange(H, device="cuda") // 128
     off = (q.double() != torch.round(xh * torch.exp2(127 - e.double())[:, block])).sum().item()
     assert off <= 3 * 8e-7 * M * H + 3, off
+
+
+def test_outlier_channels_are_reported_outside_of_captures():
+    """The first training forward of an 8-bit model warns of a channel that takes its neighbours' digits, on a model whose
+    first one is captured the first eager one; a captured step takes no host read."""
+    import warnings
+
+    from heiretsu_b200.ops._C import check_status
+    from test_objectives_gpu import batch, models
+
+    idx, tgt = batch()[:2]
+
+    def outlier():
+        m = models(act_bits=8)[1]
+        with torch.no_grad():
+            m.tr.wpe.weight[:, 5] = 9.0
+        return m
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        models(act_bits=8)[1].token_logprobs(idx, tgt).sum().backward()
+    with pytest.warns(UserWarning, match="block 0 LayerNorm: 12[0-9]"):
+        outlier().token_logprobs(idx, tgt).sum().backward()
+    m = outlier()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with torch.cuda.graph(graph):
+            m.token_logprobs(idx, tgt).sum().backward()
+    graph.replay()
+    with pytest.warns(UserWarning, match="block 0 LayerNorm"):
+        m.token_logprobs(idx, tgt)
+    torch.cuda.synchronize()
+    check_status()
