@@ -18,7 +18,7 @@ namespace hb {
 
 long logit_row_limit(int type);
 long policy_scratch_doubles();
-long preference_scratch_doubles(long tokens);
+long preference_scratch_doubles(int P, int T);
 void token_logprobs_launch(const LogitRows& a, cudaStream_t s);
 void policy_loss_launch(const LogitRows& a, const PolicyTerms& p, double* scratch, float* loss, float* stats,
                         cudaStream_t s);
@@ -186,7 +186,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> preference_loss(const at::Tensor&
   if (given(ref_logp)) check_vec(*ref_logp, at::kFloat, n, dev, op, "ref_logp");
   const auto f32 = logp.options();
   at::Tensor loss = at::empty({}, f32), rewards = at::empty({2, P}, f32), dlogp = at::empty(logp.sizes(), f32);
-  const long doubles = preference_scratch_doubles(n);
+  const long doubles = preference_scratch_doubles(static_cast<int>(P), static_cast<int>(T));
   at::Tensor scratch;
   if (doubles > 0) scratch = at::empty({doubles}, f32.dtype(at::kDouble));
   preference_loss_launch(logp.data_ptr<float>(), given(ref_logp) ? ref_logp->data_ptr<float>() : nullptr,

@@ -93,3 +93,51 @@ def test_policy_terms_past_32_bits(kl):
     assert torch.isfinite(grad).all() and (grad[9:15] == 0).all()  # weight 0; the others keep their KL term
     tol = grad_bound(d[:, None] * unit, d, x, lse64, V, x.dtype) + slack * (d[:, None] * unit).abs()
     assert ((grad.double() - d[:, None] * unit).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("P,T", [(16, 1), (17, 1), (32, 4), (16, 128), (17, 128), (8, 129), (9, 129), (1, 2049), (2, 2049),
+                                 (4096, 1), (5000, 0), (1024, 4)])
+def test_preference_pairs_on_both_sides_of_the_launch_rule(P, T):
+    """One CTA takes as many pairs as it has groups of warps (16 up to 128 tokens, then halves); loss, rewards and gradient
+    against 64 bits around that number. Only the outputs' roundings remain."""
+    from heiretsu_b200.ops import kernels as K
+    from heiretsu_b200.ops._C import check_status
+    from post_oracle import IGNORE, preference
+
+    g = torch.Generator(device="cuda").manual_seed(P + T)
+    lp = -torch.rand(2 * P, T, device="cuda", generator=g)
+    t = torch.randint(0, 9, (2 * P, T), device="cuda", generator=g)
+    t[torch.rand(2 * P, T, device="cuda", generator=g) < 0.3] = IGNORE
+    loss, rewards, d = K.preference_loss(lp, t, beta=0.4, label_smoothing=0.1)
+    torch.cuda.synchronize()
+    check_status()
+    l64, r64, d64 = preference(lp, t, None, 0.4, 0.1)
+    for a, b in ((loss, l64), (rewards, r64), (d, d64)):
+        assert ((a.double() - b).abs() <= 2.0 ** -24 * b.abs() + 1e-12).all()
+
+
+def test_many_short_preference_pairs_spread_over_the_gpu():
+    """4096 pairs of one token are no queue on one SM: within 20 times of 16 pairs (in one CTA they took 160 times as long,
+    on all SMs 2 times)."""
+    from heiretsu_b200.ops import kernels as K
+
+    def us(P):
+        lp = -torch.rand(2 * P, 1, device="cuda")
+        t = torch.zeros(2 * P, 1, device="cuda", dtype=torch.long)
+        K.preference_loss(lp, t)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(10):
+                K.preference_loss(lp, t)
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert us(4096) <= 20 * us(16)
