@@ -71,3 +71,24 @@ def test_outlier_channels_are_reported_outside_of_captures():
         m.token_logprobs(idx, tgt)
     torch.cuda.synchronize()
     check_status()
+
+
+def test_column_sums_round_once_behind_the_ctas():
+    """dgamma and dbeta of whole numbers: a CTA's sum of at most 2^6 rows of values below 2^18 is exact in 32 bits, the sum
+    of all CTAs (2^30) only in 64, so what is added to the accumulators is off by its own rounding alone."""
+    from heiretsu_b200.ops import kernels as K
+    from heiretsu_b200.ops._C import check_status
+
+    M, H = 8192, 1280
+    g = torch.Generator(device="cuda").manual_seed(9)
+    dy = torch.randint(2 ** 16, 2 ** 18, (M, H), device="cuda", generator=g).float()
+    q = torch.ones(M, H, device="cuda", dtype=torch.int8)  # xh = 1 everywhere
+    e = torch.full((M, H // 128), 127, device="cuda", dtype=torch.uint8)
+    w, b, rstd = torch.ones(H, device="cuda"), torch.zeros(H, device="cuda"), torch.ones(M, device="cuda")
+    res, d16 = torch.zeros(M, H, device="cuda"), torch.empty(M, H, device="cuda", dtype=torch.bfloat16)
+    dg, db = torch.full((H,), 0.5, device="cuda"), torch.zeros(H, device="cuda")
+    K.layernorm_bwd_act8(dy, q, e, rstd, w, b, res, res, d16, dg, db)
+    torch.cuda.synchronize()
+    check_status()
+    want = dy.double().sum(0)
+    assert torch.equal(db, want.float()) and torch.equal(dg, (want + 0.5).float())
