@@ -7,9 +7,9 @@
 // Scaling by a power of two is exact, so the code's rounding is the only error: at most 2^e / 2 <= max|x| / 127
 // per value, and the codes of a given input do not depend on the order of any arithmetic. A power of two
 // costs up to one bit against a scale of max|x| / 127; in exchange the scale is one byte for 128 values and
-// encoding needs no division. The bound goes by the block's largest value: a column 50 times larger than the other 127
-// leaves these off by 15% of their size, one 300 times larger by 70 to 90% (all codes 0). A block that holds an infinity or NaN gets byte 255 and comes back as NaN, so a
-// broken activation still shows in the gradient norm.
+// encoding needs no division. The bound goes by the block's largest value: a column 50 times larger than the other
+// 127 leaves these off by 15% of their size, one 300 times larger by 70% and more (most codes 0). A block that holds an
+// infinity or NaN gets byte 255 and comes back as NaN, so a broken activation still shows in the gradient norm.
 #pragma once
 
 #include "common.cuh"

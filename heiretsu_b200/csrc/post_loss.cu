@@ -199,9 +199,10 @@ struct Deal {
 // So a row crosses DRAM once each way. Rows may start at any element: the columns before the first 16-byte
 // boundary (`head`, fewer than one piece) are read by single threads of the first CTA.
 // Measured: 8192 x 50257 bf16 with a quarter of the rows ignored, 255 to 275 us by the run: 1.44 GB, 5.2 to 5.6 TB/s (a
-// copy reaches 6.4); with none ignored 305 us, 5.4 TB/s; without a gradient 113 and 143 us (5.5, 5.8 TB/s). The arithmetic (8 instructions an
-// element and pass) fills 56% of the issue slots and 62% of the transcendental unit. More warps, copies waited for
-// in two or four groups and packed arithmetic do not change the time; the two CTAs of an SM overlap their phases.
+// copy reaches 6.4); with none ignored 305 us, 5.4 TB/s; without a gradient 113 and 143 us (5.5, 5.8 TB/s). The
+// arithmetic (8 instructions an element and pass) fills 56% of the issue slots and 62% of the transcendental unit. More
+// warps, copies waited for in two or four groups and packed arithmetic do not change the time; the two CTAs of an SM
+// overlap their phases.
 template <int TYPE, int MODE, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreadsPerSm / kThreads)
     logit_rows_kernel(const LogitRows a, const PolicyTerms p, const Deal d, double* __restrict__ part) {

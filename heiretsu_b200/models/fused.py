@@ -115,7 +115,7 @@ def _dropout_of(blk):
 #
 # One scale serves 128 channels, so the format holds channels of like sizes: each value is off by at most 1/254 to
 # 1/127 of the largest among the 128, about 1% of a standard deviation where they are alike. A channel
-# 50 times larger leaves its 127 neighbours off by 15%, one 300 times larger by 70 to 90%, and their part of the
+# 50 times larger leaves its 127 neighbours off by 15%, one 300 times larger by 70% and more, and their part of the
 # gradients with it. Trained models can have such channels; the first training forward looks for them.
 class _Act8:
     """Saved state of a sub-layer in 8 bits."""
