@@ -49,6 +49,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_logprobs", &hb::token_logprobs);
   m.def("policy_loss", &hb::policy_loss);
   m.def("preference_loss", &hb::preference_loss);
+  m.def("kv_write", &hb::kv_write);
+  m.def("kv_read", &hb::kv_read);
+  m.def("decode_attention", &hb::decode_attention);
+  m.def("sample_tokens", &hb::sample_tokens);
   m.def("act8_pack", &hb::act8_pack);
   m.def("act8_unpack", &hb::act8_unpack);
   m.def("layernorm_fwd_act8", &hb::layernorm_fwd_act8);

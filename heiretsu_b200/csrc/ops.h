@@ -72,6 +72,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layernorm_fwd_act8(co
 at::Tensor layernorm_bwd_act8(const at::Tensor& dy, const at::Tensor& q, const at::Tensor& e, const at::Tensor& rstd,
                               const at::Tensor& w, const at::Tensor& b, const at::Tensor& dres_in, at::Tensor& dres,
                               at::Tensor& dres16, at::Tensor& dgamma, at::Tensor& dbeta);
+void kv_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, const at::Tensor& k_pages,
+              const at::Tensor& v_pages, const c10::optional<at::Tensor>& k_exp, const c10::optional<at::Tensor>& v_exp);
+std::tuple<at::Tensor, at::Tensor> kv_read(const at::Tensor& slots, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                                           const c10::optional<at::Tensor>& k_exp, const c10::optional<at::Tensor>& v_exp,
+                                           const c10::optional<at::ScalarType>& dtype);
+std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor& k_pages,
+                                                    const at::Tensor& v_pages, const at::Tensor& table,
+                                                    const at::Tensor& lengths, const c10::optional<at::Tensor>& k_exp,
+                                                    const c10::optional<at::Tensor>& v_exp,
+                                                    const c10::optional<double>& scale);
+at::Tensor sample_tokens(const at::Tensor& logits, int64_t V, const at::Tensor& u,
+                         const c10::optional<at::Tensor>& temperature, double temperature0,
+                         const c10::optional<at::Tensor>& top_k, int64_t top_k0, const c10::optional<at::Tensor>& top_p,
+                         double top_p0, const c10::optional<at::Tensor>& min_p, double min_p0);
 uint64_t raw_malloc(int64_t bytes);
 void raw_free(uint64_t ptr);
 at::Tensor tensor_from_ptr(uint64_t ptr, int64_t numel, at::ScalarType dtype, int64_t device);

@@ -177,6 +177,70 @@ def layernorm_bwd_act8(dy, q, e, rstd, w, b, dres_in, dres, dres16, dgamma, dbet
 
 
 # ---------------------------------------------------------------------------
+# Decoding: a paged key/value cache, attention of one new token over it, and the choice of the next token
+# ---------------------------------------------------------------------------
+# A cache is k_pages and v_pages [pages, heads, page size, head dim] (bf16 or fp16; the page size a multiple of 16, any
+# strides that are multiples of 16 bytes). In 8 bits they are int8 and k_exp and v_exp (uint8 [pages, heads, page size]) hold
+# the exponent byte of each head of each token: the format of act8_pack with a block per head of a token.
+def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+             k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None) -> None:
+    """Writes K and V of new tokens ([tokens, heads, head dim], bf16 or fp16; any strides, such as views of a projection's
+    output) into the cache, quantised where it holds 8 bits.
+
+    ``slots`` int64 [tokens]: page * page size + place in the page. A negative slot's token is not kept; one behind the
+    cache is not either, and sets the bad-argument status. Slots must differ: of two tokens with one slot either may be kept,
+    or a mixture of both. An 8-bit head that holds an infinity or NaN comes back as NaN."""
+    _ext().kv_write(k, v, slots, k_pages, v_pages, k_exp, v_exp)
+
+
+def kv_read(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_exp: Optional[torch.Tensor] = None,
+            v_exp: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None):
+    """K and V of ``slots`` (as in ``kv_write``; the same slot may come more than once): (k, v) [tokens, heads, head dim].
+
+    An 8-bit cache is read in ``dtype`` (bf16, the default, fp16 or fp32; values beyond the type's range become its
+    largest), a 16-bit one in its own. A negative slot reads as zeros; one behind the cache as NaN, and sets the
+    bad-argument status."""
+    return _ext().kv_read(slots, k_pages, v_pages, k_exp, v_exp, dtype)
+
+
+def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                     lengths: torch.Tensor, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None):
+    """Attention of one new token per sequence over its cached tokens: (out like q, lse fp32 [sequences, heads]).
+
+    ``q`` [sequences, heads, head dim] in bf16 or fp16 (any strides; a 16-bit cache has its dtype), heads a multiple of
+    the cache's: query heads i * g .. i * g + g - 1 share K/V head i. ``table`` int32 [sequences, pages]: the pages of a
+    sequence in order; ``lengths`` int32 [sequences]: how many of its tokens count, the new one's own K and V among them when
+    it has been written. Entries and slots behind them are not read. ``scale`` defaults to head dim ** -0.5; ``lse`` is the natural
+    log-sum-exp of the scores, so that outputs over parts of a cache can be joined. A sequence of length 0 gives 0 and
+    -inf; a length or page out of range gives NaN in its rows, and sets the bad-argument status."""
+    return _ext().decode_attention(q, k_pages, v_pages, table, lengths, k_exp, v_exp, scale)
+
+
+def _per_row(value):
+    """A setting of ``sample_tokens`` as (tensor or None, number)."""
+    return (value, 0) if isinstance(value, torch.Tensor) else (None, value)
+
+
+def sample_tokens(logits: torch.Tensor, V: int, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> torch.Tensor:
+    """A token per row of ``logits`` [M, >= V] (bf16, fp16 or fp32, contiguous rows): int64 [M].
+
+    ``u`` fp32 [M]: uniform numbers in [0, 1). Settings are numbers, or tensors [M] with one for each row (fp32; ``top_k``
+    int64). Token i weighs w_i = exp((x_i - max) / temperature). In the order by logit, descending, equal ones by index, kept
+    are the first ``top_k`` (0, or V and more: all), of these the shortest start whose weight reaches ``top_p`` of theirs, of
+    these the ones with w_i >= ``min_p``; the first always is. The token drawn is the first kept one, in the
+    vocabulary's order, at which the running weight exceeds u times the kept weight: the same u, logits and settings
+    give the same token whatever the other rows are. ``temperature`` <= 0 takes the largest logit (equal ones: the lowest
+    index). A row that holds +inf or NaN, or nothing but -inf, and a setting or u that is NaN, gives -1. V is at most 524288."""
+    t, t0 = _per_row(temperature)
+    k, k0 = _per_row(top_k)
+    p, p0 = _per_row(top_p)
+    m, m0 = _per_row(min_p)
+    return _ext().sample_tokens(logits, V, u, t, float(t0), k, int(k0), p, float(p0), m, float(m0))
+
+
+# ---------------------------------------------------------------------------
 # Embedding
 # ---------------------------------------------------------------------------
 def embedding_fwd(idx: torch.Tensor, wte: torch.Tensor, wpe: torch.Tensor) -> torch.Tensor:
