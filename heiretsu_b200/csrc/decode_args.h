@@ -44,6 +44,8 @@ struct DecodeArgs {
   float scale;
   void* out;                       // [seqs, heads_q, dim]
   float* lse;                      // [seqs, heads_q]
+  float* part;                     // per CTA, two unfinished units: maxima, sums and outputs of their columns
+  long* record;                    // and which they are: 2 * unit + (the unit ends there), -1: none
   int* status;
 };
 

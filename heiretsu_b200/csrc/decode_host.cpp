@@ -21,13 +21,16 @@ namespace hb {
 void kv_write_launch(const KvTokens& t, const KvPool& p, int* status, cudaStream_t s);
 void kv_read_launch(const int64_t* slots, const KvPool& p, void* k, void* v, int n, int out, int* status,
                     cudaStream_t s);
-void decode_attention_launch(const DecodeArgs& a, cudaStream_t s);
+int decode_attention_ctas(int seqs, int units, long longest);
+int decode_attention_seqs();
+void decode_attention_launch(const DecodeArgs& a, int ctas, cudaStream_t s);
 void sample_tokens_launch(const SampleArgs& a, cudaStream_t s);
 
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
 constexpr int64_t kIntMax = std::numeric_limits<int>::max();
+constexpr int64_t kLongest = 1 << 24;   // tokens of a sequence: the tiles of 1024 sequences are counted in 32 bits
 constexpr int64_t kMaxVocab = 1 << 19;  // weights of 2^-44 then sum to less than 2^63
 
 bool given(const OptTensor& t) { return t && t->defined(); }
@@ -193,7 +196,7 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
   TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B &&
                   (table.size(1) <= 1 || table.stride(1) == 1) && table.stride(0) >= 0,
               op, ": table must be int32 [sequences, pages] with contiguous rows");
-  TORCH_CHECK(table.size(1) <= kIntMax / a.pool.size, op, ": table is too wide");
+  TORCH_CHECK(table.size(1) <= kLongest / a.pool.size, op, ": table is too wide: at most ", std::to_string(kLongest), " tokens");
   check_plain(lengths, at::kInt, {B}, op, "lengths (int32 [sequences])");
   a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(a.pool.dim)));
   TORCH_CHECK(std::isfinite(a.scale), op, ": scale must be finite");
@@ -204,15 +207,27 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
   TORCH_CHECK(k_pages.is_cuda(), op, ": the cache must be on a CUDA device");
   c10::cuda::CUDAGuard g(dev);
   at::Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
-  a.q = q.data_ptr(), a.qt = q.stride(0), a.qh = q.stride(1);
+  a.qt = q.stride(0), a.qh = q.stride(1);
   a.q_vec = rows_aligned(q);
   a.f16 = q.scalar_type() == at::kHalf;
-  a.table = table.data_ptr<int>(), a.tt = table.stride(0), a.width = static_cast<int>(table.size(1));
-  a.lengths = lengths.data_ptr<int>();
-  a.seqs = static_cast<int>(B), a.heads_q = static_cast<int>(q.size(1));
-  a.out = out.data_ptr(), a.lse = lse.data_ptr<float>();
+  a.tt = table.stride(0), a.width = static_cast<int>(table.size(1));
+  a.heads_q = static_cast<int>(q.size(1));
   a.status = device_status_ptr(dev.index());
-  decode_attention_launch(a, at::cuda::getCurrentCUDAStream());
+  const int most = decode_attention_seqs(), G = a.heads_q / a.pool.heads, cols = std::min(G, 8);
+  for (int64_t b = 0; b < B; b += most) {  // a launch for each 1024 sequences
+    a.seqs = static_cast<int>(std::min<int64_t>(most, B - b));
+    a.q = static_cast<const uint16_t*>(q.data_ptr()) + b * a.qt;
+    a.table = table.data_ptr<int>() + b * a.tt;
+    a.lengths = lengths.data_ptr<int>() + b;
+    a.out = static_cast<uint16_t*>(out.data_ptr()) + b * out.stride(0);
+    a.lse = lse.data_ptr<float>() + b * a.heads_q;
+    const int ctas = decode_attention_ctas(a.seqs, a.pool.heads * ((G + 7) / 8), static_cast<long>(a.width) * a.pool.size);
+    // 2 * ctas records, then 2 * ctas parts
+    at::Tensor part = at::empty({2l * ctas * (2 + static_cast<long>(cols) * (a.pool.dim + 2))}, lse.options());
+    a.record = reinterpret_cast<long*>(part.data_ptr<float>());
+    a.part = part.data_ptr<float>() + 4l * ctas;
+    decode_attention_launch(a, ctas, at::cuda::getCurrentCUDAStream());
+  }
   return {out, lse};
 }
 
