@@ -2,6 +2,8 @@
 // checks (decode_host.cpp).
 #pragma once
 
+#include <vector_types.h>
+
 #include <cstdint>
 
 namespace hb {
@@ -16,7 +18,9 @@ struct KvPool {
   uint8_t *ke, *ve;                // null unless type is kKvCodes
   long kp, kh, ks, vp, vh, vs;     // strides in elements
   long kep, keh, vep, veh;
+  uint32_t kp16, ks16, vp16, vs16; // strides of a page and a slot in units of 16 bytes (32 bits: decode_attention only)
   int pages, heads, size, dim;     // size: slots of a page
+  int groups;                      // of 16 slots in a page
   int type;                        // KvType
 };
 
@@ -38,15 +42,22 @@ struct DecodeArgs {
   bool f16;                        // of q and out
   const int* table;                // [seqs, width], row stride tt
   long tt;
-  int width;
   const int* lengths;              // [seqs]
+  int longest;                     // tokens that a row of the table holds
   int seqs, heads_q;
   float scale;
   void* out;                       // [seqs, heads_q, dim]
   float* lse;                      // [seqs, heads_q]
   float* part;                     // per CTA, two unfinished units: maxima, sums and outputs of their columns
-  long* record;                    // and which they are: 2 * unit + (the unit ends there), -1: none
+  int2* record;                    // and which they are: (unit or -1, CTAs behind that have more of it)
   int* status;
+};
+
+// How decode_attention deals out its work: a launch of `ctas` CTAs for each `seqs` sequences (0: more tiles than 32 bits
+// count); `whole`: CTAs take whole units.
+struct DecodePlan {
+  int seqs = 0, ctas = 0;
+  bool whole = false;
 };
 
 struct SampleArgs {

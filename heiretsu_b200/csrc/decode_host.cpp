@@ -21,9 +21,8 @@ namespace hb {
 void kv_write_launch(const KvTokens& t, const KvPool& p, int* status, cudaStream_t s);
 void kv_read_launch(const int64_t* slots, const KvPool& p, void* k, void* v, int n, int out, int* status,
                     cudaStream_t s);
-int decode_attention_ctas(int seqs, int units, long longest);
-int decode_attention_seqs();
-void decode_attention_launch(const DecodeArgs& a, int ctas, cudaStream_t s);
+DecodePlan decode_attention_plan(int seqs, int units, int longest);
+void decode_attention_launch(const DecodeArgs& a, const DecodePlan& d, cudaStream_t s);
 void sample_tokens_launch(const SampleArgs& a, cudaStream_t s);
 
 namespace {
@@ -97,6 +96,7 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
   p.vp = v.stride(0), p.vh = v.stride(1), p.vs = v.stride(2);
   p.pages = static_cast<int>(k.size(0)), p.heads = static_cast<int>(k.size(1));
   p.size = static_cast<int>(size), p.dim = static_cast<int>(D);
+  p.groups = p.size / 16;
   p.type = dt == at::kChar ? kKvCodes : dt == at::kHalf ? kKvF16 : kKvBf16;
   check_same_device(v, k.device(), op, "v_pages");
   TORCH_CHECK(given(ke) == (dt == at::kChar) && given(ve) == (dt == at::kChar), op,
@@ -115,6 +115,16 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
   return p;
 }
 
+// The attention kernel counts slots in units of 16 bytes, and exponent bytes, in 32 bits.
+void check_reach(KvPool& p, const char* op) {
+  const int64_t es = p.type == kKvCodes ? 1 : 2, most = int64_t{1} << 32;
+  const auto reach = [&](long page, long slot) { return (p.pages * page + p.size * slot) * es / 16; };
+  TORCH_CHECK(reach(p.kp, p.ks) < most && reach(p.vp, p.vs) < most && p.pages * p.kep + p.size < most &&
+                  p.pages * p.vep + p.size < most,
+              op, ": k_pages and v_pages must each span less than 64 GB");
+  p.kp16 = static_cast<uint32_t>(p.kp * es / 16), p.ks16 = static_cast<uint32_t>(p.ks * es / 16);
+  p.vp16 = static_cast<uint32_t>(p.vp * es / 16), p.vs16 = static_cast<uint32_t>(p.vs * es / 16);
+}
 void check_slots(const at::Tensor& slots, const char* op) {
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), op,
               ": slots must be contiguous int64 [tokens]");
@@ -198,6 +208,7 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
               op, ": table must be int32 [sequences, pages] with contiguous rows");
   TORCH_CHECK(table.size(1) <= kLongest / a.pool.size, op, ": table is too wide: at most ", std::to_string(kLongest), " tokens");
   check_plain(lengths, at::kInt, {B}, op, "lengths (int32 [sequences])");
+  check_reach(a.pool, op);
   a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(a.pool.dim)));
   TORCH_CHECK(std::isfinite(a.scale), op, ": scale must be finite");
   const at::Device dev = k_pages.device();
@@ -210,23 +221,26 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
   a.qt = q.stride(0), a.qh = q.stride(1);
   a.q_vec = rows_aligned(q);
   a.f16 = q.scalar_type() == at::kHalf;
-  a.tt = table.stride(0), a.width = static_cast<int>(table.size(1));
+  a.tt = table.stride(0);
+  a.longest = a.pool.pages == 0 ? 0 : static_cast<int>(table.size(1)) * a.pool.size;
   a.heads_q = static_cast<int>(q.size(1));
   a.status = device_status_ptr(dev.index());
-  const int most = decode_attention_seqs(), G = a.heads_q / a.pool.heads, cols = std::min(G, 8);
-  for (int64_t b = 0; b < B; b += most) {  // a launch for each 1024 sequences
-    a.seqs = static_cast<int>(std::min<int64_t>(most, B - b));
+  const int G = a.heads_q / a.pool.heads, cols = std::min(G, 8);
+  DecodePlan plan;
+  for (int64_t b = 0; b < B; b += plan.seqs) {
+    plan = decode_attention_plan(static_cast<int>(B - b), a.pool.heads * ((G + 7) / 8), a.longest);
+    TORCH_CHECK(plan.seqs > 0, op, ": the table is too wide for so many heads");
+    a.seqs = plan.seqs;
     a.q = static_cast<const uint16_t*>(q.data_ptr()) + b * a.qt;
     a.table = table.data_ptr<int>() + b * a.tt;
     a.lengths = lengths.data_ptr<int>() + b;
     a.out = static_cast<uint16_t*>(out.data_ptr()) + b * out.stride(0);
     a.lse = lse.data_ptr<float>() + b * a.heads_q;
-    const int ctas = decode_attention_ctas(a.seqs, a.pool.heads * ((G + 7) / 8), static_cast<long>(a.width) * a.pool.size);
-    // 2 * ctas records, then 2 * ctas parts
-    at::Tensor part = at::empty({2l * ctas * (2 + static_cast<long>(cols) * (a.pool.dim + 2))}, lse.options());
-    a.record = reinterpret_cast<long*>(part.data_ptr<float>());
-    a.part = part.data_ptr<float>() + 4l * ctas;
-    decode_attention_launch(a, ctas, at::cuda::getCurrentCUDAStream());
+    // two parts and their records for each CTA; each launch its own, as the next may begin before the last has joined its
+    at::Tensor part = at::empty({2l * plan.ctas * (2 + cols * (a.pool.dim + 2))}, lse.options());
+    a.record = reinterpret_cast<int2*>(part.data_ptr<float>());
+    a.part = part.data_ptr<float>() + 4l * plan.ctas;
+    decode_attention_launch(a, plan, at::cuda::getCurrentCUDAStream());
   }
   return {out, lse};
 }
