@@ -18,7 +18,6 @@ struct KvPool {
   uint8_t *ke, *ve;                // null unless type is kKvCodes
   long kp, kh, ks, vp, vh, vs;     // strides in elements
   long kep, keh, vep, veh;
-  uint32_t kp16, ks16, vp16, vs16; // strides of a page and a slot in units of 16 bytes (32 bits: decode_attention only)
   int pages, heads, size, dim;     // size: slots of a page
   int groups;                      // of 16 slots in a page
   int type;                        // KvType

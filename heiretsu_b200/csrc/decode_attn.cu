@@ -48,19 +48,30 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// W words from global memory.
-template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&r)[W], const void* p) {
-  if constexpr (W == 4) {
-    const uint4 x = __ldg(static_cast<const uint4*>(p));
-    r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
-  } else if constexpr (W == 2) {
-    const uint2 x = __ldg(static_cast<const uint2*>(p));
-    r[0] = x.x, r[1] = x.y;
-  } else {
-    static_assert(W == 1);
-    r[0] = __ldg(static_cast<const uint32_t*>(p));
-  }
+// Four 8 x 8 matrices of 16-bit values from shared memory (two with X2); lane i gives the address of row i % 8 of number i / 8.
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {  // each transposed
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+// Asynchronous copies into this CTA's shared memory: a box of a 4-D tensor, and 16 bytes.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load_16(uint32_t dst, const void* src, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst),
+               "l"(src), "r"(bar)
+               : "memory");
 }
 
 // Four signed bytes as fp16. A byte with its sign flipped is code + 128; under 0x64 it reads as 1024 + 128 + code, and 1152
@@ -82,28 +93,34 @@ __device__ __forceinline__ uint32_t widen_pair(uint32_t pair) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// How a warp holds a tile of 16 * KT tokens. In the matrix instructions' layout lane (g = lane / 4, t = lane % 4)
-// holds, of each 16 tokens, K of the tokens g and g + 8 and V of 2t, 2t + 1, 2t + 8 and 2t + 9. Which channel an index of
-// a product stands for is free as long as both operands agree, so a lane's channels are taken to be consecutive ones:
-//   K: KE channels from c * 4 KE + t KE, for NKC chunks c (scores: K times q, sums over channels)
-//   V: 2 VW channels from c * 16 VW + g 2 VW, for NVC chunks c (output: V^T times weights, sums over tokens)
-// and tiles go from memory into registers in wide loads, with no shared memory between.
+// A tile of 16 * KT tokens of one K/V head, as it lies in a stage of a warp's ring in shared memory: K, then V, each
+// [KT groups of 16 tokens][boxes of up to 128 bytes of a token][16 tokens][box]; codes have [KT][16 exponent bytes of K, 16
+// of V] besides. The copies swizzle 16-byte chunks of a box by its token, so that the 8 rows of a matrix load
+// lie in different banks.
 template <int D, bool CODES>
 struct Shape {
-  static constexpr int kBytes = CODES ? 1 : 2;
-  static constexpr int KE = CODES ? (D / 4 < 16 ? D / 4 : 16) : (D / 4 < 8 ? D / 4 : 8);
-  static constexpr int NKC = D / (4 * KE);
-  static constexpr int KW = KE * kBytes / 4;  // words of a chunk
-  static constexpr int QW = KE / 2;           // words of q of a chunk
-  static constexpr int VW = CODES ? D / 16 : (D / 16 < 4 ? D / 16 : 4);
-  static constexpr int NVC = D / (16 * VW);
-  static constexpr int VB = 2 * VW * kBytes;  // bytes of a chunk
-  static constexpr int VL = VB < 4 ? 1 : VB / 4;
-  static constexpr int KT = D >= 128 ? 1 : D == 64 ? 2 : 4;
+  static constexpr int kRow = D * (CODES ? 1 : 2);       // bytes of a token
+  static constexpr int kBox = kRow < 128 ? kRow : 128;
+  static constexpr int kBoxes = kRow / kBox;
+  static constexpr int kGroup = 16 * kRow;               // bytes of 16 tokens
+  // 4 KB of K and V (head dim 128 in 16 bits: 8; head dim 16 in codes: 2)
+  static constexpr int KT = kGroup >= 2048 ? 1 : kGroup == 1024 ? 2 : 4;
   static constexpr int kTokens = 16 * KT;
+  static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
+  static constexpr int kStage = 2 * kKv;
+  static constexpr int kExps = CODES ? KT * 32 : 0;      // exponent bytes of a tile, kept apart
+  static constexpr int kCtas = kGroup >= 4096 ? 1 : 2;   // on an SM: what the shared memory holds
+  static constexpr int kSteps = D / 16;                  // matrix instructions along the channels
+  // byte offset of 16-byte chunk c of token r in a group
+  static __device__ __forceinline__ uint32_t chunk(int r, int c) {
+    constexpr int per = kBox / 16;  // chunks of a box: 8, 4, 2 or 1
+    const int x = per == 8 ? r & 7 : per == 4 ? r >> 1 & 3 : per == 2 ? r >> 2 & 1 : 0;
+    return (c / per) * (16 * kBox) + r * kBox + (((c % per) ^ x) << 4);
+  }
 };
 
 constexpr int kMaxSeqs = 1024;  // of one launch: their tile counts are summed in shared memory
+constexpr int kMaxStages = 4;
 
 // A unit: a K/V head of a sequence and up to 8 of its query heads.
 struct Heads {
@@ -155,15 +172,19 @@ __device__ __forceinline__ int share(int total, int c, int n) {
 // that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. WHOLE: CTAs take whole
 // units, and nothing is left to join.
 template <int D, bool F16, bool CODES>
-__global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeArgs a, const bool whole_units) {
+__global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
+    decode_attn_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const int stages, const bool whole_units) {
   using S = Shape<D, CODES>;
   constexpr int KT = S::KT;
-  constexpr bool QK16 = F16 || CODES;   // codes times q run in fp16 (q scaled by a power of two): two instructions less a pair
+  constexpr bool QK16 = F16 || CODES;   // codes times q run in fp16 (q scaled by a power of two): fewer instructions to widen
   constexpr bool PV16 = F16 && !CODES;  // weights times codes run in bf16: 2^e of a head's scale has any exponent
-  extern __shared__ float parts[];      // two per warp
+  extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1];  // tiles of a unit before each sequence
   __shared__ int sums[kWarps];
   __shared__ int seg_unit[2 * kWarps], seg_first[2 * kWarps], seg_last[2 * kWarps], seg_tiles[2 * kWarps];
+  __shared__ uint64_t full[kWarps][kMaxStages];
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -186,6 +207,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
     }
     if (lane == 31) sums[warp] = run;
     if (lane < 2) seg_unit[2 * warp + lane] = -1;
+    if (lane < stages) mbar_init(&full[warp][lane], KT);
+    fence_barrier_init();
     __syncthreads();
     run -= sum;
     for (int w = 0; w < warp; ++w) run += sums[w];
@@ -221,93 +244,102 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
     const bool idle = static_cast<int>(blockIdx.x) >= busy;
     c0 = idle ? total : share(total, blockIdx.x, busy), c1 = idle ? total : share(total, blockIdx.x + 1, busy);
   }
+  // number 2 w: where the run of warp w begins; 2 w + 1: where it ends, in its ring
+  const auto part = [&](int i) {
+    return reinterpret_cast<float*>(smem + (i & 1 ? (i >> 1) * stages * S::kStage : kWarps * stages * (S::kStage + S::kExps) + (i >> 1) * n.cols * (D + 2) * 4));
+  };
   const int w0 = c0 + share(c1 - c0, warp, kWarps), w1 = c0 + share(c1 - c0, warp + 1, kWarps);
 
-  for (int at = w0; at < w1;) {
-    int b = 0;  // the last sequence whose tiles begin at or before `at`
+  // The ring. The copies of a tile are issued as soon as its stage has been read, in the order of the warp's run and across
+  // its units, by the lanes that know the pages: lane i knows that of group number group0 + i of the sequence.
+  uint8_t* const ring = smem + warp * stages * S::kStage;
+  uint8_t* const exps = smem + kWarps * stages * S::kStage + warp * stages * S::kExps;
+  const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(&full[warp][0]);
+  struct {
+    int at, b, u, tile, tiles, groups, group0, page, slot;
+  } next;  // the tile to be copied next
+  next.at = w0;
+  uint32_t lost_pages = 0, lost = 0;  // lanes whose page is none; of the stages' groups, KT bits each
+  const auto unit_at = [&](int at, int& b, int& u, int& tile, int& tiles) {
+    b = 0;  // the last sequence whose tiles begin at or before `at`
     for (int hi = a.seqs; hi - b > 1;) {
       const int mid = (b + hi) >> 1;
       if (prefix[mid] * n.units <= at) b = mid;
       else hi = mid;
     }
-    const int tiles = prefix[b + 1] - prefix[b], in_seq = at - prefix[b] * n.units;
-    const int u = in_seq / tiles, first = in_seq - u * tiles, last = min(tiles, first + (w1 - at));
+    tiles = prefix[b + 1] - prefix[b];
+    const int in_seq = at - prefix[b] * n.units;
+    u = in_seq / tiles;
+    tile = in_seq - u * tiles;
+  };
+  const auto find_pages = [&]() {
+    next.group0 = next.tile * KT;
+    const int mine = min(next.group0 + lane, next.groups - 1), page = mine / p.groups;
+    next.slot = (mine - page * p.groups) * 16;
+    next.page = a.table[next.b * a.tt + page];
+    lost_pages = __ballot_sync(kFull, next.page < 0 || next.page >= p.pages);
+    if (lost_pages && lane == 0) record_error(a.status, kBadArg, kSite);
+  };
+  const auto copy_next = [&](int stage) {
+    if (next.at >= w1) return;
+    if (next.at == w0 || next.tile == next.tiles) {  // another unit
+      unit_at(next.at, next.b, next.u, next.tile, next.tiles);
+      next.groups = (a.lengths[next.b] + 15) >> 4;
+      find_pages();
+    } else if (next.tile * KT >= next.group0 + 32) {
+      find_pages();
+    }
+    const int first = next.tile * KT - next.group0, i = lane - first;
+    lost = (lost & ~(((1u << KT) - 1) << (stage * KT))) | ((lost_pages >> first & ((1u << KT) - 1)) << (stage * KT));
+    if (i >= 0 && i < KT) {
+      const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * S::kStage + i * S::kGroup;
+      if (next.tile * KT + i < next.groups) {
+        mbar_arrive_expect_tx(&full[warp][stage], 2 * S::kGroup + (CODES ? 32 : 0));
+        const int h = next.u / n.chunks;
+#pragma unroll
+        for (int x = 0; x < S::kBoxes; ++x) {
+          tma_load_4d(dst + x * 16 * S::kBox, &k_map, bar, x * (S::kBox / (CODES ? 1 : 2)), next.slot, h, next.page);
+          tma_load_4d(dst + S::kKv + x * 16 * S::kBox, &v_map, bar, x * (S::kBox / (CODES ? 1 : 2)), next.slot, h, next.page);
+        }
+        if constexpr (CODES) {
+          const long page = next.page < 0 || next.page >= p.pages ? 0 : next.page;
+          const uint32_t e = smem_u32(exps) + stage * S::kExps + i * 32;
+          bulk_load_16(e, p.ke + page * p.kep + h * p.keh + next.slot, bar);
+          bulk_load_16(e + 16, p.ve + page * p.vep + h * p.veh + next.slot, bar);
+        }
+      } else {
+        mbar_arrive(&full[warp][stage]);
+      }
+    }
+    ++next.at, ++next.tile;
+  };
+  for (int s = 0; s < stages; ++s) copy_next(s);
+
+  int stage = 0;
+  uint32_t parity = 0;
+  bool broken = false;  // a copy that did not arrive in time
+  // where this lane's rows of matrix loads are: K of the tokens and chunks, V of the same, by Shape::chunk
+  const int row_k = (lane & 7) + (lane & 8), chunk_k = lane >> 4;
+  const int row_v = CODES ? row_k : (lane & 7) + (lane >> 4) * 8, chunk_v = CODES ? chunk_k : lane >> 3 & 1;
+
+  for (int at = w0; at < w1 && !broken;) {
+    int b, u, first, tiles;
+    unit_at(at, b, u, first, tiles);
+    const int last = min(tiles, first + (w1 - at));
     const Columns c(n, u);
     const int len = a.lengths[b], groups = (len + 15) >> 4;  // of 16 tokens
 
-    // Lane i knows where the group number group0 + i is: K and V in units of 16 bytes, the exponent bytes in bytes, from the
-    // lane's own place in slot 0 of page 0. A page outside the cache is replaced by page 0 and noted in `lost`.
-    int group0;
-    uint32_t k_at, v_at, ke_at = 0, ve_at = 0, lost;
-    const auto find_pages = [&](int group) {
-      group0 = group;
-      const int mine = min(group + lane, groups - 1);
-      const int page = mine / p.groups, slot = (mine - page * p.groups) * 16;
-      int id = a.table[b * a.tt + page];
-      const bool bad = id < 0 || id >= p.pages;
-      if (bad) id = 0;
-      lost = __ballot_sync(kFull, bad);
-      if (lost && lane == 0) record_error(a.status, kBadArg, kSite);
-      k_at = id * p.kp16 + slot * p.ks16, v_at = id * p.vp16 + slot * p.vs16;
-      if constexpr (CODES) ke_at = id * static_cast<uint32_t>(p.kep) + slot, ve_at = id * static_cast<uint32_t>(p.vep) + slot;
-    };
-    const char* const kb = static_cast<const char*>(p.k) + (c.h * p.kh + g * p.ks + t * S::KE) * S::kBytes;
-    const char* const vb = static_cast<const char*>(p.v) + (c.h * p.vh + 2 * t * p.vs + g * 2 * S::VW) * S::kBytes;
-    const uint8_t *keb = nullptr, *veb = nullptr;
-    if constexpr (CODES) keb = p.ke + c.h * p.keh + g, veb = p.ve + c.h * p.veh + g;
-    const long k8 = 8 * p.ks * S::kBytes, v1 = p.vs * S::kBytes;
-
-    uint32_t kr[KT][2][S::NKC][S::KW], vr[KT][4][S::NVC][S::VL], vo[KT];
-    uint32_t ke[KT][2], ve[KT][2];  // exponent bytes of the tokens g and g + 8
-    // Slots behind the length are read too (they are slots of the page): K's scores and V are blanked out below.
-    const auto load_k = [&](int tile) {
-      if (tile * KT >= group0 + 32) find_pages(tile * KT);
-#pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        const int i = tile * KT + j - group0;
-        const char* src = kb + static_cast<uint64_t>(__shfl_sync(kFull, k_at, i)) * 16;
-        vo[j] = __shfl_sync(kFull, v_at, i);
-#pragma unroll
-        for (int x = 0; x < S::NKC; ++x) {
-          load_words<S::KW>(kr[j][0][x], src + x * 4 * S::KE * S::kBytes);
-          load_words<S::KW>(kr[j][1][x], src + k8 + x * 4 * S::KE * S::kBytes);
-        }
-        if constexpr (CODES) {
-          const uint8_t* ks = keb + __shfl_sync(kFull, ke_at, i);
-          const uint8_t* vs = veb + __shfl_sync(kFull, ve_at, i);
-          ke[j][0] = __ldg(ks), ke[j][1] = __ldg(ks + 8);
-          ve[j][0] = __ldg(vs), ve[j][1] = __ldg(vs + 8);
-        }
-      }
-    };
-    const auto load_v = [&]() {
-#pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        const char* src = vb + static_cast<uint64_t>(vo[j]) * 16;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int x = 0; x < S::NVC; ++x) {
-            const char* s = src + ((r & 1) + 8 * (r >> 1)) * v1 + x * 16 * S::VW * S::kBytes;
-            if constexpr (S::VB >= 4) load_words<S::VL>(vr[j][r][x], s);
-            else vr[j][r][x][0] = __ldg(reinterpret_cast<const uint16_t*>(s));
-          }
-      }
-    };
-    find_pages(first * KT);
-    load_k(first);
-    load_v();
-
-    // q of query head g of the unit, in the order of K's channels
+    // q of query head g of the unit, in the order of K's channels: index 2t of 16 is channel 2t (codes: 4t), 2t + 8 is 2t + 8
+    // (codes: 4t + 2)
     float unit = a.scale * kLog2e;
-    uint32_t q[S::NKC][S::QW];
+    uint32_t q[S::kSteps][2];
     {
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qt + (c.q0 + g) * a.qh + t * S::KE;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qt + (c.q0 + g) * a.qh + (CODES ? 4 * t : 2 * t);
 #pragma unroll
-      for (int x = 0; x < S::NKC; ++x)
+      for (int x = 0; x < S::kSteps; ++x)
 #pragma unroll
-        for (int i = 0; i < S::QW; ++i) {
-          const uint16_t* s = src + x * 4 * S::KE + 2 * i;
+        for (int i = 0; i < 2; ++i) {
+          const uint16_t* s = src + 16 * x + (CODES ? 2 : 8) * i;
           if (g >= c.nq) q[x][i] = 0;
           else if (a.q_vec) q[x][i] = *reinterpret_cast<const uint32_t*>(s);
           else q[x][i] = s[0] | (static_cast<uint32_t>(s[1]) << 16);
@@ -318,9 +350,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
       // bf16 q in fp16: times 2^(14 - exponent of the head's largest), so that 2^-29 of it is still exact
       uint32_t top = 0;
 #pragma unroll
-      for (int x = 0; x < S::NKC; ++x)
+      for (int x = 0; x < S::kSteps; ++x)
 #pragma unroll
-        for (int i = 0; i < S::QW; ++i) top = max(top, max(q[x][i] & 0x7FFFu, q[x][i] >> 16 & 0x7FFFu));
+        for (int i = 0; i < 2; ++i) top = max(top, max(q[x][i] & 0x7FFFu, q[x][i] >> 16 & 0x7FFFu));
       top = max(top, __shfl_xor_sync(kFull, top, 1));
       top = max(top, __shfl_xor_sync(kFull, top, 2));
       const int e = min(max(static_cast<int>(top >> 7), 40), 254);  // biased; 255: infinity or NaN, which stay
@@ -328,9 +360,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
       const int s0 = (141 - e) / 2, s1 = 141 - e - s0;
       const float f0 = __uint_as_float((127 + s0) << 23), f1 = __uint_as_float((127 + s1) << 23);
 #pragma unroll
-      for (int x = 0; x < S::NKC; ++x)
+      for (int x = 0; x < S::kSteps; ++x)
 #pragma unroll
-        for (int i = 0; i < S::QW; ++i) q[x][i] = pack_f16(lo16<false>(q[x][i]) * f0 * f1, hi16<false>(q[x][i]) * f0 * f1);
+        for (int i = 0; i < 2; ++i) q[x][i] = pack_f16(lo16<false>(q[x][i]) * f0 * f1, hi16<false>(q[x][i]) * f0 * f1);
       const float back0 = __uint_as_float((127 - s0) << 23), back1 = __uint_as_float((127 - s1) << 23);
       const float b0 = __shfl_sync(kFull, back0, 8 * t), b1 = __shfl_sync(kFull, back1, 8 * t);
       const float d0 = __shfl_sync(kFull, back0, 8 * t + 4), d1 = __shfl_sync(kFull, back1, 8 * t + 4);
@@ -344,55 +376,71 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
     for (int tile = first; tile < last; ++tile) {
+      const uint32_t k0 = ring0 + stage * S::kStage, v0 = k0 + S::kKv;
+      if (!mbar_wait(&full[warp][stage], parity, a.status, kSite)) {
+        broken = true;
+        break;
+      }
       // scores: rows are tokens g and g + 8, columns query heads 2t and 2t + 1
       float s[KT][4], vs[KT][2];
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        if constexpr (CODES) {
 #pragma unroll
-        for (int x = 0; x < S::NKC; ++x)
+          for (int x = 0; x < S::kSteps; x += 2) {  // a load is 2 chunks of 16 channels (head dim 16: one, twice)
+            uint32_t r[4];
+            load_matrices(r, k0 + j * S::kGroup + S::chunk(row_k, S::kSteps == 1 ? 0 : x + chunk_k));
+            uint32_t w[4][2];
 #pragma unroll
-          for (int i = 0; i < S::KE / 4; ++i) {  // 16 channels
-            if constexpr (CODES) {
-              uint32_t r0[2], r1[2];
-              widen_word(kr[j][0][x][i], r0);
-              widen_word(kr[j][1][x][i], r1);
-              mma<true>(s[j], r0[0], r1[0], r0[1], r1[1], q[x][2 * i], q[x][2 * i + 1]);
-            } else {
-              mma<F16>(s[j], kr[j][0][x][2 * i], kr[j][1][x][2 * i], kr[j][0][x][2 * i + 1], kr[j][1][x][2 * i + 1],
-                       q[x][2 * i], q[x][2 * i + 1]);
-            }
+            for (int i = 0; i < 4; ++i) widen_word(r[i], w[i]);
+            mma<true>(s[j], w[0][0], w[1][0], w[0][1], w[1][1], q[x][0], q[x][1]);
+            if (x + 1 < S::kSteps) mma<true>(s[j], w[2][0], w[3][0], w[2][1], w[3][1], q[x + 1 < S::kSteps ? x + 1 : 0][0], q[x + 1 < S::kSteps ? x + 1 : 0][1]);
           }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (CODES) s[j][i] *= act8_scale(ke[j][i >> 1]) * q_unit[i & 1];
-          else s[j][i] *= unit;
+          for (int x = 0; x < S::kSteps; ++x) {
+            uint32_t r[4];
+            load_matrices(r, k0 + j * S::kGroup + S::chunk(row_k, 2 * x + chunk_k));
+            mma<F16>(s[j], r[0], r[1], r[2], r[3], q[x][0], q[x][1]);
+          }
         }
-        if constexpr (CODES) vs[j][0] = act8_scale(ve[j][0]), vs[j][1] = act8_scale(ve[j][1]);
+        if constexpr (CODES) {
+          const uint8_t* e = exps + stage * S::kExps + j * 32 + g;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float by = act8_scale(e[8 * r]);
+            vs[j][r] = act8_scale(e[16 + 8 * r]);
+            s[j][2 * r] *= by * q_unit[0], s[j][2 * r + 1] *= by * q_unit[1];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[j][i] *= unit;
+        }
       }
-      if (lost | (tile * KT + KT >= groups)) {  // the last tile, or pages that are none
+      const uint32_t none = lost >> (stage * KT) & ((1u << KT) - 1);
+      if (none | (tile * KT + KT >= groups)) {  // the last tile, or pages that are none
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          const int group = tile * KT + j;
-          const bool none = lost >> (min(group, groups - 1) - group0) & 1;
+          const int token = (tile * KT + j) * 16;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (none) s[j][i] = quiet_nan();
-            if (group * 16 + g + 8 * (i >> 1) >= len) {
+            if (none >> j & 1) s[j][i] = quiet_nan();
+            if (token + g + 8 * (i >> 1) >= len) {
               s[j][i] = -INFINITY;
               if constexpr (CODES) vs[j][i >> 1] = 0.f;
             }
           }
+          if (token + (lane & 15) >= len)  // V behind the length, whatever it is, becomes 0
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (none || group * 16 + 2 * t + (r & 1) + 8 * (r >> 1) >= len)
-#pragma unroll
-              for (int x = 0; x < S::NVC; ++x)
-#pragma unroll
-                for (int i = 0; i < S::VL; ++i) vr[j][r][x][i] = 0;
+            for (int x = 0; x < S::kRow / 16; ++x)
+              if ((x & 1) == lane >> 4 || S::kRow == 16)
+                *reinterpret_cast<uint4*>(ring + stage * S::kStage + S::kKv + j * S::kGroup + (x / (S::kBox / 16)) * 16 * S::kBox +
+                                          (lane & 15) * S::kBox + (x % (S::kBox / 16)) * 16) = make_uint4(0, 0, 0, 0);
         }
+        fence_proxy_async_smem();
+        __syncwarp();
       }
-      if (tile + 1 < last) load_k(tile + 1);  // on its way during the rest of this tile
       // running maximum of each column
       float top[2] = {m[0], m[1]};
 #pragma unroll
@@ -432,34 +480,41 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
           rest[r] = transpose8(pack16<PV16>(w[2 * r] - lo16<PV16>(x), w[2 * r + 1] - hi16<PV16>(x)));
           hi[r] = transpose8(x);
         }
+        // output: rows are channels
+        if constexpr (CODES) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const int x = i / S::VW, k = i % S::VW;
-          uint32_t v[4];
+          for (int i = 0; i < D / 16; i += 2) {
+            uint32_t r[4];
+            load_matrices_t(r, v0 + j * S::kGroup + S::chunk(row_v, S::kSteps == 1 ? 0 : i + chunk_v));
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if constexpr (CODES) {
-              const uint32_t e = vr[j][2 * r][x][k / 2], f = vr[j][2 * r + 1][x][k / 2];
-              v[2 * r] = widen_pair(__byte_perm(e, f, k & 1 ? 0x0602 : 0x0400));
-              v[2 * r + 1] = widen_pair(__byte_perm(e, f, k & 1 ? 0x0703 : 0x0501));
-            } else {
-              const uint32_t e = vr[j][2 * r][x][k], f = vr[j][2 * r + 1][x][k];
-              v[2 * r] = __byte_perm(e, f, 0x5410);
-              v[2 * r + 1] = __byte_perm(e, f, 0x7632);
+            for (int x = 0; x < 2 && i + x < D / 16; ++x) {  // a word: channels 2g and 2g + 1 of two tokens
+              const uint32_t v[4] = {widen_pair(r[2 * x]), widen_pair(r[2 * x] >> 8), widen_pair(r[2 * x + 1]), widen_pair(r[2 * x + 1] >> 8)};
+              mma<PV16>(o[i + x < D / 16 ? i + x : 0], v[0], v[1], v[2], v[3], hi[0], hi[1]);
+              mma<PV16>(o[i + x < D / 16 ? i + x : 0], v[0], v[1], v[2], v[3], rest[0], rest[1]);
             }
           }
-          mma<PV16>(o[i], v[0], v[1], v[2], v[3], hi[0], hi[1]);
-          mma<PV16>(o[i], v[0], v[1], v[2], v[3], rest[0], rest[1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t r[4];
+            load_matrices_t(r, v0 + j * S::kGroup + S::chunk(row_v, 2 * i + chunk_v));
+            mma<PV16>(o[i], r[0], r[1], r[2], r[3], hi[0], hi[1]);
+            mma<PV16>(o[i], r[0], r[1], r[2], r[3], rest[0], rest[1]);
+          }
         }
       }
-      if (tile + 1 < last) load_v();
+      __syncwarp();  // the stage has been read
+      copy_next(stage);
+      if (++stage == stages) stage = 0, parity ^= 1;
     }
+    if (broken) break;
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) {
       l[0] += __shfl_xor_sync(kFull, l[0], x);
       l[1] += __shfl_xor_sync(kFull, l[1], x);
     }
-    const auto channel = [&](int i) { return (i / S::VW) * 16 * S::VW + g * 2 * S::VW + 2 * (i % S::VW); };
+    // channel of row g (x = 0) or g + 8 (x = 1) of output tile i
+    const auto channel = [&](int i, int x) { return 16 * i + (CODES ? 2 * g + x : g + 8 * x); };
     if (first == 0 && last == tiles) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -467,29 +522,40 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
         if (col < c.nq) {
           const long row = static_cast<long>(b) * a.heads_q + c.q0 + col;
           const float inv = 1.f / l[x];
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + row * D;
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * D + channel(i)) =
-                pack16<F16>(o[i][x] * inv, o[i][2 + x] * inv);
+          for (int i = 0; i < D / 16; ++i) {
+            dst[channel(i, 0)] = from_f32<F16>(o[i][x] * inv);
+            dst[channel(i, 1)] = from_f32<F16>(o[i][2 + x] * inv);
+          }
           if (g == 0) a.lse[row] = (m[x] + log2f(l[x])) * kLn2;
         }
       }
     } else {
-      const int mine = 2 * warp + (at != w0 ? 1 : 0);  // a run has at most two such: where it begins, and where it ends
+      // a run has at most two such: where it begins, and where it ends, when the ring is no longer used
+      const int mine = 2 * warp + (at != w0 ? 1 : 0);
       if (lane == 0) seg_unit[mine] = b * n.units + u, seg_first[mine] = first, seg_last[mine] = last, seg_tiles[mine] = tiles;
-      float* dst = part_of<D>(parts, mine, n.cols);
+      float* dst = part(mine);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int col = 2 * t + x;
         if (col < n.cols) {
           if (g == 0) dst[col] = m[x], dst[n.cols + col] = l[x];
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            *reinterpret_cast<float2*>(dst + 2 * n.cols + col * D + channel(i)) = make_float2(o[i][x], o[i][2 + x]);
+          for (int i = 0; i < D / 16; ++i) {
+            dst[2 * n.cols + col * D + channel(i, 0)] = o[i][x];
+            dst[2 * n.cols + col * D + channel(i, 1)] = o[i][2 + x];
+          }
         }
       }
     }
     at += last - first;
+  }
+  if (broken) {  // wait (with a limit) for what is still on its way, which must not outlive the CTA
+    for (int s = 0; s < stages; ++s) {
+      mbar_wait(&full[warp][stage], parity, a.status, kSite);
+      if (++stage == stages) stage = 0, parity ^= 1;
+    }
   }
   if (tid < 2) a.record[2 * blockIdx.x + tid] = make_int2(-1, 0);
   __syncthreads();
@@ -524,9 +590,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attn_kernel(const DecodeAr
       }
       if (col >= c.nq) continue;
       Join j;
-      for (uint32_t s = members; s; s &= s - 1) j.look(part_of<D>(parts, __ffs(s) - 1, n.cols), col);
+      for (uint32_t s = members; s; s &= s - 1) j.look(part(__ffs(s) - 1), col);
       j.looked();
-      for (uint32_t s = members; s; s &= s - 1) j.add(part_of<D>(parts, __ffs(s) - 1, n.cols), n.cols, col, e);
+      for (uint32_t s = members; s; s &= s - 1) j.add(part(__ffs(s) - 1), n.cols, col, e);
       if (whole) {
         j.finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, d, D);
       } else {
@@ -561,19 +627,44 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const DecodeArgs a) {
   j.finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, d, D);
 }
 
+// The cache as a tensor of (channel, slot, head, page), copied 16 slots at a time.
+template <int D, bool CODES>
+CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, long slot) {
+  using S = Shape<D, CODES>;
+  const uint64_t es = CODES ? 1 : 2;
+  const uint64_t sizes[4] = {D, static_cast<uint64_t>(p.size), static_cast<uint64_t>(p.heads), static_cast<uint64_t>(p.pages)};
+  // (the stride of a dimension of one element is whatever it was given, and of no use)
+  const uint64_t strides[3] = {slot * es, p.heads > 1 ? head * es : 16, p.pages > 1 ? page * es : 16};
+  const uint32_t box[4] = {S::kBox / static_cast<uint32_t>(es), 16, 1, 1};
+  return make_tmap(CODES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, sizes, strides, box,
+                   S::kBox == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                   : S::kBox == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                   : S::kBox == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                   : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <int D, bool F16, bool CODES>
 void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
-  const int cols = std::min(a.heads_q / a.pool.heads, kCols);
-  const size_t smem = sizeof(float) * 2 * kWarps * cols * (D + 2);
+  using S = Shape<D, CODES>;
+  const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * cols * (D + 2) * 4 + 1024;
+  // 227 KB of an SM, less 1 KB a CTA and what the kernel declares
+  constexpr int kRoom = (227 * 1024) / S::kCtas - 1024 - 5 * 1024;
+  const int stages = std::min(kMaxStages, (kRoom - parts) / (kWarps * (S::kStage + S::kExps)));
+  const size_t smem = static_cast<size_t>(kWarps) * stages * (S::kStage + S::kExps) + parts;
   const auto kernel = decode_attn_kernel<D, F16, CODES>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use that much shared memory
   const int dev = current_device();
   if (!(ready.load() >> dev & 1)) {
-    HB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(sizeof(float) * 2 * kWarps * kCols * (D + 2))));
+    HB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoom));
     ready.fetch_or(1ull << dev);
   }
-  kernel<<<ctas, kThreads, smem, s>>>(a, whole);
+  const KvPool& p = a.pool;
+  CUtensorMap k_map{}, v_map{};  // a cache of no pages is not read
+  if (p.pages > 0) {
+    k_map = cache_map<D, CODES>(p, p.k, p.kp, p.kh, p.ks);
+    v_map = cache_map<D, CODES>(p, p.v, p.vp, p.vh, p.vs);
+  }
+  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, whole);
   HB_CUDA_CHECK(cudaGetLastError());
   if (whole || ctas == 1) return;
   cudaLaunchConfig_t cfg{};  // launched while the kernel above runs: it waits for its end by itself
@@ -595,17 +686,29 @@ void launch_dim(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
 
 constexpr int kWholeTokens = 256;
 
+// CTAs on an SM, and tokens of a tile.
+struct Fit {
+  int ctas, tokens;
+};
+template <int D>
+Fit fit_dim(bool codes) {
+  if (codes) return {Shape<D, true>::kCtas, Shape<D, true>::kTokens};
+  return {Shape<D, false>::kCtas, Shape<D, false>::kTokens};
+}
+
 }  // namespace
 
-// Two CTAs on every SM, or fewer where the table cannot hold a tile for each of their warps.
-DecodePlan decode_attention_plan(int seqs, int units, int longest) {
+// As many CTAs as the SMs hold, or fewer where the table cannot hold a tile for each of their warps.
+DecodePlan decode_attention_plan(const KvPool& p, int seqs, int units, int longest) {
+  const bool codes = p.type == kKvCodes;
+  const Fit f = p.dim == 16 ? fit_dim<16>(codes) : p.dim == 32 ? fit_dim<32>(codes) : p.dim == 64 ? fit_dim<64>(codes) : fit_dim<128>(codes);
   DecodePlan d;
-  const long tiles = (longest + 15) / 16, fit = (1l << 31) - 1;
-  d.seqs = static_cast<int>(std::min<long>(std::min(seqs, kMaxSeqs), fit / std::max(1l, units * tiles)));
+  const long tiles = (longest + f.tokens - 1) / f.tokens, most = (1l << 31) - 1;
+  d.seqs = static_cast<int>(std::min<long>(std::min(seqs, kMaxSeqs), most / std::max(1l, units * tiles)));
   if (d.seqs == 0) return d;
   d.whole = longest <= kWholeTokens;
-  const long all = static_cast<long>(d.seqs) * units;
-  d.ctas = static_cast<int>(std::max(1l, std::min(2l * num_sms(current_device()), d.whole ? all : (all * tiles + kWarps - 1) / kWarps)));
+  const long all = static_cast<long>(d.seqs) * units, sms = num_sms(current_device());
+  d.ctas = static_cast<int>(std::max(1l, std::min(f.ctas * sms, d.whole ? all : (all * tiles + kWarps - 1) / kWarps)));
   return d;
 }
 

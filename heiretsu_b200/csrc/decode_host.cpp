@@ -21,7 +21,7 @@ namespace hb {
 void kv_write_launch(const KvTokens& t, const KvPool& p, int* status, cudaStream_t s);
 void kv_read_launch(const int64_t* slots, const KvPool& p, void* k, void* v, int n, int out, int* status,
                     cudaStream_t s);
-DecodePlan decode_attention_plan(int seqs, int units, int longest);
+DecodePlan decode_attention_plan(const KvPool& p, int seqs, int units, int longest);
 void decode_attention_launch(const DecodeArgs& a, const DecodePlan& d, cudaStream_t s);
 void sample_tokens_launch(const SampleArgs& a, cudaStream_t s);
 
@@ -106,6 +106,8 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
       TORCH_CHECK(t->scalar_type() == at::kByte && t->sizes() == k.sizes().slice(0, 3) &&
                       (t->stride(2) == 1) && disjoint(*t),
                   op, ": k_exp and v_exp must be uint8 [pages, heads, page size] with contiguous slots");
+      TORCH_CHECK(aligned16(*t) && (t->size(0) <= 1 || t->stride(0) % 16 == 0) && (t->size(1) <= 1 || t->stride(1) % 16 == 0),
+                  op, ": the exponent bytes of a head of a page must start on a 16-byte boundary");
       check_same_device(*t, k.device(), op, "k_exp and v_exp");
     }
     TORCH_CHECK(ke->numel() == 0 || ke->data_ptr() != ve->data_ptr(), op, ": k_exp and v_exp must not be one buffer");
@@ -115,16 +117,6 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
   return p;
 }
 
-// The attention kernel counts slots in units of 16 bytes, and exponent bytes, in 32 bits.
-void check_reach(KvPool& p, const char* op) {
-  const int64_t es = p.type == kKvCodes ? 1 : 2, most = int64_t{1} << 32;
-  const auto reach = [&](long page, long slot) { return (p.pages * page + p.size * slot) * es / 16; };
-  TORCH_CHECK(reach(p.kp, p.ks) < most && reach(p.vp, p.vs) < most && p.pages * p.kep + p.size < most &&
-                  p.pages * p.vep + p.size < most,
-              op, ": k_pages and v_pages must each span less than 64 GB");
-  p.kp16 = static_cast<uint32_t>(p.kp * es / 16), p.ks16 = static_cast<uint32_t>(p.ks * es / 16);
-  p.vp16 = static_cast<uint32_t>(p.vp * es / 16), p.vs16 = static_cast<uint32_t>(p.vs * es / 16);
-}
 void check_slots(const at::Tensor& slots, const char* op) {
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), op,
               ": slots must be contiguous int64 [tokens]");
@@ -208,7 +200,6 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
               op, ": table must be int32 [sequences, pages] with contiguous rows");
   TORCH_CHECK(table.size(1) <= kLongest / a.pool.size, op, ": table is too wide: at most ", std::to_string(kLongest), " tokens");
   check_plain(lengths, at::kInt, {B}, op, "lengths (int32 [sequences])");
-  check_reach(a.pool, op);
   a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(a.pool.dim)));
   TORCH_CHECK(std::isfinite(a.scale), op, ": scale must be finite");
   const at::Device dev = k_pages.device();
@@ -228,7 +219,7 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
   const int G = a.heads_q / a.pool.heads, cols = std::min(G, 8);
   DecodePlan plan;
   for (int64_t b = 0; b < B; b += plan.seqs) {
-    plan = decode_attention_plan(static_cast<int>(B - b), a.pool.heads * ((G + 7) / 8), a.longest);
+    plan = decode_attention_plan(a.pool, static_cast<int>(B - b), a.pool.heads * ((G + 7) / 8), a.longest);
     TORCH_CHECK(plan.seqs > 0, op, ": the table is too wide for so many heads");
     a.seqs = plan.seqs;
     a.q = static_cast<const uint16_t*>(q.data_ptr()) + b * a.qt;
