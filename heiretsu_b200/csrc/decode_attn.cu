@@ -74,48 +74,60 @@ __device__ __forceinline__ void bulk_load_16(uint32_t dst, const void* src, uint
                : "memory");
 }
 
-// Four signed bytes as fp16. A byte with its sign flipped is code + 128; under 0x64 it reads as 1024 + 128 + code, and 1152
-// is taken off.
-__device__ __forceinline__ void widen_word(uint32_t codes, uint32_t (&r)[2]) {
+// Four signed bytes as fp16, in pairs: bytes 0 and 1, 2 and 3 (ALONG), or 0 and 2, 1 and 3. A byte with its sign flipped is
+// code + 128; under 0x64 it reads as 1024 + 128 + code, and 1152 is taken off.
+template <bool ALONG>
+__device__ __forceinline__ void widen(uint32_t codes, uint32_t (&r)[2]) {
   codes ^= 0x80808080u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t x = __byte_perm(codes, 0x64646464u, i ? 0x4342 : 0x4140);
+    const uint32_t x = __byte_perm(codes, 0x64646464u, ALONG ? (i ? 0x4342 : 0x4140) : (i ? 0x4341 : 0x4240));
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-// Two signed bytes (the low ones of `pair`'s halves, whatever lies above them) as bf16, which has 7 fraction bits: under
-// 0x43 the low 7 bits u read as 128 + u, the sign bit as 128 or 256, and their difference is u - 128 sign.
-__device__ __forceinline__ uint32_t widen_pair(uint32_t pair) {
-  const uint32_t x = (pair & 0x007F007Fu) | 0x43004300u, y = (pair & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// The exponent that an exponent byte stands for, NaN for 255.
+__device__ __forceinline__ float exponent_of(uint32_t byte) {
+  return byte == kAct8Nan ? quiet_nan() : __uint_as_float(0x4B000000u | byte) - 8388735.f;  // 2^23 + 127
 }
 
-// A tile of 16 * KT tokens of one K/V head, as it lies in a stage of a warp's ring in shared memory: K, then V, each
-// [KT groups of 16 tokens][boxes of up to 128 bytes of a token][16 tokens][box]; codes have [KT][16 exponent bytes of K, 16
-// of V] besides. The copies swizzle 16-byte chunks of a box by its token, so that the 8 rows of a matrix load
-// lie in different banks.
+// A tile of 16 * KT tokens of one K/V head, as it lies in a stage of a warp's ring in shared memory: K, then V; codes have
+// 16 * KT exponent bytes of K and as many of V besides. A box is what one copy brings: rows of up to 128 bytes, whose 16-byte
+// chunks are swizzled by the row, so that the 8 tokens of a matrix load lie in different banks.
 template <int D, bool CODES>
 struct Shape {
-  static constexpr int kRow = D * (CODES ? 1 : 2);       // bytes of a token
-  static constexpr int kBox = kRow < 128 ? kRow : 128;
-  static constexpr int kBoxes = kRow / kBox;
+  static constexpr int kSize = CODES ? 1 : 2;
+  static constexpr int kRow = D * kSize;                 // bytes of a token
+  static constexpr int kBoxes = kRow <= 128 ? 1 : kRow / 128;  // along the channels
   static constexpr int kGroup = 16 * kRow;               // bytes of 16 tokens
   // 4 KB of K and V (head dim 128 in 16 bits: 8; head dim 16 in codes: 2)
   static constexpr int KT = kGroup >= 2048 ? 1 : kGroup == 1024 ? 2 : 4;
   static constexpr int kTokens = 16 * KT;
   static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
   static constexpr int kStage = 2 * kKv;
-  static constexpr int kExps = CODES ? KT * 32 : 0;      // exponent bytes of a tile, kept apart
+  static constexpr int kExps = CODES ? 2 * kTokens : 0;
   static constexpr int kCtas = kGroup >= 4096 ? 1 : 2;   // on an SM: what the shared memory holds
   static constexpr int kSteps = D / 16;                  // matrix instructions along the channels
-  // byte offset of 16-byte chunk c of token r in a group
-  static __device__ __forceinline__ uint32_t chunk(int r, int c) {
-    constexpr int per = kBox / 16;  // chunks of a box: 8, 4, 2 or 1
-    const int x = per == 8 ? r & 7 : per == 4 ? r >> 1 & 3 : per == 2 ? r >> 2 & 1 : 0;
-    return (c / per) * (16 * kBox) + r * kBox + (((c % per) ^ x) << 4);
+};
+// Where a lane's row of a matrix load is in 16 tokens, the group number j of a tile: chunk(c, j) is that of chunk c (known when
+// compiled) of token r, c without its bits in `c0`. `packed`: the cache's slots follow one another, and where a token is
+// shorter than 128 bytes a row of a box holds several, which the copies bring 2 to 8 times as fast; else a row is a token.
+template <int ROW>
+struct Place {
+  uint32_t at, x, groups;
+  __device__ __forceinline__ Place(int r, int c0, bool packed) : groups(0) {
+    if (ROW >= 128) {
+      at = r * 128, x = (r & 7) ^ c0;
+    } else if (packed) {
+      at = r * ROW & ~127, x = ((r * ROW & 127) >> 4) ^ (r * ROW >> 7 & 7) ^ c0;
+      groups = 7;  // 16 tokens may be fewer than the 8 rows after which the swizzle repeats
+    } else {
+      at = r * ROW, x = (ROW == 64 ? r >> 1 & 3 : ROW == 32 ? r >> 2 & 1 : 0) ^ c0;
+    }
+  }
+  __device__ __forceinline__ uint32_t chunk(int c, int j) const {  // 8 chunks to a box of 16 tokens
+    const uint32_t y = ROW < 64 ? x ^ (j * 16 * ROW / 128 & groups) : x;
+    return j * 16 * ROW + (c >> 3) * 2048 + at + ((y ^ (c & 7)) << 4);
   }
 };
 
@@ -171,14 +183,22 @@ __device__ __forceinline__ int share(int total, int c, int n) {
 // unit that is not wholly its own goes to shared memory, the CTA joins these, and what the CTA has of a unit
 // that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. WHOLE: CTAs take whole
 // units, and nothing is left to join.
+// How copies bring tiles: `packed` as in Place; `joint`: a page holds whole tiles, and one copy brings K of one.
+struct Boxes {
+  bool packed, joint;
+};
+
 template <int D, bool F16, bool CODES>
 __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     decode_attn_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                       const int stages, const bool whole_units) {
+                       const int stages, const Boxes boxes, const bool whole_units) {
   using S = Shape<D, CODES>;
   constexpr int KT = S::KT;
-  constexpr bool QK16 = F16 || CODES;   // codes times q run in fp16 (q scaled by a power of two): fewer instructions to widen
-  constexpr bool PV16 = F16 && !CODES;  // weights times codes run in bf16: 2^e of a head's scale has any exponent
+  // Codes are widened to fp16, in fewer instructions than to bf16. bf16 q is scaled by a power of two for it, and the weights
+  // are those of V times its scale, under a running maximum of their own, so that they fit. fp16 weights are at
+  // most 2^15 instead of 1: then 2^-39 of the largest is still not lost.
+  constexpr bool HALF = F16 || CODES;
+  constexpr float kLift = HALF ? 15.f : 0.f;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1];  // tiles of a unit before each sequence
@@ -187,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   __shared__ uint64_t full[kWarps][kMaxStages];
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x < 2) tma_prefetch_desc(threadIdx.x ? &v_map : &k_map);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const KvPool& p = a.pool;
   const Heads n(a);
@@ -207,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     }
     if (lane == 31) sums[warp] = run;
     if (lane < 2) seg_unit[2 * warp + lane] = -1;
-    if (lane < stages) mbar_init(&full[warp][lane], KT);
+    if (lane < stages) mbar_init(&full[warp][lane], CODES ? 33 : 1);
     fence_barrier_init();
     __syncthreads();
     run -= sum;
@@ -250,103 +271,145 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   };
   const int w0 = c0 + share(c1 - c0, warp, kWarps), w1 = c0 + share(c1 - c0, warp + 1, kWarps);
 
-  // The ring. The copies of a tile are issued as soon as its stage has been read, in the order of the warp's run and across
-  // its units, by the lanes that know the pages: lane i knows that of group number group0 + i of the sequence.
-  uint8_t* const ring = smem + warp * stages * S::kStage;
-  uint8_t* const exps = smem + kWarps * stages * S::kStage + warp * stages * S::kExps;
-  const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(&full[warp][0]);
-  struct {
-    int at, b, u, tile, tiles, groups, group0, page, slot;
-  } next;  // the tile to be copied next
-  next.at = w0;
-  uint32_t lost_pages = 0, lost = 0;  // lanes whose page is none; of the stages' groups, KT bits each
-  const auto unit_at = [&](int at, int& b, int& u, int& tile, int& tiles) {
-    b = 0;  // the last sequence whose tiles begin at or before `at`
-    for (int hi = a.seqs; hi - b > 1;) {
-      const int mid = (b + hi) >> 1;
-      if (prefix[mid] * n.units <= at) b = mid;
+  // A unit on the way through a run.
+  struct Walk {
+    int b, u, h, chunk, tile, tiles;
+  };
+  const auto walk_from = [&](int at) {
+    Walk w{};  // the last sequence whose tiles begin at or before `at`
+    for (int hi = a.seqs; hi - w.b > 1;) {
+      const int mid = (w.b + hi) >> 1;
+      if (prefix[mid] * n.units <= at) w.b = mid;
       else hi = mid;
     }
-    tiles = prefix[b + 1] - prefix[b];
-    const int in_seq = at - prefix[b] * n.units;
-    u = in_seq / tiles;
-    tile = in_seq - u * tiles;
+    w.tiles = prefix[w.b + 1] - prefix[w.b];
+    const int in_seq = at - prefix[w.b] * n.units;
+    w.u = in_seq / w.tiles;
+    w.tile = in_seq - w.u * w.tiles;
+    w.h = w.u / n.chunks;
+    w.chunk = w.u - w.h * n.chunks;
+    return w;
   };
+  const auto next_unit = [&](Walk& w) {
+    w.tile = 0;
+    ++w.u;
+    if (++w.chunk == n.chunks) w.chunk = 0, ++w.h;
+    if (w.u == n.units) {
+      w.u = w.h = 0;
+      do ++w.b;
+      while (prefix[w.b + 1] == prefix[w.b]);
+      w.tiles = prefix[w.b + 1] - prefix[w.b];
+    }
+  };
+
+  // The ring. The copies of a tile are issued as soon as its stage has been read, in the order of the warp's run and across
+  // its units. Lane i knows the page and the first slot of group number group0 + i of the sequence.
+  uint8_t* const ring = smem + warp * stages * S::kStage;
+  uint8_t* const exps = smem + kWarps * stages * S::kStage + warp * stages * S::kExps;
+  const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(&full[warp][0]), exps0 = smem_u32(exps);
+  int left = w1 - w0;  // tiles yet to be copied
+  Walk nx{};
+  int groups = 0, in_window = 32, page = 0, slot = 0;
+  uint32_t lost_pages = 0, lost = 0;  // lanes whose page is none; of the stages' groups, KT bits each
   const auto find_pages = [&]() {
-    next.group0 = next.tile * KT;
-    const int mine = min(next.group0 + lane, next.groups - 1), page = mine / p.groups;
-    next.slot = (mine - page * p.groups) * 16;
-    next.page = a.table[next.b * a.tt + page];
-    lost_pages = __ballot_sync(kFull, next.page < 0 || next.page >= p.pages);
+    const int mine = min(nx.tile * KT + lane, groups - 1), i = mine / p.groups;
+    slot = (mine - i * p.groups) * 16;
+    page = a.table[nx.b * a.tt + i];
+    lost_pages = __ballot_sync(kFull, page < 0 || page >= p.pages);
     if (lost_pages && lane == 0) record_error(a.status, kBadArg, kSite);
+    in_window = 0;
   };
   const auto copy_next = [&](int stage) {
-    if (next.at >= w1) return;
-    if (next.at == w0 || next.tile == next.tiles) {  // another unit
-      unit_at(next.at, next.b, next.u, next.tile, next.tiles);
-      next.groups = (a.lengths[next.b] + 15) >> 4;
-      find_pages();
-    } else if (next.tile * KT >= next.group0 + 32) {
-      find_pages();
+    if (left == 0) return;
+    --left;
+    if (in_window == 32) find_pages();
+    const uint32_t dst = ring0 + stage * S::kStage, bar = bar0 + 8 * stage;
+    const int behind = groups - nx.tile * KT;  // groups of the sequence from here on
+    if (lost | lost_pages) {
+      constexpr uint32_t mask = (1u << KT) - 1;
+      lost = (lost & ~(mask << (stage * KT))) | ((lost_pages >> in_window & mask) << (stage * KT));
     }
-    const int first = next.tile * KT - next.group0, i = lane - first;
-    lost = (lost & ~(((1u << KT) - 1) << (stage * KT))) | ((lost_pages >> first & ((1u << KT) - 1)) << (stage * KT));
-    if (i >= 0 && i < KT) {
-      const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * S::kStage + i * S::kGroup;
-      if (next.tile * KT + i < next.groups) {
-        mbar_arrive_expect_tx(&full[warp][stage], 2 * S::kGroup + (CODES ? 32 : 0));
-        const int h = next.u / n.chunks;
+    if (boxes.joint) {
+      const int pg = __shfl_sync(kFull, page, in_window), at = __shfl_sync(kFull, slot, in_window);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&full[warp][stage], S::kStage);
+        const int row = boxes.packed && S::kRow < 128 ? at * S::kRow / 128 : at;
 #pragma unroll
         for (int x = 0; x < S::kBoxes; ++x) {
-          tma_load_4d(dst + x * 16 * S::kBox, &k_map, bar, x * (S::kBox / (CODES ? 1 : 2)), next.slot, h, next.page);
-          tma_load_4d(dst + S::kKv + x * 16 * S::kBox, &v_map, bar, x * (S::kBox / (CODES ? 1 : 2)), next.slot, h, next.page);
+          tma_load_4d(dst + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, pg);
+          tma_load_4d(dst + S::kKv + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, pg);
         }
-        if constexpr (CODES) {
-          const long page = next.page < 0 || next.page >= p.pages ? 0 : next.page;
-          const uint32_t e = smem_u32(exps) + stage * S::kExps + i * 32;
-          bulk_load_16(e, p.ke + page * p.kep + h * p.keh + next.slot, bar);
-          bulk_load_16(e + 16, p.ve + page * p.vep + h * p.veh + next.slot, bar);
+      }
+    } else {
+      int pg[KT], at[KT];
+#pragma unroll
+      for (int j = 0; j < KT; ++j) pg[j] = __shfl_sync(kFull, page, in_window + j), at[j] = __shfl_sync(kFull, slot, in_window + j);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&full[warp][stage], min(KT, behind) * 2 * S::kGroup);
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          if (j >= behind) break;
+          const int row = boxes.packed && S::kRow < 128 ? at[j] * S::kRow / 128 : at[j];
+#pragma unroll
+          for (int x = 0; x < S::kBoxes; ++x) {
+            tma_load_4d(dst + j * S::kGroup + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, pg[j]);
+            tma_load_4d(dst + S::kKv + j * S::kGroup + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, pg[j]);
+          }
         }
-      } else {
-        mbar_arrive(&full[warp][stage]);
       }
     }
-    ++next.at, ++next.tile;
+    if constexpr (CODES) {  // lane j copies the exponent bytes of K of group j, lane KT + j those of V
+      const int j = lane % KT, pg = __shfl_sync(kFull, page, in_window + j), at = __shfl_sync(kFull, slot, in_window + j);
+      if (lane < 2 * KT && j < behind && pg >= 0 && pg < p.pages) {
+        const uint8_t* src = lane < KT ? p.ke + pg * p.kep + nx.h * p.keh + at : p.ve + pg * p.vep + nx.h * p.veh + at;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(exps0 + stage * S::kExps + lane * 16), "l"(src) : "memory");
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    }
+    in_window += KT;
+    if (++nx.tile == nx.tiles && left > 0) {
+      next_unit(nx);
+      groups = (a.lengths[nx.b] + 15) >> 4;
+      in_window = 32;
+    }
   };
+  Walk w{};
+  if (left > 0) {
+    w = nx = walk_from(w0);
+    groups = (a.lengths[nx.b] + 15) >> 4;
+  }
   for (int s = 0; s < stages; ++s) copy_next(s);
 
   int stage = 0;
   uint32_t parity = 0;
   bool broken = false;  // a copy that did not arrive in time
-  // where this lane's rows of matrix loads are: K of the tokens and chunks, V of the same, by Shape::chunk
-  const int row_k = (lane & 7) + (lane & 8), chunk_k = lane >> 4;
-  const int row_v = CODES ? row_k : (lane & 7) + (lane >> 4) * 8, chunk_v = CODES ? chunk_k : lane >> 3 & 1;
+  const Place<S::kRow> k_row((lane & 7) + (lane & 8), lane >> 4, boxes.packed);
+  const Place<S::kRow> v_row(CODES ? (lane & 7) + (lane & 8) : (lane & 7) + (lane >> 4) * 8,
+                             CODES ? lane >> 4 : lane >> 3 & 1, boxes.packed);
 
-  for (int at = w0; at < w1 && !broken;) {
-    int b, u, first, tiles;
-    unit_at(at, b, u, first, tiles);
-    const int last = min(tiles, first + (w1 - at));
-    const Columns c(n, u);
-    const int len = a.lengths[b], groups = (len + 15) >> 4;  // of 16 tokens
+  for (int at = w0; at < w1;) {
+    const int first = w.tile, last = min(w.tiles, first + (w1 - at)), b = w.b;
+    const int q0 = w.h * n.G + w.chunk * kCols, nq = min(kCols, n.G - w.chunk * kCols);
+    const int len = a.lengths[b];
 
     // q of query head g of the unit, in the order of K's channels: index 2t of 16 is channel 2t (codes: 4t), 2t + 8 is 2t + 8
     // (codes: 4t + 2)
-    float unit = a.scale * kLog2e;
     uint32_t q[S::kSteps][2];
     {
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qt + (c.q0 + g) * a.qh + (CODES ? 4 * t : 2 * t);
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qt + (q0 + g) * a.qh + (CODES ? 4 * t : 2 * t);
 #pragma unroll
       for (int x = 0; x < S::kSteps; ++x)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint16_t* s = src + 16 * x + (CODES ? 2 : 8) * i;
-          if (g >= c.nq) q[x][i] = 0;
+          if (g >= nq) q[x][i] = 0;
           else if (a.q_vec) q[x][i] = *reinterpret_cast<const uint32_t*>(s);
           else q[x][i] = s[0] | (static_cast<uint32_t>(s[1]) << 16);
         }
     }
+    const float unit = a.scale * kLog2e;
     float q_unit[2] = {unit, unit};  // of columns 2t and 2t + 1
-    if constexpr (QK16 && !F16) {
+    if constexpr (CODES && !F16) {
       // bf16 q in fp16: times 2^(14 - exponent of the head's largest), so that 2^-29 of it is still exact
       uint32_t top = 0;
 #pragma unroll
@@ -368,7 +431,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       const float d0 = __shfl_sync(kFull, back0, 8 * t + 4), d1 = __shfl_sync(kFull, back1, 8 * t + 4);
       q_unit[0] = b0 * unit * b1, q_unit[1] = d0 * unit * d1;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of columns 2t and 2t + 1, in powers of 2; l: this lane's rows
+    // Of columns 2t and 2t + 1, in powers of 2: the largest score; codes: the largest score plus exponent of V
+    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY};
+    float l[2] = {0.f, 0.f};  // sum of the weights of this lane's rows
     float o[D / 16][4];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
@@ -382,102 +447,112 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         break;
       }
       // scores: rows are tokens g and g + 8, columns query heads 2t and 2t + 1
-      float s[KT][4], vs[KT][2];
+      float s[KT][4], sv[KT][4];
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
         if constexpr (CODES) {
 #pragma unroll
-          for (int x = 0; x < S::kSteps; x += 2) {  // a load is 2 chunks of 16 channels (head dim 16: one, twice)
-            uint32_t r[4];
-            load_matrices(r, k0 + j * S::kGroup + S::chunk(row_k, S::kSteps == 1 ? 0 : x + chunk_k));
-            uint32_t w[4][2];
+          for (int x = 0; x < S::kSteps; x += 2) {  // a load is 2 chunks of 16 channels (head dim 16: one, and what lies behind)
+            uint32_t r[4], y[4][2];
+            load_matrices(r, k0 + k_row.chunk(x, j));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) widen_word(r[i], w[i]);
-            mma<true>(s[j], w[0][0], w[1][0], w[0][1], w[1][1], q[x][0], q[x][1]);
-            if (x + 1 < S::kSteps) mma<true>(s[j], w[2][0], w[3][0], w[2][1], w[3][1], q[x + 1 < S::kSteps ? x + 1 : 0][0], q[x + 1 < S::kSteps ? x + 1 : 0][1]);
+            for (int i = 0; i < 4; ++i) widen<true>(r[i], y[i]);
+            mma<true>(s[j], y[0][0], y[1][0], y[0][1], y[1][1], q[x][0], q[x][1]);
+            if constexpr (S::kSteps > 1) mma<true>(s[j], y[2][0], y[3][0], y[2][1], y[3][1], q[x + 1][0], q[x + 1][1]);
+          }
+          const uint8_t* e = exps + stage * S::kExps + j * 16 + g;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float by = act8_scale(e[8 * r]), ev = exponent_of(e[S::kTokens + 8 * r]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              s[j][2 * r + i] *= by * q_unit[i];
+              sv[j][2 * r + i] = s[j][2 * r + i] + ev;
+            }
           }
         } else {
 #pragma unroll
           for (int x = 0; x < S::kSteps; ++x) {
             uint32_t r[4];
-            load_matrices(r, k0 + j * S::kGroup + S::chunk(row_k, 2 * x + chunk_k));
+            load_matrices(r, k0 + k_row.chunk(2 * x, j));
             mma<F16>(s[j], r[0], r[1], r[2], r[3], q[x][0], q[x][1]);
           }
-        }
-        if constexpr (CODES) {
-          const uint8_t* e = exps + stage * S::kExps + j * 32 + g;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float by = act8_scale(e[8 * r]);
-            vs[j][r] = act8_scale(e[16 + 8 * r]);
-            s[j][2 * r] *= by * q_unit[0], s[j][2 * r + 1] *= by * q_unit[1];
-          }
-        } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[j][i] *= unit;
         }
       }
       const uint32_t none = lost >> (stage * KT) & ((1u << KT) - 1);
-      if (none | (tile * KT + KT >= groups)) {  // the last tile, or pages that are none
+      if (none | (tile + 1 == w.tiles)) {  // pages that are none, or the sequence's last tile
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          const int token = (tile * KT + j) * 16;
+          const int token = tile * S::kTokens + j * 16;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (none >> j & 1) s[j][i] = quiet_nan();
-            if (token + g + 8 * (i >> 1) >= len) {
-              s[j][i] = -INFINITY;
-              if constexpr (CODES) vs[j][i >> 1] = 0.f;
-            }
+            if (none >> j & 1) s[j][i] = sv[j][i] = quiet_nan();
+            if (token + g + 8 * (i >> 1) >= len) s[j][i] = sv[j][i] = -INFINITY;
           }
-          if (token + (lane & 15) >= len)  // V behind the length, whatever it is, becomes 0
+          // V behind the length, whatever it is, becomes 0
+          const int r = lane & 15;
+          if (token + r >= len) {
+            const uint32_t at0 = stage * S::kStage + S::kKv;
+            const Place<S::kRow> place(r, 0, boxes.packed);
 #pragma unroll
             for (int x = 0; x < S::kRow / 16; ++x)
-              if ((x & 1) == lane >> 4 || S::kRow == 16)
-                *reinterpret_cast<uint4*>(ring + stage * S::kStage + S::kKv + j * S::kGroup + (x / (S::kBox / 16)) * 16 * S::kBox +
-                                          (lane & 15) * S::kBox + (x % (S::kBox / 16)) * 16) = make_uint4(0, 0, 0, 0);
+              if (x % 2 == lane >> 4 || S::kRow == 16) *reinterpret_cast<uint4*>(ring + at0 + place.chunk(x, j)) = make_uint4(0, 0, 0, 0);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
       }
       // running maximum of each column
-      float top[2] = {m[0], m[1]};
+      float top[2] = {m[0], m[1]}, topv[2] = {mv[0], mv[1]};
 #pragma unroll
       for (int j = 0; j < KT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], s[j][i]);
+        for (int i = 0; i < 4; ++i) {
+          top[i & 1] = fmaxf(top[i & 1], s[j][i]);
+          if constexpr (CODES) topv[i & 1] = fmaxf(topv[i & 1], sv[j][i]);
+        }
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) {
-        top[0] = fmaxf(top[0], __shfl_xor_sync(kFull, top[0], x));
-        top[1] = fmaxf(top[1], __shfl_xor_sync(kFull, top[1], x));
-      }
-      if (__any_sync(kFull, top[0] != m[0] || top[1] != m[1])) {
+      for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[i] = fmaxf(top[i], __shfl_xor_sync(kFull, top[i], x));
+          if constexpr (CODES) topv[i] = fmaxf(topv[i], __shfl_xor_sync(kFull, topv[i], x));
+        }
+      if constexpr (!CODES) topv[0] = top[0], topv[1] = top[1];
+      if (__any_sync(kFull, top[0] != m[0] || top[1] != m[1] || (CODES && (topv[0] != mv[0] || topv[1] != mv[1])))) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float f = top[x] == m[x] ? 1.f : ex2(m[x] - top[x]);
-          m[x] = top[x];
-          l[x] *= f;
+          l[x] *= top[x] == m[x] ? 1.f : ex2(m[x] - top[x]);
+          const float f = topv[x] == mv[x] ? 1.f : ex2(mv[x] - topv[x]);
+          m[x] = top[x], mv[x] = topv[x];
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) o[i][x] *= f, o[i][2 + x] *= f;
         }
       }
-      const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+      float ref[2], refv[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        ref[x] = (m[x] == -INFINITY ? 0.f : m[x]) - (CODES ? 0.f : kLift);
+        refv[x] = (mv[x] == -INFINITY ? 0.f : mv[x]) - kLift;
+      }
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         // weights, as the sum of two 16-bit numbers: what one of 8 or 11 bits leaves would show in the output
-        float w[4];
+        float wt[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          w[i] = ex2(s[j][i] - ref[i & 1]);
-          l[i & 1] += w[i];
-          if constexpr (CODES) w[i] *= vs[j][i >> 1];
+          wt[i] = ex2(s[j][i] - ref[i & 1]);
+          l[i & 1] += wt[i];
+          if constexpr (CODES) wt[i] = ex2(sv[j][i] - refv[i & 1]);
         }
         uint32_t hi[2], rest[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t x = pack16<PV16>(w[2 * r], w[2 * r + 1]);
-          rest[r] = transpose8(pack16<PV16>(w[2 * r] - lo16<PV16>(x), w[2 * r + 1] - hi16<PV16>(x)));
+          const uint32_t x = pack16<HALF>(wt[2 * r], wt[2 * r + 1]);
+          rest[r] = transpose8(pack16<HALF>(wt[2 * r] - lo16<HALF>(x), wt[2 * r + 1] - hi16<HALF>(x)));
           hi[r] = transpose8(x);
         }
         // output: rows are channels
@@ -485,21 +560,24 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
 #pragma unroll
           for (int i = 0; i < D / 16; i += 2) {
             uint32_t r[4];
-            load_matrices_t(r, v0 + j * S::kGroup + S::chunk(row_v, S::kSteps == 1 ? 0 : i + chunk_v));
+            load_matrices_t(r, v0 + v_row.chunk(i, j));
 #pragma unroll
-            for (int x = 0; x < 2 && i + x < D / 16; ++x) {  // a word: channels 2g and 2g + 1 of two tokens
-              const uint32_t v[4] = {widen_pair(r[2 * x]), widen_pair(r[2 * x] >> 8), widen_pair(r[2 * x + 1]), widen_pair(r[2 * x + 1] >> 8)};
-              mma<PV16>(o[i + x < D / 16 ? i + x : 0], v[0], v[1], v[2], v[3], hi[0], hi[1]);
-              mma<PV16>(o[i + x < D / 16 ? i + x : 0], v[0], v[1], v[2], v[3], rest[0], rest[1]);
+            for (int x = 0; x < 2; ++x) {  // a word: channels 2g and 2g + 1 of two tokens
+              if (i + x >= D / 16) break;
+              uint32_t y[2], z[2];
+              widen<false>(r[2 * x], y);
+              widen<false>(r[2 * x + 1], z);
+              mma<HALF>(o[i + x], y[0], y[1], z[0], z[1], hi[0], hi[1]);
+              mma<HALF>(o[i + x], y[0], y[1], z[0], z[1], rest[0], rest[1]);
             }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             uint32_t r[4];
-            load_matrices_t(r, v0 + j * S::kGroup + S::chunk(row_v, 2 * i + chunk_v));
-            mma<PV16>(o[i], r[0], r[1], r[2], r[3], hi[0], hi[1]);
-            mma<PV16>(o[i], r[0], r[1], r[2], r[3], rest[0], rest[1]);
+            load_matrices_t(r, v0 + v_row.chunk(2 * i, j));
+            mma<HALF>(o[i], r[0], r[1], r[2], r[3], hi[0], hi[1]);
+            mma<HALF>(o[i], r[0], r[1], r[2], r[3], rest[0], rest[1]);
           }
         }
       }
@@ -513,14 +591,22 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       l[0] += __shfl_xor_sync(kFull, l[0], x);
       l[1] += __shfl_xor_sync(kFull, l[1], x);
     }
+    // the sums of V come under the scores' maximum again; what the weights were lifted by leaves both sums
+#pragma unroll
+    for (int x = 0; x < 2 && HALF; ++x) {
+      const float down = __uint_as_float((127u - 15u) << 23), f = CODES && mv[x] != -INFINITY ? ex2(mv[x] - m[x]) : 1.f;
+      if constexpr (!CODES) l[x] *= down;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[i][x] = o[i][x] * down * f, o[i][2 + x] = o[i][2 + x] * down * f;
+    }
     // channel of row g (x = 0) or g + 8 (x = 1) of output tile i
     const auto channel = [&](int i, int x) { return 16 * i + (CODES ? 2 * g + x : g + 8 * x); };
-    if (first == 0 && last == tiles) {
+    if (first == 0 && last == w.tiles) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int col = 2 * t + x;
-        if (col < c.nq) {
-          const long row = static_cast<long>(b) * a.heads_q + c.q0 + col;
+        if (col < nq) {
+          const long row = static_cast<long>(b) * a.heads_q + q0 + col;
           const float inv = 1.f / l[x];
           uint16_t* dst = static_cast<uint16_t*>(a.out) + row * D;
 #pragma unroll
@@ -534,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     } else {
       // a run has at most two such: where it begins, and where it ends, when the ring is no longer used
       const int mine = 2 * warp + (at != w0 ? 1 : 0);
-      if (lane == 0) seg_unit[mine] = b * n.units + u, seg_first[mine] = first, seg_last[mine] = last, seg_tiles[mine] = tiles;
+      if (lane == 0) seg_unit[mine] = b * n.units + w.u, seg_first[mine] = first, seg_last[mine] = last, seg_tiles[mine] = w.tiles;
       float* dst = part(mine);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -550,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       }
     }
     at += last - first;
+    if (at < w1) next_unit(w);
   }
   if (broken) {  // wait (with a limit) for what is still on its way, which must not outlive the CTA
     for (int s = 0; s < stages; ++s) {
@@ -627,20 +714,24 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const DecodeArgs a) {
   j.finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, d, D);
 }
 
-// The cache as a tensor of (channel, slot, head, page), copied 16 slots at a time.
+// The cache as a tensor of (channel, slot, head, page) or, packed, of (byte of 128, row of 128 bytes, head, page).
 template <int D, bool CODES>
-CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, long slot) {
+CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, long slot, Boxes boxes) {
   using S = Shape<D, CODES>;
-  const uint64_t es = CODES ? 1 : 2;
-  const uint64_t sizes[4] = {D, static_cast<uint64_t>(p.size), static_cast<uint64_t>(p.heads), static_cast<uint64_t>(p.pages)};
+  const uint64_t es = S::kSize;
+  const bool join = boxes.packed && S::kRow < 128;
+  const uint32_t tokens = boxes.joint ? S::kTokens : 16;
+  const uint64_t wide = join ? 128 / es : D, rows = join ? static_cast<uint64_t>(p.size) * S::kRow / 128 : p.size;
+  const uint64_t sizes[4] = {wide, rows, static_cast<uint64_t>(p.heads), static_cast<uint64_t>(p.pages)};
   // (the stride of a dimension of one element is whatever it was given, and of no use)
-  const uint64_t strides[3] = {slot * es, p.heads > 1 ? head * es : 16, p.pages > 1 ? page * es : 16};
-  const uint32_t box[4] = {S::kBox / static_cast<uint32_t>(es), 16, 1, 1};
+  const uint64_t strides[3] = {join ? 128 : slot * es, p.heads > 1 ? head * es : 16, p.pages > 1 ? page * es : 16};
+  const int line = join || S::kRow >= 128 ? 128 : S::kRow;
+  const uint32_t box[4] = {line / static_cast<uint32_t>(es), join ? tokens * S::kRow / 128 : tokens, 1, 1};
   return make_tmap(CODES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, sizes, strides, box,
-                   S::kBox == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                   : S::kBox == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                   : S::kBox == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
-                                   : CU_TENSOR_MAP_SWIZZLE_NONE);
+                   line == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                   : line == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                   : line == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <int D, bool F16, bool CODES>
@@ -659,12 +750,13 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
     ready.fetch_or(1ull << dev);
   }
   const KvPool& p = a.pool;
+  const Boxes boxes{p.ks == D && p.vs == D, p.size % S::kTokens == 0};
   CUtensorMap k_map{}, v_map{};  // a cache of no pages is not read
   if (p.pages > 0) {
-    k_map = cache_map<D, CODES>(p, p.k, p.kp, p.kh, p.ks);
-    v_map = cache_map<D, CODES>(p, p.v, p.vp, p.vh, p.vs);
+    k_map = cache_map<D, CODES>(p, p.k, p.kp, p.kh, p.ks, boxes);
+    v_map = cache_map<D, CODES>(p, p.v, p.vp, p.vh, p.vs, boxes);
   }
-  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, whole);
+  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, boxes, whole);
   HB_CUDA_CHECK(cudaGetLastError());
   if (whole || ctas == 1) return;
   cudaLaunchConfig_t cfg{};  // launched while the kernel above runs: it waits for its end by itself
