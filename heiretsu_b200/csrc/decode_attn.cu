@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   constexpr float kLift = HALF ? 15.f : 0.f;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int prefix[kMaxSeqs + 1];  // tiles of a unit before each sequence
+  __shared__ int prefix[kMaxSeqs + 1], lens[kMaxSeqs];  // tiles of a unit before each sequence; their lengths
   __shared__ int sums[kWarps];
   __shared__ int seg_unit[2 * kWarps], seg_first[2 * kWarps], seg_last[2 * kWarps], seg_tiles[2 * kWarps];
   __shared__ uint64_t full[kWarps][kMaxStages];
@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     int sum = 0;
     for (int b = b0; b < min(b0 + per, a.seqs); ++b) {
       const int len = a.lengths[b];
+      lens[b] = len;
       prefix[b + 1] = len > 0 && len <= a.longest ? (len + S::kTokens - 1) / S::kTokens : 0;
       sum += prefix[b + 1];
     }
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   // sequences without a tile: nothing cached, or a length that is none
   for (int b = blockIdx.x; b < a.seqs; b += gridDim.x) {
     if (prefix[b + 1] != prefix[b]) continue;
-    const bool bad = a.lengths[b] != 0;
+    const bool bad = lens[b] != 0;
     if (bad && tid == 0) record_error(a.status, kBadArg, kSite);
     for (int i = tid; i < a.heads_q * D; i += kThreads)
       static_cast<uint16_t*>(a.out)[static_cast<long>(b) * a.heads_q * D + i] = from_f32<F16>(bad ? quiet_nan() : 0.f);
@@ -309,20 +310,30 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(&full[warp][0]), exps0 = smem_u32(exps);
   int left = w1 - w0;  // tiles yet to be copied
   Walk nx{};
-  int groups = 0, in_window = 32, page = 0, slot = 0;
+  int groups = 0, in_window = 32, page = 0, slot = 0, page_ahead = 0, slot_ahead = 0;
   uint32_t lost_pages = 0, lost = 0;  // lanes whose page is none; of the stages' groups, KT bits each
-  const auto find_pages = [&]() {
-    const int mine = min(nx.tile * KT + lane, groups - 1), i = mine / p.groups;
-    slot = (mine - i * p.groups) * 16;
-    page = a.table[nx.b * a.tt + i];
+  // The next 32 groups' places are on their way while those of the present ones are used.
+  const auto look_ahead = [&](const Walk& f) {
+    const int mine = min(f.tile * KT + lane, (lens[f.b] + 15) / 16 - 1), i = mine / p.groups;
+    slot_ahead = (mine - i * p.groups) * 16;
+    page_ahead = a.table[f.b * a.tt + i];
+  };
+  const auto next_window = [&]() {
+    page = page_ahead, slot = slot_ahead;
     lost_pages = __ballot_sync(kFull, page < 0 || page >= p.pages);
     if (lost_pages && lane == 0) record_error(a.status, kBadArg, kSite);
     in_window = 0;
+    Walk f = nx;
+    const int more = nx.tiles - nx.tile - 1;  // tiles of the unit behind this one
+    if (more >= 32 / KT) f.tile += 32 / KT;
+    else if (left > more) next_unit(f);
+    else return;
+    look_ahead(f);
   };
   const auto copy_next = [&](int stage) {
     if (left == 0) return;
     --left;
-    if (in_window == 32) find_pages();
+    if (in_window == 32) next_window();
     const uint32_t dst = ring0 + stage * S::kStage, bar = bar0 + 8 * stage;
     const int behind = groups - nx.tile * KT;  // groups of the sequence from here on
     if (lost | lost_pages) {
@@ -369,14 +380,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     in_window += KT;
     if (++nx.tile == nx.tiles && left > 0) {
       next_unit(nx);
-      groups = (a.lengths[nx.b] + 15) >> 4;
+      groups = (lens[nx.b] + 15) >> 4;
       in_window = 32;
     }
   };
   Walk w{};
   if (left > 0) {
     w = nx = walk_from(w0);
-    groups = (a.lengths[nx.b] + 15) >> 4;
+    groups = (lens[nx.b] + 15) >> 4;
+    look_ahead(nx);
   }
   for (int s = 0; s < stages; ++s) copy_next(s);
 
@@ -387,25 +399,35 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   const Place<S::kRow> v_row(CODES ? (lane & 7) + (lane & 8) : (lane & 7) + (lane >> 4) * 8,
                              CODES ? lane >> 4 : lane >> 3 & 1, boxes.packed);
 
-  for (int at = w0; at < w1;) {
-    const int first = w.tile, last = min(w.tiles, first + (w1 - at)), b = w.b;
-    const int q0 = w.h * n.G + w.chunk * kCols, nq = min(kCols, n.G - w.chunk * kCols);
-    const int len = a.lengths[b];
-
-    // q of query head g of the unit, in the order of K's channels: index 2t of 16 is channel 2t (codes: 4t), 2t + 8 is 2t + 8
-    // (codes: 4t + 2)
-    uint32_t q[S::kSteps][2];
-    {
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qt + (q0 + g) * a.qh + (CODES ? 4 * t : 2 * t);
+  // q of query head g of a unit, in the order of K's channels: index 2t of 16 is channel 2t (codes: 4t), 2t + 8 is 2t + 8
+  // (codes: 4t + 2). That of the next unit is on its way during the present one.
+  uint32_t q[S::kSteps][2], q_ahead[S::kSteps][2];
+  const auto load_q = [&](const Walk& f) {
+    const int head = f.chunk * kCols + g;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + f.b * a.qt + (f.h * n.G + head) * a.qh + (CODES ? 4 * t : 2 * t);
 #pragma unroll
-      for (int x = 0; x < S::kSteps; ++x)
+    for (int x = 0; x < S::kSteps; ++x)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint16_t* s = src + 16 * x + (CODES ? 2 : 8) * i;
-          if (g >= nq) q[x][i] = 0;
-          else if (a.q_vec) q[x][i] = *reinterpret_cast<const uint32_t*>(s);
-          else q[x][i] = s[0] | (static_cast<uint32_t>(s[1]) << 16);
+      for (int i = 0; i < 2; ++i) {
+        const uint16_t* s = src + 16 * x + (CODES ? 2 : 8) * i;
+        q_ahead[x][i] = 0;
+        if (g < kCols && head < n.G) {
+          if (a.q_vec) q_ahead[x][i] = *reinterpret_cast<const uint32_t*>(s);
+          else q_ahead[x][i] = s[0] | (static_cast<uint32_t>(s[1]) << 16);
         }
+      }
+  };
+  if (w0 < w1) load_q(w);
+
+  for (int at = w0; at < w1;) {
+    const int first = w.tile, last = min(w.tiles, first + (w1 - at)), b = w.b, u = w.u, tiles = w.tiles;
+    const int q0 = w.h * n.G + w.chunk * kCols, nq = min(kCols, n.G - w.chunk * kCols);
+    const int len = lens[b];
+#pragma unroll
+    for (int x = 0; x < S::kSteps; ++x) q[x][0] = q_ahead[x][0], q[x][1] = q_ahead[x][1];
+    if (at + last - first < w1) {
+      next_unit(w);
+      load_q(w);
     }
     const float unit = a.scale * kLog2e;
     float q_unit[2] = {unit, unit};  // of columns 2t and 2t + 1
@@ -483,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         }
       }
       const uint32_t none = lost >> (stage * KT) & ((1u << KT) - 1);
-      if (none | (tile + 1 == w.tiles)) {  // pages that are none, or the sequence's last tile
+      if (none | (tile + 1 == tiles)) {  // pages that are none, or the sequence's last tile
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
           const int token = tile * S::kTokens + j * 16;
@@ -492,18 +514,20 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
             if (none >> j & 1) s[j][i] = sv[j][i] = quiet_nan();
             if (token + g + 8 * (i >> 1) >= len) s[j][i] = sv[j][i] = -INFINITY;
           }
-          // V behind the length, whatever it is, becomes 0
+          // V behind the length, whatever it is, becomes 0 (codes are numbers whatever they are)
           const int r = lane & 15;
-          if (token + r >= len) {
+          if (!CODES && token + r >= len) {
             const uint32_t at0 = stage * S::kStage + S::kKv;
             const Place<S::kRow> place(r, 0, boxes.packed);
 #pragma unroll
             for (int x = 0; x < S::kRow / 16; ++x)
-              if (x % 2 == lane >> 4 || S::kRow == 16) *reinterpret_cast<uint4*>(ring + at0 + place.chunk(x, j)) = make_uint4(0, 0, 0, 0);
+              if (x % 2 == lane >> 4) *reinterpret_cast<uint4*>(ring + at0 + place.chunk(x, j)) = make_uint4(0, 0, 0, 0);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
+        if constexpr (!CODES) {
+          if (left > 0) fence_proxy_async_smem();  // before a copy takes the stage again
+          __syncwarp();
+        }
       }
       // running maximum of each column
       float top[2] = {m[0], m[1]}, topv[2] = {mv[0], mv[1]};
@@ -599,44 +623,44 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[i][x] = o[i][x] * down * f, o[i][2 + x] = o[i][2 + x] * down * f;
     }
-    // channel of row g (x = 0) or g + 8 (x = 1) of output tile i
-    const auto channel = [&](int i, int x) { return 16 * i + (CODES ? 2 * g + x : g + 8 * x); };
-    if (first == 0 && last == w.tiles) {
+    if (first == 0 && last == tiles) {
+      const float inv[2] = {1.f / l[0], 1.f / l[1]};
+      const long row = static_cast<long>(b) * a.heads_q + q0;
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + (row + g) * D + (CODES ? 4 * t : 2 * t);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int col = 2 * t + x;
-        if (col < nq) {
-          const long row = static_cast<long>(b) * a.heads_q + q0 + col;
-          const float inv = 1.f / l[x];
-          uint16_t* dst = static_cast<uint16_t*>(a.out) + row * D;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            dst[channel(i, 0)] = from_f32<F16>(o[i][x] * inv);
-            dst[channel(i, 1)] = from_f32<F16>(o[i][2 + x] * inv);
+      for (int i = 0; i < D / 16; ++i) {  // transposed, a lane has neighbouring channels of head g
+        const uint32_t x = transpose8(pack16<F16>(o[i][0] * inv[0], o[i][1] * inv[1]));
+        const uint32_t y = transpose8(pack16<F16>(o[i][2] * inv[0], o[i][3] * inv[1]));
+        if (g < nq) {
+          if constexpr (CODES) {
+            *reinterpret_cast<uint2*>(dst + 16 * i) = make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+          } else {
+            *reinterpret_cast<uint32_t*>(dst + 16 * i) = x;
+            *reinterpret_cast<uint32_t*>(dst + 16 * i + 8) = y;
           }
-          if (g == 0) a.lse[row] = (m[x] + log2f(l[x])) * kLn2;
         }
+      }
+      if (g == 0) {
+        if (2 * t < nq) a.lse[row + 2 * t] = (m[0] + log2f(l[0])) * kLn2;
+        if (2 * t + 1 < nq) a.lse[row + 2 * t + 1] = (m[1] + log2f(l[1])) * kLn2;
       }
     } else {
       // a run has at most two such: where it begins, and where it ends, when the ring is no longer used
       const int mine = 2 * warp + (at != w0 ? 1 : 0);
-      if (lane == 0) seg_unit[mine] = b * n.units + w.u, seg_first[mine] = first, seg_last[mine] = last, seg_tiles[mine] = w.tiles;
+      if (lane == 0) seg_unit[mine] = b * n.units + u, seg_first[mine] = first, seg_last[mine] = last, seg_tiles[mine] = tiles;
       float* dst = part(mine);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int col = 2 * t + x;
         if (col < n.cols) {
           if (g == 0) dst[col] = m[x], dst[n.cols + col] = l[x];
+          float* d = dst + 2 * n.cols + col * D + (CODES ? 2 * g : g);
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            dst[2 * n.cols + col * D + channel(i, 0)] = o[i][x];
-            dst[2 * n.cols + col * D + channel(i, 1)] = o[i][2 + x];
-          }
+          for (int i = 0; i < D / 16; ++i) d[16 * i] = o[i][x], d[16 * i + (CODES ? 1 : 8)] = o[i][2 + x];
         }
       }
     }
     at += last - first;
-    if (at < w1) next_unit(w);
   }
   if (broken) {  // wait (with a limit) for what is still on its way, which must not outlive the CTA
     for (int s = 0; s < stages; ++s) {
@@ -739,7 +763,7 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   using S = Shape<D, CODES>;
   const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * cols * (D + 2) * 4 + 1024;
   // 227 KB of an SM, less 1 KB a CTA and what the kernel declares
-  constexpr int kRoom = (227 * 1024) / S::kCtas - 1024 - 5 * 1024;
+  constexpr int kRoom = (227 * 1024) / S::kCtas - 1024 - 9 * 1024;
   const int stages = std::min(kMaxStages, (kRoom - parts) / (kWarps * (S::kStage + S::kExps)));
   const size_t smem = static_cast<size_t>(kWarps) * stages * (S::kStage + S::kExps) + parts;
   const auto kernel = decode_attn_kernel<D, F16, CODES>;
