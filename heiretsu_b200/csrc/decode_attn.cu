@@ -14,7 +14,8 @@ namespace hb {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kWarps = 8;                       // that compute; one more copies
+constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kCols = 8;        // query heads of a unit: the columns of one matrix instruction
 constexpr int kSite = 430;      // status site
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -23,6 +24,16 @@ constexpr uint32_t kFull = 0xffffffffu;
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
@@ -61,6 +72,18 @@ __device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
                : "r"(at)
                : "memory");
 }
+// Whether the phase with the given parity has completed.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Asynchronous copies into this CTA's shared memory: a box of a 4-D tensor, and 16 bytes.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
@@ -68,10 +91,8 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-__device__ __forceinline__ void bulk_load_16(uint32_t dst, const void* src, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst),
-               "l"(src), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void copy_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Four signed bytes as fp16, in pairs: bytes 0 and 1, 2 and 3 (ALONG), or 0 and 2, 1 and 3. A byte with its sign flipped is
@@ -167,7 +188,7 @@ struct Join {
   template <bool F16>
   __device__ __forceinline__ void finish(const DecodeArgs& a, long row, int d, int D) const {
     static_cast<uint16_t*>(a.out)[row * D + d] = from_f32<F16>(acc / sum);
-    if (d == 0) a.lse[row] = (top + log2f(sum)) * kLn2;
+    if (d == 0) a.lse[row] = (top + lg2(sum)) * kLn2;
   }
 };
 
@@ -202,9 +223,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1], lens[kMaxSeqs];  // tiles of a unit before each sequence; their lengths
-  __shared__ int sums[kWarps];
+  __shared__ int sums[kWarps + 1];
   __shared__ int seg_unit[2 * kWarps], seg_first[2 * kWarps], seg_last[2 * kWarps], seg_tiles[2 * kWarps];
-  __shared__ uint64_t full[kWarps][kMaxStages];
+  __shared__ uint64_t full[kWarps][kMaxStages], empty[kWarps][kMaxStages];
+  __shared__ uint32_t lost[kWarps][kMaxStages];  // groups of a stage's tile whose page is none
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x < 2) tma_prefetch_desc(threadIdx.x ? &v_map : &k_map);
@@ -213,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   const Heads n(a);
 
   {  // tiles of a unit before each sequence
-    const int per = (a.seqs + kThreads - 1) / kThreads, b0 = tid * per;  // at most 4
+    const int per = (a.seqs + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, a.seqs);  // at most 4
     int sum = 0;
     for (int b = b0; b < min(b0 + per, a.seqs); ++b) {
       const int len = a.lengths[b];
@@ -228,8 +250,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       if (lane >= o) run += x;
     }
     if (lane == 31) sums[warp] = run;
-    if (lane < 2) seg_unit[2 * warp + lane] = -1;
-    if (lane < stages) mbar_init(&full[warp][lane], CODES ? 33 : 1);
+    if (tid < 2 * kWarps) seg_unit[tid] = -1;
+    if (warp < kWarps && lane < stages) {
+      mbar_init(&full[warp][lane], CODES ? 2 : 1);
+      mbar_init(&empty[warp][lane], 1);
+    }
     fence_barrier_init();
     __syncthreads();
     run -= sum;
@@ -270,8 +295,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   const auto part = [&](int i) {
     return reinterpret_cast<float*>(smem + (i & 1 ? (i >> 1) * stages * S::kStage : kWarps * stages * (S::kStage + S::kExps) + (i >> 1) * n.cols * (D + 2) * 4));
   };
-  const int w0 = c0 + share(c1 - c0, warp, kWarps), w1 = c0 + share(c1 - c0, warp + 1, kWarps);
-
   // A unit on the way through a run.
   struct Walk {
     int b, u, h, chunk, tile, tiles;
@@ -303,95 +326,112 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     }
   };
 
-  // The ring. The copies of a tile are issued as soon as its stage has been read, in the order of the warp's run and across
-  // its units. Lane i knows the page and the first slot of group number group0 + i of the sequence.
-  uint8_t* const ring = smem + warp * stages * S::kStage;
-  uint8_t* const exps = smem + kWarps * stages * S::kStage + warp * stages * S::kExps;
-  const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(&full[warp][0]), exps0 = smem_u32(exps);
-  int left = w1 - w0;  // tiles yet to be copied
-  Walk nx{};
-  int groups = 0, in_window = 32, page = 0, slot = 0, page_ahead = 0, slot_ahead = 0;
-  uint32_t lost_pages = 0, lost = 0;  // lanes whose page is none; of the stages' groups, KT bits each
-  // The next 32 groups' places are on their way while those of the present ones are used.
-  const auto look_ahead = [&](const Walk& f) {
-    const int mine = min(f.tile * KT + lane, (lens[f.b] + 15) / 16 - 1), i = mine / p.groups;
-    slot_ahead = (mine - i * p.groups) * 16;
-    page_ahead = a.table[f.b * a.tt + i];
-  };
-  const auto next_window = [&]() {
-    page = page_ahead, slot = slot_ahead;
-    lost_pages = __ballot_sync(kFull, page < 0 || page >= p.pages);
-    if (lost_pages && lane == 0) record_error(a.status, kBadArg, kSite);
-    in_window = 0;
-    Walk f = nx;
-    const int more = nx.tiles - nx.tile - 1;  // tiles of the unit behind this one
-    if (more >= 32 / KT) f.tile += 32 / KT;
-    else if (left > more) next_unit(f);
-    else return;
-    look_ahead(f);
-  };
-  const auto copy_next = [&](int stage) {
-    if (left == 0) return;
-    --left;
-    if (in_window == 32) next_window();
-    const uint32_t dst = ring0 + stage * S::kStage, bar = bar0 + 8 * stage;
-    const int behind = groups - nx.tile * KT;  // groups of the sequence from here on
-    if (lost | lost_pages) {
-      constexpr uint32_t mask = (1u << KT) - 1;
-      lost = (lost & ~(mask << (stage * KT))) | ((lost_pages >> in_window & mask) << (stage * KT));
-    }
-    if (boxes.joint) {
-      const int pg = __shfl_sync(kFull, page, in_window), at = __shfl_sync(kFull, slot, in_window);
-      if (elect_one()) {
-        mbar_arrive_expect_tx(&full[warp][stage], S::kStage);
-        const int row = boxes.packed && S::kRow < 128 ? at * S::kRow / 128 : at;
+  uint8_t* const exps_at = smem + kWarps * stages * S::kStage;
+  if (warp == kWarps) {
+    // Lane i keeps the ring of warp i filled: the copies of a tile are issued when its stage has been read, in the order of the
+    // warp's run and across its units. The places of the next tile are on their way meanwhile.
+    const int run = min(lane, kWarps - 1), w0 = c0 + share(c1 - c0, run, kWarps);
+    int left = lane < kWarps ? c0 + share(c1 - c0, run + 1, kWarps) - w0 : 0;
+    Walk nx{};
+    int len = 0, index = 0, slot = 0, page[KT];  // index, slot: of the tile's first token in the row of the table and in its page
+    const auto look_ahead = [&]() {
+      int i = index, s = slot;
 #pragma unroll
-        for (int x = 0; x < S::kBoxes; ++x) {
-          tma_load_4d(dst + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, pg);
-          tma_load_4d(dst + S::kKv + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, pg);
-        }
+      for (int j = 0; j < KT; ++j) {
+        page[j] = -1;
+        if (nx.tile * S::kTokens + 16 * j < len) page[j] = __ldg(a.table + nx.b * a.tt + i);
+        if (boxes.joint) break;
+        s += 16;
+        if (s == p.size) s = 0, ++i;
       }
-    } else {
-      int pg[KT], at[KT];
+    };
+    const auto enter = [&]() {
+      len = lens[nx.b];
+      index = nx.tile * S::kTokens / p.size;
+      slot = nx.tile * S::kTokens - index * p.size;
+    };
+    if (left > 0) {
+      nx = walk_from(w0);
+      enter();
+      look_ahead();
+    }
+    int stage = 0;
+    uint32_t parity = 1;
+    uint64_t since = globaltimer_ns();
+    for (uint32_t turn = 0; __any_sync(kFull, left > 0); ++turn) {
+      const bool ready = left > 0 && mbar_test(&empty[run][stage], parity);
+      if (ready) {
+        const uint32_t dst = smem_u32(smem) + (run * stages + stage) * S::kStage, bar = smem_u32(&full[run][stage]);
+        const int behind = (len + 15) / 16 - nx.tile * KT;  // groups of the sequence from here on
+        uint32_t none = 0;
+        int i = index, s = slot;
 #pragma unroll
-      for (int j = 0; j < KT; ++j) pg[j] = __shfl_sync(kFull, page, in_window + j), at[j] = __shfl_sync(kFull, slot, in_window + j);
-      if (elect_one()) {
-        mbar_arrive_expect_tx(&full[warp][stage], min(KT, behind) * 2 * S::kGroup);
+        for (int j = 0; j < KT; ++j) {
+          const int pg = boxes.joint ? page[0] : page[j];
+          const bool bad = pg < 0 || pg >= p.pages;
+          if (j < behind && bad) none |= 1u << j;
+        }
+        if (none) record_error(a.status, kBadArg, kSite);
+        lost[run][stage] = none;
+        mbar_arrive_expect_tx(&full[run][stage], boxes.joint ? S::kStage : min(KT, behind) * 2 * S::kGroup);
+        if (boxes.joint) {
+          const int row = boxes.packed && S::kRow < 128 ? s * S::kRow / 128 : s;
+#pragma unroll
+          for (int x = 0; x < S::kBoxes; ++x) {
+            tma_load_4d(dst + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, page[0]);
+            tma_load_4d(dst + S::kKv + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, page[0]);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
           if (j >= behind) break;
-          const int row = boxes.packed && S::kRow < 128 ? at[j] * S::kRow / 128 : at[j];
+          const int pg = boxes.joint ? page[0] : page[j];
+          if (!boxes.joint) {
+            const int row = boxes.packed && S::kRow < 128 ? s * S::kRow / 128 : s;
 #pragma unroll
-          for (int x = 0; x < S::kBoxes; ++x) {
-            tma_load_4d(dst + j * S::kGroup + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, pg[j]);
-            tma_load_4d(dst + S::kKv + j * S::kGroup + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, pg[j]);
+            for (int x = 0; x < S::kBoxes; ++x) {
+              tma_load_4d(dst + j * S::kGroup + x * 2048, &k_map, bar, x * (128 / S::kSize), row, nx.h, pg);
+              tma_load_4d(dst + S::kKv + j * S::kGroup + x * 2048, &v_map, bar, x * (128 / S::kSize), row, nx.h, pg);
+            }
           }
+          if (CODES && !(none >> j & 1)) {
+            const uint32_t e = smem_u32(exps_at) + (run * stages + stage) * S::kExps + j * 16;
+            copy_16(e, p.ke + pg * p.kep + nx.h * p.keh + s);
+            copy_16(e + S::kTokens, p.ve + pg * p.vep + nx.h * p.veh + s);
+          }
+          s += 16;
+          if (s == p.size) s = 0, ++i;
+        }
+        if constexpr (CODES) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+        if (++stage == stages) stage = 0, parity ^= 1;
+        if (--left > 0) {
+          if (++nx.tile == nx.tiles) {
+            next_unit(nx);
+            enter();
+          } else {
+            index = i, slot = s;
+          }
+          look_ahead();
+        }
+      }
+      if (__any_sync(kFull, ready)) {
+        turn = ~0u;
+      } else if (turn % 1024 == 0) {  // nothing to do: give up where that lasts
+        if (turn == 0) since = globaltimer_ns();
+        else if (globaltimer_ns() - since > HB_WAIT_TIMEOUT_NS) {
+          record_error(a.status, kMbarTimeout, kSite);
+          break;
         }
       }
     }
-    if constexpr (CODES) {  // lane j copies the exponent bytes of K of group j, lane KT + j those of V
-      const int j = lane % KT, pg = __shfl_sync(kFull, page, in_window + j), at = __shfl_sync(kFull, slot, in_window + j);
-      if (lane < 2 * KT && j < behind && pg >= 0 && pg < p.pages) {
-        const uint8_t* src = lane < KT ? p.ke + pg * p.kep + nx.h * p.keh + at : p.ve + pg * p.vep + nx.h * p.veh + at;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(exps0 + stage * S::kExps + lane * 16), "l"(src) : "memory");
-      }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-    }
-    in_window += KT;
-    if (++nx.tile == nx.tiles && left > 0) {
-      next_unit(nx);
-      groups = (lens[nx.b] + 15) >> 4;
-      in_window = 32;
-    }
-  };
-  Walk w{};
-  if (left > 0) {
-    w = nx = walk_from(w0);
-    groups = (lens[nx.b] + 15) >> 4;
-    look_ahead(nx);
+    __syncwarp();
   }
-  for (int s = 0; s < stages; ++s) copy_next(s);
-
+  const int w0 = warp < kWarps ? c0 + share(c1 - c0, warp, kWarps) : 0, w1 = warp < kWarps ? c0 + share(c1 - c0, warp + 1, kWarps) : 0;
+  uint8_t* const ring = smem + warp * stages * S::kStage;
+  uint8_t* const exps = exps_at + warp * stages * S::kExps;
+  const uint32_t ring0 = smem_u32(ring);
+  Walk w{};
+  if (w0 < w1) w = walk_from(w0);
   int stage = 0;
   uint32_t parity = 0;
   bool broken = false;  // a copy that did not arrive in time
@@ -504,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           for (int i = 0; i < 4; ++i) s[j][i] *= unit;
         }
       }
-      const uint32_t none = lost >> (stage * KT) & ((1u << KT) - 1);
+      const uint32_t none = lost[warp][stage];
       if (none | (tile + 1 == tiles)) {  // pages that are none, or the sequence's last tile
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
@@ -525,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           }
         }
         if constexpr (!CODES) {
-          if (left > 0) fence_proxy_async_smem();  // before a copy takes the stage again
+          fence_proxy_async_smem();  // before a copy takes the stage again
           __syncwarp();
         }
       }
@@ -606,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         }
       }
       __syncwarp();  // the stage has been read
-      copy_next(stage);
+      if (lane == 0) mbar_arrive(&empty[warp][stage]);
       if (++stage == stages) stage = 0, parity ^= 1;
     }
     if (broken) break;
@@ -624,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       for (int i = 0; i < D / 16; ++i) o[i][x] = o[i][x] * down * f, o[i][2 + x] = o[i][2 + x] * down * f;
     }
     if (first == 0 && last == tiles) {
-      const float inv[2] = {1.f / l[0], 1.f / l[1]};
+      const float inv[2] = {rcp(l[0]), rcp(l[1])};
       const long row = static_cast<long>(b) * a.heads_q + q0;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + (row + g) * D + (CODES ? 4 * t : 2 * t);
 #pragma unroll
@@ -641,8 +681,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         }
       }
       if (g == 0) {
-        if (2 * t < nq) a.lse[row + 2 * t] = (m[0] + log2f(l[0])) * kLn2;
-        if (2 * t + 1 < nq) a.lse[row + 2 * t + 1] = (m[1] + log2f(l[1])) * kLn2;
+        if (2 * t < nq) a.lse[row + 2 * t] = (m[0] + lg2(l[0])) * kLn2;
+        if (2 * t + 1 < nq) a.lse[row + 2 * t + 1] = (m[1] + lg2(l[1])) * kLn2;
       }
     } else {
       // a run has at most two such: where it begins, and where it ends, when the ring is no longer used
@@ -662,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     }
     at += last - first;
   }
-  if (broken) {  // wait (with a limit) for what is still on its way, which must not outlive the CTA
+  if (broken && warp < kWarps) {  // wait (with a limit) for what is still on its way, which must not outlive the CTA
     for (int s = 0; s < stages; ++s) {
       mbar_wait(&full[warp][stage], parity, a.status, kSite);
       if (++stage == stages) stage = 0, parity ^= 1;
@@ -677,6 +717,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   const uint32_t used = __ballot_sync(kFull, unit >= 0), before = used & ((1u << lane) - 1);
   const int prev = __shfl_sync(kFull, unit, before ? 31 - __clz(before) : 0);
   uint32_t starts = __ballot_sync(kFull, unit >= 0 && (before == 0 || prev != unit));
+  if (warp == kWarps) starts = 0;
   for (int item = warp; starts; starts &= starts - 1) {
     const int i0 = __ffs(starts) - 1;
     const uint32_t rest = starts & (starts - 1);
