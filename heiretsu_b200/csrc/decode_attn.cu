@@ -170,25 +170,71 @@ struct Columns {
   }
 };
 
-// Part of a unit: [cols] maxima, [cols] sums, [cols][D] weighted sums of V.
+// Part of a unit: [cols] maxima, [cols] sums, [cols][D] weighted sums of V; every part and row on 16-byte boundaries.
+__host__ __device__ constexpr int part_head(int cols) { return (2 * cols + 3) & ~3; }
 template <int D>
 __device__ __forceinline__ float* part_of(float* base, int i, int cols) {
-  return base + i * (cols * (D + 2));
+  return base + i * (part_head(cols) + cols * D);
 }
-// Joins element e = column * D + channel of parts: add() each, in order, twice: once for the maximum, once for the sums.
+// A warp joins column `col` of n parts, in order; part(i) gives the address of the i-th. Lane i works out the factor of
+// part i; then each lane sums its share of the D channels, E consecutive ones.
+template <int D>
 struct Join {
-  float top = -INFINITY, ref = 0.f, sum = 0.f, acc = 0.f;
-  __device__ __forceinline__ void look(const float* part, int col) { top = fmaxf(top, part[col]); }
-  __device__ __forceinline__ void looked() { ref = top == -INFINITY ? 0.f : top; }
-  __device__ __forceinline__ void add(const float* part, int cols, int col, int e) {
-    const float f = ex2(part[col] - ref);
-    sum = fmaf(part[cols + col], f, sum);
-    acc = fmaf(part[2 * cols + e], f, acc);
+  static constexpr int E = D >= 32 ? D / 32 : 1;  // head dim 16: half of the lanes have none
+  float top = -INFINITY, sum = 0.f, acc[E] = {};
+  template <class Part>
+  __device__ __forceinline__ void run(int n, int cols, int col, int lane, Part part) {
+    const int d = min(lane * E, D - E);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      float m = -INFINITY, l = 0.f;
+      if (i < n) m = part(i)[col], l = part(i)[cols + col];
+      float t = m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, o));
+      t = fmaxf(t, top);
+      const float ref = t == -INFINITY ? 0.f : t, f = ex2(m - ref), old = ex2(top - ref);
+      l = i < n ? l * f : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(kFull, l, o);
+      sum = sum * old + l;
+#pragma unroll
+      for (int k = 0; k < E; ++k) acc[k] *= old;
+      top = t;
+      const int left = min(32, n - i0);
+#pragma unroll 4
+      for (int k = 0; k < left; ++k) {
+        const float* src = part(i0 + k) + part_head(cols) + col * D + d;
+        const float by = __shfl_sync(kFull, f, k);
+        if constexpr (E == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src);
+          acc[0] = fmaf(v.x, by, acc[0]), acc[1] = fmaf(v.y, by, acc[1]);
+          acc[2] = fmaf(v.z, by, acc[2]), acc[3] = fmaf(v.w, by, acc[3]);
+        } else if constexpr (E == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src);
+          acc[0] = fmaf(v.x, by, acc[0]), acc[1] = fmaf(v.y, by, acc[1]);
+        } else {
+          acc[0] = fmaf(*src, by, acc[0]);
+        }
+      }
+    }
   }
   template <bool F16>
-  __device__ __forceinline__ void finish(const DecodeArgs& a, long row, int d, int D) const {
-    static_cast<uint16_t*>(a.out)[row * D + d] = from_f32<F16>(acc / sum);
-    if (d == 0) a.lse[row] = (top + lg2(sum)) * kLn2;
+  __device__ __forceinline__ void finish(const DecodeArgs& a, long row, int lane) const {
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + row * D + lane * E;
+    const float inv = rcp(sum);
+    if (lane * E < D) {
+      if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
+      else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = pack16<F16>(acc[0] * inv, acc[1] * inv);
+      else *dst = from_f32<F16>(acc[0] * inv);
+    }
+    if (lane == 0) a.lse[row] = (top + lg2(sum)) * kLn2;
+  }
+  __device__ __forceinline__ void keep(float* dst, int cols, int col, int lane) const {
+    if (lane * E < D)
+#pragma unroll
+      for (int k = 0; k < E; ++k) dst[part_head(cols) + col * D + lane * E + k] = acc[k];
+    if (lane == 0) dst[col] = top, dst[cols + col] = sum;
   }
 };
 
@@ -293,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   }
   // number 2 w: where the run of warp w begins; 2 w + 1: where it ends, in its ring
   const auto part = [&](int i) {
-    return reinterpret_cast<float*>(smem + (i & 1 ? (i >> 1) * stages * S::kStage : kWarps * stages * (S::kStage + S::kExps) + (i >> 1) * n.cols * (D + 2) * 4));
+    return reinterpret_cast<float*>(smem + (i & 1 ? (i >> 1) * stages * S::kStage : kWarps * stages * (S::kStage + S::kExps) + (i >> 1) * (part_head(n.cols) + n.cols * D) * 4));
   };
   // A unit on the way through a run.
   struct Walk {
@@ -694,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         const int col = 2 * t + x;
         if (col < n.cols) {
           if (g == 0) dst[col] = m[x], dst[n.cols + col] = l[x];
-          float* d = dst + 2 * n.cols + col * D + (CODES ? 2 * g : g);
+          float* d = dst + part_head(n.cols) + col * D + (CODES ? 2 * g : g);
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) d[16 * i] = o[i][x], d[16 * i + (CODES ? 1 : 8)] = o[i][2 + x];
         }
@@ -711,14 +757,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   if (tid < 2) a.record[2 * blockIdx.x + tid] = make_int2(-1, 0);
   __syncthreads();
 
-  // Parts of units that warps share. Lane i looks at segment i; neighbouring ones of one unit are a set; 32 elements
-  // of a set are an item, and the warps take the items in turn.
+  // Parts of units that warps share. Lane i looks at segment i; neighbouring ones of one unit are a set: the first of them,
+  // and those with which the runs of the warps behind it begin. The warps take the columns of all sets in turn.
   const int unit = lane < 2 * kWarps ? seg_unit[lane] : -1;
   const uint32_t used = __ballot_sync(kFull, unit >= 0), before = used & ((1u << lane) - 1);
   const int prev = __shfl_sync(kFull, unit, before ? 31 - __clz(before) : 0);
   uint32_t starts = __ballot_sync(kFull, unit >= 0 && (before == 0 || prev != unit));
-  if (warp == kWarps) starts = 0;
-  for (int item = warp; starts; starts &= starts - 1) {
+  for (int col = warp; starts; starts &= starts - 1) {
     const int i0 = __ffs(starts) - 1;
     const uint32_t rest = starts & (starts - 1);
     const uint32_t members = used & ~((1u << i0) - 1) & (rest ? (1u << (__ffs(rest) - 1)) - 1 : kFull);
@@ -726,11 +771,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     const Columns c(n, id - b * n.units);
     const bool whole = first == 0 && seg_last[end] == seg_tiles[i0];
     const int slot = 2 * blockIdx.x + (first == 0 ? 1 : 0);
-    float* dst = part_of<D>(a.part, slot, n.cols);
-    const int items = c.nq * D / 32 + (c.nq * D % 32 != 0);
-    for (; item < items; item += kWarps) {
-      const int e = item * 32 + lane, col = e / D, d = e % D;
-      if (item == 0 && lane == 0 && !whole) {
+    for (; col < c.nq; col += kWarps + 1) {
+      if (col == 0 && lane == 0 && !whole) {
         // how many CTAs behind this one have a part of a unit that begins here
         const int left = seg_tiles[i0] - seg_last[end];
         int last_cta = blockIdx.x;
@@ -740,43 +782,31 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         }
         a.record[slot] = make_int2(id, last_cta - blockIdx.x);
       }
-      if (col >= c.nq) continue;
-      Join j;
-      for (uint32_t s = members; s; s &= s - 1) j.look(part(__ffs(s) - 1), col);
-      j.looked();
-      for (uint32_t s = members; s; s &= s - 1) j.add(part(__ffs(s) - 1), n.cols, col, e);
-      if (whole) {
-        j.finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, d, D);
-      } else {
-        dst[2 * n.cols + e] = j.acc;
-        if (d == 0) dst[col] = j.top, dst[n.cols + col] = j.sum;
-      }
+      Join<D> j;
+      j.run(__popc(members), n.cols, col, lane, [&](int i) { return part(i == 0 ? i0 : (i0 | 1) - 1 + 2 * i); });
+      if (whole) j.template finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, lane);
+      else j.keep(part_of<D>(a.part, slot, n.cols), n.cols, col, lane);
     }
-    item -= items;
+    col -= c.nq;
   }
 }
 
-// Joins the parts of the units that CTAs share. CTA (c, y): the unit that begins in CTA c of the kernel above and does not end
-// there, if any; its other parts are the first ones of the CTAs behind. y: which kJoin elements of the unit.
-constexpr int kJoin = 128;
+// Joins the parts of the units that CTAs share. Warp (c, y): column y of the unit that begins in CTA c of the kernel above and does
+// not end there, if any; its other parts are the first ones of the CTAs behind.
 template <int D, bool F16>
-__global__ void __launch_bounds__(kJoin) join_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(32) join_kernel(const DecodeArgs a) {
   const Heads n(a);
-  const int e = blockIdx.y * kJoin + threadIdx.x, col = e / D, d = e % D;
+  const int col = blockIdx.y, lane = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 rec = a.record[2 * blockIdx.x + 1];
   if (rec.x < 0) return;
   const int b = rec.x / n.units;
   const Columns c(n, rec.x - b * n.units);
   if (col >= c.nq) return;
-  const auto part = [&](int i) { return part_of<D>(a.part, 2 * (blockIdx.x + i) + (i == 0 ? 1 : 0), n.cols); };
-  Join j;
-#pragma unroll 4
-  for (int i = 0; i <= rec.y; ++i) j.look(part(i), col);
-  j.looked();
-#pragma unroll 4
-  for (int i = 0; i <= rec.y; ++i) j.add(part(i), n.cols, col, e);
-  j.finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, d, D);
+  Join<D> j;
+  j.run(rec.y + 1, n.cols, col, lane,
+        [&](int i) { return part_of<D>(a.part, 2 * (static_cast<int>(blockIdx.x) + i) + (i == 0 ? 1 : 0), n.cols); });
+  j.template finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, lane);
 }
 
 // The cache as a tensor of (channel, slot, head, page) or, packed, of (byte of 128, row of 128 bytes, head, page).
@@ -802,7 +832,7 @@ CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, l
 template <int D, bool F16, bool CODES>
 void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   using S = Shape<D, CODES>;
-  const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * cols * (D + 2) * 4 + 1024;
+  const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * (part_head(cols) + cols * D) * 4 + 1024;
   // 227 KB of an SM, less 1 KB a CTA and what the kernel declares
   constexpr int kRoom = (227 * 1024) / S::kCtas - 1024 - 9 * 1024;
   const int stages = std::min(kMaxStages, (kRoom - parts) / (kWarps * (S::kStage + S::kExps)));
@@ -825,8 +855,8 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   HB_CUDA_CHECK(cudaGetLastError());
   if (whole || ctas == 1) return;
   cudaLaunchConfig_t cfg{};  // launched while the kernel above runs: it waits for its end by itself
-  cfg.gridDim = dim3(ctas, (cols * D + kJoin - 1) / kJoin);
-  cfg.blockDim = dim3(kJoin);
+  cfg.gridDim = dim3(ctas, cols);
+  cfg.blockDim = dim3(32);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

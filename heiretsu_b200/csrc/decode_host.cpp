@@ -228,7 +228,7 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
     a.out = static_cast<uint16_t*>(out.data_ptr()) + b * out.stride(0);
     a.lse = lse.data_ptr<float>() + b * a.heads_q;
     // two parts and their records for each CTA; each launch its own, as the next may begin before the last has joined its
-    at::Tensor part = at::empty({2l * plan.ctas * (2 + cols * (a.pool.dim + 2))}, lse.options());
+    at::Tensor part = at::empty({2l * plan.ctas * (2 + ((2 * cols + 3) & ~3) + static_cast<long>(cols) * a.pool.dim)}, lse.options());
     a.record = reinterpret_cast<int2*>(part.data_ptr<float>());
     a.part = part.data_ptr<float>() + 4l * plan.ctas;
     decode_attention_launch(a, plan, at::cuda::getCurrentCUDAStream());
