@@ -26,10 +26,11 @@ namespace {
 
 using u64 = unsigned long long;
 constexpr uint32_t kFull = 0xffffffffu;
-constexpr int kEach = 4;   // candidates a thread holds
-constexpr int kBins = 256; // of the histogram of weights, 8 to a factor of 2
-constexpr int kTable = 32; // of 2^(j / 32)
+constexpr int kEach = 4;      // candidates a thread holds
+constexpr int kBins = 256;    // of the histogram of weights, 8 to a factor of 2
+constexpr int kTable = 256;   // of 2^(j / 256)
 constexpr float kFaint = -46.f;  // 2^kFaint is no more than half of 2^-44, with room for the rounding of the exponent
+constexpr float kInf = INFINITY;
 
 // Element types as the host numbers them; keys are unsigned numbers in the order of the logits (-0 counts as 0).
 template <int TYPE>
@@ -37,12 +38,14 @@ struct Type {
   static constexpr bool kWide = TYPE == 2;
   static constexpr int kElems = kWide ? 4 : 8, kBytes = kWide ? 4 : 2;  // of a 16-byte piece, of an element
   static constexpr int kBits = kWide ? 32 : 16;                         // of a key
-  static __device__ __forceinline__ uint32_t key(uint32_t b) {
+  static constexpr uint32_t kNone = TYPE == 2 ? 0xFF800000u : TYPE == 1 ? 0xFC00u : 0xFF80u;  // -inf
+  static __device__ __forceinline__ uint32_t key(float x) {
+    uint32_t b;
     if constexpr (kWide) {
-      if (b == 0x80000000u) b = 0;
+      b = __float_as_uint(x + 0.f);
       return b ^ (static_cast<int>(b) < 0 ? 0xFFFFFFFFu : 0x80000000u);
     } else {
-      if (b == 0x8000u) b = 0;
+      b = from_f32<TYPE == 1>(x + 0.f);
       return b ^ (b & 0x8000u ? 0xFFFFu : 0x8000u);
     }
   }
@@ -54,82 +57,83 @@ struct Type {
     if constexpr (kWide) return value(key ^ (static_cast<int>(key) < 0 ? 0x80000000u : 0xFFFFFFFFu));
     else return value(key ^ (key & 0x8000u ? 0x8000u : 0xFFFFu));
   }
-  // the least key of a logit >= x, x finite or -inf
-  static __device__ __forceinline__ uint32_t key_from(float x) {
+  // the least logit of the type that is >= x, x finite
+  static __device__ __forceinline__ float round_up(float x) {
+    if constexpr (kWide) return x;
+    else if constexpr (TYPE == 1) return __half2float(__float2half_ru(x));
+    else return __bfloat162float(__float2bfloat16_ru(x));
+  }
+  static __device__ __forceinline__ float at(const uint4& r, int e) {  // element e, known when compiled
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (kWide) return value(w[e]);
+    else return e & 1 ? hi16<TYPE == 1>(w[e >> 1]) : lo16<TYPE == 1>(w[e >> 1]);
+  }
+  // the largest element of a piece, NaN where there is one
+  static __device__ __forceinline__ float largest(const uint4& r) {
     if constexpr (kWide) {
-      return key(__float_as_uint(x));
+      return max_nan(max_nan(value(r.x), value(r.y)), max_nan(value(r.z), value(r.w)));
     } else {
-      const uint16_t b = TYPE == 1 ? __half_as_ushort(__float2half_ru(x)) : __bfloat16_as_ushort(__float2bfloat16_ru(x));
-      return key(b);
+      const uint32_t w = max2(max2(r.x, r.y), max2(r.z, r.w));
+      return max_nan(lo16<TYPE == 1>(w), hi16<TYPE == 1>(w));
     }
   }
-  static __device__ __forceinline__ uint32_t bits(const uint4& r, int e) {  // element e, known when compiled
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    if constexpr (kWide) return w[e];
-    else return e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
+  static __device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (TYPE == 1) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
   }
 };
 
-// The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 32) 2^r with |r| <= 1 / 64; the last
-// factor is e^(r ln 2) by its series to degree 5, whose remainder is below (ln 2 / 64)^6 / 720 < 3e-15.
+// The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 256) 2^r with |r| <= 1 / 512; the last
+// factor is e^(r ln 2) by its series to degree 3, whose remainder is below (ln 2 / 512)^4 / 24 < 1.5e-13.
 struct Weigher {
   double top, by;    // by: log2 e / T
   float top32, by32;
-  const double* table;  // 2^(44 + j / 32)
+  const double* table;  // 2^(44 + j / 256)
   __device__ __forceinline__ float exponent(float x) const { return (x - top32) * by32; }  // about; monotone
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (x == top32) return 1ull << 44;
-    if (!(exponent(x) > kFaint)) return 0;
-    const double t = (static_cast<double>(x) - top) * by, shift = 211106232532992.0;  // 1.5 * 2^47
+    const double t = (static_cast<double>(x) - top) * by, shift = 26388279066624.0;  // 1.5 * 2^44
     const double s = t + shift, r = t - (s - shift);
     const int k = __double2loint(s);
-    double p = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);  // (ln 2)^5/5!, (ln 2)^4/4!
-    p = fma(r, p, 5.5504108664821580e-2);                             // (ln 2)^3/3!
-    p = fma(r, p, 2.4022650695910071e-1);                             // (ln 2)^2/2!
+    double p = fma(r, 5.5504108664821580e-2, 2.4022650695910071e-1);  // (ln 2)^3/3!, (ln 2)^2/2!
     p = fma(r, p, 6.9314718055994531e-1);                             // ln 2
     p = fma(r, p, 1.0);
-    p *= table[k & (kTable - 1)];
-    p = __hiloint2double(__double2hiint(p) + (k >> 5 << 20), __double2loint(p));
-    return __double_as_longlong(p + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
-  }
-};
-
-template <int WARPS>
-struct Block {
-  u64 buf[WARPS];
-  __device__ __forceinline__ u64 sum(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = buf[threadIdx.x % WARPS];
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    return v;
+    const double q = table[k & (kTable - 1)];
+    const double scale = __hiloint2double(__double2hiint(q) + (k >> 8 << 20), __double2loint(q));
+    const u64 w = __double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
+    return exponent(x) > kFaint ? w : 0;
   }
 };
 
 // A row as a block sees it: pieces of 16 bytes from the 16-byte boundary at or before its start, `off` elements of the first
 // lying before the row. Warp w has the pieces [w per, (w + 1) per), 32 at a time.
-template <int TYPE, int WARPS>
+template <int TYPE>
 struct Row {
   using P = Type<TYPE>;
   static constexpr int E = P::kElems;
   const char* base;  // of the row
   uint4* copy;       // the pieces in shared memory, or null
-  int V, off, pieces, per;
+  int V, off, pieces, per, first, end;  // first: this thread's first piece; end: behind its warp's last
 
   __device__ __forceinline__ bool inside(int piece) const { return piece * E >= off && (piece + 1) * E <= off + V; }
+  __device__ __forceinline__ uint32_t bits(int i) const {  // of element i of the row
+    if constexpr (P::kWide) return copy ? reinterpret_cast<const uint32_t*>(copy)[off + i] : reinterpret_cast<const uint32_t*>(base)[i];
+    else return copy ? reinterpret_cast<const uint16_t*>(copy)[off + i] : reinterpret_cast<const uint16_t*>(base)[i];
+  }
   // elements outside the row read as -inf
   __device__ __forceinline__ uint4 load(int piece) const {
     if (inside(piece)) return __ldg(reinterpret_cast<const uint4*>(base + (static_cast<long>(piece) * E - off) * P::kBytes));
-    constexpr uint32_t none = TYPE == 2 ? 0xFF800000u : TYPE == 1 ? 0xFC00u : 0xFF80u;
     uint32_t b[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = piece * E - off + e;
-      b[e] = none;
+      b[e] = P::kNone;
       if (i >= 0 && i < V) {
         if constexpr (P::kWide) b[e] = reinterpret_cast<const uint32_t*>(base)[i];
         else b[e] = reinterpret_cast<const uint16_t*>(base)[i];
@@ -138,25 +142,55 @@ struct Row {
     if constexpr (P::kWide) return make_uint4(b[0], b[1], b[2], b[3]);
     else return make_uint4(b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16);
   }
-  __device__ __forceinline__ uint4 again(int piece) const { return copy != nullptr ? copy[piece] : load(piece); }
-  // f(bits, index) for each element of a piece that is in the row
+  // f(piece, its number) for this thread's pieces
   template <class F>
-  __device__ __forceinline__ void each(const uint4& r, int piece, F f) const {
-    const int i0 = piece * E - off;
-    if (inside(piece)) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) f(P::bits(r, e), i0 + e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (i0 + e >= 0 && i0 + e < V) f(P::bits(r, e), i0 + e);
-    }
+  __device__ __forceinline__ void pieces_of(F f) const {
+    if (copy != nullptr)
+      for (int p = first; p < end; p += 32) f(copy[p], p);
+    else
+      for (int p = first; p < end; p += 32) f(load(p), p);
   }
-  // f(bits, index) for each element of this thread's pieces, after the first pass
+  // f(logit, index) for each element of a piece that is in the row and >= from
   template <class F>
-  __device__ __forceinline__ void all(F f) const {
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, end = min((w + 1) * per, pieces);
-    for (int p = w * per + lane; p < end; p += 32) each(again(p), p, f);
+  __device__ __forceinline__ void each(const uint4& r, int piece, float from, F f) const {
+    if (!(P::largest(r) >= from)) return;
+    const int i0 = piece * E - off;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (P::at(r, e) >= from && i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
+  }
+  // f(weight, logit) for each element, all of a piece at once (elements outside the row weigh 0)
+  template <class F>
+  __device__ __forceinline__ void weigh(const uint4& r, const Weigher& weight, F f) const {
+    if (!(weight.exponent(P::largest(r)) > kFaint)) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(weight(P::at(r, e)), P::at(r, e));
+  }
+};
+
+// Sums over a block, in one barrier each: parts of 22, 22 and 20 bits that warps add up in one instruction and the
+// block in shared memory (whole numbers: in any order). Each sum takes new slots, set to 0 beforehand.
+constexpr int kSums = 2 * 33 + 8;  // two searches of 32 bits, and a few
+struct Sums {
+  uint32_t (*slots)[3];
+  int used = 0;
+  __device__ __forceinline__ u64 operator()(u64 v) {
+    uint32_t* s = slots[used++];
+    const uint32_t part[3] = {static_cast<uint32_t>(v & 0x3FFFFF), static_cast<uint32_t>(v >> 22 & 0x3FFFFF), static_cast<uint32_t>(v >> 44)};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t x = __reduce_add_sync(kFull, part[i]);
+      if ((threadIdx.x & 31) == 0 && x != 0) atomicAdd(&s[i], x);
+    }
+    __syncthreads();
+    return s[0] + (static_cast<u64>(s[1]) << 22) + (static_cast<u64>(s[2]) << 44);
+  }
+  __device__ __forceinline__ uint32_t count(uint32_t v) {
+    uint32_t* s = slots[used++];
+    v = __reduce_add_sync(kFull, v);
+    if ((threadIdx.x & 31) == 0 && v != 0) atomicAdd(&s[0], v);
+    __syncthreads();
+    return s[0];
   }
 };
 
@@ -166,16 +200,16 @@ struct Row {
 //      top_k-th largest of the threads' own maxima), go to a list, and the cuts are found among them.
 //      top_p alone: all weights, their sum and a histogram of them, which tells in which bins the cut lies; then the
 //      sum above those bins, and the list of what is in them.
-//   3. the kept weight of each warp's part of the row; the warp whose part holds u times the whole walks its part again.
+//   3. the kept weight of each warp's part of the row; the part that holds u times the whole is looked at by all.
 // Where a list overflows, the cuts are found by halving over the whole row.
 template <int TYPE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const SampleArgs a, const bool resident) {
   constexpr int kWarps = THREADS / 32, kList = kEach * THREADS;
   using P = Type<TYPE>;
   extern __shared__ uint4 smem[];
-  __shared__ Block<kWarps> block;
   __shared__ u64 warp_sums[kWarps];
-  __shared__ uint32_t list[kList], hist[kBins], s_max[kWarps];
+  __shared__ uint32_t list[kList], hist[kBins], slots[kSums][3], warp_ties[kWarps];
+  __shared__ float warp_max[kWarps];
   __shared__ double table[kTable];
   __shared__ int s_bad, s_pick, s_listed, s_bins[2];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -184,91 +218,99 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   const double top_p = a.top_p ? a.top_p[row] : a.top_p0, min_p = a.min_p ? a.min_p[row] : a.min_p0;
   const int64_t top_k = a.top_k ? a.top_k[row] : a.top_k0;
   const double u = a.u[row];
-  Row<TYPE, kWarps> x;
+  Row<TYPE> x;
   x.base = static_cast<const char*>(a.x) + row * a.ld * P::kBytes;
   x.copy = resident ? smem : nullptr;
   x.V = a.V;
   x.off = static_cast<int>(reinterpret_cast<uintptr_t>(x.base) & 15) / P::kBytes;
   x.pieces = (x.off + a.V + x.E - 1) / x.E;
-  x.per = ((x.pieces + kWarps - 1) / kWarps + 31) / 32 * 32;
-  if (x.per * (kWarps - 1) >= x.pieces) x.per = (x.pieces + kWarps - 1) / kWarps;
+  x.per = (x.pieces + kWarps - 1) / kWarps;
+  x.first = warp * x.per + lane;
+  x.end = min((warp + 1) * x.per, x.pieces);
 
-  if (tid == 0) s_bad = T != T || top_p != top_p || min_p != min_p || u != u, s_pick = a.V, s_listed = 0;
-  if (tid < kTable) table[tid] = exp2(44.0 + tid / static_cast<double>(kTable));
-  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
-  uint32_t mine = 0;  // this thread's largest key
-  bool bad = false;
-  {
-    const int end = min((warp + 1) * x.per, x.pieces);
-#pragma unroll 4
-    for (int p = warp * x.per + lane; p < end; p += 32) {
-      const uint4 r = x.load(p);
-      if (resident) smem[p] = r;
-#pragma unroll
-      for (int e = 0; e < x.E; ++e) {
-        bad |= !(P::value(P::bits(r, e)) < INFINITY);
-        mine = max(mine, P::key(P::bits(r, e)));
-      }
-    }
+  float mine = -kInf;  // this thread's largest
+  const auto take = [&](const uint4& r, int p) {
+    if (resident) smem[p] = r;
+    mine = P::max_nan(mine, P::largest(r));
+  };
+  if (x.inside(warp * x.per) && x.inside(x.end - 1)) {  // all of the warp's pieces: their loads are issued together
+    const uint4* src = reinterpret_cast<const uint4*>(x.base - x.off * P::kBytes);
+#pragma unroll 8
+    for (int p = x.first; p < x.end; p += 32) take(__ldg(src + p), p);
+  } else {
+    for (int p = x.first; p < x.end; p += 32) take(x.load(p), p);
   }
-  const uint32_t warp_max = __reduce_max_sync(kFull, mine);
-  if (lane == 0) s_max[warp] = warp_max;
-  __syncthreads();  // also: s_bad is set up
-  if (bad) s_bad = 1;
-  const uint32_t kmax = __reduce_max_sync(kFull, s_max[lane % kWarps]);
+  if (tid == 0) s_pick = a.V, s_listed = 0;
+  for (int i = tid; i < kTable; i += THREADS) table[i] = exp2(44.0 + i / static_cast<double>(kTable));
+  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+  for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
+  float top = mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = P::max_nan(top, __shfl_xor_sync(kFull, top, o));
+  if (lane == 0) warp_max[warp] = top;
   __syncthreads();
-  Weigher weight;
-  weight.top32 = P::logit(kmax);
-  if (s_bad || weight.top32 == -INFINITY) {  // NaN or +inf among the logits, nothing but -inf, a setting that is no number
+  top = warp_max[lane % kWarps];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = P::max_nan(top, __shfl_xor_sync(kFull, top, o));
+  // NaN or +inf among the logits, nothing but -inf, a setting that is no number
+  if (!(top < kInf) || top == -kInf || T != T || top_p != top_p || min_p != min_p || u != u) {
     if (tid == 0) a.tokens[row] = -1;
     return;
   }
   if (T <= 0 || min_p > 1 || top_p <= 0) {  // the first token of the order
-    x.all([&](uint32_t b, int i) {
-      if (P::key(b) == kmax) atomicMin(&s_pick, i);
-    });
+    x.pieces_of([&](const uint4& r, int p) { x.each(r, p, top, [&](float, int i) { atomicMin(&s_pick, i); }); });
     __syncthreads();
     if (tid == 0) a.tokens[row] = s_pick;
     return;
   }
-  weight.top = weight.top32;
+  Weigher weight;
+  weight.top = weight.top32 = top;
   weight.by = fmin(1.4426950408889634 / T, 1.6069380442589903e60);  // 2^200: no two logits are closer than 2^-149
   weight.by32 = static_cast<float>(fmin(weight.by, 3e38));
   weight.table = table;
+  Sums sums{slots};
 
   uint32_t t = 0;  // kept: keys above t, and the first `ties` equal to it
   u64 ties = ~0ull;
+  const uint32_t kmax = P::key(top);
   const bool use_k = top_k > 0 && top_k < a.V, use_p = top_p < 1;
   uint32_t floor_key = 0;  // of min_p
-  if (min_p > 0 && T < INFINITY) floor_key = P::key_from(fmaxf(__double2float_ru(weight.top + T * log(min_p)), -3.4028234663852886e38f));
+  if (min_p > 0 && T < INFINITY)
+    floor_key = min(kmax, P::key(P::round_up(fmaxf(__double2float_ru(weight.top + T * log(min_p)), -3.4028234663852886e38f))));
   const auto need_of = [&](u64 total) { return max(__double2ull_ru(top_p * static_cast<double>(total)), 1ull); };
+  // the largest key c with enough(c), which holds for `low` and not above kmax: only bits below those that low and kmax share
+  const auto search = [&](uint32_t low, auto&& enough) {
+    const int bits = low >= kmax ? 0 : 32 - __clz(low ^ kmax);
+    uint32_t c = bits >= 32 ? 0 : kmax >> bits << bits;
+    for (int bit = bits - 1; bit >= 0; --bit)
+      if ((c | (1u << bit)) <= low || enough(c | (1u << bit))) c |= 1u << bit;
+    return bits == 0 ? kmax : c;
+  };
 
   // ---- candidates
   uint32_t from = 0;        // keys at or above it are listed
   bool listing = false;
   u64 above = 0, need = 0;  // top_p alone: the weight above the listed bins, and what the kept weight has to reach
-  int bin0 = 0, bin1 = kBins;
-  const auto bin_of = [&](float v) { return static_cast<int>(fminf(weight.exponent(v) * -8.f, static_cast<float>(kBins))); };
+  u64 mine_above = 0;       // this thread's part of `above`
+  float e_list = 0.f, e_above = 0.f;  // exponents of the listed bins: above e_list and not above e_above
+  const bool bins = use_p && !use_k;
   if (use_k) {
-    const int have = __syncthreads_count(mine != 0);
-    if (top_k <= have) {
-      for (int bit = P::kBits - 1; bit >= 0; --bit) {
-        const uint32_t c = from | (1u << bit);
-        if (__syncthreads_count(mine >= c) >= top_k) from = c;
-      }
+    const uint32_t key = x.first < x.end ? P::key(mine) : 0;
+    if (top_k <= __syncthreads_count(key != 0)) {
+      from = search(0, [&](uint32_t c) { return __syncthreads_count(key >= c) >= top_k; });
       listing = true;
     }
     if (!use_p && floor_key > from) from = floor_key, listing = true;
   } else if (use_p) {
     u64 sum = 0;
-    x.all([&](uint32_t b, int) {
-      const float v = P::value(b);
-      const u64 w = weight(v);
-      sum += w;
-      const int bin = bin_of(v);
-      if (bin < kBins) atomicAdd(&hist[bin], static_cast<uint32_t>(w >> (32 - (bin >> 3))));  // 11 bits or 12
+    x.pieces_of([&](const uint4& r, int) {
+      x.weigh(r, weight, [&](u64 w, float v) {
+        sum += w;
+        const int bin = static_cast<int>(fminf(weight.exponent(v) * -8.f, static_cast<float>(kBins)));
+        if (bin < kBins) atomicAdd(&hist[bin], static_cast<uint32_t>(w >> (32 - (bin >> 3))));  // 11 bits or 12
+      });
     });
-    need = need_of(block.sum(sum));
+    need = need_of(sums(sum));
     if (warp == 0) {  // first bin whose end may reach `need`, first whose end does
       u64 run = 0, part[kBins / 32];
 #pragma unroll
@@ -297,7 +339,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       if (lane == 0) s_bins[0] = may, s_bins[1] = does;
     }
     __syncthreads();
-    bin0 = s_bins[0], bin1 = s_bins[1];
+    e_above = s_bins[0] / -8.f;
+    e_list = s_bins[1] >= kBins ? -kInf : (s_bins[1] + 1) / -8.f;
     listing = true;
   } else if (floor_key > 0) {
     from = floor_key;
@@ -306,39 +349,43 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   uint32_t key[kEach];
   int n = 0;
   if (listing) {
-    const bool bins = use_p && !use_k;
-    u64 sum = 0;
-    x.all([&](uint32_t b, int) {
-      const uint32_t k = P::key(b);
-      bool take = k >= from;
-      if (bins) {
-        const int bin = bin_of(P::value(b));
-        take = bin >= bin0 && bin <= bin1;
-        if (bin < bin0) sum += weight(P::value(b));
-      }
-      if (take) {
-        const int at = atomicAdd(&s_listed, 1);
-        if (at < kList) list[at] = k;
-      }
-    });
-    if (bins) above = block.sum(sum);
-    __syncthreads();
+    const auto put = [&](float v) {
+      const int at = atomicAdd(&s_listed, 1);
+      if (at < kList) list[at] = P::key(v);
+    };
+    if (bins) {
+      x.pieces_of([&](const uint4& r, int p) {
+        const float e = weight.exponent(P::largest(r));
+        if (e > e_above) x.weigh(r, weight, [&](u64 w, float v) { mine_above += weight.exponent(v) > e_above ? w : 0; });
+        if (!(e > e_list) && e_list > -kInf) return;
+        x.each(r, p, -kInf, [&](float v, int) {
+          const float e = weight.exponent(v);
+          if (!(e > e_above) && (e > e_list || e_list == -kInf)) put(v);
+        });
+      });
+      above = sums(mine_above);
+    } else {
+      const float low = from == 0 ? -kInf : P::logit(from);
+      x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int) { put(v); }); });
+      __syncthreads();
+    }
     n = s_listed;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) key[i] = i * THREADS + tid < n ? list[min(i * THREADS + tid, kList - 1)] : 0;  // 0: none
   }
-  const bool listed = listing && n <= kList && (!use_p || use_k || above < need);
+  const bool listed = listing && n <= kList && (!bins || above < need);
 
   // ---- cuts: counts and sums over the list where there is one, else over the row
-  const auto count = [&](uint32_t c) -> u64 {
+  const auto count = [&](uint32_t c) -> uint32_t {
     uint32_t m = 0;
     if (listed) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) m += key[i] >= c;
     } else {
-      x.all([&](uint32_t b, int) { m += P::key(b) >= c; });
+      const float low = P::logit(c);
+      x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float, int) { ++m; }); });
     }
-    return block.sum(m);
+    return sums.count(m);
   };
   u64 w[kEach];  // of the list
   const auto mass = [&](uint32_t c) -> u64 {
@@ -346,25 +393,26 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     if (listed) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) m += key[i] >= c ? w[i] : 0;
-    } else {
-      x.all([&](uint32_t b, int) {
-        if (P::key(b) >= c) m += weight(P::value(b));
-      });
+      return sums(m);
     }
-    return block.sum(m);
+    const float low = P::logit(c);
+    x.pieces_of([&](const uint4& r, int) {
+      if (P::largest(r) >= low) x.weigh(r, weight, [&](u64 y, float v) { m += v >= low ? y : 0; });
+    });
+    return sums(m);
   };
+  constexpr uint32_t kLowest = TYPE == 2 ? 0x007FFFFFu : TYPE == 1 ? 0x03FFu : 0x007Fu;  // the key of -inf
   if (use_k) {
-    const bool few = listed && static_cast<u64>(n) < static_cast<u64>(top_k);  // min_p leaves fewer than top_k
+    const bool few = listed && n < top_k;  // min_p leaves fewer than top_k
     if (!few) {
-      for (int bit = P::kBits - 1; bit >= 0; --bit)
-        if (count(t | (1u << bit)) >= static_cast<u64>(top_k)) t |= 1u << bit;
-      ties = top_k - count(t + 1);
+      t = search(listed ? from : kLowest, [&](uint32_t c) { return count(c) >= top_k; });
+      ties = top_k - (t >= kmax ? 0 : count(t + 1));
     }
   }
   if (use_p) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) w[i] = listed && key[i] != 0 ? weight(P::logit(key[i])) : 0;
-    u64 over = mass(t + 1);  // of the keys above t
+    u64 over = t >= kmax ? 0 : mass(max(t + 1, kLowest));  // of the keys above t
     if (use_k || !listed) {
       above = 0;
       const u64 total = t == 0 ? over : over + ties * weight(P::logit(t));
@@ -372,15 +420,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     uint32_t t2 = t;
     if (above + over >= need) {
-      t2 = 0;
-      for (int bit = P::kBits - 1; bit >= 0; --bit) {
-        const uint32_t c = t2 | (1u << bit);
-        if (c <= t || above + mass(c) >= need) t2 = c;
-      }
-      over = mass(t2 + 1);
+      t2 = search(max(t, kLowest), [&](uint32_t c) { return above + mass(c) >= need; });
+      over = t2 >= kmax ? 0 : mass(t2 + 1);
     }
-    const u64 each = weight(P::logit(t2));
-    if (each > 0 && t2 > 0) {
+    const u64 each = t2 > kLowest ? weight(P::logit(t2)) : 0;
+    if (each > 0) {
       const u64 m = (need - min(above + over, need) + each - 1) / each;
       ties = t2 == t ? min(ties, m) : m;
     }
@@ -388,81 +432,95 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   }
   if (floor_key > t) t = floor_key, ties = ~0ull;
 
-  // ---- the draw. Equal keys of the warps before this one count first
-  u64 tie = 0;
-  if (ties != ~0ull) {
-    uint32_t m = 0;
-    x.all([&](uint32_t b, int) { m += P::key(b) == t; });
-    m = __reduce_add_sync(kFull, m);
-    __syncthreads();
-    if (lane == 0) block.buf[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < warp; ++i) tie += block.buf[i];
-  }
-  const int end = min((warp + 1) * x.per, x.pieces);
-  // what this thread's piece of a round holds; `seen`: equal keys before the round, which it moves behind
-  const auto round = [&](const uint4& r, int piece, u64& seen, auto&& f) {
-    u64 rank = seen;
-    if (ties != ~0ull) {
-      uint32_t m = 0;
-      if (piece < end) x.each(r, piece, [&](uint32_t b, int) { m += P::key(b) == t; });
-      if (__any_sync(kFull, m != 0)) {
-        uint32_t run = m;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(kFull, run, o);
-          if (lane >= o) run += y;
-        }
-        rank += run - m;
-        seen += __shfl_sync(kFull, run, 31);
+  // ---- the draw. `low`: the least logit kept; equal ones of the warps before this one count first
+  const float low = t <= kLowest ? -kInf : P::logit(t);
+  const bool limited = ties != ~0ull;
+  u64 kept = 0;
+  {
+    const float e_low = weight.exponent(low);
+    uint32_t equal = 0;
+    x.pieces_of([&](const uint4& r, int p) {
+      if (!(P::largest(r) >= low)) return;
+      if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
+      // (top_p alone: what lies above the listed bins has been weighed)
+      if (bins && listed && !(e_low > e_above)) {
+        x.each(r, p, low, [&](float v, int) {
+          if (v > low && !(weight.exponent(v) > e_above)) kept += weight(v);
+        });
+      } else {
+        x.weigh(r, weight, [&](u64 y, float v) { kept += v > low || (v == low && !limited) ? y : 0; });
+      }
+    });
+    if (bins && listed && !(e_low > e_above)) {
+      kept += mine_above;
+      if (!limited) {  // (equal ones that were left out above)
+        x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int) { kept += v == low ? weight(v) : 0; }); });
       }
     }
-    if (piece < end)
-      x.each(r, piece, [&](uint32_t b, int i) {
-        const uint32_t k = P::key(b);
-        if (k > t || (k == t && rank++ < ties)) f(P::value(b), i);
-      });
-  };
-  u64 kept = 0, seen = tie;
-  for (int p0 = warp * x.per; p0 < end; p0 += 32) {
-    const int p = p0 + lane;
-    round(p < end ? x.again(p) : uint4{}, p, seen, [&](float v, int) { kept += weight(v); });
-  }
+    if (limited) {
+      equal = __reduce_add_sync(kFull, equal);
+      if (lane == 0) warp_ties[warp] = equal;
+      __syncthreads();
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(kFull, kept, o);
+    for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(kFull, kept, o);
+  }
+  u64 tie_before = 0;  // equal ones of the warps before
+  if (limited) {
+    for (int i = 0; i < warp; ++i) tie_before += warp_ties[i];
+    const u64 own = tie_before >= ties ? 0 : min(ties - tie_before, static_cast<u64>(warp_ties[warp]));
+    kept += own * weight(low);
+  }
   if (lane == 0) warp_sums[warp] = kept;
   __syncthreads();
-  u64 total = 0, run = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i == warp) run = total;
-    total += warp_sums[i];
+  u64 total = 0;
+  for (int i = 0; i < kWarps; ++i) total += warp_sums[i];
+  u64 target = min(static_cast<u64>(max(u, 0.0) * static_cast<double>(total)), total - 1);
+  int owner = 0;
+  u64 tie0 = 0;
+  while (target >= warp_sums[owner]) {
+    target -= warp_sums[owner];
+    if (limited) tie0 += warp_ties[owner];
+    ++owner;
   }
-  const u64 target = min(static_cast<u64>(max(u, 0.0) * static_cast<double>(total)), total - 1);
-  if (target < run || target >= run + kept) return;
-  seen = tie;
-  for (int p0 = warp * x.per; p0 < end; p0 += 32) {
-    const int p = p0 + lane;
-    const uint4 r = p < end ? x.again(p) : uint4{};
-    u64 part = 0, old = seen;
-    round(r, p, seen, [&](float v, int) { part += weight(v); });
-    u64 upto = part;
+  // The part of warp `owner`, THREADS elements at a time, one to a thread.
+  const int i1 = min((owner + 1) * x.per * x.E - x.off, a.V);
+  __syncthreads();
+  for (int i0 = max(owner * x.per * x.E - x.off, 0); i0 < i1; i0 += THREADS) {
+    const int i = i0 + tid;
+    const float v = i < i1 ? P::value(x.bits(i)) : -kInf;
+    const bool equal = i < i1 && v == low;
+    u64 y = i < i1 && (v > low || equal) ? weight(v) : 0;
+    if (limited) {
+      const uint32_t vote = __ballot_sync(kFull, equal);
+      if (lane == 0) warp_ties[warp] = __popc(vote);
+      __syncthreads();
+      u64 rank = tie0 + __popc(vote & ((1u << lane) - 1));
+      for (int j = 0; j < kWarps; ++j) {
+        if (j < warp) rank += warp_ties[j];
+        tie0 += warp_ties[j];
+      }
+      if (equal && rank >= ties) y = 0;
+    }
+    u64 upto = y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(kFull, upto, o);
-      if (lane >= o) upto += y;
+      const u64 z = __shfl_up_sync(kFull, upto, o);
+      if (lane >= o) upto += z;
     }
-    const u64 all = __shfl_sync(kFull, upto, 31);
-    if (target < run + all) {
-      u64 at = run + upto - part;
-      const bool here = target >= at && target < at + part;
-      round(r, p, old, [&](float v, int i) {
-        const u64 next = at + weight(v);
-        if (here && at <= target && target < next) a.tokens[row] = i;
-        at = next;
-      });
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    u64 all = 0;
+    for (int j = 0; j < kWarps; ++j) {
+      if (j < warp) upto += warp_sums[j];
+      all += warp_sums[j];
+    }
+    if (target < all) {
+      if (target >= upto - y && target < upto) a.tokens[row] = i;
       return;
     }
-    run += all;
+    target -= all;
+    __syncthreads();
   }
 }
 
