@@ -28,7 +28,7 @@ using u64 = unsigned long long;
 constexpr uint32_t kFull = 0xffffffffu;
 constexpr int kEach = 4;      // candidates a thread holds
 constexpr int kBins = 256;    // of the histogram of weights, 8 to a factor of 2
-constexpr int kTable = 256;   // of 2^(j / 256)
+constexpr int kTable = 16;    // of 2^(j / 16): as many as shared memory has pairs of banks, so that no two lanes wait for each other
 constexpr float kFaint = -46.f;  // 2^kFaint is no more than half of 2^-44, with room for the rounding of the exponent
 constexpr float kInf = INFINITY;
 
@@ -90,29 +90,41 @@ struct Type {
   }
 };
 
-// The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 256) 2^r with |r| <= 1 / 512; the last
-// factor is e^(r ln 2) by its series to degree 3, whose remainder is below (ln 2 / 512)^4 / 24 < 1.5e-13.
+// The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 16) 2^r with |r| <= 1 / 32; the last
+// factor is e^(r ln 2) by its series to degree 5, whose remainder is below (ln 2 / 32)^6 / 720 < 1.5e-13.
 struct Weigher {
   double top, by;    // by: log2 e / T
   float top32, by32;
-  const double* table;  // 2^(44 + j / 256)
+  const double* table;  // 2^(44 + j / 16)
+  __device__ __forceinline__ Weigher(float t, double T, const double* tab) : top(t), top32(t), table(tab) {
+    by = fmin(1.4426950408889634 / T, 1.6069380442589903e60);  // 2^200: no two logits are closer than 2^-149
+    by32 = static_cast<float>(fmin(by, 3e38));
+  }
   __device__ __forceinline__ float exponent(float x) const { return (x - top32) * by32; }  // about; monotone
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double t = (static_cast<double>(x) - top) * by, shift = 26388279066624.0;  // 1.5 * 2^44
+    const double t = (static_cast<double>(x) - top) * by, shift = 422212465065984.0;  // 1.5 * 2^48
     const double s = t + shift, r = t - (s - shift);
     const int k = __double2loint(s);
-    double p = fma(r, 5.5504108664821580e-2, 2.4022650695910071e-1);  // (ln 2)^3/3!, (ln 2)^2/2!
+    double p = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);  // (ln 2)^5/5!, (ln 2)^4/4!
+    p = fma(r, p, 5.5504108664821580e-2);                             // (ln 2)^3/3!
+    p = fma(r, p, 2.4022650695910071e-1);                             // (ln 2)^2/2!
     p = fma(r, p, 6.9314718055994531e-1);                             // ln 2
     p = fma(r, p, 1.0);
     const double q = table[k & (kTable - 1)];
-    const double scale = __hiloint2double(__double2hiint(q) + (k >> 8 << 20), __double2loint(q));
+    const double scale = __hiloint2double(__double2hiint(q) + (k >> 4 << 20), __double2loint(q));
     const u64 w = __double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
-    return exponent(x) > kFaint ? w : 0;
+    return exponent(x) > kFaint ? w : 0;  // (what w is otherwise has no meaning; NaN for -inf at T = inf)
   }
 };
 
 // A row as a block sees it: pieces of 16 bytes from the 16-byte boundary at or before its start, `off` elements of the first
 // lying before the row. Warp w has the pieces [w per, (w + 1) per), 32 at a time.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <int TYPE>
 struct Row {
   using P = Type<TYPE>;
@@ -155,9 +167,15 @@ struct Row {
   __device__ __forceinline__ void each(const uint4& r, int piece, float from, F f) const {
     if (!(P::largest(r) >= from)) return;
     const int i0 = piece * E - off;
+    if (from > -kInf || inside(piece)) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (P::at(r, e) >= from && i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
+      for (int e = 0; e < E; ++e)
+        if (P::at(r, e) >= from) f(P::at(r, e), i0 + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
+    }
   }
   // f(weight, logit) for each element, all of a piece at once (elements outside the row weigh 0)
   template <class F>
@@ -211,7 +229,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   __shared__ uint32_t list[kList], hist[kBins], slots[kSums][3], warp_ties[kWarps];
   __shared__ float warp_max[kWarps];
   __shared__ double table[kTable];
-  __shared__ int s_bad, s_pick, s_listed, s_bins[2];
+  __shared__ int s_pick, s_listed, s_bins[2];
+  __shared__ uint32_t s_range[2];  // of the list's keys
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   const double T = a.temperature ? a.temperature[row] : a.temperature0;
@@ -240,8 +259,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   } else {
     for (int p = x.first; p < x.end; p += 32) take(x.load(p), p);
   }
-  if (tid == 0) s_pick = a.V, s_listed = 0;
-  for (int i = tid; i < kTable; i += THREADS) table[i] = exp2(44.0 + i / static_cast<double>(kTable));
+  if (tid == 0) s_pick = a.V, s_listed = 0, s_range[0] = ~0u, s_range[1] = 0;
+  if (tid < kTable) table[tid] = exp2(44.0 + tid / static_cast<double>(kTable));
   for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
   for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
   float top = mine;
@@ -263,11 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     if (tid == 0) a.tokens[row] = s_pick;
     return;
   }
-  Weigher weight;
-  weight.top = weight.top32 = top;
-  weight.by = fmin(1.4426950408889634 / T, 1.6069380442589903e60);  // 2^200: no two logits are closer than 2^-149
-  weight.by32 = static_cast<float>(fmin(weight.by, 3e38));
-  weight.table = table;
+  const Weigher weight(top, T, table);
   Sums sums{slots};
 
   uint32_t t = 0;  // kept: keys above t, and the first `ties` equal to it
@@ -278,14 +293,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   if (min_p > 0 && T < INFINITY)
     floor_key = min(kmax, P::key(P::round_up(fmaxf(__double2float_ru(weight.top + T * log(min_p)), -3.4028234663852886e38f))));
   const auto need_of = [&](u64 total) { return max(__double2ull_ru(top_p * static_cast<double>(total)), 1ull); };
-  // the largest key c with enough(c), which holds for `low` and not above kmax: only bits below those that low and kmax share
-  const auto search = [&](uint32_t low, auto&& enough) {
-    const int bits = low >= kmax ? 0 : 32 - __clz(low ^ kmax);
-    uint32_t c = bits >= 32 ? 0 : kmax >> bits << bits;
+  // the largest key c with enough(c), which holds for `low` and not above `high`: only the bits below those they share
+  const auto search = [&](uint32_t low, uint32_t high, auto&& enough) {
+    if (low >= high) return low;
+    const int bits = 32 - __clz(low ^ high);
+    uint32_t c = bits >= 32 ? 0 : high >> bits << bits;
     for (int bit = bits - 1; bit >= 0; --bit)
       if ((c | (1u << bit)) <= low || enough(c | (1u << bit))) c |= 1u << bit;
-    return bits == 0 ? kmax : c;
+    return c;
   };
+  constexpr uint32_t kLowest = TYPE == 2 ? 0x007FFFFFu : TYPE == 1 ? 0x03FFu : 0x007Fu;  // the key of -inf
 
   // ---- candidates
   uint32_t from = 0;        // keys at or above it are listed
@@ -296,44 +313,52 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   const bool bins = use_p && !use_k;
   if (use_k) {
     const uint32_t key = x.first < x.end ? P::key(mine) : 0;
+    const uint32_t least = __reduce_min_sync(kFull, key != 0 ? key : ~0u);
+    if (lane == 0) atomicMin(&s_range[0], least);
     if (top_k <= __syncthreads_count(key != 0)) {
-      from = search(0, [&](uint32_t c) { return __syncthreads_count(key >= c) >= top_k; });
+      from = search(s_range[0], kmax, [&](uint32_t c) { return __syncthreads_count(key >= c) >= top_k; });
       listing = true;
     }
+    __syncthreads();
+    if (tid == 0) s_range[0] = ~0u;
     if (!use_p && floor_key > from) from = floor_key, listing = true;
   } else if (use_p) {
-    u64 sum = 0;
+    // in 32 bits: which bins the cut may be in
     x.pieces_of([&](const uint4& r, int) {
-      x.weigh(r, weight, [&](u64 w, float v) {
-        sum += w;
-        const int bin = static_cast<int>(fminf(weight.exponent(v) * -8.f, static_cast<float>(kBins)));
-        if (bin < kBins) atomicAdd(&hist[bin], static_cast<uint32_t>(w >> (32 - (bin >> 3))));  // 11 bits or 12
-      });
+      if (!(weight.exponent(P::largest(r)) * -8.f < kBins)) return;
+#pragma unroll
+      for (int e = 0; e < x.E; ++e) {
+        const float at = weight.exponent(P::at(r, e)) * -8.f;
+        const int bin = static_cast<int>(fminf(at, static_cast<float>(kBins)));
+        // 2^12 times the weight over that of the bin's octave: 2^(12 - at / 8 + bin / 8 whole)
+        if (bin < kBins) atomicAdd(&hist[bin], static_cast<uint32_t>(ex2(fmaf(at, -0.125f, static_cast<float>((bin >> 3) + 12))) + 0.5f));
+      }
     });
-    need = need_of(sums(sum));
-    if (warp == 0) {  // first bin whose end may reach `need`, first whose end does
-      u64 run = 0, part[kBins / 32];
+    __syncthreads();
+    if (warp == 0) {  // first bin whose end may reach top_p of the whole, first whose end is sure to
+      float part[kBins / 32], run = 0.f;
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
         const int bin = lane * (kBins / 32) + i;
-        part[i] = static_cast<u64>(hist[bin]) << (32 - (bin >> 3));
+        part[i] = hist[bin] * ex2(-12.f - (bin >> 3));
         run += part[i];
       }
-      u64 before = run;
+      float before = run;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(kFull, before, o);
+        const float y = __shfl_up_sync(kFull, before, o);
         if (lane >= o) before += y;
       }
+      // roundings of up to 1 in 2^12, 32-bit exponentials and sums, and up to 2^19 logits below the bins: by 1 in 2^10
+      const float all = __shfl_sync(kFull, before, 31), goal = static_cast<float>(top_p) * all;
       before -= run;
       int may = kBins, does = kBins;
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
         before += part[i];
         const int bin = lane * (kBins / 32) + i;
-        // what was cut off is less than 1 in 2^11 of a bin; 2^30: the exponent's rounding, near a bin's edge
-        if (before + (before >> 10) + (1ull << 30) >= need) may = min(may, bin);
-        if (before >= need) does = min(does, bin);
+        if (before >= goal * (1.f - 1.f / 1024)) may = min(may, bin);
+        if (before >= goal * (1.f + 1.f / 1024)) does = min(does, bin);
       }
       may = __reduce_min_sync(kFull, may), does = __reduce_min_sync(kFull, does);
       if (lane == 0) s_bins[0] = may, s_bins[1] = does;
@@ -354,15 +379,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       if (at < kList) list[at] = P::key(v);
     };
     if (bins) {
+      u64 sum = 0;
       x.pieces_of([&](const uint4& r, int p) {
-        const float e = weight.exponent(P::largest(r));
-        if (e > e_above) x.weigh(r, weight, [&](u64 w, float v) { mine_above += weight.exponent(v) > e_above ? w : 0; });
-        if (!(e > e_list) && e_list > -kInf) return;
+        x.weigh(r, weight, [&](u64 w, float v) {
+          sum += w;
+          mine_above += weight.exponent(v) > e_above ? w : 0;
+        });
+        if (!(weight.exponent(P::largest(r)) > e_list) && e_list > -kInf) return;
         x.each(r, p, -kInf, [&](float v, int) {
           const float e = weight.exponent(v);
           if (!(e > e_above) && (e > e_list || e_list == -kInf)) put(v);
         });
       });
+      need = need_of(sums(sum));
       above = sums(mine_above);
     } else {
       const float low = from == 0 ? -kInf : P::logit(from);
@@ -372,8 +401,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     n = s_listed;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) key[i] = i * THREADS + tid < n ? list[min(i * THREADS + tid, kList - 1)] : 0;  // 0: none
+    if (bins) {
+      uint32_t least = ~0u, most = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) least = min(least, key[i] != 0 ? key[i] : ~0u), most = max(most, key[i]);
+      least = __reduce_min_sync(kFull, least), most = __reduce_max_sync(kFull, most);
+      if (lane == 0) atomicMin(&s_range[0], least), atomicMax(&s_range[1], most);
+      __syncthreads();
+    }
   }
-  const bool listed = listing && n <= kList && (!bins || above < need);
+  bool listed = listing && n <= kList && (!bins || above < need);
 
   // ---- cuts: counts and sums over the list where there is one, else over the row
   const auto count = [&](uint32_t c) -> uint32_t {
@@ -401,17 +438,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     });
     return sums(m);
   };
-  constexpr uint32_t kLowest = TYPE == 2 ? 0x007FFFFFu : TYPE == 1 ? 0x03FFu : 0x007Fu;  // the key of -inf
   if (use_k) {
     const bool few = listed && n < top_k;  // min_p leaves fewer than top_k
     if (!few) {
-      t = search(listed ? from : kLowest, [&](uint32_t c) { return count(c) >= top_k; });
+      t = search(listed ? from : kLowest, kmax, [&](uint32_t c) { return count(c) >= top_k; });
       ties = top_k - (t >= kmax ? 0 : count(t + 1));
     }
   }
   if (use_p) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) w[i] = listed && key[i] != 0 ? weight(P::logit(key[i])) : 0;
+    if (bins && listed && above + mass(kLowest) < need) listed = false;  // the bins did not hold the cut after all
     u64 over = t >= kmax ? 0 : mass(max(t + 1, kLowest));  // of the keys above t
     if (use_k || !listed) {
       above = 0;
@@ -420,7 +457,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     uint32_t t2 = t;
     if (above + over >= need) {
-      t2 = search(max(t, kLowest), [&](uint32_t c) { return above + mass(c) >= need; });
+      const bool few = bins && listed;
+      t2 = search(few ? s_range[0] : max(t, kLowest), few ? s_range[1] : kmax, [&](uint32_t c) { return above + mass(c) >= need; });
       over = t2 >= kmax ? 0 : mass(t2 + 1);
     }
     const u64 each = t2 > kLowest ? weight(P::logit(t2)) : 0;
@@ -439,24 +477,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   {
     const float e_low = weight.exponent(low);
     uint32_t equal = 0;
+    const bool weighed = bins && listed && !(e_low > e_above);  // what lies above the listed bins has been
+    const bool few = weighed || (listed && !bins) || floor_key > 0;
     x.pieces_of([&](const uint4& r, int p) {
       if (!(P::largest(r) >= low)) return;
       if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
-      // (top_p alone: what lies above the listed bins has been weighed)
-      if (bins && listed && !(e_low > e_above)) {
+      if (few) {
         x.each(r, p, low, [&](float v, int) {
-          if (v > low && !(weight.exponent(v) > e_above)) kept += weight(v);
+          if ((v > low || !limited) && !(weighed && weight.exponent(v) > e_above)) kept += weight(v);
         });
       } else {
         x.weigh(r, weight, [&](u64 y, float v) { kept += v > low || (v == low && !limited) ? y : 0; });
       }
     });
-    if (bins && listed && !(e_low > e_above)) {
-      kept += mine_above;
-      if (!limited) {  // (equal ones that were left out above)
-        x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int) { kept += v == low ? weight(v) : 0; }); });
-      }
-    }
+    if (weighed) kept += mine_above;
     if (limited) {
       equal = __reduce_add_sync(kFull, equal);
       if (lane == 0) warp_ties[warp] = equal;
@@ -465,24 +499,31 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(kFull, kept, o);
   }
-  u64 tie_before = 0;  // equal ones of the warps before
+  // of lanes: the warps' ties, weights, and both up to and with each
+  const auto scan = [&](u64 v) {
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const u64 y = __shfl_up_sync(kFull, v, o);
+      if (lane >= o) v += y;
+    }
+    return v;
+  };
+  uint32_t tie_upto = 0, tie_own = 0;
   if (limited) {
-    for (int i = 0; i < warp; ++i) tie_before += warp_ties[i];
-    const u64 own = tie_before >= ties ? 0 : min(ties - tie_before, static_cast<u64>(warp_ties[warp]));
-    kept += own * weight(low);
+    tie_own = lane < kWarps ? warp_ties[lane] : 0;
+    tie_upto = static_cast<uint32_t>(scan(tie_own));
+    const uint32_t upto = __shfl_sync(kFull, tie_upto, warp), own = __shfl_sync(kFull, tie_own, warp);
+    const u64 left = ties > upto - own ? ties - (upto - own) : 0;
+    kept += min(left, static_cast<u64>(own)) * weight(low);
   }
   if (lane == 0) warp_sums[warp] = kept;
   __syncthreads();
-  u64 total = 0;
-  for (int i = 0; i < kWarps; ++i) total += warp_sums[i];
+  const u64 own = lane < kWarps ? warp_sums[lane] : 0, upto_all = scan(own);
+  const u64 total = __shfl_sync(kFull, upto_all, kWarps - 1);
   u64 target = min(static_cast<u64>(max(u, 0.0) * static_cast<double>(total)), total - 1);
-  int owner = 0;
-  u64 tie0 = 0;
-  while (target >= warp_sums[owner]) {
-    target -= warp_sums[owner];
-    if (limited) tie0 += warp_ties[owner];
-    ++owner;
-  }
+  const int owner = __ffs(__ballot_sync(kFull, lane < kWarps && target < upto_all)) - 1;
+  target -= __shfl_sync(kFull, upto_all - own, owner);
+  u64 tie0 = __shfl_sync(kFull, tie_upto - tie_own, owner);
   // The part of warp `owner`, THREADS elements at a time, one to a thread.
   const int i1 = min((owner + 1) * x.per * x.E - x.off, a.V);
   __syncthreads();
@@ -495,11 +536,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       const uint32_t vote = __ballot_sync(kFull, equal);
       if (lane == 0) warp_ties[warp] = __popc(vote);
       __syncthreads();
-      u64 rank = tie0 + __popc(vote & ((1u << lane) - 1));
-      for (int j = 0; j < kWarps; ++j) {
-        if (j < warp) rank += warp_ties[j];
-        tie0 += warp_ties[j];
-      }
+      const uint32_t o = lane < kWarps ? warp_ties[lane] : 0, s = static_cast<uint32_t>(scan(o));
+      const u64 rank = tie0 + __shfl_sync(kFull, s - o, warp) + __popc(vote & ((1u << lane) - 1));
+      tie0 += __shfl_sync(kFull, s, kWarps - 1);
       if (equal && rank >= ties) y = 0;
     }
     u64 upto = y;
@@ -510,11 +549,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    u64 all = 0;
-    for (int j = 0; j < kWarps; ++j) {
-      if (j < warp) upto += warp_sums[j];
-      all += warp_sums[j];
-    }
+    const u64 o = lane < kWarps ? warp_sums[lane] : 0, s = scan(o), all = __shfl_sync(kFull, s, kWarps - 1);
+    upto += __shfl_sync(kFull, s - o, warp);
     if (target < all) {
       if (target >= upto - y && target < upto) a.tokens[row] = i;
       return;
