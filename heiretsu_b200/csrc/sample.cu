@@ -26,8 +26,8 @@ namespace {
 
 using u64 = unsigned long long;
 constexpr uint32_t kFull = 0xffffffffu;
-constexpr int kEach = 4;      // candidates a thread holds
-constexpr int kBins = 256;    // of the histogram of weights, 8 to a factor of 2
+constexpr int kEach = 2;      // candidates a thread holds
+constexpr int kBins = 512;    // of the histogram of weights, 16 to a factor of 2
 constexpr int kTable = 16;    // of 2^(j / 16): as many as shared memory has pairs of banks, so that no two lanes wait for each other
 constexpr float kFaint = -46.f;  // 2^kFaint is no more than half of 2^-44, with room for the rounding of the exponent
 constexpr float kInf = INFINITY;
@@ -101,7 +101,10 @@ struct Weigher {
     by32 = static_cast<float>(fmin(by, 3e38));
   }
   __device__ __forceinline__ float exponent(float x) const { return (x - top32) * by32; }  // about; monotone
-  __device__ __forceinline__ u64 operator()(float x) const {
+  // Which bin of the histogram a logit is in, in the order of falling weights: 0x4B000000 + 16 times the exponent, rounded.
+  static __device__ __forceinline__ int bin(float exponent) { return __float_as_int(fmaf(exponent, -16.f, 8388608.f)); }
+  // of a logit whose exponent is above kFaint
+  __device__ __forceinline__ u64 raw(float x) const {
     const double t = (static_cast<double>(x) - top) * by, shift = 422212465065984.0;  // 1.5 * 2^48
     const double s = t + shift, r = t - (s - shift);
     const int k = __double2loint(s);
@@ -111,14 +114,15 @@ struct Weigher {
     p = fma(r, p, 6.9314718055994531e-1);                             // ln 2
     p = fma(r, p, 1.0);
     const double q = table[k & (kTable - 1)];
-    const double scale = __hiloint2double(__double2hiint(q) + (k >> 4 << 20), __double2loint(q));
-    const u64 w = __double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
+    const double scale = __hiloint2double(__double2hiint(q) + ((k & ~(kTable - 1)) << 16), __double2loint(q));
+    return __double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    const u64 w = raw(x);
     return exponent(x) > kFaint ? w : 0;  // (what w is otherwise has no meaning; NaN for -inf at T = inf)
   }
 };
 
-// A row as a block sees it: pieces of 16 bytes from the 16-byte boundary at or before its start, `off` elements of the first
-// lying before the row. Warp w has the pieces [w per, (w + 1) per), 32 at a time.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -177,12 +181,16 @@ struct Row {
         if (i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
     }
   }
-  // f(weight, logit) for each element, all of a piece at once (elements outside the row weigh 0)
+  // f(weight, logit, exponent, index) for each element that weighs anything, all of a piece at once
   template <class F>
-  __device__ __forceinline__ void weigh(const uint4& r, const Weigher& weight, F f) const {
+  __device__ __forceinline__ void weigh(const uint4& r, int piece, const Weigher& weight, F f) const {
     if (!(weight.exponent(P::largest(r)) > kFaint)) return;
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(weight(P::at(r, e)), P::at(r, e));
+    for (int e = 0; e < E; ++e) {
+      const float v = P::at(r, e), at = weight.exponent(v);
+      const u64 w = weight.raw(v);
+      if (at > kFaint) f(w, v, at, piece * E - off + e);
+    }
   }
 };
 
@@ -226,7 +234,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   using P = Type<TYPE>;
   extern __shared__ uint4 smem[];
   __shared__ u64 warp_sums[kWarps];
-  __shared__ uint32_t list[kList], hist[kBins], slots[kSums][3], warp_ties[kWarps];
+  __shared__ uint2 list[kList];  // (key, index)
+  __shared__ uint32_t hist[kBins], slots[kSums][3], warp_ties[kWarps], warp_parts[kWarps][3];
   __shared__ float warp_max[kWarps];
   __shared__ double table[kTable];
   __shared__ int s_pick, s_listed, s_bins[2];
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   bool listing = false;
   u64 above = 0, need = 0;  // top_p alone: the weight above the listed bins, and what the kept weight has to reach
   u64 mine_above = 0;       // this thread's part of `above`
-  float e_list = 0.f, e_above = 0.f;  // exponents of the listed bins: above e_list and not above e_above
+  int bin0 = 0, bin1 = 0;   // the listed bins
   const bool bins = use_p && !use_k;
   if (use_k) {
     const uint32_t key = x.first < x.end ? P::key(mine) : 0;
@@ -325,13 +334,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   } else if (use_p) {
     // in 32 bits: which bins the cut may be in
     x.pieces_of([&](const uint4& r, int) {
-      if (!(weight.exponent(P::largest(r)) * -8.f < kBins)) return;
+      if (Weigher::bin(weight.exponent(P::largest(r))) >= 0x4B000000 + kBins) return;
 #pragma unroll
       for (int e = 0; e < x.E; ++e) {
-        const float at = weight.exponent(P::at(r, e)) * -8.f;
-        const int bin = static_cast<int>(fminf(at, static_cast<float>(kBins)));
-        // 2^12 times the weight over that of the bin's octave: 2^(12 - at / 8 + bin / 8 whole)
-        if (bin < kBins) atomicAdd(&hist[bin], static_cast<uint32_t>(ex2(fmaf(at, -0.125f, static_cast<float>((bin >> 3) + 12))) + 0.5f));
+        const float at = weight.exponent(P::at(r, e));
+        const int bin = Weigher::bin(at) - 0x4B000000;
+        // the weight over that of the bin's factor of 2, in units of 2^-12: 2^23 is added, whose fraction takes it
+        const float w = __uint_as_float(__float_as_uint(ex2(at)) + ((bin & ~15) << 19));
+        if (bin < kBins) atomicAdd(&hist[bin], __float_as_uint(fmaf(w, 4096.f, 8388608.f)) & 0xFFFFu);
       }
     });
     __syncthreads();
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
         const int bin = lane * (kBins / 32) + i;
-        part[i] = hist[bin] * ex2(-12.f - (bin >> 3));
+        part[i] = hist[bin] * ex2(-12.f - (bin >> 4));
         run += part[i];
       }
       float before = run;
@@ -364,43 +374,39 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       if (lane == 0) s_bins[0] = may, s_bins[1] = does;
     }
     __syncthreads();
-    e_above = s_bins[0] / -8.f;
-    e_list = s_bins[1] >= kBins ? -kInf : (s_bins[1] + 1) / -8.f;
+    bin0 = 0x4B000000 + s_bins[0], bin1 = s_bins[1] >= kBins ? 0x7F800000 : 0x4B000000 + s_bins[1];
     listing = true;
   } else if (floor_key > 0) {
-    from = floor_key;
+    from = floor_key, listing = true;
   }
 
   uint32_t key[kEach];
   int n = 0;
   if (listing) {
-    const auto put = [&](float v) {
+    const auto put = [&](float v, int i) {
       const int at = atomicAdd(&s_listed, 1);
-      if (at < kList) list[at] = P::key(v);
+      if (at < kList) list[at] = make_uint2(P::key(v), i);
     };
     if (bins) {
       u64 sum = 0;
       x.pieces_of([&](const uint4& r, int p) {
-        x.weigh(r, weight, [&](u64 w, float v) {
+        x.weigh(r, p, weight, [&](u64 w, float v, float at, int i) {
+          const int bin = Weigher::bin(at);
           sum += w;
-          mine_above += weight.exponent(v) > e_above ? w : 0;
-        });
-        if (!(weight.exponent(P::largest(r)) > e_list) && e_list > -kInf) return;
-        x.each(r, p, -kInf, [&](float v, int) {
-          const float e = weight.exponent(v);
-          if (!(e > e_above) && (e > e_list || e_list == -kInf)) put(v);
+          if (bin < bin0) mine_above += w;
+          else if (bin <= bin1) put(v, i);
         });
       });
       need = need_of(sums(sum));
       above = sums(mine_above);
     } else {
       const float low = from == 0 ? -kInf : P::logit(from);
-      x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int) { put(v); }); });
+      x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int i) { put(v, i); }); });
       __syncthreads();
     }
     n = s_listed;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) key[i] = i * THREADS + tid < n ? list[min(i * THREADS + tid, kList - 1)] : 0;  // 0: none
+    for (int i = 0; i < kEach; ++i) key[i] = i * THREADS + tid < n ? list[min(i * THREADS + tid, kList - 1)].x : 0;  // 0: none
     if (bins) {
       uint32_t least = ~0u, most = 0;
 #pragma unroll
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     return sums.count(m);
   };
-  u64 w[kEach];  // of the list
+  u64 w[kEach] = {};  // of the list
   const auto mass = [&](uint32_t c) -> u64 {
     u64 m = 0;
     if (listed) {
@@ -433,11 +439,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       return sums(m);
     }
     const float low = P::logit(c);
-    x.pieces_of([&](const uint4& r, int) {
-      if (P::largest(r) >= low) x.weigh(r, weight, [&](u64 y, float v) { m += v >= low ? y : 0; });
+    x.pieces_of([&](const uint4& r, int p) {
+      if (P::largest(r) >= low)
+        x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
+          if (v >= low) m += y;
+        });
     });
     return sums(m);
   };
+  if (listed)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (key[i] != 0) w[i] = weight(P::logit(key[i]));
   if (use_k) {
     const bool few = listed && n < top_k;  // min_p leaves fewer than top_k
     if (!few) {
@@ -446,8 +459,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
   }
   if (use_p) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) w[i] = listed && key[i] != 0 ? weight(P::logit(key[i])) : 0;
     if (bins && listed && above + mass(kLowest) < need) listed = false;  // the bins did not hold the cut after all
     u64 over = t >= kmax ? 0 : mass(max(t + 1, kLowest));  // of the keys above t
     if (use_k || !listed) {
@@ -475,22 +486,37 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   const bool limited = ties != ~0ull;
   u64 kept = 0;
   {
-    const float e_low = weight.exponent(low);
     uint32_t equal = 0;
-    const bool weighed = bins && listed && !(e_low > e_above);  // what lies above the listed bins has been
-    const bool few = weighed || (listed && !bins) || floor_key > 0;
-    x.pieces_of([&](const uint4& r, int p) {
-      if (!(P::largest(r) >= low)) return;
-      if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
-      if (few) {
-        x.each(r, p, low, [&](float v, int) {
-          if ((v > low || !limited) && !(weighed && weight.exponent(v) > e_above)) kept += weight(v);
-        });
-      } else {
-        x.weigh(r, weight, [&](u64 y, float v) { kept += v > low || (v == low && !limited) ? y : 0; });
+    // Where the list holds all that is kept, or all but what has been weighed above its bins, it tells; else the row.
+    if (listed && !(bins && Weigher::bin(weight.exponent(low)) < bin0)) {
+      for (int i = tid; i < kWarps * 3; i += THREADS) warp_parts[i / 3][i % 3] = 0;
+      if (tid < kWarps) warp_ties[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (key[i] == 0 || key[i] < t) continue;
+        const int owner = (static_cast<int>(list[i * THREADS + tid].y) + x.off) / x.E / x.per;
+        if (limited && key[i] == t) {
+          atomicAdd(&warp_ties[owner], 1u);
+        } else {  // parts of 20 bits: kList of them add up to less than 2^32
+          atomicAdd(&warp_parts[owner][0], static_cast<uint32_t>(w[i] & 0xFFFFF));
+          atomicAdd(&warp_parts[owner][1], static_cast<uint32_t>(w[i] >> 20 & 0xFFFFF));
+          atomicAdd(&warp_parts[owner][2], static_cast<uint32_t>(w[i] >> 40));
+        }
       }
-    });
-    if (weighed) kept += mine_above;
+      __syncthreads();
+      equal = lane == 0 ? warp_ties[warp] : 0;
+      kept = mine_above;
+      if (lane == 0) kept += warp_parts[warp][0] + (static_cast<u64>(warp_parts[warp][1]) << 20) + (static_cast<u64>(warp_parts[warp][2]) << 40);
+    } else {
+      x.pieces_of([&](const uint4& r, int p) {
+        if (!(P::largest(r) >= low)) return;
+        if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
+        x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
+          if (v > low || (v == low && !limited)) kept += y;
+        });
+      });
+    }
     if (limited) {
       equal = __reduce_add_sync(kFull, equal);
       if (lane == 0) warp_ties[warp] = equal;
@@ -562,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 
 template <int TYPE, int THREADS>
 void launch(const SampleArgs& a, cudaStream_t s) {
-  constexpr int kRoom = (227 * 1024 - 1024 * (1024 / THREADS)) / (1024 / THREADS) - (THREADS == 1024 ? 20 : 11) * 1024;
+  constexpr int kRoom = (227 * 1024 - 1024 * (1024 / THREADS)) / (1024 / THREADS) - (THREADS == 1024 ? 21 : 12) * 1024;
   const size_t bytes = (static_cast<size_t>(a.V) * Type<TYPE>::kBytes + 15 + 15) / 16 * 16 + 16;
   const bool resident = bytes <= kRoom;
   const auto kernel = sample_kernel<TYPE, THREADS>;
