@@ -95,7 +95,7 @@ struct Type {
 struct Weigher {
   double top, by;    // by: log2 e / T
   float top32, by32;
-  const double* table;  // 2^(44 + j / 16)
+  const double* table;  // 2^(44 + j / 16), the j that k << 16 adds to its exponent field taken off
   __device__ __forceinline__ Weigher(float t, double T, const double* tab) : top(t), top32(t), table(tab) {
     by = fmin(1.4426950408889634 / T, 1.6069380442589903e60);  // 2^200: no two logits are closer than 2^-149
     by32 = static_cast<float>(fmin(by, 3e38));
@@ -105,8 +105,8 @@ struct Weigher {
   static __device__ __forceinline__ int bin(float exponent) { return __float_as_int(fmaf(exponent, -16.f, 8388608.f)); }
   // of a logit whose exponent is above kFaint
   __device__ __forceinline__ u64 raw(float x) const {
-    const double t = (static_cast<double>(x) - top) * by, shift = 422212465065984.0;  // 1.5 * 2^48
-    const double s = t + shift, r = t - (s - shift);
+    const double d = static_cast<double>(x) - top, shift = 422212465065984.0;  // 1.5 * 2^48
+    const double s = fma(d, by, shift), r = fma(d, by, shift - s);
     const int k = __double2loint(s);
     double p = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);  // (ln 2)^5/5!, (ln 2)^4/4!
     p = fma(r, p, 5.5504108664821580e-2);                             // (ln 2)^3/3!
@@ -114,8 +114,9 @@ struct Weigher {
     p = fma(r, p, 6.9314718055994531e-1);                             // ln 2
     p = fma(r, p, 1.0);
     const double q = table[k & (kTable - 1)];
-    const double scale = __hiloint2double(__double2hiint(q) + ((k & ~(kTable - 1)) << 16), __double2loint(q));
-    return __double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // 2^52: the fraction is the number
+    const double scale = __hiloint2double(__double2hiint(q) + (k << 16), __double2loint(q));
+    // 2^52 is added, whose fraction takes the number
+    return static_cast<u64>(__double_as_longlong(fma(p, scale, 4503599627370496.0))) - 0x4330000000000000ull;
   }
   __device__ __forceinline__ u64 operator()(float x) const {
     const u64 w = raw(x);
@@ -269,7 +270,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     for (int p = x.first; p < x.end; p += 32) take(x.load(p), p);
   }
   if (tid == 0) s_pick = a.V, s_listed = 0, s_range[0] = ~0u, s_range[1] = 0;
-  if (tid < kTable) table[tid] = exp2(44.0 + tid / static_cast<double>(kTable));
+  if (tid < kTable) {
+    const double q = exp2(44.0 + tid / static_cast<double>(kTable));
+    table[tid] = __hiloint2double(__double2hiint(q) - (tid << 16), __double2loint(q));
+  }
   for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
   for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
   float top = mine;
@@ -509,7 +513,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       kept = mine_above;
       if (lane == 0) kept += warp_parts[warp][0] + (static_cast<u64>(warp_parts[warp][1]) << 20) + (static_cast<u64>(warp_parts[warp][2]) << 40);
     } else {
-      x.pieces_of([&](const uint4& r, int p) {
+      if (t == 0) {  // nothing is cut
+        x.pieces_of([&](const uint4& r, int p) { x.weigh(r, p, weight, [&](u64 y, float, float, int) { kept += y; }); });
+      } else x.pieces_of([&](const uint4& r, int p) {
         if (!(P::largest(r) >= low)) return;
         if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
         x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
