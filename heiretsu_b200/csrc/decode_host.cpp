@@ -10,7 +10,6 @@
 #include <cmath>
 #include <limits>
 #include <string>
-#include <vector>
 
 #include "decode_args.h"
 #include "host_utils.h"
@@ -30,6 +29,7 @@ namespace {
 using OptTensor = c10::optional<at::Tensor>;
 constexpr int64_t kIntMax = std::numeric_limits<int>::max();
 constexpr int64_t kLongest = 1 << 24;   // tokens of a sequence: the tiles of 1024 sequences are counted in 32 bits
+constexpr int64_t kStride = int64_t{1} << 32;
 constexpr int64_t kMaxVocab = 1 << 19;  // weights of 2^-44 then sum to less than 2^63
 
 bool given(const OptTensor& t) { return t && t->defined(); }
@@ -42,16 +42,20 @@ std::string dims(const at::Tensor& t) {
   return s + "]";
 }
 
-// No two elements at one address.
+// No two elements at one address: sorted by stride, each dimension steps over all that lies within the ones before.
 bool disjoint(const at::Tensor& t) {
-  std::vector<std::pair<int64_t, int64_t>> d;  // (stride, size)
-  for (int64_t i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
-  std::sort(d.begin(), d.end());
+  int64_t stride[4], size[4];
+  int n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) <= 1) continue;
+    int j = n++;
+    for (; j > 0 && stride[j - 1] > t.stride(i); --j) stride[j] = stride[j - 1], size[j] = size[j - 1];
+    stride[j] = t.stride(i), size[j] = t.size(i);
+  }
   int64_t reach = 1;
-  for (const auto& [stride, size] : d) {
-    if (stride < reach) return false;
-    reach = stride * size;
+  for (int j = 0; j < n; ++j) {
+    if (stride[j] < reach) return false;
+    reach = stride[j] * size[j];
   }
   return true;
 }
@@ -89,6 +93,8 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
     bool even = aligned16(*t);
     for (int i = 0; i < 3; ++i) even = even && (t->size(i) <= 1 || t->stride(i) % per == 0);
     TORCH_CHECK(even, op, ": the cache's slots must start on 16-byte boundaries");
+    TORCH_CHECK(t->stride(0) < kStride && t->stride(1) < kStride && t->stride(2) < kStride, op,
+                ": the cache's strides must be below 2^32 elements");
   }
   TORCH_CHECK(k.numel() == 0 || k.data_ptr() != v.data_ptr(), op, ": k_pages and v_pages must not be one buffer");
   p.k = k.data_ptr(), p.v = v.data_ptr();
@@ -106,6 +112,7 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
       TORCH_CHECK(t->scalar_type() == at::kByte && t->sizes() == k.sizes().slice(0, 3) &&
                       (t->stride(2) == 1) && disjoint(*t),
                   op, ": k_exp and v_exp must be uint8 [pages, heads, page size] with contiguous slots");
+      TORCH_CHECK(t->stride(0) < kStride && t->stride(1) < kStride, op, ": the cache's strides must be below 2^32 elements");
       TORCH_CHECK(aligned16(*t) && (t->size(0) <= 1 || t->stride(0) % 16 == 0) && (t->size(1) <= 1 || t->stride(1) % 16 == 0),
                   op, ": the exponent bytes of a head of a page must start on a 16-byte boundary");
       check_same_device(*t, k.device(), op, "k_exp and v_exp");
@@ -141,6 +148,8 @@ void kv_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
                   k.size(2) == p.dim,
               op, ": k and v must both be [tokens, heads, head dim] of the slots and the cache, got ", dims(k), " and ", dims(v));
   TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, op, ": the channels of k and v must be contiguous");
+  for (const at::Tensor* x : {&k, &v})
+    TORCH_CHECK(x->stride(0) < kStride && x->stride(1) < kStride, op, ": the strides of k and v must be below 2^32 elements");
   check_rows(k.size(0), p.heads, op);
   const at::Device dev = k_pages.device();
   check_same_device(k, dev, op, "k");
