@@ -66,26 +66,59 @@ def _forward_cached(model, idx: torch.Tensor, cache: KVCache) -> torch.Tensor:
     return model.lm_head(model.tr.ln_f(x[:, -1:, :]))[:, -1, :]
 
 
-def _pick(logits: torch.Tensor, temperature: float, top_k: Optional[int], generator) -> torch.Tensor:
+def _cut(logits: torch.Tensor, top_p: float, min_p: float) -> torch.Tensor:
+    """-inf where a token is not kept: in the order by logit, the shortest start that has ``top_p`` of the probability, of it the
+    tokens with at least ``min_p`` times the largest; the first always is."""
+    x, order = logits.sort(dim=-1, descending=True, stable=True)
+    p = torch.softmax(x.double(), dim=-1)
+    drop = (p.cumsum(-1) - p >= top_p * p.sum(-1, keepdim=True)) if top_p < 1 else torch.zeros_like(x, dtype=torch.bool)
+    if min_p > 0:
+        drop |= p < min_p * p[..., :1]
+    drop[..., 0] = False
+    return logits.masked_fill(torch.zeros_like(drop).scatter_(-1, order, drop), float("-inf"))
+
+
+def _pick(logits: torch.Tensor, temperature: float, top_k: Optional[int], generator, top_p: float = 1.0,
+          min_p: float = 0.0) -> torch.Tensor:
     if temperature <= 0:
         return logits.argmax(dim=-1, keepdim=True)
     logits = logits.float() / temperature
     if top_k is not None and top_k < logits.size(-1):
         kth = torch.topk(logits, top_k, dim=-1).values[:, -1:]
         logits = logits.masked_fill(logits < kth, float("-inf"))
+    if top_p < 1 or min_p > 0:
+        logits = _cut(logits, top_p, min_p)
     probs = torch.softmax(logits, dim=-1)
     return torch.multinomial(probs, 1, generator=generator)
 
 
 @torch.no_grad()
 def generate(model, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0, top_k: Optional[int] = None,
-             generator: Optional[torch.Generator] = None, kv_cache: bool = True) -> torch.Tensor:
+             generator: Optional[torch.Generator] = None, kv_cache: bool = True, top_p: float = 1.0, min_p: float = 0.0,
+             engine: str = "plain", cache_bits: int = 16) -> torch.Tensor:
     """Extend ``idx`` [B, T0] by ``max_new_tokens`` sampled tokens; returns [B, T0 + new].
 
-    ``temperature <= 0`` picks the most likely token. With ``kv_cache`` the total
-    length must fit in ``block_size``; without it the context is cropped to the
-    last ``block_size`` tokens, as training saw them."""
+    ``temperature <= 0`` picks the most likely token; ``top_k``, ``top_p`` and ``min_p`` cut the distribution. With
+    ``kv_cache`` the total length must fit in ``block_size``; without it the context is cropped to the
+    last ``block_size`` tokens, as training saw them. ``engine`` "fused" decodes with the native kernels
+    (models/decode.py; flattened parameters on a GPU): 16-bit weights, a cache of 16 or 8 bits, a CUDA graph per token.
+    Its random numbers are used differently: the same generator gives other samples of the same distribution."""
     cfg = model.cfg
+    if engine not in ("plain", "fused"):
+        raise ValueError(f"engine must be plain or fused, got {engine!r}")
+    if engine == "fused":
+        from .decode import Decoder
+        if not kv_cache:
+            raise ValueError("the fused engine decodes from a cache")
+        if idx.size(1) + max_new_tokens > cfg.block_size:
+            raise ValueError(f"prompt {idx.size(1)} + {max_new_tokens} new tokens > block_size {cfg.block_size}")
+        if max_new_tokens < 1:
+            return idx
+        d = Decoder(model, idx.size(0), cache_bits=cache_bits)
+        d.append(idx)
+        return torch.cat([idx, d.generate(max_new_tokens, temperature, top_k, top_p, min_p, generator)], dim=1)
+    if cache_bits != 16:
+        raise ValueError("the plain modules keep their cache in the weights' type (engine \"fused\" has 8 bits)")
     was_training, was_fused = model.training, getattr(model, "fused", False)
     model.eval()
     model.fused = False  # plain modules: any sequence length, fp32 master weights
@@ -97,7 +130,7 @@ def generate(model, idx: torch.Tensor, max_new_tokens: int, temperature: float =
             cache = KVCache(model, idx.size(0), idx.device, model.tr.wte.weight.dtype)
             logits = _forward_cached(model, idx, cache)
             for i in range(max_new_tokens):
-                nxt = _pick(logits, temperature, top_k, generator)
+                nxt = _pick(logits, temperature, top_k, generator, top_p, min_p)
                 idx = torch.cat([idx, nxt], dim=1)
                 if i + 1 < max_new_tokens:
                     logits = _forward_cached(model, nxt, cache)
@@ -105,7 +138,7 @@ def generate(model, idx: torch.Tensor, max_new_tokens: int, temperature: float =
         for _ in range(max_new_tokens):
             ctx = idx[:, -cfg.block_size:]
             logits, _, _ = model(ctx)
-            nxt = _pick(logits[:, -1, :], temperature, top_k, generator)
+            nxt = _pick(logits[:, -1, :], temperature, top_k, generator, top_p, min_p)
             idx = torch.cat([idx, nxt], dim=1)
         return idx
     finally:

@@ -319,6 +319,12 @@ class GPT(nn.Module):
         from .objectives import preference_loss
         return preference_loss(self, idx, targets, ref_logp, beta, label_smoothing)
 
+    def generate(self, idx: torch.Tensor, max_new_tokens: int, **kw) -> torch.Tensor:
+        """``idx`` [B, T] extended by sampled tokens (models/generate.py), by the native kernels where the model is fused."""
+        from .generate import generate
+        kw.setdefault("engine", "fused" if self.fused and idx.is_cuda else "plain")
+        return generate(self, idx, max_new_tokens, **kw)
+
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())
 

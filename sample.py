@@ -40,6 +40,11 @@ def main(argv=None) -> None:
     ap.add_argument("--max_new_tokens", type=int, default=64)
     ap.add_argument("--temperature", type=float, default=0.8, help="<= 0: always the most likely token")
     ap.add_argument("--top_k", type=int, default=200)
+    ap.add_argument("--top_p", type=float, default=1.0, help="keep the likeliest tokens that have this share of the probability")
+    ap.add_argument("--min_p", type=float, default=0.0, help="keep tokens with this share of the likeliest one's probability")
+    ap.add_argument("--engine", choices=("plain", "fused"), default="plain",
+                    help="fused: bf16 weights, paged cache and the native kernels (one GPU)")
+    ap.add_argument("--cache_bits", type=int, choices=(16, 8), default=16, help="with --engine fused: bits of a cached value")
     ap.add_argument("--seed", type=int, default=1337)
     ap.add_argument("--device", default="auto")
     ap.add_argument("--no_kv_cache", action="store_true", help="re-run the whole context every token")
@@ -47,6 +52,9 @@ def main(argv=None) -> None:
     device = torch.device("cuda" if a.device == "auto" and torch.cuda.is_available() else
                           ("cpu" if a.device == "auto" else a.device))
     model = load_model(a.ckpt, device)
+    if a.engine == "fused":
+        from heiretsu_b200.parallel.flat import FlatParams
+        FlatParams(model, device)  # the 16-bit weights that the kernels read
     try:
         import tiktoken
         enc = tiktoken.get_encoding("gpt2")
@@ -61,7 +69,7 @@ def main(argv=None) -> None:
     g = torch.Generator(device=device).manual_seed(a.seed)
     idx = torch.tensor([ids] * a.num_samples, dtype=torch.long, device=device)
     out = generate(model, idx, a.max_new_tokens, temperature=a.temperature, top_k=a.top_k, generator=g,
-                   kv_cache=not a.no_kv_cache)
+                   kv_cache=not a.no_kv_cache, top_p=a.top_p, min_p=a.min_p, engine=a.engine, cache_bits=a.cache_bits)
     for row in out.tolist():
         print(",".join(str(t) for t in row))
         if enc is not None:
