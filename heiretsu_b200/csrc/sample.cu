@@ -90,6 +90,13 @@ struct Type {
   }
 };
 
+// 2^(44 + j / 16)
+__device__ const double kPowers[kTable] = {
+    17592186044416, 18371058661769.059, 19184414915921.48, 20033781527906.219,
+    20920752812471.082, 21846993670708.133, 22814242715178.152, 23824315533396.16,
+    24879108095803.801, 25980600314625.527, 27130859760288.855, 28332045542384.562,
+    29586412362451.676, 30896314746194.609, 32264211463076.527, 33692670141584.852};
+
 // The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 16) 2^r with |r| <= 1 / 32; the last
 // factor is e^(r ln 2) by its series to degree 5, whose remainder is below (ln 2 / 32)^6 / 720 < 1.5e-13.
 struct Weigher {
@@ -182,7 +189,8 @@ struct Row {
         if (i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
     }
   }
-  // f(weight, logit, exponent, index) for each element that weighs anything, all of a piece at once
+  // f(weight, logit, exponent, index) for each element, all of a piece at once, where any weighs something (elements outside the
+  // row weigh nothing)
   template <class F>
   __device__ __forceinline__ void weigh(const uint4& r, int piece, const Weigher& weight, F f) const {
     if (!(weight.exponent(P::largest(r)) > kFaint)) return;
@@ -190,7 +198,7 @@ struct Row {
     for (int e = 0; e < E; ++e) {
       const float v = P::at(r, e), at = weight.exponent(v);
       const u64 w = weight.raw(v);
-      if (at > kFaint) f(w, v, at, piece * E - off + e);
+      f(at > kFaint ? w : 0, v, at, piece * E - off + e);
     }
   }
 };
@@ -241,6 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   __shared__ double table[kTable];
   __shared__ int s_pick, s_listed, s_bins[2];
   __shared__ uint32_t s_range[2];  // of the list's keys
+
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   const double T = a.temperature ? a.temperature[row] : a.temperature0;
@@ -257,6 +266,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   x.first = warp * x.per + lane;
   x.end = min((warp + 1) * x.per, x.pieces);
 
+  if (tid == 0) s_pick = a.V, s_listed = 0, s_range[0] = ~0u, s_range[1] = 0;
+  if (tid < kTable) table[tid] = __hiloint2double(__double2hiint(kPowers[tid]) - (tid << 16), __double2loint(kPowers[tid]));
+  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+  for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
   float mine = -kInf;  // this thread's largest
   const auto take = [&](const uint4& r, int p) {
     if (resident) smem[p] = r;
@@ -269,13 +282,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   } else {
     for (int p = x.first; p < x.end; p += 32) take(x.load(p), p);
   }
-  if (tid == 0) s_pick = a.V, s_listed = 0, s_range[0] = ~0u, s_range[1] = 0;
-  if (tid < kTable) {
-    const double q = exp2(44.0 + tid / static_cast<double>(kTable));
-    table[tid] = __hiloint2double(__double2hiint(q) - (tid << 16), __double2loint(q));
-  }
-  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
-  for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
   float top = mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = P::max_nan(top, __shfl_xor_sync(kFull, top, o));
@@ -387,9 +393,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   uint32_t key[kEach];
   int n = 0;
   if (listing) {
-    const auto put = [&](float v, int i) {
-      const int at = atomicAdd(&s_listed, 1);
-      if (at < kList) list[at] = make_uint2(P::key(v), i);
+    // the elements of a piece that are in the row and for which `take` says so
+    const auto put = [&](const uint4& r, int p, auto&& take) {
+      uint32_t which = 0;
+#pragma unroll
+      for (int e = 0; e < x.E; ++e) which |= take(P::at(r, e)) ? 1u << e : 0u;
+      const int i0 = p * x.E - x.off;
+      if (!x.inside(p)) {
+#pragma unroll
+        for (int e = 0; e < x.E; ++e)
+          if (i0 + e < 0 || i0 + e >= x.V) which &= ~(1u << e);
+      }
+      if (which == 0) return;
+      for (int at = atomicAdd(&s_listed, __popc(which)); which; which &= which - 1, ++at) {
+        const int i = i0 + __ffs(which) - 1;
+        if (at < kList) list[at] = make_uint2(P::key(P::value(x.bits(i))), i);
+      }
     };
     if (bins) {
       u64 sum = 0;
@@ -397,15 +416,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         x.weigh(r, p, weight, [&](u64 w, float v, float at, int i) {
           const int bin = Weigher::bin(at);
           sum += w;
-          if (bin < bin0) mine_above += w;
-          else if (bin <= bin1) put(v, i);
+          mine_above += bin < bin0 ? w : 0;
         });
+        if (Weigher::bin(weight.exponent(P::largest(r))) <= bin1)
+          put(r, p, [&](float v) {
+            const int bin = Weigher::bin(weight.exponent(v));
+            return bin >= bin0 && bin <= bin1;
+          });
       });
       need = need_of(sums(sum));
       above = sums(mine_above);
     } else {
       const float low = from == 0 ? -kInf : P::logit(from);
-      x.pieces_of([&](const uint4& r, int p) { x.each(r, p, low, [&](float v, int i) { put(v, i); }); });
+      x.pieces_of([&](const uint4& r, int p) {
+        if (P::largest(r) >= low) put(r, p, [&](float v) { return v >= low; });
+      });
       __syncthreads();
     }
     n = s_listed;
@@ -422,7 +447,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   }
   bool listed = listing && n <= kList && (!bins || above < need);
 
-  // ---- cuts: counts and sums over the list where there is one, else over the row
+  // ---- cuts, from count(c) and mass(c), of the keys >= c: over the list where there is one, else over the row
+  u64 w[kEach] = {};  // of the list
+  if (listed)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (key[i] != 0) w[i] = weight(P::logit(key[i]));
   const auto count = [&](uint32_t c) -> uint32_t {
     uint32_t m = 0;
     if (listed) {
@@ -434,7 +464,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     return sums.count(m);
   };
-  u64 w[kEach] = {};  // of the list
   const auto mass = [&](uint32_t c) -> u64 {
     u64 m = 0;
     if (listed) {
@@ -444,17 +473,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     }
     const float low = P::logit(c);
     x.pieces_of([&](const uint4& r, int p) {
-      if (P::largest(r) >= low)
-        x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
-          if (v >= low) m += y;
-        });
+      if (P::largest(r) >= low) x.weigh(r, p, weight, [&](u64 y, float v, float, int) { m += v >= low ? y : 0; });
     });
     return sums(m);
   };
-  if (listed)
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (key[i] != 0) w[i] = weight(P::logit(key[i]));
   if (use_k) {
     const bool few = listed && n < top_k;  // min_p leaves fewer than top_k
     if (!few) {
@@ -519,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         if (!(P::largest(r) >= low)) return;
         if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
         x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
-          if (v > low || (v == low && !limited)) kept += y;
+          kept += v > low || (v == low && !limited) ? y : 0;
         });
       });
     }
