@@ -107,11 +107,6 @@ __device__ __forceinline__ void widen(uint32_t codes, uint32_t (&r)[2]) {
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-// The exponent that an exponent byte stands for, NaN for 255.
-__device__ __forceinline__ float exponent_of(uint32_t byte) {
-  return byte == kAct8Nan ? quiet_nan() : __uint_as_float(0x4B000000u | byte) - 8388735.f;  // 2^23 + 127
-}
-
 // A tile of 16 * KT tokens of one K/V head, as it lies in a stage of a warp's ring in shared memory: K, then V; codes have
 // 16 * KT exponent bytes of K and as many of V besides. A box is what one copy brings: rows of up to 128 bytes, whose 16-byte
 // chunks are swizzled by the row, so that the 8 tokens of a matrix load lie in different banks.
@@ -261,11 +256,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
                        const int stages, const Boxes boxes, const bool whole_units) {
   using S = Shape<D, CODES>;
   constexpr int KT = S::KT;
-  // Codes are widened to fp16, in fewer instructions than to bf16. bf16 q is scaled by a power of two for it, and the weights
-  // are those of V times its scale, under a running maximum of their own, so that they fit. fp16 weights are at
-  // most 2^15 instead of 1: then 2^-39 of the largest is still not lost.
+  // Codes are widened to fp16, in fewer instructions than to bf16. bf16 q is scaled by a power of two for it, and a weight
+  // takes the scale of its token's V with it, over the largest so far.
   constexpr bool HALF = F16 || CODES;
-  constexpr float kLift = HALF ? 15.f : 0.f;
+  // The scores' reference is raised only where one passes it by more than 2^kSlack: maxima across lanes cost more than the
+  // rest of a tile's softmax. fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest.
+  constexpr float kSlack = 8.f, kLift = HALF ? 7.f : 0.f;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1], lens[kMaxSeqs];  // tiles of a unit before each sequence; their lengths
@@ -539,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       const float d0 = __shfl_sync(kFull, back0, 8 * t + 4), d1 = __shfl_sync(kFull, back1, 8 * t + 4);
       q_unit[0] = b0 * unit * b1, q_unit[1] = d0 * unit * d1;
     }
-    // Of columns 2t and 2t + 1, in powers of 2: the largest score; codes: the largest score plus exponent of V
-    float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY};
+    float m[2] = {-INFINITY, -INFINITY};  // reference of the scores of columns 2t and 2t + 1, in powers of 2
+    uint32_t v_top = 0;                   // codes: the largest exponent byte of V so far; o is in units of its scale
     float l[2] = {0.f, 0.f};  // sum of the weights of this lane's rows
     float o[D / 16][4];
 #pragma unroll
@@ -555,7 +551,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         break;
       }
       // scores: rows are tokens g and g + 8, columns query heads 2t and 2t + 1
-      float s[KT][4], sv[KT][4];
+      float s[KT][4], vs[KT][2];
+      uint32_t byte[KT];
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
@@ -569,15 +566,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
             mma<true>(s[j], y[0][0], y[1][0], y[0][1], y[1][1], q[x][0], q[x][1]);
             if constexpr (S::kSteps > 1) mma<true>(s[j], y[2][0], y[3][0], y[2][1], y[3][1], q[x + 1][0], q[x + 1][1]);
           }
-          const uint8_t* e = exps + stage * S::kExps + j * 16 + g;
+          // lane i has the exponent byte of K of token i of the 16, lane 16 + i that of V; behind the length: 0
+          const int i = lane & 15;
+          byte[j] = exps[stage * S::kExps + (lane >> 4) * S::kTokens + j * 16 + i];
+          if (tile * S::kTokens + j * 16 + i >= len) byte[j] = 0;
+          const float scale = act8_scale(byte[j]);
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float by = act8_scale(e[8 * r]), ev = exponent_of(e[S::kTokens + 8 * r]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              s[j][2 * r + i] *= by * q_unit[i];
-              sv[j][2 * r + i] = s[j][2 * r + i] + ev;
-            }
+            const float by = __shfl_sync(kFull, scale, g + 8 * r);
+            vs[j][r] = __shfl_sync(kFull, scale, 16 + g + 8 * r);
+            s[j][2 * r] *= by * q_unit[0], s[j][2 * r + 1] *= by * q_unit[1];
           }
         } else {
 #pragma unroll
@@ -597,8 +595,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           const int token = tile * S::kTokens + j * 16;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (none >> j & 1) s[j][i] = sv[j][i] = quiet_nan();
-            if (token + g + 8 * (i >> 1) >= len) s[j][i] = sv[j][i] = -INFINITY;
+            if (none >> j & 1) s[j][i] = quiet_nan();
+            if (token + g + 8 * (i >> 1) >= len) s[j][i] = -INFINITY;
           }
           // V behind the length, whatever it is, becomes 0 (codes are numbers whatever they are)
           const int r = lane & 15;
@@ -615,48 +613,54 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           __syncwarp();
         }
       }
-      // running maximum of each column
-      float top[2] = {m[0], m[1]}, topv[2] = {mv[0], mv[1]};
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < KT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          top[i & 1] = fmaxf(top[i & 1], s[j][i]);
-          if constexpr (CODES) topv[i & 1] = fmaxf(topv[i & 1], sv[j][i]);
-        }
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[i] = fmaxf(top[i], __shfl_xor_sync(kFull, top[i], x));
-          if constexpr (CODES) topv[i] = fmaxf(topv[i], __shfl_xor_sync(kFull, topv[i], x));
-        }
-      if constexpr (!CODES) topv[0] = top[0], topv[1] = top[1];
-      if (__any_sync(kFull, top[0] != m[0] || top[1] != m[1] || (CODES && (topv[0] != mv[0] || topv[1] != mv[1])))) {
+        for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], s[j][i]);
+      if (__any_sync(kFull, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          l[x] *= top[x] == m[x] ? 1.f : ex2(m[x] - top[x]);
-          const float f = topv[x] == mv[x] ? 1.f : ex2(mv[x] - topv[x]);
-          m[x] = top[x], mv[x] = topv[x];
+          top[x] = fmaxf(top[x], m[x]);
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) top[x] = fmaxf(top[x], __shfl_xor_sync(kFull, top[x], i));
+          const float f = top[x] == m[x] ? 1.f : ex2(m[x] - top[x]);
+          m[x] = top[x];
+          l[x] *= f;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) o[i][x] *= f, o[i][2 + x] *= f;
         }
       }
-      float ref[2], refv[2];
+      float lift = 1.f;
+      if constexpr (CODES) {
+        uint32_t most = 0;  // of the tile's V; a head of NaN has no say
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        ref[x] = (m[x] == -INFINITY ? 0.f : m[x]) - (CODES ? 0.f : kLift);
-        refv[x] = (mv[x] == -INFINITY ? 0.f : mv[x]) - kLift;
+        for (int j = 0; j < KT; ++j) most = max(most, lane < 16 || byte[j] == kAct8Nan ? 0u : byte[j]);
+        most = __reduce_max_sync(kFull, most);
+        if (most > v_top) {
+          const int down = 127 + static_cast<int>(v_top) - static_cast<int>(most);
+          const float f = down > 0 ? __uint_as_float(static_cast<uint32_t>(down) << 23) : 0.f;
+          v_top = most;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[i][x] *= f;
+        }
+        lift = v_top == 0 ? 0.f : __uint_as_float((254u - v_top) << 23) * 128.f;  // 2^kLift over the scale of v_top
       }
+      float ref[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) ref[x] = (m[x] == -INFINITY ? 0.f : m[x]) - (CODES ? 0.f : kLift);
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         // weights, as the sum of two 16-bit numbers: what one of 8 or 11 bits leaves would show in the output
         float wt[4];
+        if constexpr (CODES) vs[j][0] *= lift, vs[j][1] *= lift;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           wt[i] = ex2(s[j][i] - ref[i & 1]);
           l[i & 1] += wt[i];
-          if constexpr (CODES) wt[i] = ex2(sv[j][i] - refv[i & 1]);
+          if constexpr (CODES) wt[i] *= vs[j][i >> 1];
         }
         uint32_t hi[2], rest[2];
 #pragma unroll
@@ -701,13 +705,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       l[0] += __shfl_xor_sync(kFull, l[0], x);
       l[1] += __shfl_xor_sync(kFull, l[1], x);
     }
-    // the sums of V come under the scores' maximum again; what the weights were lifted by leaves both sums
+    if constexpr (HALF) {  // what the weights were lifted by leaves both sums; the scale of V returns
+      const float down = __uint_as_float((127u - 7u) << 23), f = CODES ? __uint_as_float(v_top << 23) : 1.f;
+      if constexpr (!CODES) l[0] *= down, l[1] *= down;
 #pragma unroll
-    for (int x = 0; x < 2 && HALF; ++x) {
-      const float down = __uint_as_float((127u - 15u) << 23), f = CODES && mv[x] != -INFINITY ? ex2(mv[x] - m[x]) : 1.f;
-      if constexpr (!CODES) l[x] *= down;
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) o[i][x] = o[i][x] * down * f, o[i][2 + x] = o[i][2 + x] * down * f;
+        for (int x = 0; x < 4; ++x) o[i][x] = o[i][x] * down * f;
     }
     if (first == 0 && last == tiles) {
       const float inv[2] = {rcp(l[0]), rcp(l[1])};
