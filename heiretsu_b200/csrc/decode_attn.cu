@@ -795,21 +795,32 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   }
 }
 
-// Joins the parts of the units that CTAs share. Warp (c, y): column y of the unit that begins in CTA c of the kernel above and does
-// not end there, if any; its other parts are the first ones of the CTAs behind.
-template <int D, bool F16>
-__global__ void __launch_bounds__(32) join_kernel(const DecodeArgs a) {
+// Joins the parts of the units that CTAs share. CTA (c, y): column y of the unit that begins in CTA c of the kernel above and does
+// not end there, if any; its other parts are the first ones of the CTAs behind. WARPS > 1, for units of many parts: the
+// warps take equal runs of them first.
+template <int D, bool F16, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) join_kernel(const DecodeArgs a) {
   const Heads n(a);
-  const int col = blockIdx.y, lane = threadIdx.x;
+  const int col = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 rec = a.record[2 * blockIdx.x + 1];
   if (rec.x < 0) return;
-  const int b = rec.x / n.units;
+  const int b = rec.x / n.units, parts = rec.y + 1;
   const Columns c(n, rec.x - b * n.units);
   if (col >= c.nq) return;
+  const int i0 = share(parts, warp, WARPS), i1 = share(parts, warp + 1, WARPS);
   Join<D> j;
-  j.run(rec.y + 1, n.cols, col, lane,
-        [&](int i) { return part_of<D>(a.part, 2 * (static_cast<int>(blockIdx.x) + i) + (i == 0 ? 1 : 0), n.cols); });
+  j.run(i1 - i0, n.cols, col, lane, [&](int i) {
+    return part_of<D>(a.part, 2 * (static_cast<int>(blockIdx.x) + i0 + i) + (i0 + i == 0 ? 1 : 0), n.cols);
+  });
+  if constexpr (WARPS > 1) {
+    __shared__ __align__(16) float own[WARPS * (part_head(1) + D)];
+    j.keep(part_of<D>(own, warp, 1), 1, 0, lane);
+    __syncthreads();
+    if (warp > 0) return;
+    j = Join<D>();
+    j.run(WARPS, 1, 0, lane, [&](int i) { return part_of<D>(own, i, 1); });
+  }
   j.template finish<F16>(a, static_cast<long>(b) * a.heads_q + c.q0 + col, lane);
 }
 
@@ -858,16 +869,21 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, boxes, whole);
   HB_CUDA_CHECK(cudaGetLastError());
   if (whole || ctas == 1) return;
+  // Where a unit is spread over more than 16 CTAs on average, 8 warps join its parts (one sequence of 131072 tokens and one K/V
+  // head: 24 us in all instead of 34); elsewhere one does, and a larger block would only start later (1 x 1024 tokens of 12 heads:
+  // 10.8 us instead of 8.5).
+  const int units = a.seqs * p.heads * ((a.heads_q / p.heads + kCols - 1) / kCols);
+  const bool spread = ctas / 16 > units;
   cudaLaunchConfig_t cfg{};  // launched while the kernel above runs: it waits for its end by itself
   cfg.gridDim = dim3(ctas, cols);
-  cfg.blockDim = dim3(32);
+  cfg.blockDim = dim3(spread ? 8 * 32 : 32);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = early;
   cfg.numAttrs = 1;
-  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<D, F16>, a));
+  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, spread ? join_kernel<D, F16, 8> : join_kernel<D, F16, 1>, a));
 }
 template <int D>
 void launch_dim(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
