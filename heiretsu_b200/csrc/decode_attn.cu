@@ -891,6 +891,9 @@ void launch_dim(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   else a.f16 ? launch<D, true, false>(a, ctas, whole, s) : launch<D, false, false>(a, ctas, whole, s);
 }
 
+// Tables of at most this many tokens: CTAs take whole units, which saves the second kernel (12 heads of 64, bf16: 1 sequence of up
+// to 256 tokens 6.9 us instead of 8.2, 8 sequences 7.3 instead of 9.3, 128 sequences 20.3 instead of 19.8; of up to 512
+// tokens 8.8 instead of 7.9, 8.9 instead of 9.6, 32.9 instead of 29.1).
 constexpr int kWholeTokens = 256;
 
 // CTAs on an SM, and tokens of a tile.
