@@ -48,15 +48,15 @@ struct DecodeArgs {
   void* out;                       // [seqs, heads_q, dim]
   float* lse;                      // [seqs, heads_q]
   float* part;                     // per CTA, two unfinished units: maxima, sums and outputs of their columns
-  int2* record;                    // and which they are: (unit or -1, CTAs behind that have more of it)
+  int2* record;                    // and which they are: (unit or -1, CTAs behind that have more of it); null: CTAs take whole units
   int* status;
 };
 
 // How decode_attention deals out its work: a launch of `ctas` CTAs for each `seqs` sequences (0: more tiles than 32 bits
-// count); `whole`: CTAs take whole units.
+// count); `split`: a unit may be spread over CTAs.
 struct DecodePlan {
   int seqs = 0, ctas = 0;
-  bool whole = false;
+  bool split = false;
 };
 
 struct SampleArgs {

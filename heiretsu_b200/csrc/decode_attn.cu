@@ -243,7 +243,7 @@ __device__ __forceinline__ int share(int total, int c, int n) {
 // and every warp an equal run of the CTA's, whatever the lengths are: a unit may lie inside a warp's run, or be
 // spread over warps and CTAs. A warp walks its run with a running maximum and sum per query head; what it has of a
 // unit that is not wholly its own goes to shared memory, the CTA joins these, and what the CTA has of a unit
-// that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. WHOLE: CTAs take whole
+// that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. Without a.record CTAs take whole
 // units, and nothing is left to join.
 // How copies bring tiles: `packed` as in Place; `joint`: a page holds whole tiles, and one copy brings K of one.
 struct Boxes {
@@ -253,7 +253,7 @@ struct Boxes {
 template <int D, bool F16, bool CODES>
 __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     decode_attn_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                       const int stages, const Boxes boxes, const bool whole_units) {
+                       const int stages, const Boxes boxes) {
   using S = Shape<D, CODES>;
   constexpr int KT = S::KT;
   // Codes are widened to fp16, in fewer instructions than to bf16. bf16 q is scaled by a power of two for it, and a weight
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
 
   const int total = prefix[a.seqs] * n.units;
   int c0, c1, busy = gridDim.x;  // this CTA's run
-  if (whole_units) {
+  if (a.record == nullptr) {
     const auto start = [&](int c) {
       const int i = share(a.seqs * n.units, c, gridDim.x), b = i / n.units;
       return b == a.seqs ? total : prefix[b] * n.units + (i - b * n.units) * (prefix[b + 1] - prefix[b]);
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       if (++stage == stages) stage = 0, parity ^= 1;
     }
   }
-  if (tid < 2) a.record[2 * blockIdx.x + tid] = make_int2(-1, 0);
+  if (tid < 2 && a.record != nullptr) a.record[2 * blockIdx.x + tid] = make_int2(-1, 0);
   __syncthreads();
 
   // Parts of units that warps share. Lane i looks at segment i; neighbouring ones of one unit are a set: the first of them,
@@ -845,7 +845,7 @@ CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, l
 }
 
 template <int D, bool F16, bool CODES>
-void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
+void launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
   using S = Shape<D, CODES>;
   const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * (part_head(cols) + cols * D) * 4 + 1024;
   // 227 KB of an SM, less 1 KB a CTA and what the kernel declares
@@ -866,9 +866,9 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
     k_map = cache_map<D, CODES>(p, p.k, p.kp, p.kh, p.ks, boxes);
     v_map = cache_map<D, CODES>(p, p.v, p.vp, p.vh, p.vs, boxes);
   }
-  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, boxes, whole);
+  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, boxes);
   HB_CUDA_CHECK(cudaGetLastError());
-  if (whole || ctas == 1) return;
+  if (a.record == nullptr) return;
   // Where a unit is spread over more than 16 CTAs on average, 8 warps join its parts (one sequence of 131072 tokens and one K/V
   // head: 24 us in all instead of 34); elsewhere one does, and a larger block would only start later (1 x 1024 tokens of 12 heads:
   // 10.8 us instead of 8.5).
@@ -886,9 +886,9 @@ void launch(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
   HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, spread ? join_kernel<D, F16, 8> : join_kernel<D, F16, 1>, a));
 }
 template <int D>
-void launch_dim(const DecodeArgs& a, int ctas, bool whole, cudaStream_t s) {
-  if (a.pool.type == kKvCodes) a.f16 ? launch<D, true, true>(a, ctas, whole, s) : launch<D, false, true>(a, ctas, whole, s);
-  else a.f16 ? launch<D, true, false>(a, ctas, whole, s) : launch<D, false, false>(a, ctas, whole, s);
+void launch_dim(const DecodeArgs& a, int ctas, cudaStream_t s) {
+  if (a.pool.type == kKvCodes) a.f16 ? launch<D, true, true>(a, ctas, s) : launch<D, false, true>(a, ctas, s);
+  else a.f16 ? launch<D, true, false>(a, ctas, s) : launch<D, false, false>(a, ctas, s);
 }
 
 // Tables of at most this many tokens: CTAs take whole units, which saves the second kernel (12 heads of 64, bf16: 1 sequence of up
@@ -916,18 +916,19 @@ DecodePlan decode_attention_plan(const KvPool& p, int seqs, int units, int longe
   const long tiles = (longest + f.tokens - 1) / f.tokens, most = (1l << 31) - 1;
   d.seqs = static_cast<int>(std::min<long>(std::min(seqs, kMaxSeqs), most / std::max(1l, units * tiles)));
   if (d.seqs == 0) return d;
-  d.whole = longest <= kWholeTokens;
   const long all = static_cast<long>(d.seqs) * units, sms = num_sms(current_device());
-  d.ctas = static_cast<int>(std::max(1l, std::min(f.ctas * sms, d.whole ? all : (all * tiles + kWarps - 1) / kWarps)));
+  const bool whole = longest <= kWholeTokens;
+  d.ctas = static_cast<int>(std::max(1l, std::min(f.ctas * sms, whole ? all : (all * tiles + kWarps - 1) / kWarps)));
+  d.split = !whole && d.ctas > 1;
   return d;
 }
 
 void decode_attention_launch(const DecodeArgs& a, const DecodePlan& d, cudaStream_t s) {
   switch (a.pool.dim) {
-    case 16: launch_dim<16>(a, d.ctas, d.whole, s); break;
-    case 32: launch_dim<32>(a, d.ctas, d.whole, s); break;
-    case 64: launch_dim<64>(a, d.ctas, d.whole, s); break;
-    default: launch_dim<128>(a, d.ctas, d.whole, s); break;
+    case 16: launch_dim<16>(a, d.ctas, s); break;
+    case 32: launch_dim<32>(a, d.ctas, s); break;
+    case 64: launch_dim<64>(a, d.ctas, s); break;
+    default: launch_dim<128>(a, d.ctas, s); break;
   }
 }
 

@@ -3,6 +3,7 @@
 // every other refusal shows on a machine without one. Numbers go into the messages as strings: an extension whose
 // linker brought its own static libstdc++ faults when it streams them.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -31,6 +32,11 @@ constexpr int64_t kIntMax = std::numeric_limits<int>::max();
 constexpr int64_t kLongest = 1 << 24;   // tokens of a sequence: the tiles of 1024 sequences are counted in 32 bits
 constexpr int64_t kStride = int64_t{1} << 32;
 constexpr int64_t kMaxVocab = 1 << 19;  // weights of 2^-44 then sum to less than 2^63
+
+// An output, allocated without the dispatcher: a short call is bound by the host.
+at::Tensor output(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, dt, dev, c10::nullopt);
+}
 
 bool given(const OptTensor& t) { return t && t->defined(); }
 bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
@@ -181,9 +187,8 @@ std::tuple<at::Tensor, at::Tensor> kv_read(const at::Tensor& slots, const at::Te
   check_same_device(slots, dev, op, "slots");
   TORCH_CHECK(k_pages.is_cuda(), op, ": the cache must be on a CUDA device");
   c10::cuda::CUDAGuard g(dev);
-  const auto opts = k_pages.options().dtype(dt);
   const int64_t n = slots.size(0);
-  at::Tensor k = at::empty({n, p.heads, p.dim}, opts), v = at::empty({n, p.heads, p.dim}, opts);
+  at::Tensor k = output({n, p.heads, p.dim}, dt, dev), v = output({n, p.heads, p.dim}, dt, dev);
   kv_read_launch(slots.data_ptr<int64_t>(), p, k.data_ptr(), v.data_ptr(), static_cast<int>(n),
                  dt == at::kFloat ? 2 : dt == at::kHalf ? 1 : 0, device_status_ptr(dev.index()),
                  at::cuda::getCurrentCUDAStream());
@@ -217,7 +222,7 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
   check_same_device(lengths, dev, op, "lengths");
   TORCH_CHECK(k_pages.is_cuda(), op, ": the cache must be on a CUDA device");
   c10::cuda::CUDAGuard g(dev);
-  at::Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({B, q.size(1)}, q.options().dtype(at::kFloat));
+  at::Tensor out = output(q.sizes(), q.scalar_type(), dev), lse = output({B, q.size(1)}, at::kFloat, dev);
   a.qt = q.stride(0), a.qh = q.stride(1);
   a.q_vec = rows_aligned(q);
   a.f16 = q.scalar_type() == at::kHalf;
@@ -237,9 +242,13 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
     a.out = static_cast<uint16_t*>(out.data_ptr()) + b * out.stride(0);
     a.lse = lse.data_ptr<float>() + b * a.heads_q;
     // two parts and their records for each CTA; each launch its own, as the next may begin before the last has joined its
-    at::Tensor part = at::empty({2l * plan.ctas * (2 + ((2 * cols + 3) & ~3) + static_cast<long>(cols) * a.pool.dim)}, lse.options());
-    a.record = reinterpret_cast<int2*>(part.data_ptr<float>());
-    a.part = part.data_ptr<float>() + 4l * plan.ctas;
+    at::Tensor part;
+    a.record = nullptr;
+    if (plan.split) {
+      part = output({2l * plan.ctas * (2 + ((2 * cols + 3) & ~3) + static_cast<long>(cols) * a.pool.dim)}, at::kFloat, dev);
+      a.record = reinterpret_cast<int2*>(part.data_ptr<float>());
+      a.part = part.data_ptr<float>() + 4l * plan.ctas;
+    }
     decode_attention_launch(a, plan, at::cuda::getCurrentCUDAStream());
   }
   return {out, lse};
@@ -278,7 +287,7 @@ at::Tensor sample_tokens(const at::Tensor& logits, int64_t V, const at::Tensor& 
   TORCH_CHECK(!std::isnan(temperature0) && !std::isnan(top_p0) && !std::isnan(min_p0), op, ": a setting is not a number");
   TORCH_CHECK(logits.is_cuda(), op, ": logits must be on a CUDA device");
   c10::cuda::CUDAGuard g(dev);
-  at::Tensor tokens = at::empty({M}, logits.options().dtype(at::kLong));
+  at::Tensor tokens = output({M}, at::kLong, dev);
   a.x = logits.data_ptr(), a.ld = logits.stride(0);
   a.rows = static_cast<int>(M), a.V = static_cast<int>(V);
   a.u = u.data_ptr<float>();
