@@ -95,17 +95,23 @@ __device__ __forceinline__ void copy_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// Four signed bytes as fp16, in pairs: bytes 0 and 1, 2 and 3 (ALONG), or 0 and 2, 1 and 3. A byte with its sign flipped is
-// code + 128; under 0x64 it reads as 1024 + 128 + code, and 1152 is taken off.
-template <bool ALONG>
+// Four signed bytes as fp16, in pairs: bytes 0 and 1, 2 and 3. A byte with its sign flipped is code + 128; under 0x64 it reads as
+// 1024 + 128 + code, and 1152 is taken off.
 __device__ __forceinline__ void widen(uint32_t codes, uint32_t (&r)[2]) {
   codes ^= 0x80808080u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t x = __byte_perm(codes, 0x64646464u, ALONG ? (i ? 0x4342 : 0x4140) : (i ? 0x4341 : 0x4240));
+    const uint32_t x = __byte_perm(codes, 0x64646464u, i ? 0x4342 : 0x4140);
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+// Two signed bytes (the low ones of `pair`'s halves, whatever lies above them) as bf16, which has 7 fraction bits: under 0x43
+// the low 7 bits u read as 128 + u, the sign bit as 128 or 256, and their difference is u - 128 sign.
+__device__ __forceinline__ uint32_t widen_bf16(uint32_t pair) {
+  const uint32_t x = (pair & 0x007F007Fu) | 0x43004300u, y = (pair & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 // A tile of 16 * KT tokens of one K/V head, as it lies in a stage of a warp's ring in shared memory: K, then V; codes have
 // 16 * KT exponent bytes of K and as many of V besides. A box is what one copy brings: rows of up to 128 bytes, whose 16-byte
@@ -256,12 +262,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
                        const int stages, const Boxes boxes) {
   using S = Shape<D, CODES>;
   constexpr int KT = S::KT;
-  // Codes are widened to fp16, in fewer instructions than to bf16. bf16 q is scaled by a power of two for it, and a weight
-  // takes the scale of its token's V with it, over the largest so far.
-  constexpr bool HALF = F16 || CODES;
+  // Codes of K are widened to fp16, in fewer instructions than to bf16, and bf16 q is scaled by a power of two for it. Codes of V
+  // are widened to bf16: a weight takes the scale of its head of a token with it, and these may lie further apart than fp16 goes.
+  constexpr bool V16 = F16 && !CODES;
   // The scores' reference is raised only where one passes it by more than 2^kSlack: maxima across lanes cost more than the
-  // rest of a tile's softmax. fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest.
-  constexpr float kSlack = 8.f, kLift = HALF ? 7.f : 0.f;
+  // rest of a tile's softmax. fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest;
+  // bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
+  constexpr float kSlack = 8.f, kLift = V16 ? 7.f : -kSlack;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1], lens[kMaxSeqs];  // tiles of a unit before each sequence; their lengths
@@ -536,7 +543,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       q_unit[0] = b0 * unit * b1, q_unit[1] = d0 * unit * d1;
     }
     float m[2] = {-INFINITY, -INFINITY};  // reference of the scores of columns 2t and 2t + 1, in powers of 2
-    uint32_t v_top = 0;                   // codes: the largest exponent byte of V so far; o is in units of its scale
     float l[2] = {0.f, 0.f};  // sum of the weights of this lane's rows
     float o[D / 16][4];
 #pragma unroll
@@ -552,7 +558,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       }
       // scores: rows are tokens g and g + 8, columns query heads 2t and 2t + 1
       float s[KT][4], vs[KT][2];
-      uint32_t byte[KT];
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
@@ -562,15 +567,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
             uint32_t r[4], y[4][2];
             load_matrices(r, k0 + k_row.chunk(x, j));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) widen<true>(r[i], y[i]);
+            for (int i = 0; i < 4; ++i) widen(r[i], y[i]);
             mma<true>(s[j], y[0][0], y[1][0], y[0][1], y[1][1], q[x][0], q[x][1]);
             if constexpr (S::kSteps > 1) mma<true>(s[j], y[2][0], y[3][0], y[2][1], y[3][1], q[x + 1][0], q[x + 1][1]);
           }
           // lane i has the exponent byte of K of token i of the 16, lane 16 + i that of V; behind the length: 0
           const int i = lane & 15;
-          byte[j] = exps[stage * S::kExps + (lane >> 4) * S::kTokens + j * 16 + i];
-          if (tile * S::kTokens + j * 16 + i >= len) byte[j] = 0;
-          const float scale = act8_scale(byte[j]);
+          uint32_t byte = exps[stage * S::kExps + (lane >> 4) * S::kTokens + j * 16 + i];
+          if (tile * S::kTokens + j * 16 + i >= len) byte = 0;
+          const float scale = act8_scale(byte);
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float by = __shfl_sync(kFull, scale, g + 8 * r);
@@ -631,31 +636,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           for (int i = 0; i < D / 16; ++i) o[i][x] *= f, o[i][2 + x] *= f;
         }
       }
-      float lift = 1.f;
-      if constexpr (CODES) {
-        uint32_t most = 0;  // of the tile's V; a head of NaN has no say
-#pragma unroll
-        for (int j = 0; j < KT; ++j) most = max(most, lane < 16 || byte[j] == kAct8Nan ? 0u : byte[j]);
-        most = __reduce_max_sync(kFull, most);
-        if (most > v_top) {
-          const int down = 127 + static_cast<int>(v_top) - static_cast<int>(most);
-          const float f = down > 0 ? __uint_as_float(static_cast<uint32_t>(down) << 23) : 0.f;
-          v_top = most;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[i][x] *= f;
-        }
-        lift = v_top == 0 ? 0.f : __uint_as_float((254u - v_top) << 23) * 128.f;  // 2^kLift over the scale of v_top
-      }
       float ref[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) ref[x] = (m[x] == -INFINITY ? 0.f : m[x]) - (CODES ? 0.f : kLift);
+      for (int x = 0; x < 2; ++x) ref[x] = (m[x] == -INFINITY ? 0.f : m[x]) - kLift;
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         // weights, as the sum of two 16-bit numbers: what one of 8 or 11 bits leaves would show in the output
         float wt[4];
-        if constexpr (CODES) vs[j][0] *= lift, vs[j][1] *= lift;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           wt[i] = ex2(s[j][i] - ref[i & 1]);
@@ -665,8 +652,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
         uint32_t hi[2], rest[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t x = pack16<HALF>(wt[2 * r], wt[2 * r + 1]);
-          rest[r] = transpose8(pack16<HALF>(wt[2 * r] - lo16<HALF>(x), wt[2 * r + 1] - hi16<HALF>(x)));
+          const uint32_t x = pack16<V16>(wt[2 * r], wt[2 * r + 1]);
+          rest[r] = transpose8(pack16<V16>(wt[2 * r] - lo16<V16>(x), wt[2 * r + 1] - hi16<V16>(x)));
           hi[r] = transpose8(x);
         }
         // output: rows are channels
@@ -678,11 +665,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // a word: channels 2g and 2g + 1 of two tokens
               if (i + x >= D / 16) break;
-              uint32_t y[2], z[2];
-              widen<false>(r[2 * x], y);
-              widen<false>(r[2 * x + 1], z);
-              mma<HALF>(o[i + x], y[0], y[1], z[0], z[1], hi[0], hi[1]);
-              mma<HALF>(o[i + x], y[0], y[1], z[0], z[1], rest[0], rest[1]);
+              const uint32_t y[4] = {widen_bf16(r[2 * x]), widen_bf16(r[2 * x] >> 8), widen_bf16(r[2 * x + 1]), widen_bf16(r[2 * x + 1] >> 8)};
+              mma<V16>(o[i + x], y[0], y[1], y[2], y[3], hi[0], hi[1]);
+              mma<V16>(o[i + x], y[0], y[1], y[2], y[3], rest[0], rest[1]);
             }
           }
         } else {
@@ -690,8 +675,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
           for (int i = 0; i < D / 16; ++i) {
             uint32_t r[4];
             load_matrices_t(r, v0 + v_row.chunk(2 * i, j));
-            mma<HALF>(o[i], r[0], r[1], r[2], r[3], hi[0], hi[1]);
-            mma<HALF>(o[i], r[0], r[1], r[2], r[3], rest[0], rest[1]);
+            mma<V16>(o[i], r[0], r[1], r[2], r[3], hi[0], hi[1]);
+            mma<V16>(o[i], r[0], r[1], r[2], r[3], rest[0], rest[1]);
           }
         }
       }
@@ -705,14 +690,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
       l[0] += __shfl_xor_sync(kFull, l[0], x);
       l[1] += __shfl_xor_sync(kFull, l[1], x);
     }
-    if constexpr (HALF) {  // what the weights were lifted by leaves both sums; the scale of V returns
-      const float down = __uint_as_float((127u - 7u) << 23), f = CODES ? __uint_as_float(v_top << 23) : 1.f;
-      if constexpr (!CODES) l[0] *= down, l[1] *= down;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[i][x] = o[i][x] * down * f;
-    }
+    m[0] -= kLift, m[1] -= kLift;  // what the sums' weights are relative to
     if (first == 0 && last == tiles) {
       const float inv[2] = {rcp(l[0]), rcp(l[1])};
       const long row = static_cast<long>(b) * a.heads_q + q0;

@@ -213,7 +213,8 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     sequence in order; ``lengths`` int32 [sequences]: how many of its tokens count, the new one's own K and V among them when
     it has been written. Entries and slots behind them are not read. ``scale`` defaults to head dim ** -0.5; ``lse`` is the natural
     log-sum-exp of the scores, so that outputs over parts of a cache can be joined. A sequence of length 0 gives 0 and
-    -inf; a length or page out of range gives NaN in its rows, and sets the bad-argument status."""
+    -inf; a length or page out of range gives NaN in its rows, and sets the bad-argument status. A NaN or infinity in a counted
+    token's V makes its channel NaN, in its K the row (-inf scores weigh nothing)."""
     return _ext().decode_attention(q, k_pages, v_pages, table, lengths, k_exp, v_exp, scale)
 
 

@@ -267,6 +267,58 @@ def test_attention_of_infinities_and_nan_in_counted_tokens():
     _status()
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 2, 128)])
+def test_attention_of_broken_heads_in_8_bits(heads, kv, dim):
+    """A head of one token whose K or V held an infinity or NaN: NaN in the query heads that share it, in its own sequence, and
+    nowhere else; heads of zeros, and scales far apart, are like any others."""
+    K = _k()
+    q, c, table, n, held = _batch([40, 33, 50, 64], heads, kv, dim, 16, BF16, 8, seed=3)
+    held = [(k.clone(), v.clone()) for k, v in held]
+
+    def put(b, tok, h, name, byte=None, zero=False):
+        pg, at = int(table[b, tok // 16]), tok % 16
+        i = 0 if name == "k" else 1
+        if byte is not None:
+            c.pools[name + "_exp"][pg, h, at] = byte
+            held[b][i][tok, h] = math.nan
+        if zero:
+            c.pools[name + "_exp"][pg, h, at], c.pools[name + "_pages"][pg, h, at] = 1, 0
+            held[b][i][tok, h] = 0
+
+    put(0, 17, 1, "k", 255)
+    put(1, 32, 0, "v", 255)
+    for tok in range(50):
+        put(2, tok, 0, "v", zero=True)
+        put(2, tok, 1, "k", zero=True)
+    pg, at = int(table[3, 0]), 5
+    c.pools["v_exp"][pg, 0, at] += 30  # one token's V a billion times as large
+    held[3][1][5, 0] *= 2.0 ** 30
+    out, lse = K.decode_attention(q, table=table, lengths=n, **c.pools)
+    G = heads // kv
+    for b, (k, v) in enumerate(held):
+        want, wl, size, mean_v = O.attention(q[b], k, v, dim ** -0.5)
+        near, near_lse = O.attention_bounds(want, wl, size, mean_v, dim, k.shape[0], BF16)
+        for h in range(heads):
+            if (b, h // G) == (0, 1):
+                assert bool(out[b, h].isnan().all()) and bool(lse[b, h].isnan())
+            elif (b, h // G) == (1, 0):
+                assert bool(out[b, h].isnan().all()) and abs(float(lse[b, h] - wl[h])) <= float(near_lse[h])
+            else:
+                assert bool(((out[b, h].double() - want[h]).abs() <= near[h]).all()), (b, h)
+                assert abs(float(lse[b, h] - wl[h])) <= float(near_lse[h])
+    _status()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_of_more_sequences_than_one_launch_takes(bits):
+    K = _k()
+    lengths = [(7 * i) % 40 for i in range(1030)] + [300, 0, 5]
+    q, c, table, n, held = _batch(lengths, 2, 1, 32, 16, BF16, bits, seed=4)
+    out, lse = K.decode_attention(q, table=table, lengths=n, **c.pools)
+    _compare(out, lse, q, held)
+    _status()
+
+
 def test_attention_reports_bad_pages_and_lengths():
     K = _k()
     q, c, table, n, held = _batch([100, 33, 70, 260, 48], 4, 2, 64, 16, BF16, 16, seed=6)
@@ -497,6 +549,37 @@ def test_sampling_strides_and_sizes():
     many = _rows(700, 517, F32, g)
     uu = torch.rand(700, device="cuda", generator=g)
     assert K.sample_tokens(many, 517, uu, 0.9, 0, 0.8).tolist() == _want(many, 517, uu, 0.9, 0, 0.8, 0.0)
+
+
+@pytest.mark.parametrize("dtype,V", [(BF16, 60000), (F32, 60000), (F16, 130001), (F32, 130001), (BF16, 300000)])
+def test_sampling_where_nothing_short_holds_what_is_kept(dtype, V):
+    """Flat logits, cuts far down, ties without end: more candidates than a list has, rows that shared memory does not hold."""
+    K, g = _k(), _gen(V)
+    x = _rows(4, V, dtype, g, spread=1.0)
+    x[1] = 0.5
+    x[2] = (x[2] * 4).round() / 4  # few different values
+    x[3, ::2] = -math.inf
+    u = torch.rand(4, device="cuda", generator=g)
+    for s in [(1.0, 0, 1.0, 0.0), (1.0, 900, 1.0, 0.0), (1.3, 5000, 0.7, 0.0), (1.0, V - 1, 0.999, 0.0), (2.0, 0, 0.99, 0.0),
+              (1.5, 0, 0.5, 0.0), (1.0, 0, 0.99999, 0.0), (1.0, 0, 1.0, 1e-7), (0.6, 0, 0.9, 1e-4), (3.0, 3000, 0.95, 0.001)]:
+        assert K.sample_tokens(x, V, u, *s).tolist() == _want(x, V, u, *s), s
+    _status()
+
+
+def test_sampling_many_rows_of_unlike_settings():
+    """More rows than the GPU has SMs, each of its own kind."""
+    K, g = _k(), _gen(21)
+    M, V = 400, 20011
+    x = _rows(M, V, BF16, g)
+    x[::7] *= 0.3
+    u = torch.rand(M, device="cuda", generator=g)
+    r = torch.rand(4, M, device="cuda", generator=g)
+    t = torch.where(r[0] < 0.1, 0.0, 0.2 + 1.5 * r[0])
+    k = torch.where(r[1] < 0.4, 0, (800 * r[1]).long())
+    p = torch.where(r[2] < 0.3, 1.0, r[2])
+    m = torch.where(r[3] < 0.6, 0.0, 0.1 * r[3])
+    got = K.sample_tokens(x, V, u, t, k, p, m)
+    assert got.tolist() == _want(x, V, u, t, k, p, m)
 
 
 def test_sampling_follows_the_distribution():
