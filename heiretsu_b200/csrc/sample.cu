@@ -29,7 +29,7 @@ constexpr uint32_t kFull = 0xffffffffu;
 constexpr int kEach = 2;      // candidates a thread holds
 constexpr int kBins = 512;    // of the histogram of weights, 16 to a factor of 2
 constexpr int kTable = 16;    // of 2^(j / 16): as many as shared memory has pairs of banks, so that no two lanes wait for each other
-constexpr float kFaint = -46.f;  // 2^kFaint is no more than half of 2^-44, with room for the rounding of the exponent
+constexpr int kFine = 256;    // steps of a bin
 constexpr float kInf = INFINITY;
 
 // Element types as the host numbers them; keys are unsigned numbers in the order of the logits (-0 counts as 0).
@@ -97,20 +97,33 @@ __device__ const double kPowers[kTable] = {
     24879108095803.801, 25980600314625.527, 27130859760288.855, 28332045542384.562,
     29586412362451.676, 30896314746194.609, 32264211463076.527, 33692670141584.852};
 
-// The weight of a logit in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 16) 2^r with |r| <= 1 / 32; the last
+// The weight of a logit x in units of 2^-44. 2^(d log2 e / T), d = x - top, is 2^n 2^(j / 16) 2^r with |r| <= 1 / 32; the last
 // factor is e^(r ln 2) by its series to degree 5, whose remainder is below (ln 2 / 32)^6 / 720 < 1.5e-13.
+// x is raised to `least` first, whose weight of 2^-46 or less is rounded to 0 as that of all below it is: so n stays small,
+// and -inf is like the others. That `least` is finite, and not `top`, takes
+// - x and T in units of 2^56 where one of them is so large that top - 46 T ln 2 is no number of 32 bits,
+// - T ln 2 of at most 2^174, which has all finite logits weigh 1 as an infinite T does, and
+// - T ln 2 of at least 1 / 50 of the distance to the next number of 32 bits below top, which still weighs 0.
 struct Weigher {
   double top, by;    // by: log2 e / T
-  float top32, by32;
+  float unit, least, top32, inv32, steps;  // inv32: T ln 2; steps: of bins, to a logit
   const double* table;  // 2^(44 + j / 16), the j that k << 16 adds to its exponent field taken off
-  __device__ __forceinline__ Weigher(float t, double T, const double* tab) : top(t), top32(t), table(tab) {
-    by = fmin(1.4426950408889634 / T, 1.6069380442589903e60);  // 2^200: no two logits are closer than 2^-149
-    by32 = static_cast<float>(fmin(by, 3e38));
+  __device__ __forceinline__ Weigher(float t, double T, const double* tab) : table(tab) {
+    double inv = fmin(T * 0.69314718055994531, 2.3945242826029513e52);
+    unit = t < -1e38f || t - 46 * inv < -3.4028234663852886e38 ? 1.3877787807814457e-17f : 1.f;
+    top32 = t * unit, top = top32;
+    const float below = nextafterf(top32, -INFINITY);
+    inv = fmax(inv * unit, (top - below) * 0.02);
+    by = 1 / inv;
+    least = fminf(__double2float_rd(top - 46 * inv), below);
+    inv32 = static_cast<float>(inv);
+    steps = static_cast<float>(fmin(by * 16 * kFine, 1e38));
   }
-  __device__ __forceinline__ float exponent(float x) const { return (x - top32) * by32; }  // about; monotone
-  // Which bin of the histogram a logit is in, in the order of falling weights: 0x4B000000 + 16 times the exponent, rounded.
-  static __device__ __forceinline__ int bin(float exponent) { return __float_as_int(fmaf(exponent, -16.f, 8388608.f)); }
-  // of a logit whose exponent is above kFaint
+  __device__ __forceinline__ float raised(float x) const { return fmaxf(x * unit, least); }
+  __device__ __forceinline__ bool any(float largest) const { return largest * unit > least; }
+  // In the histogram: 0x4B000000 + the steps below top, rounded; more where the logit is far below it.
+  __device__ __forceinline__ int place(float x) const { return __float_as_int(fmaf(top32 - x * unit, steps, 8388608.f)); }
+  // of a logit that has been raised
   __device__ __forceinline__ u64 raw(float x) const {
     const double d = static_cast<double>(x) - top, shift = 422212465065984.0;  // 1.5 * 2^48
     const double s = fma(d, by, shift), r = fma(d, by, shift - s);
@@ -125,10 +138,7 @@ struct Weigher {
     // 2^52 is added, whose fraction takes the number
     return static_cast<u64>(__double_as_longlong(fma(p, scale, 4503599627370496.0))) - 0x4330000000000000ull;
   }
-  __device__ __forceinline__ u64 operator()(float x) const {
-    const u64 w = raw(x);
-    return exponent(x) > kFaint ? w : 0;  // (what w is otherwise has no meaning; NaN for -inf at T = inf)
-  }
+  __device__ __forceinline__ u64 operator()(float x) const { return raw(raised(x)); }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -189,17 +199,17 @@ struct Row {
         if (i0 + e >= 0 && i0 + e < V) f(P::at(r, e), i0 + e);
     }
   }
-  // f(weight, logit, exponent, index) for each element, all of a piece at once, where any weighs something (elements outside the
-  // row weigh nothing)
-  template <class F>
-  __device__ __forceinline__ void weigh(const uint4& r, int piece, const Weigher& weight, F f) const {
-    if (!(weight.exponent(P::largest(r)) > kFaint)) return;
+  // the weight of a piece's elements, ALL or those that are not below `from` (elements outside the row weigh nothing)
+  template <bool ALL = false>
+  __device__ __forceinline__ u64 weigh(const uint4& r, const Weigher& weight, float from = 0) const {
+    u64 sum = 0;
+    if (!weight.any(P::largest(r))) return sum;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float v = P::at(r, e), at = weight.exponent(v);
-      const u64 w = weight.raw(v);
-      f(at > kFaint ? w : 0, v, at, piece * E - off + e);
+      const u64 w = weight(P::at(r, e));
+      if (ALL || P::at(r, e) >= from) sum += w;
     }
+    return sum;
   }
 };
 
@@ -243,8 +253,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   using P = Type<TYPE>;
   extern __shared__ uint4 smem[];
   __shared__ u64 warp_sums[kWarps];
-  __shared__ uint2 list[kList];  // (key, index)
-  __shared__ uint32_t hist[kBins], slots[kSums][3], warp_ties[kWarps], warp_parts[kWarps][3];
+  __shared__ __align__(16) uint2 list[kList];  // (key, index); before that the histogram, four copies of a bin side by side
+  __shared__ uint32_t slots[kSums][3], warp_ties[kWarps], warp_parts[kWarps][3];
   __shared__ float warp_max[kWarps];
   __shared__ double table[kTable];
   __shared__ int s_pick, s_listed, s_bins[2];
@@ -268,7 +278,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 
   if (tid == 0) s_pick = a.V, s_listed = 0, s_range[0] = ~0u, s_range[1] = 0;
   if (tid < kTable) table[tid] = __hiloint2double(__double2hiint(kPowers[tid]) - (tid << 16), __double2loint(kPowers[tid]));
-  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
   for (int i = tid; i < kSums * 3; i += THREADS) slots[i / 3][i % 3] = 0;
   float mine = -kInf;  // this thread's largest
   const auto take = [&](const uint4& r, int p) {
@@ -310,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   const bool use_k = top_k > 0 && top_k < a.V, use_p = top_p < 1;
   uint32_t floor_key = 0;  // of min_p
   if (min_p > 0 && T < INFINITY)
-    floor_key = min(kmax, P::key(P::round_up(fmaxf(__double2float_ru(weight.top + T * log(min_p)), -3.4028234663852886e38f))));
+    floor_key = min(kmax, P::key(P::round_up(fmaxf(__double2float_ru(top + T * log(min_p)), -3.4028234663852886e38f))));
   const auto need_of = [&](u64 total) { return max(__double2ull_ru(top_p * static_cast<double>(total)), 1ull); };
   // the largest key c with enough(c), which holds for `low` and not above `high`: only the bits below those they share
   const auto search = [&](uint32_t low, uint32_t high, auto&& enough) {
@@ -328,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   bool listing = false;
   u64 above = 0, need = 0;  // top_p alone: the weight above the listed bins, and what the kept weight has to reach
   u64 mine_above = 0;       // this thread's part of `above`
-  int bin0 = 0, bin1 = 0;   // the listed bins
+  float listed_from = 0, listed_to = 0;  // of raised logits, those >= the first and < the second
   const bool bins = use_p && !use_k;
   if (use_k) {
     const uint32_t key = x.first < x.end ? P::key(mine) : 0;
@@ -342,16 +351,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     if (tid == 0) s_range[0] = ~0u;
     if (!use_p && floor_key > from) from = floor_key, listing = true;
   } else if (use_p) {
-    // in 32 bits: which bins the cut may be in
+    // In 32 bits: which bins the cut may be in. Within a bin a weight falls from 6038 to 5783 steps of equal size, which is off
+    // by no more than 1 in 2^12; the sum of 2^19 stays below 2^32. Lanes that add to one bin wait for each other: with four copies
+    // of the bins few do.
+    uint32_t* const hist = reinterpret_cast<uint32_t*>(list);
+    static_assert(4 * kBins <= 2 * kList, "");
+    for (int i = tid; i < 4 * kBins; i += THREADS) hist[i] = 0;
+    __syncthreads();
     x.pieces_of([&](const uint4& r, int) {
-      if (Weigher::bin(weight.exponent(P::largest(r))) >= 0x4B000000 + kBins) return;
+      if (weight.place(P::largest(r)) >= 0x4B000000 + kBins * kFine) return;
 #pragma unroll
       for (int e = 0; e < x.E; ++e) {
-        const float at = weight.exponent(P::at(r, e));
-        const int bin = Weigher::bin(at) - 0x4B000000;
-        // the weight over that of the bin's factor of 2, in units of 2^-12: 2^23 is added, whose fraction takes it
-        const float w = __uint_as_float(__float_as_uint(ex2(at)) + ((bin & ~15) << 19));
-        if (bin < kBins) atomicAdd(&hist[bin], __float_as_uint(fmaf(w, 4096.f, 8388608.f)) & 0xFFFFu);
+        const int at = weight.place(P::at(r, e)) - 0x4B000000;
+        if (at < kBins * kFine) atomicAdd(&hist[at / kFine * 4 + (lane & 3)], 6038u - static_cast<uint32_t>(at % kFine));
       }
     });
     __syncthreads();
@@ -360,7 +372,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
         const int bin = lane * (kBins / 32) + i;
-        part[i] = hist[bin] * ex2(-12.f - (bin >> 4));
+        const uint4 h = reinterpret_cast<const uint4*>(hist)[bin];
+        part[i] = (h.x + h.y + h.z + h.w) * ex2(bin * -0.0625f);
         run += part[i];
       }
       float before = run;
@@ -369,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
         const float y = __shfl_up_sync(kFull, before, o);
         if (lane >= o) before += y;
       }
-      // roundings of up to 1 in 2^12, 32-bit exponentials and sums, and up to 2^19 logits below the bins: by 1 in 2^10
+      // weights to 1 in 2^12, sums in 32 bits, and up to 2^19 logits below the bins: by 1 in 2^10
       const float all = __shfl_sync(kFull, before, 31), goal = static_cast<float>(top_p) * all;
       before -= run;
       int may = kBins, does = kBins;
@@ -384,7 +397,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       if (lane == 0) s_bins[0] = may, s_bins[1] = does;
     }
     __syncthreads();
-    bin0 = 0x4B000000 + s_bins[0], bin1 = s_bins[1] >= kBins ? 0x7F800000 : 0x4B000000 + s_bins[1];
+    // (1 / 16 of a bin more on either side, for the roundings)
+    listed_to = s_bins[0] == 0 ? kInf : __fadd_ru(weight.top32, (1.f / 256 - s_bins[0] * 0.0625f) * weight.inv32);
+    listed_from = s_bins[1] >= kBins ? -kInf : __fadd_rd(weight.top32, (-1.f / 256 - (s_bins[1] + 1) * 0.0625f) * weight.inv32);
     listing = true;
   } else if (floor_key > 0) {
     from = floor_key, listing = true;
@@ -393,11 +408,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   uint32_t key[kEach];
   int n = 0;
   if (listing) {
-    // the elements of a piece that are in the row and for which `take` says so
-    const auto put = [&](const uint4& r, int p, auto&& take) {
-      uint32_t which = 0;
-#pragma unroll
-      for (int e = 0; e < x.E; ++e) which |= take(P::at(r, e)) ? 1u << e : 0u;
+    // the elements `which` of a piece, those that are in the row
+    const auto put = [&](int p, uint32_t which) {
       const int i0 = p * x.E - x.off;
       if (!x.inside(p)) {
 #pragma unroll
@@ -413,23 +425,32 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     if (bins) {
       u64 sum = 0;
       x.pieces_of([&](const uint4& r, int p) {
-        x.weigh(r, p, weight, [&](u64 w, float v, float at, int i) {
-          const int bin = Weigher::bin(at);
-          sum += w;
-          mine_above += bin < bin0 ? w : 0;
-        });
-        if (Weigher::bin(weight.exponent(P::largest(r))) <= bin1)
-          put(r, p, [&](float v) {
-            const int bin = Weigher::bin(weight.exponent(v));
-            return bin >= bin0 && bin <= bin1;
-          });
+        uint32_t which = 0;
+        if (weight.any(P::largest(r))) {
+#pragma unroll
+          for (int e = 0; e < x.E; ++e) {
+            const float y = weight.raised(P::at(r, e));
+            const u64 w = weight.raw(y);
+            sum += w;
+            if (y >= listed_to) mine_above += w;
+            else if (y >= listed_from) which |= 1u << e;
+          }
+        } else if (weight.least >= listed_from) {
+          which = (1u << x.E) - 1;
+        }
+        put(p, which);
       });
       need = need_of(sums(sum));
       above = sums(mine_above);
     } else {
       const float low = from == 0 ? -kInf : P::logit(from);
       x.pieces_of([&](const uint4& r, int p) {
-        if (P::largest(r) >= low) put(r, p, [&](float v) { return v >= low; });
+        if (!(P::largest(r) >= low)) return;
+        uint32_t which = 0;
+#pragma unroll
+        for (int e = 0; e < x.E; ++e)
+          if (P::at(r, e) >= low) which |= 1u << e;
+        put(p, which);
       });
       __syncthreads();
     }
@@ -472,8 +493,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       return sums(m);
     }
     const float low = P::logit(c);
-    x.pieces_of([&](const uint4& r, int p) {
-      if (P::largest(r) >= low) x.weigh(r, p, weight, [&](u64 y, float v, float, int) { m += v >= low ? y : 0; });
+    x.pieces_of([&](const uint4& r, int) {
+      if (P::largest(r) >= low) m += x.weigh(r, weight, low);
     });
     return sums(m);
   };
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   {
     uint32_t equal = 0;
     // Where the list holds all that is kept, or all but what has been weighed above its bins, it tells; else the row.
-    if (listed && !(bins && Weigher::bin(weight.exponent(low)) < bin0)) {
+    if (listed && !(bins && weight.raised(low) >= listed_to)) {
       for (int i = tid; i < kWarps * 3; i += THREADS) warp_parts[i / 3][i % 3] = 0;
       if (tid < kWarps) warp_ties[tid] = 0;
       __syncthreads();
@@ -535,14 +556,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       kept = mine_above;
       if (lane == 0) kept += warp_parts[warp][0] + (static_cast<u64>(warp_parts[warp][1]) << 20) + (static_cast<u64>(warp_parts[warp][2]) << 40);
     } else {
-      if (t == 0) {  // nothing is cut
-        x.pieces_of([&](const uint4& r, int p) { x.weigh(r, p, weight, [&](u64 y, float, float, int) { kept += y; }); });
-      } else x.pieces_of([&](const uint4& r, int p) {
+      const float above_ties = !limited ? low : t >= kmax ? kInf : P::logit(t + 1);
+      if (t == 0) x.pieces_of([&](const uint4& r, int) { kept += x.template weigh<true>(r, weight); });  // nothing is cut
+      else x.pieces_of([&](const uint4& r, int p) {
         if (!(P::largest(r) >= low)) return;
         if (limited) x.each(r, p, low, [&](float v, int) { equal += v == low; });
-        x.weigh(r, p, weight, [&](u64 y, float v, float, int) {
-          kept += v > low || (v == low && !limited) ? y : 0;
-        });
+        kept += x.weigh(r, weight, above_ties);
       });
     }
     if (limited) {
