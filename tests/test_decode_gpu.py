@@ -582,6 +582,26 @@ def test_sampling_many_rows_of_unlike_settings():
     assert got.tolist() == _want(x, V, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_sampling_at_the_ends_of_the_range(dtype):
+    """Logits and temperatures from the smallest to the largest numbers: all in one row, and next to masks of either kind."""
+    K, g = _k(), _gen(31)
+    top = torch.finfo(dtype).max
+    x = _rows(8, 2003, dtype, g)
+    x[1], x[2], x[3] = x[1] * 1e-30, x[2] * (top / 64), x[3] * 1e-38
+    x[4] = -top
+    x[4, ::7], x[4, 5::7] = -math.inf, -top * 0.99
+    x[5, ::2], x[5, 1::4] = top, -top
+    x[6] = 0.0
+    x[6, 3::5], x[6, 4::5] = -torch.finfo(dtype).tiny, -math.inf
+    x[7, 1:] = -math.inf
+    u = torch.rand(8, device="cuda", generator=g)
+    for t in (1e-40, 1e-30, 1e-7, 1e5, 1e30, 2.0 ** 121, 3e38, 1e300, math.inf):
+        for k, p, m in ((0, 1.0, 0.0), (9, 1.0, 0.0), (0, 0.6, 0.0), (50, 0.9, 0.1)):
+            assert K.sample_tokens(x, 2003, u, t, k, p, m).tolist() == _want(x, 2003, u, t, k, p, m), (t, k, p, m)
+    _status()
+
+
 def test_sampling_follows_the_distribution():
     """Numbers spread evenly over [0, 1) give every token its share: each border is at its running probability."""
     K, g = _k(), _gen(13)
