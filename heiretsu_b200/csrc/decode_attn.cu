@@ -122,13 +122,16 @@ struct Shape {
   static constexpr int kRow = D * kSize;                 // bytes of a token
   static constexpr int kBoxes = kRow <= 128 ? 1 : kRow / 128;  // along the channels
   static constexpr int kGroup = 16 * kRow;               // bytes of 16 tokens
-  // 4 KB of K and V (head dim 128 in 16 bits: 8; head dim 16 in codes: 2)
-  static constexpr int KT = kGroup >= 2048 ? 1 : kGroup == 1024 ? 2 : 4;
+  // What a warp takes at a time. In 16 bits 8 KB (head dim 16: 4): 61 x up to 1024 tokens of 12 heads of 64 take 26.9 us, with 4 KB
+  // 28.2. In codes the arithmetic is the longer part, and 4 KB are what two CTAs an SM have registers for: 256 x up to 1024 tokens
+  // of 20 heads of 64 100 us, with 2 KB 129, with 8 KB 110. Head dim 128 in codes: 8 KB and one CTA, 64 x up to 8192 tokens
+  // of 8 heads 115 us (pages of 16 tokens: 153); 4 KB and two CTAs, which have to spill, 141 with either page.
+  static constexpr int KT = CODES ? (kGroup >= 1024 ? 2 : 4) : (kGroup == 4096 ? 1 : kGroup == 2048 ? 2 : 4);
   static constexpr int kTokens = 16 * KT;
   static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
   static constexpr int kStage = 2 * kKv;
   static constexpr int kExps = CODES ? 2 * kTokens : 0;
-  static constexpr int kCtas = kGroup >= 4096 ? 1 : 2;   // on an SM: what the shared memory holds
+  static constexpr int kCtas = D == 128 ? 1 : 2;         // on an SM: what shared memory (16 bits) and registers (codes) hold
   static constexpr int kSteps = D / 16;                  // matrix instructions along the channels
 };
 // Where a lane's row of a matrix load is in 16 tokens, the group number j of a tile: chunk(c, j) is that of chunk c (known when
@@ -825,11 +828,15 @@ CUtensorMap cache_map(const KvPool& p, const void* base, long page, long head, l
 template <int D, bool F16, bool CODES>
 void launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
   using S = Shape<D, CODES>;
-  const int cols = std::min(a.heads_q / a.pool.heads, kCols), parts = kWarps * (part_head(cols) + cols * D) * 4 + 1024;
+  const auto parts_of = [](int cols) constexpr { return kWarps * (part_head(cols) + cols * D) * 4 + 1024; };
+  constexpr int kRing = kWarps * (S::kStage + S::kExps);  // a stage of every warp
+  const int parts = parts_of(std::min(a.heads_q / a.pool.heads, kCols));
   // 227 KB of an SM, less 1 KB a CTA and what the kernel declares
   constexpr int kRoom = (227 * 1024) / S::kCtas - 1024 - 9 * 1024;
-  const int stages = std::min(kMaxStages, (kRoom - parts) / (kWarps * (S::kStage + S::kExps)));
-  const size_t smem = static_cast<size_t>(kWarps) * stages * (S::kStage + S::kExps) + parts;
+  constexpr int kLeast = std::min(kMaxStages, (kRoom - parts_of(kCols)) / kRing);  // stages, with 8 query heads a K/V head
+  static_assert(kLeast >= 1 && kLeast * S::kStage >= (part_head(kCols) + kCols * D) * 4, "a stage and a part have to fit");
+  const int stages = std::min(kMaxStages, (kRoom - parts) / kRing);
+  const size_t smem = static_cast<size_t>(stages) * kRing + parts;
   const auto kernel = decode_attn_kernel<D, F16, CODES>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use that much shared memory
   const int dev = current_device();
@@ -853,7 +860,7 @@ void launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
   const int units = a.seqs * p.heads * ((a.heads_q / p.heads + kCols - 1) / kCols);
   const bool spread = ctas / 16 > units;
   cudaLaunchConfig_t cfg{};  // launched while the kernel above runs: it waits for its end by itself
-  cfg.gridDim = dim3(ctas, cols);
+  cfg.gridDim = dim3(ctas, std::min(a.heads_q / p.heads, kCols));
   cfg.blockDim = dim3(spread ? 8 * 32 : 32);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
