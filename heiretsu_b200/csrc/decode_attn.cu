@@ -2,6 +2,18 @@
 //   s_j = scale q.k_j,  j < length;  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m);  lse = m + log sum_j e^(s_j - m)
 // A sequence of length 0 gives 0 and -inf. A length outside [0, width * page size] or a page outside the cache gives NaN in
 // the sequence's rows, and the bad-argument status.
+//
+// Every K and V is read once and takes part in 4 operations a query head that shares it: bound by memory. So the tiles lie where
+// copies put them, and the products take the small matrix instructions (8 query heads are a column each; those of 128 rows
+// would be all but empty). Device times on a B200, and what the bytes alone take at a copy's 6.5 TB/s:
+//   64 sequences of up to 8192 tokens, 8 K/V heads of 128 with 4 query heads each, bf16    181 us    169
+//   1 of 100003, the same heads, fp16                                                       73       63
+//   61 of up to 1024, 12 heads of 64, bf16                                                  26.9     14.6
+//   256 of up to 1024, 20 heads of 64, in codes                                            100       54
+//   1 of 57, 12 heads of 64                                                                  5.7      0.03
+// Long sequences are near their bytes. Short ones pay the start, the joins and the second kernel (about 3 us each); codes
+// pay their widening, 5 to 7 instructions for 4 codes, beside copies that would take 70 us alone.
+// Tried and slower: tiles loaded into registers (64 x 8192 227 us), every warp copying for itself (256 in codes 109).
 #include <algorithm>
 #include <atomic>
 
@@ -248,17 +260,17 @@ __device__ __forceinline__ int share(int total, int c, int n) {
   return c * each + min(c, more);
 }
 
+// How copies bring tiles: `packed` as in Place; `joint`: a page holds whole tiles, and one copy brings K of one.
+struct Boxes {
+  bool packed, joint;
+};
+
 // Work is a list of tiles of 16 * KT tokens, ordered by sequence, then unit, then token. Every CTA takes an equal run of it
 // and every warp an equal run of the CTA's, whatever the lengths are: a unit may lie inside a warp's run, or be
 // spread over warps and CTAs. A warp walks its run with a running maximum and sum per query head; what it has of a
 // unit that is not wholly its own goes to shared memory, the CTA joins these, and what the CTA has of a unit
 // that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. Without a.record CTAs take whole
 // units, and nothing is left to join.
-// How copies bring tiles: `packed` as in Place; `joint`: a page holds whole tiles, and one copy brings K of one.
-struct Boxes {
-  bool packed, joint;
-};
-
 template <int D, bool F16, bool CODES>
 __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     decode_attn_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -269,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   // are widened to bf16: a weight takes the scale of its head of a token with it, and these may lie further apart than fp16 goes.
   constexpr bool V16 = F16 && !CODES;
   // The scores' reference is raised only where one passes it by more than 2^kSlack: maxima across lanes cost more than the
-  // rest of a tile's softmax. fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest;
+  // rest of a tile's softmax (64 x 8192: 180.6 us instead of 181.2). fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest;
   // bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
   constexpr float kSlack = 8.f, kLift = V16 ? 7.f : -kSlack;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
@@ -876,9 +888,10 @@ void launch_dim(const DecodeArgs& a, int ctas, cudaStream_t s) {
   else a.f16 ? launch<D, true, false>(a, ctas, s) : launch<D, false, false>(a, ctas, s);
 }
 
-// Tables of at most this many tokens: CTAs take whole units, which saves the second kernel (12 heads of 64, bf16: 1 sequence of up
-// to 256 tokens 6.9 us instead of 8.2, 8 sequences 7.3 instead of 9.3, 128 sequences 20.3 instead of 19.8; of up to 512
-// tokens 8.8 instead of 7.9, 8.9 instead of 9.6, 32.9 instead of 29.1).
+// Tables of at most this many tokens, and of at most three times as many for each CTA that fits: CTAs take whole units, which
+// saves the second kernel. 12 heads of 64, bf16: 8 sequences of up to 256 tokens 6.8 us instead of 9.6, 64 of them 13.5
+// instead of 14.8 (664 tokens a CTA); but 128 of up to 200 19.9 instead of 19.1 (1038), 512 of up to 256 56 instead of 48; and 8 of up
+// to 512 8.9 instead of 9.6, but 1 of up to 512 8.8 instead of 7.9.
 constexpr int kWholeTokens = 256;
 
 // CTAs on an SM, and tokens of a tile.
@@ -902,7 +915,7 @@ DecodePlan decode_attention_plan(const KvPool& p, int seqs, int units, int longe
   d.seqs = static_cast<int>(std::min<long>(std::min(seqs, kMaxSeqs), most / std::max(1l, units * tiles)));
   if (d.seqs == 0) return d;
   const long all = static_cast<long>(d.seqs) * units, sms = num_sms(current_device());
-  const bool whole = longest <= kWholeTokens;
+  const bool whole = longest <= kWholeTokens && all * longest <= 3l * kWholeTokens * f.ctas * sms;
   d.ctas = static_cast<int>(std::max(1l, std::min(f.ctas * sms, whole ? all : (all * tiles + kWarps - 1) / kWarps)));
   d.split = !whole && d.ctas > 1;
   return d;

@@ -10,6 +10,12 @@
 // out whatever the launch, and equal logits weigh exactly the same. A sum over the 2^19 columns allowed stays below 2^64.
 // 32-bit exponentials would not do: the chance that a number falls on another token is twice the error of the running
 // weights times the number of tokens in play, about 5% a row for 10,000 tokens at 2^-18.
+//
+// The row is read once, and its passes are made in shared memory: bound by the arithmetic of the weights (10 instructions
+// in 64 bits and about 20 others each) and, for few rows, by the chain of barriers. Device times on a B200, and what the
+// bytes alone take: rows of 50257, 1 by top_k 15.0 us (0.02), 64 whole ones in 32 bits 17.0 us (2.0), 256 by top_p 54.8 us
+// (3.9); 101 of 32003 with settings of their own 28.7 us (1.0).
+// Tried and slower: searches by one warp (1 row 22.5 us) or of two bits a step (17.7), tables of 256 exponentials.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -650,7 +656,8 @@ void launch(const SampleArgs& a, cudaStream_t s) {
 }
 template <int TYPE>
 void launch_type(const SampleArgs& a, cudaStream_t s) {
-  // More rows than SMs: two blocks of half the threads share one and overlap their passes
+  // More rows than SMs: two blocks of half the threads share one and overlap their passes (256 rows by top_p 55 us instead
+  // of 68). Fewer: a row takes all threads of its SM (64 rows 17 us instead of 22, 1 row 15 instead of 17).
   if (a.rows > num_sms(current_device())) launch<TYPE, 512>(a, s);
   else launch<TYPE, 1024>(a, s);
 }
