@@ -144,13 +144,13 @@ class Decoder:
         if self.pending is not None:
             idx, lengths = torch.cat([self.pending[:, None], idx], 1), [n + 1 for n in lengths]
         self._reserve(lengths)
-        self.pending = self.logits = None
         training = self.model.training
         self.model.eval()
         try:
             self.logits = self._prefill(idx.contiguous(), lengths)
         finally:
             self.model.train(training)
+        self.pending = None
         self.lens = [a + n for a, n in zip(self.lens, lengths)]
         self.lengths.copy_(torch.tensor(self.lens, dtype=torch.int32))
         return self.logits[:, : self.model.cfg.vocab_size]
@@ -212,11 +212,11 @@ class Decoder:
             at.add_(1)
             return token
 
-        training = self.model.training
+        training, logits = self.model.training, self.logits
         self.model.eval()
         try:
-            if self.logits is not None:
-                token = sample(self.logits)
+            if logits is not None:
+                token = sample(logits)
                 self.logits = None
             else:
                 token = self.pending
@@ -233,6 +233,10 @@ class Decoder:
                     g.replay()
                 torch.cuda.current_stream().synchronize()  # before the graph and its memory go
                 del g
+        except BaseException:  # nothing was generated: the next call begins where this one did
+            self.logits = logits
+            self.lengths.copy_(torch.tensor(self.lens, dtype=torch.int32))
+            raise
         finally:
             self.model.train(training)
         self.lens = [a + steps for a in self.lens]

@@ -66,6 +66,48 @@ def test_prompts_of_unlike_lengths_and_what_is_added_later(monkeypatch):
     assert d.lens == [n1[i] + n2[i] + 6 + 9 for i in range(3)]
 
 
+@pytest.mark.parametrize("steps", [1, 4])
+def test_a_call_that_fails_can_be_made_again(monkeypatch, steps):
+    """An error in the middle of append or generate (memory that runs out, say) leaves the sequences as they were."""
+    from heiretsu_b200.models import decode
+
+    emulate(monkeypatch)
+    m = _model()
+    idx = _ids(2, 5)
+    want = generate(m, idx, 12, temperature=0)
+    d = Decoder(m, 2, page_size=16)
+    calls = []
+
+    def failing(name, at):
+        real = getattr(decode.K, name)
+
+        def call(*a, **kw):
+            calls.append(name)
+            if len(calls) == at:
+                raise RuntimeError("out of memory")
+            return real(*a, **kw)
+
+        calls.clear()
+        monkeypatch.setattr(decode.K, name, call)
+        return lambda: monkeypatch.setattr(decode.K, name, real)
+
+    for prompt in (idx[:, :3], idx[:, 3:]):
+        undo = failing("kv_write", 2)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            d.append(prompt)
+        undo()
+        d.append(prompt)
+    out = []
+    for _ in range(2):
+        undo = failing("sample_tokens", steps)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            d.generate(6, temperature=0)
+        undo()
+        assert d.lengths.tolist() == d.lens and m.training
+        out.append(d.generate(6, temperature=0))
+    assert torch.equal(torch.cat([idx, *out], 1), want)
+
+
 def test_mixture_of_experts_and_8_bits(monkeypatch):
     from moe_emulation import emulate_moe
 

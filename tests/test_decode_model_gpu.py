@@ -134,6 +134,13 @@ def test_sampled_tokens_train_a_policy():
     assert abs(float(loss.detach()) + 1) < 1e-5  # -(mean of ratio 1 times advantage 1)
 
 
+def test_model_method_without_a_cache():
+    m = _model()
+    idx = _ids(2, 6)
+    out = m.generate(idx, 5, temperature=0, kv_cache=False)
+    assert torch.equal(out, m.generate(idx, 5, temperature=0, engine="plain"))
+
+
 def test_sample_script_on_the_fused_engine(tmp_path):
     m = _model(vocab=300)
     torch.save({"model": m.state_dict(), "cfg": asdict(m.cfg), "step": 1}, tmp_path / "dense.pt")
