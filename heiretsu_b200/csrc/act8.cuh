@@ -35,12 +35,12 @@ __device__ __forceinline__ float act8_scale(uint32_t byte) {
   return byte == kAct8Nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
 }
 // Four codes, the first in the low byte. Rounding by adding 1.5 * 2^23: the sum's low byte is the code in two's
-// complement (|x 2^-e| <= 127). Blocks with byte 255 get codes 0 (an infinity or NaN times 0 is NaN).
+// complement (|x 2^-e| <= 127; the product is exact, or too small to count). Blocks with byte 255 get codes 0 (an infinity or NaN times 0 is NaN).
 __device__ __forceinline__ uint32_t act8_codes(const float (&x)[4], uint32_t byte) {
   const float inv = act8_inv_scale(byte);
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+  for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fmaf_rn(x[i], inv, 12582912.f));
   const uint32_t all = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
   return byte == kAct8Nan ? 0u : all;
 }

@@ -19,7 +19,7 @@ struct KvPool {
   long kp, kh, ks, vp, vh, vs;     // strides in elements
   long kep, keh, vep, veh;
   int pages, heads, size, dim;     // size: slots of a page
-  int groups;                      // of 16 slots in a page
+  uint32_t per_head, per_slot;     // 2^32 over heads and size, rounded down (below 2^32)
   int type;                        // KvType
 };
 

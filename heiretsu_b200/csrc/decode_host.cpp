@@ -108,7 +108,8 @@ KvPool check_pool(const at::Tensor& k, const at::Tensor& v, const OptTensor& ke,
   p.vp = v.stride(0), p.vh = v.stride(1), p.vs = v.stride(2);
   p.pages = static_cast<int>(k.size(0)), p.heads = static_cast<int>(k.size(1));
   p.size = static_cast<int>(size), p.dim = static_cast<int>(D);
-  p.groups = p.size / 16;
+  p.per_head = static_cast<uint32_t>(std::min((int64_t{1} << 32) / p.heads, (int64_t{1} << 32) - 1));
+  p.per_slot = static_cast<uint32_t>((int64_t{1} << 32) / p.size);
   p.type = dt == at::kChar ? kKvCodes : dt == at::kHalf ? kKvF16 : kKvBf16;
   check_same_device(v, k.device(), op, "v_pages");
   TORCH_CHECK(given(ke) == (dt == at::kChar) && given(ve) == (dt == at::kChar), op,

@@ -2,7 +2,7 @@
 // written (the format of act8.cuh with a block per head of a token), and back:
 //   byte = e + 127, e >= -126 the least with max |x| <= 127 * 2^e over a head of a token;  code = rint(x / 2^e);  x' = code * 2^e
 // Bound by memory (one pass, 16 bytes a load), and for a step's few tokens by the launch. B200, write and read together:
-// 8192 tokens of 20 heads of 64 into 8 bits and back 28.4 us (126 MB, 4.5 TB/s), 4099 of 12 heads in 16 bits 8.6 us,
+// 8192 tokens of 20 heads of 64 into 8 bits and back 26.2 us (126 MB, 4.8 TB/s), 4099 of 12 heads in 16 bits 8.6 us,
 // 16 tokens into 8 bits 3.9 us.
 #include "act8.cuh"
 #include "common.cuh"
@@ -41,15 +41,24 @@ __device__ __forceinline__ uint2 quantise8(const uint4& r, uint32_t& byte) {
   return make_uint2(act8_codes(a, byte), act8_codes(b, byte));
 }
 
-// Where a token's slot is. (A division in 64 bits costs five times one in 32.)
+// x / d and what remains, from 2^32 / d rounded down (at most 2^32 - 1): x times that, over 2^32, is less than 1 below x / d, so
+// the quotient is right or one too small. Shorter than a division (8192 tokens 28.4 -> 26.2 us).
+__device__ __forceinline__ uint32_t divide(uint32_t x, uint32_t d, uint32_t per, uint32_t& left) {
+  uint32_t q = __umulhi(x, per);
+  left = x - q * d;
+  if (left >= d) ++q, left -= d;
+  return q;
+}
+
+// Where a token's slot is.
 struct Place {
   bool in;
   uint32_t page, at;
   __device__ __forceinline__ Place(int64_t slot, const KvPool& p) {
     in = slot >= 0 && slot < static_cast<int64_t>(p.pages) * p.size;
-    const uint32_t size = p.size;
-    page = !in ? 0 : slot <= 0xFFFFFFFFll ? static_cast<uint32_t>(slot) / size : static_cast<uint32_t>(slot / p.size);
-    at = in ? static_cast<uint32_t>(slot - static_cast<int64_t>(page) * p.size) : 0;
+    page = at = 0;
+    if (in && slot <= 0xFFFFFFFFll) page = divide(static_cast<uint32_t>(slot), p.size, p.per_slot, at);
+    else if (in) page = static_cast<uint32_t>(slot / p.size), at = static_cast<uint32_t>(slot % p.size);
   }
 };
 // Strides are below 2^32 elements: one instruction a product.
@@ -62,19 +71,20 @@ __device__ __forceinline__ long times(uint32_t a, long stride) {
 struct Share {
   int part, head, token;
   template <int LANES>
-  __device__ __forceinline__ static Share of(int heads) {
+  __device__ __forceinline__ static Share of(const KvPool& p) {
     const uint32_t row = (blockIdx.x * kThreads + threadIdx.x) / LANES;
     Share s;
     s.part = threadIdx.x % LANES;
-    s.token = row / static_cast<uint32_t>(heads);
-    s.head = row - s.token * heads;
+    uint32_t head;
+    s.token = divide(row, p.heads, p.per_head, head);
+    s.head = head;
     return s;
   }
 };
 
 template <int LANES, bool CODES, bool F16>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvTokens t, const KvPool p, int* status) {
-  const Share me = Share::of<LANES>(p.heads);
+  const Share me = Share::of<LANES>(p);
   const int token = min(me.token, t.n - 1);  // threads without a token only take part in the exchange of lanes
   const int64_t slot = t.slots[token];
   const uint4 k = load8(t.k, times(token, t.kt) + times(me.head, t.kh) + me.part * 8, t.vec);
@@ -137,7 +147,7 @@ __device__ __forceinline__ void decode8(const uint2& codes, uint32_t byte, float
 template <int LANES, bool CODES, int OUT>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const int64_t* __restrict__ slots, const KvPool p, void* k,
                                                            void* v, int n, int* status) {
-  const Share me = Share::of<LANES>(p.heads);
+  const Share me = Share::of<LANES>(p);
   if (me.token >= n) return;
   const int64_t slot = slots[me.token];
   const Place s(slot, p);
