@@ -13,7 +13,7 @@
 //
 // The row is read once, and its passes are made in shared memory: bound by the arithmetic of the weights (10 instructions
 // in 64 bits and about 20 others each) and, for few rows, by the chain of barriers. Device times on a B200, and what the
-// bytes alone take: rows of 50257, 1 by top_k 15.0 us (0.02), 64 whole ones in 32 bits 17.0 us (2.0), 256 by top_p 54.8 us
+// bytes alone take: rows of 50257, 1 by top_k 15.0 us (0.02), 64 whole ones in 32 bits 17.0 us (2.0), 256 by top_p 53.5 us
 // (3.9); 101 of 32003 with settings of their own 28.7 us (1.0).
 // Tried and slower: searches by one warp (1 row 22.5 us) or of two bits a step (17.7), tables of 256 exponentials.
 #include <cuda_bf16.h>
@@ -603,24 +603,41 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
   const int owner = __ffs(__ballot_sync(kFull, lane < kWarps && target < upto_all)) - 1;
   target -= __shfl_sync(kFull, upto_all - own, owner);
   u64 tie0 = __shfl_sync(kFull, tie_upto - tie_own, owner);
-  // The part of warp `owner`, THREADS elements at a time, one to a thread.
+  // The part of warp `owner`, kRun elements in turn to a thread: with 512 threads a part is 1 / 16 of the row, and fewer rounds
+  // count (256 rows by top_p 53.5 us, with 1 element 54.7); with 1024 the first result does (1 row 15.0 us, with 4 elements 15.7).
+  constexpr int kRun = THREADS == 512 ? 4 : 1;
   const int i1 = min((owner + 1) * x.per * x.E - x.off, a.V);
   __syncthreads();
-  for (int i0 = max(owner * x.per * x.E - x.off, 0); i0 < i1; i0 += THREADS) {
-    const int i = i0 + tid;
-    const float v = i < i1 ? P::value(x.bits(i)) : -kInf;
-    const bool equal = i < i1 && v == low;
-    u64 y = i < i1 && (v > low || equal) ? weight(v) : 0;
+  for (int i0 = max(owner * x.per * x.E - x.off, 0); i0 < i1; i0 += kRun * THREADS) {
+    const int i = i0 + kRun * tid;
+    u64 y[kRun];
+    uint32_t equal = 0;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      const float v = i + e < i1 ? P::value(x.bits(i + e)) : -kInf;
+      y[e] = v >= low ? weight(v) : 0;
+      equal |= i + e < i1 && v == low ? 1u << e : 0;
+    }
     if (limited) {
-      const uint32_t vote = __ballot_sync(kFull, equal);
-      if (lane == 0) warp_ties[warp] = __popc(vote);
+      uint32_t upto = __popc(equal);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t z = __shfl_up_sync(kFull, upto, o);
+        if (lane >= o) upto += z;
+      }
+      if (lane == 31) warp_ties[warp] = upto;
       __syncthreads();
       const uint32_t o = lane < kWarps ? warp_ties[lane] : 0, s = static_cast<uint32_t>(scan(o));
-      const u64 rank = tie0 + __shfl_sync(kFull, s - o, warp) + __popc(vote & ((1u << lane) - 1));
+      u64 rank = tie0 + __shfl_sync(kFull, s - o, warp) + upto - __popc(equal);
       tie0 += __shfl_sync(kFull, s, kWarps - 1);
-      if (equal && rank >= ties) y = 0;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (equal >> e & 1 && rank++ >= ties) y[e] = 0;
     }
-    u64 upto = y;
+    u64 upto = 0;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) upto += y[e];
+    const u64 mine_all = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 z = __shfl_up_sync(kFull, upto, o);
@@ -631,7 +648,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
     const u64 o = lane < kWarps ? warp_sums[lane] : 0, s = scan(o), all = __shfl_sync(kFull, s, kWarps - 1);
     upto += __shfl_sync(kFull, s - o, warp);
     if (target < all) {
-      if (target >= upto - y && target < upto) a.tokens[row] = i;
+      u64 at = upto - mine_all;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        if (target >= at && target < at + y[e]) a.tokens[row] = i + e;
+        at += y[e];
+      }
       return;
     }
     target -= all;
@@ -656,7 +678,7 @@ void launch(const SampleArgs& a, cudaStream_t s) {
 }
 template <int TYPE>
 void launch_type(const SampleArgs& a, cudaStream_t s) {
-  // More rows than SMs: two blocks of half the threads share one and overlap their passes (256 rows by top_p 55 us instead
+  // More rows than SMs: two blocks of half the threads share one and overlap their passes (256 rows by top_p 54 us instead
   // of 68). Fewer: a row takes all threads of its SM (64 rows 17 us instead of 22, 1 row 15 instead of 17).
   if (a.rows > num_sms(current_device())) launch<TYPE, 512>(a, s);
   else launch<TYPE, 1024>(a, s);
