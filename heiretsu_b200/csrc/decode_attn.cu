@@ -26,8 +26,7 @@ namespace hb {
 
 namespace {
 
-constexpr int kWarps = 8;                       // that compute; one more copies
-constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kWarps = 8;                       // that compute
 constexpr int kCols = 8;        // query heads of a unit: the columns of one matrix instruction
 constexpr int kSite = 430;      // status site
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -137,7 +136,7 @@ struct Shape {
   // What a warp takes at a time. In 16 bits 8 KB (head dim 16: 4): 61 x up to 1024 tokens of 12 heads of 64 take 26.9 us, with 4 KB
   // 28.2. In codes the arithmetic is the longer part, and 4 KB are what two CTAs an SM have registers for: 256 x up to 1024 tokens
   // of 20 heads of 64 100 us, with 2 KB 129, with 8 KB 110. Head dim 128 in codes: 8 KB and one CTA, 64 x up to 8192 tokens
-  // of 8 heads 115 us (pages of 16 tokens: 153); 4 KB and two CTAs, which have to spill, 141 with either page.
+  // of 8 heads 115 us; 4 KB and two CTAs, which have to spill, 141.
   static constexpr int KT = CODES ? (kGroup >= 1024 ? 2 : 4) : (kGroup == 4096 ? 1 : kGroup == 2048 ? 2 : 4);
   static constexpr int kTokens = 16 * KT;
   static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
@@ -145,6 +144,11 @@ struct Shape {
   static constexpr int kExps = CODES ? 2 * kTokens : 0;
   static constexpr int kCtas = D == 128 ? 1 : 2;         // on an SM: what shared memory (16 bits) and registers (codes) hold
   static constexpr int kSteps = D / 16;                  // matrix instructions along the channels
+  // Warps that issue copies, which a warp does one lane after the other. As many as leave the registers to the rest: 64 x up to 8192
+  // tokens of 8 heads of 128 take 174.5 us (with two such warps 177.8, with one 179.6), in codes with pages of 16 tokens
+  // 113 (115, 152), 256 x up to 1024 of 20 heads of 64 in codes with such pages 101 with two (114 with one).
+  static constexpr int kMovers = kCtas == 1 ? 4 : 2;
+  static constexpr int kThreads = 32 * (kWarps + kMovers);
 };
 // Where a lane's row of a matrix load is in 16 tokens, the group number j of a tile: chunk(c, j) is that of chunk c (known when
 // compiled) of token r, c without its bits in `c0`. `packed`: the cache's slots follow one another, and where a token is
@@ -272,11 +276,11 @@ struct Boxes {
 // that is not wholly its own goes to a.part, for join_kernel. Sums have a fixed order. Without a.record CTAs take whole
 // units, and nothing is left to join.
 template <int D, bool F16, bool CODES>
-__global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
+__global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>::kCtas))
     decode_attn_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                        const int stages, const Boxes boxes) {
   using S = Shape<D, CODES>;
-  constexpr int KT = S::KT;
+  constexpr int KT = S::KT, kThreads = S::kThreads, kEach = kWarps / S::kMovers;
   // Codes of K are widened to fp16, in fewer instructions than to bf16, and bf16 q is scaled by a power of two for it. Codes of V
   // are widened to bf16: a weight takes the scale of its head of a token with it, and these may lie further apart than fp16 goes.
   constexpr bool V16 = F16 && !CODES;
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int prefix[kMaxSeqs + 1], lens[kMaxSeqs];  // tiles of a unit before each sequence; their lengths
-  __shared__ int sums[kWarps + 1];
+  __shared__ int sums[kWarps + S::kMovers];
   __shared__ int seg_unit[2 * kWarps], seg_first[2 * kWarps], seg_last[2 * kWarps], seg_tiles[2 * kWarps];
   __shared__ uint64_t full[kWarps][kMaxStages], empty[kWarps][kMaxStages];
   __shared__ uint32_t lost[kWarps][kMaxStages];  // groups of a stage's tile whose page is none
@@ -391,11 +395,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
   };
 
   uint8_t* const exps_at = smem + kWarps * stages * S::kStage;
-  if (warp == kWarps) {
-    // Lane i keeps the ring of warp i filled: the copies of a tile are issued when its stage has been read, in the order of the
+  if (warp >= kWarps) {
+    // Lane i of the first such warp keeps the ring of warp i filled, of the next one that of warp kEach + i: the copies of a tile are issued when its stage has been read, in the order of the
     // warp's run and across its units. The places of the next tile are on their way meanwhile.
-    const int run = min(lane, kWarps - 1), w0 = c0 + share(c1 - c0, run, kWarps);
-    int left = lane < kWarps ? c0 + share(c1 - c0, run + 1, kWarps) - w0 : 0;
+    const int run = (warp - kWarps) * kEach + min(lane, kEach - 1), w0 = c0 + share(c1 - c0, run, kWarps);
+    int left = lane < kEach ? c0 + share(c1 - c0, run + 1, kWarps) - w0 : 0;
     Walk nx{};
     int len = 0, index = 0, slot = 0, page[KT];  // index, slot: of the tile's first token in the row of the table and in its page
     const auto look_ahead = [&]() {
@@ -768,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, CODES>::kCtas))
     const Columns c(n, id - b * n.units);
     const bool whole = first == 0 && seg_last[end] == seg_tiles[i0];
     const int slot = 2 * blockIdx.x + (first == 0 ? 1 : 0);
-    for (; col < c.nq; col += kWarps + 1) {
+    for (; col < c.nq; col += kWarps + S::kMovers) {
       if (col == 0 && lane == 0 && !whole) {
         // how many CTAs behind this one have a part of a unit that begins here
         const int left = seg_tiles[i0] - seg_last[end];
@@ -895,7 +899,7 @@ void launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
     k_map = cache_map<D, CODES>(p, p.k, p.kp, p.kh, p.ks, boxes);
     v_map = cache_map<D, CODES>(p, p.v, p.vp, p.vh, p.vs, boxes);
   }
-  kernel<<<ctas, kThreads, smem, s>>>(a, k_map, v_map, stages, boxes);
+  kernel<<<ctas, S::kThreads, smem, s>>>(a, k_map, v_map, stages, boxes);
   HB_CUDA_CHECK(cudaGetLastError());
   if (a.record == nullptr) return;
   // Where a unit is spread over more than 16 CTAs on average, 8 warps join its parts (one sequence of 131072 tokens and one K/V
