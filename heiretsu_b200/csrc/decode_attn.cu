@@ -6,14 +6,15 @@
 // Every K and V is read once and takes part in 4 operations a query head that shares it: bound by memory. So the tiles lie where
 // copies put them, and the products take the small matrix instructions (8 query heads are a column each; those of 128 rows
 // would be all but empty). Device times on a B200, and what the bytes alone take at a copy's 6.5 TB/s:
-//   64 sequences of up to 8192 tokens, 8 K/V heads of 128 with 4 query heads each, bf16    180 us    169
-//   1 of 100003, the same heads, fp16                                                       73       63
-//   61 of up to 1024, 12 heads of 64, bf16                                                  25.7     14.6
-//   256 of up to 1024, 20 heads of 64, in codes                                             99       54
+//   64 sequences of up to 8192 tokens, 8 K/V heads of 128 with 4 query heads each, bf16    174 us    169
+//   1 of 100003, the same heads, fp16                                                       71       63
+//   61 of up to 1024, 12 heads of 64, bf16                                                  25.1     14.6
+//   256 of up to 1024, 20 heads of 64, in codes                                             96       54
 //   1 of 57, 12 heads of 64                                                                  5.7      0.03
 // Long sequences are near their bytes. Short ones pay the start, the joins and the second kernel (about 3 us each); codes
-// pay their widening, 5 to 7 instructions for 4 codes, beside copies that would take 70 us alone.
-// Tried and slower: tiles loaded into registers (64 x 8192 227 us), every warp copying for itself (256 in codes 109).
+// pay their widening, 5 to 7 instructions for 4 codes.
+// Tried and slower: tiles loaded into registers (64 x 8192 227 us instead of 191), every warp copying for itself (256 in
+// codes 109 instead of 95), stages of K and of V apart (64 x 8192 184 instead of 174).
 #include <algorithm>
 #include <atomic>
 
@@ -133,16 +134,17 @@ struct Shape {
   static constexpr int kRow = D * kSize;                 // bytes of a token
   static constexpr int kBoxes = kRow <= 128 ? 1 : kRow / 128;  // along the channels
   static constexpr int kGroup = 16 * kRow;               // bytes of 16 tokens
-  // What a warp takes at a time. In 16 bits 8 KB (head dim 16: 4): 61 x up to 1024 tokens of 12 heads of 64 take 26.9 us, with 4 KB
-  // 28.2. In codes the arithmetic is the longer part, and 4 KB are what two CTAs an SM have registers for: 256 x up to 1024 tokens
-  // of 20 heads of 64 100 us, with 2 KB 129, with 8 KB 110. Head dim 128 in codes: 8 KB and one CTA, 64 x up to 8192 tokens
-  // of 8 heads 115 us; 4 KB and two CTAs, which have to spill, 141.
-  static constexpr int KT = CODES ? (kGroup >= 1024 ? 2 : 4) : (kGroup == 4096 ? 1 : kGroup == 2048 ? 2 : 4);
+  // What a warp takes at a time: 8 KB of K and V (head dim 16, and 32 in codes: 4, 16 in codes: 2). 61 x up to 1024 tokens of 12
+  // heads of 64 take 26.9 us in bf16, with 4 KB 28.2. In codes the registers for that are there with one CTA an SM: 256 x up to
+  // 1024 tokens of 20 heads of 64 96.5 us, 1 x 60000 of 2 heads 15.3; with 4 KB and two CTAs 99 and 19.1 (but 16 x up to 384
+  // of 12 heads 9.1 instead of 10.0), with 2 KB 129. Head dim 128 in codes, 64 x up to 8192 tokens of 8 heads: 115 us; 4 KB and
+  // two CTAs, which have to spill, 141.
+  static constexpr int KT = kGroup == 4096 ? 1 : kGroup == 2048 ? 2 : 4;
   static constexpr int kTokens = 16 * KT;
   static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
   static constexpr int kStage = 2 * kKv;
   static constexpr int kExps = CODES ? 2 * kTokens : 0;
-  static constexpr int kCtas = D == 128 ? 1 : 2;         // on an SM: what shared memory (16 bits) and registers (codes) hold
+  static constexpr int kCtas = D == 128 || (CODES && D == 64) ? 1 : 2;  // on an SM: what its memory (16 bits) and registers hold
   static constexpr int kSteps = D / 16;                  // matrix instructions along the channels
   // Warps that issue copies, which a warp does one lane after the other. As many as leave the registers to the rest: 64 x up to 8192
   // tokens of 8 heads of 128 take 174.5 us (with two such warps 177.8, with one 179.6), in codes with pages of 16 tokens
