@@ -927,9 +927,10 @@ void launch_dim(const DecodeArgs& a, int ctas, cudaStream_t s) {
 }
 
 // Tables of at most this many tokens, and of at most three times as many for each CTA that fits: CTAs take whole units, which
-// saves the second kernel. 12 heads of 64, bf16: 8 sequences of up to 256 tokens 6.8 us instead of 9.6, 64 of them 13.5
-// instead of 14.8 (664 tokens a CTA); but 128 of up to 200 19.9 instead of 19.1 (1038), 512 of up to 256 56 instead of 48; and 8 of up
-// to 512 8.9 instead of 9.6, but 1 of up to 512 8.8 instead of 7.9.
+// saves the second kernel. 12 heads of 64, bf16: 8 sequences of up to 256 tokens 6.4 us instead of 8.4, 64 of them 12.9
+// instead of 13.9 (664 tokens a CTA); but 128 of up to 200 19.2 instead of 18.1 (1038), 512 of up to 256 53 instead of 45; and 8 of up
+// to 512 8.0 instead of 9.4, but 1 of up to 512 8.3 instead of 7.3. (8 heads of 128, 4 query heads each, would gain beyond
+// that: 128 of up to 200 19.7 instead of 22.3; 20 heads of 64 in codes would lose, 25 instead of 21.)
 constexpr int kWholeTokens = 256;
 
 // CTAs on an SM, and tokens of a tile.
