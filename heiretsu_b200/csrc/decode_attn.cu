@@ -287,8 +287,8 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
   // are widened to bf16: a weight takes the scale of its head of a token with it, and these may lie further apart than fp16 goes.
   constexpr bool V16 = F16 && !CODES;
   // The scores' reference is raised only where one passes it by more than 2^kSlack: maxima across lanes cost more than the
-  // rest of a tile's softmax (64 x 8192: 180.6 us instead of 181.2). fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest;
-  // bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
+  // rest of a tile's softmax (64 x 8192: 180.6 us instead of 181.2). fp16 weights are lifted by 2^kLift, which keeps them
+  // below 2^15 and what is 2^-31 of the largest; bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
   constexpr float kSlack = 8.f, kLift = V16 ? 7.f : -kSlack;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -794,14 +794,9 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
   }
 }
 
-// Joins the parts of the units that CTAs share. CTA (c, y): column y of the unit that begins in CTA c of the kernel above and does
-// not end there, if any; its other parts are the first ones of the CTAs behind. WARPS > 1, for units of many parts: the
-// warps take equal runs of them first.
-//
-// Most units have two parts, whose places are known without the record. So a warp asks for both along with it: one
-// round trip to memory instead of three (61 x up to 1024 tokens 26.7 -> 25.7 us).
+// Loads at this place in the program, not where the values are used.
 template <int N>
-__device__ __forceinline__ void ask(const float* at, float (&v)[N]) {  // here, not where the values are used
+__device__ __forceinline__ void ask(const float* at, float (&v)[N]) {
   if constexpr (N == 4)
     asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(at) : "memory");
   else if constexpr (N == 2)
@@ -809,6 +804,13 @@ __device__ __forceinline__ void ask(const float* at, float (&v)[N]) {  // here, 
   else
     asm volatile("ld.global.f32 %0, [%1];" : "=f"(v[0]) : "l"(at) : "memory");
 }
+
+// Joins the parts of the units that CTAs share. CTA (c, y): column y of the unit that begins in CTA c of the kernel above and does
+// not end there, if any; its other parts are the first ones of the CTAs behind. WARPS > 1, for units of many parts: the
+// warps take equal runs of them first.
+//
+// Most units have two parts, whose places are known without the record. So a warp asks for both along with it: one
+// round trip to memory instead of three (61 x up to 1024 tokens 26.7 -> 25.7 us).
 template <int D, bool F16, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) join_kernel(const DecodeArgs a) {
   const Heads n(a);
