@@ -13,6 +13,9 @@ Sequences may have unlike lengths. Pages are dealt out as sequences grow, from o
 """
 from __future__ import annotations
 
+import contextlib
+import functools
+import gc
 from typing import List, Optional, Sequence
 
 import torch
@@ -22,6 +25,33 @@ from ..ops import kernels as K
 from .fused import LN_EPS, _dt, _is_moe, _vpad, fused_supported
 
 GRAPH_STEPS = 8  # a capture costs some 5 steps: fewer are run one by one
+
+
+def _on_its_device(method):
+    """The method of a decoder with the decoder's device as the current one."""
+    @functools.wraps(method)
+    def call(self, *a, **kw):
+        with torch.cuda.device(self.device) if self.device.type == "cuda" else contextlib.nullcontext():
+            return method(self, *a, **kw)
+    return call
+
+
+def _capture(device: torch.device, fn):
+    """The launches of ``fn`` on ``device``, the current one, as a graph; nothing runs yet.
+
+    ``torch.cuda.graph`` would capture on one stream for the whole process, of the device that was current at the first capture:
+    kernels for another device run at once then, and its graph is empty."""
+    stream, g = torch.cuda.Stream(device), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize(device)
+    gc.collect()  # nothing that owns device memory may go during a capture
+    torch.cuda.empty_cache()
+    with torch.cuda.stream(stream):
+        g.capture_begin()
+        try:
+            fn()
+        finally:
+            g.capture_end()
+    return g
 
 
 class Decoder:
@@ -132,6 +162,7 @@ class Decoder:
 
     # ---- what a user calls ---------------------------------------------------
     @torch.no_grad()
+    @_on_its_device
     def append(self, idx: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Adds ``idx`` [batch, n] to the sequences (``lengths[b]`` >= 1 of its first tokens; default all n), behind what was
         generated last. Returns the logits [batch, vocabulary] of the token that follows each, in 16 bits."""
@@ -187,6 +218,7 @@ class Decoder:
         return self._head(y.view(B, S, -1)[torch.arange(B, device=dev), n[:, 0] - 1].contiguous())
 
     @torch.no_grad()
+    @_on_its_device
     def generate(self, n: int, temperature: float = 1.0, top_k: Optional[int] = None, top_p: float = 1.0, min_p: float = 0.0,
                  generator: Optional[torch.Generator] = None, cuda_graph: bool = True) -> torch.Tensor:
         """``n`` sampled tokens of every sequence, [batch, n] (``temperature`` <= 0: the most likely ones).
@@ -226,9 +258,7 @@ class Decoder:
                 token = sample(self._step(token))
             if graph:
                 token = token.clone()
-                g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g):
-                    token.copy_(sample(self._step(token)))
+                g = _capture(self.device, lambda: token.copy_(sample(self._step(token))))
                 for _ in range(steps - eager):
                     g.replay()
                 torch.cuda.current_stream().synchronize()  # before the graph and its memory go

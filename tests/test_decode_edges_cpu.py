@@ -1,0 +1,103 @@
+"""Calls of the decoder and of the decoding operators that are easy to get wrong: other devices, padded batches, broken rows,
+settings at their ends. The host code, on emulated kernels (``decode_emulation``)."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from decode_emulation import emulate
+
+from heiretsu_b200.config import GPTConfig
+from heiretsu_b200.models import decode
+from heiretsu_b200.models.decode import Decoder
+from heiretsu_b200.models.gpt import GPT
+
+CFG = dict(block_size=64, vocab_size=200, n_layer=2, n_head=2, n_embed=128)
+
+
+def _model(seed=0, **kw):
+    from heiretsu_b200.parallel.flat import FlatParams
+
+    torch.manual_seed(seed)
+    m = GPT(GPTConfig(**CFG), **kw)
+    FlatParams(m, torch.device("cpu"), dtype16=torch.float32)
+    return m
+
+
+def _ids(b, n, seed=1):
+    return torch.randint(0, 200, (b, n), generator=torch.Generator().manual_seed(seed))
+
+
+class FakeCuda:
+    """As much of ``torch.cuda`` as generation uses, with device 0 current; notes the device of every capture, replay and wait."""
+
+    def __init__(self):
+        self.current, self.seen = 0, []
+        fake = self
+
+        class Stream:
+            def __init__(self, device=None):
+                self.index = fake.current if device is None else torch.device(device).index
+
+            def wait_stream(self, other):
+                pass
+
+            def synchronize(self):
+                fake.seen.append(("wait", self.index))
+
+        class CUDAGraph:
+            def capture_begin(self, *a, **kw):
+                fake.seen.append(("capture", fake.current))
+
+            def capture_end(self):
+                pass
+
+            def replay(self):
+                fake.seen.append(("replay", fake.current))
+
+        self.Stream, self.CUDAGraph = Stream, CUDAGraph
+        self.default = Stream()  # where a capture without a stream of its own runs: the device of the first one
+
+    @contextlib.contextmanager
+    def device(self, device):
+        old, self.current = self.current, torch.device(device).index
+        yield
+        self.current = old
+
+    @contextlib.contextmanager
+    def stream(self, s):
+        with self.device(torch.device("cuda", s.index)):
+            yield
+
+    @contextlib.contextmanager
+    def graph(self, g, stream=None):
+        with self.stream(self.default if stream is None else stream):
+            g.capture_begin()
+            yield
+            g.capture_end()
+
+    def current_stream(self, device=None):
+        return self.Stream(device)
+
+    def synchronize(self, device=None):
+        self.seen.append(("wait", self.Stream(device).index))
+
+    def empty_cache(self):
+        pass
+
+
+def test_a_graph_is_captured_and_replayed_on_the_models_device(monkeypatch):
+    """The model is on device 1, device 0 is current: what is captured, replayed and waited for is device 1's."""
+    emulate(monkeypatch)
+    d = Decoder(_model(), 2, page_size=16)
+    d.append(_ids(2, 5))
+    fake = FakeCuda()
+    here = lambda f: lambda *a, **kw: f(*a, **{k: v for k, v in kw.items() if k != "device"})  # noqa: E731
+    torch_ = {n: getattr(torch, n) for n in dir(torch)} | {n: here(getattr(torch, n)) for n in ("rand", "zeros", "tensor")}
+    torch_ |= {"cuda": fake, "empty": here(torch.zeros)}
+    monkeypatch.setattr(decode, "torch", SimpleNamespace(**torch_))
+    d.device = torch.device("cuda", 1)
+    d.generate(20, temperature=0)
+    assert [w for w, _ in fake.seen].count("capture") == 1 and [w for w, _ in fake.seen].count("replay") == 18
+    assert {i for _, i in fake.seen} == {1} and fake.seen[-1][0] == "wait" and fake.current == 0

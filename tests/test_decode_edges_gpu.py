@@ -1,0 +1,75 @@
+"""Calls of the decoder and of the decoding operators that are easy to get wrong, on a GPU."""
+import pytest
+import torch
+
+from heiretsu_b200.config import GPTConfig
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(dtype=torch.bfloat16, moe=False, heads=4, width=256, vocab=1000, device="cuda"):
+    from heiretsu_b200.models.gpt import GPT
+    from heiretsu_b200.parallel.flat import FlatParams
+
+    torch.manual_seed(0)
+    kw = dict(num_experts=4, top_k=2, moe_freq=2) if moe else {}
+    m = GPT(GPTConfig(block_size=256, vocab_size=vocab, n_layer=3, n_head=heads, n_embed=width, dropout=0.0, **kw)).to(device)
+    with torch.no_grad():
+        for blk in m.tr.h:
+            blk.attn.c_attn.weight.mul_(4)
+    FlatParams(m, torch.device(device), dtype16=dtype)
+    m.fused = True
+    return m.eval()
+
+
+def _ids(b, n, vocab=1000, seed=1):
+    return torch.randint(0, vocab, (b, n), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _status():
+    from heiretsu_b200.ops._C import check_status
+    check_status(torch.cuda.current_device())
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_a_model_on_the_device_that_is_not_current(first):
+    """A graph gives the tokens of single steps, whether the process has captured on the current device before or not."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    from heiretsu_b200.models.decode import Decoder
+
+    if first:
+        Decoder(_model(), 1).append(_ids(1, 3))
+        x, g = torch.zeros(4, device="cuda:0"), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            x += 1
+    m = _model(device="cuda:1")
+    out = []
+    for graph in (True, False):
+        d = Decoder(m, 3)
+        d.append(_ids(3, 9))
+        out.append(d.generate(30, temperature=0, cuda_graph=graph))
+        assert d.lengths.tolist() == d.lens and torch.cuda.current_device() == 0
+    assert torch.equal(*out)
+
+
+def test_captures_between_other_captures():
+    """A decoder's graph neither takes nor leaves anything of another graph's, and the current stream may be any."""
+    from heiretsu_b200.models.decode import Decoder
+
+    m, idx = _model(), _ids(3, 9)
+    x, g = torch.zeros(4, device="cuda"), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x += 1
+    out = []
+    for graph in (True, False):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            d = Decoder(m, 3)
+            d.append(idx)
+            out.append(d.generate(30, temperature=0, cuda_graph=graph))
+            g.replay()
+        torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(*out) and x.tolist() == [2.0] * 4
+    _status()
