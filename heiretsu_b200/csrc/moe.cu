@@ -52,7 +52,8 @@ __global__ void moe_router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const
   const float inv = 1.f / s;
   for (int e = 0; e < E; ++e) logit[e] *= inv;  // probabilities
   for (int e = lane; e < E; e += 32) probs[(long)t * E + e] = logit[e];
-  // top-k (largest first, lowest index on ties)
+  // top-k (largest first, lowest index on ties). A token whose logits are no numbers has NaN everywhere, which no comparison
+  // picks: it takes the first K experts, with NaN weights, so that its rows have a place like any others and stay its own.
   if (lane == 0) {
     unsigned long long taken = 0ull;
     float wsum = 0.f;
@@ -62,7 +63,7 @@ __global__ void moe_router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const
       int best = -1;
       float bv = -1.f;
       for (int e = 0; e < E; ++e) {
-        if (!((taken >> e) & 1ull) && logit[e] > bv) {
+        if (!((taken >> e) & 1ull) && (best < 0 || logit[e] > bv)) {
           bv = logit[e];
           best = e;
         }
