@@ -164,8 +164,8 @@ class Decoder:
     @torch.no_grad()
     @_on_its_device
     def append(self, idx: torch.Tensor, lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
-        """Adds ``idx`` [batch, n] to the sequences (``lengths[b]`` >= 1 of its first tokens; default all n), behind what was
-        generated last. Returns the logits [batch, vocabulary] of the token that follows each, in 16 bits."""
+        """Adds ``idx`` [batch, n] to the sequences (``lengths[b]`` >= 1 of its first tokens, default all n; the others may be
+        anything), behind what was generated last. Returns the logits [batch, vocabulary] of the token that follows each, in 16 bits."""
         if idx.dim() != 2 or idx.size(0) != self.batch or idx.size(1) < 1:
             raise ValueError(f"expected tokens [{self.batch}, n], got {tuple(idx.shape)}")
         lengths = [idx.size(1)] * self.batch if lengths is None else [int(n) for n in lengths]
@@ -193,6 +193,7 @@ class Decoder:
         at = torch.arange(S, device=dev)[None]
         old = self.lengths.long()[:, None]
         pos = (old + at).clamp_max_(self.model.cfg.block_size - 1)
+        idx = torch.where(at < n, idx, 0)  # padding may be no token, whose row would be NaN: a weight of 0 does not take that out
         x = K.embedding_fwd(idx.view(1, -1), tr.wte.weight, tr.wpe.weight.index_select(0, pos.view(-1)))
         # tokens behind a sequence's own are rows like others, but leave nothing in the cache
         slots = torch.where(at < n, self._slots(pos), -1).view(-1)

@@ -101,3 +101,21 @@ def test_a_graph_is_captured_and_replayed_on_the_models_device(monkeypatch):
     d.generate(20, temperature=0)
     assert [w for w, _ in fake.seen].count("capture") == 1 and [w for w, _ in fake.seen].count("replay") == 18
     assert {i for _, i in fake.seen} == {1} and fake.seen[-1][0] == "wait" and fake.current == 0
+
+
+@pytest.mark.parametrize("pad", [-1, -100, 10 ** 9])
+def test_tokens_behind_a_sequences_own_may_be_anything(monkeypatch, pad):
+    """Padding that is no token of the vocabulary, in a first prompt and in tokens added later."""
+    emulate(monkeypatch)
+    m = _model()
+    out = []
+    for fill in (0, pad):
+        d = Decoder(m, 3, page_size=16)
+        logits = []
+        for seed, n in ((1, [9, 1, 4]), (2, [2, 11, 5])):
+            idx = _ids(3, 11, seed)
+            for b in range(3):
+                idx[b, n[b]:] = fill
+            logits.append(d.append(idx, n))
+        out.append((logits, d.generate(5, temperature=0)))
+    assert all(torch.equal(a, b) for a, b in zip(out[0][0], out[1][0])) and torch.equal(out[0][1], out[1][1])

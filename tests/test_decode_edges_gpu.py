@@ -73,3 +73,21 @@ def test_captures_between_other_captures():
         torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(*out) and x.tolist() == [2.0] * 4
     _status()
+
+
+@pytest.mark.parametrize("moe", [False, True])
+def test_tokens_behind_a_sequences_own_may_be_anything(moe):
+    """Padding that is no token of the vocabulary changes nothing, in a first prompt and in tokens added later, and is no error."""
+    from heiretsu_b200.models.decode import Decoder
+
+    m, out = _model(moe=moe), []
+    for fill in (0, -100):
+        d, logits = Decoder(m, 3), []
+        for seed, n in ((1, [90, 1, 37]), (2, [2, 41, 33])):
+            idx = _ids(3, 90, seed=seed)
+            for b in range(3):
+                idx[b, n[b]:] = fill
+            logits.append(d.append(idx, n))
+        out.append((*logits, d.generate(12, temperature=0)))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    _status()
