@@ -22,6 +22,7 @@ import torch
 
 from ..ops import gemm as G
 from ..ops import kernels as K
+from ..ops._C import check_status
 from .fused import LN_EPS, _dt, _is_moe, _vpad, fused_supported
 
 GRAPH_STEPS = 8  # a capture costs some 5 steps: fewer are run one by one
@@ -218,13 +219,27 @@ class Decoder:
             y = self._blocks(x, slots, attend)
         return self._head(y.view(B, S, -1)[torch.arange(B, device=dev), n[:, 0] - 1].contiguous())
 
+    def _check(self, tokens: torch.Tensor) -> None:
+        """An error where a sequence got no token (``tokens`` [steps, batch]); waits for the device."""
+        broken = (tokens < 0).any(0).nonzero()[:, 0].tolist()
+        if not broken:
+            return
+        text = f"no token for sequences {broken}: their logits hold NaN or +inf, or nothing but -inf"
+        if self.device.type == "cuda":  # what the steps behind such a token made of it is reported here, and not later
+            try:
+                check_status(self.device.index)
+            except RuntimeError as e:
+                raise RuntimeError(text) from e
+        raise RuntimeError(text)
+
     @torch.no_grad()
     @_on_its_device
     def generate(self, n: int, temperature: float = 1.0, top_k: Optional[int] = None, top_p: float = 1.0, min_p: float = 0.0,
                  generator: Optional[torch.Generator] = None, cuda_graph: bool = True) -> torch.Tensor:
         """``n`` sampled tokens of every sequence, [batch, n] (``temperature`` <= 0: the most likely ones).
 
-        The settings are ``sample_tokens``'s. The last one is run through the model when more is generated or appended."""
+        The settings are ``sample_tokens``'s. The last one is run through the model when more is generated or appended. Logits
+        that give no token (NaN, say) are an error; it leaves the sequences as they were."""
         if self.logits is None and self.pending is None:
             raise ValueError("append a prompt first")
         if n < 1:
@@ -264,6 +279,7 @@ class Decoder:
                     g.replay()
                 torch.cuda.current_stream().synchronize()  # before the graph and its memory go
                 del g
+            self._check(out)
         except BaseException:  # nothing was generated: the next call begins where this one did
             self.logits = logits
             self.lengths.copy_(torch.tensor(self.lens, dtype=torch.int32))

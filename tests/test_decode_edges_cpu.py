@@ -119,3 +119,26 @@ def test_tokens_behind_a_sequences_own_may_be_anything(monkeypatch, pad):
             logits.append(d.append(idx, n))
         out.append((logits, d.generate(5, temperature=0)))
     assert all(torch.equal(a, b) for a, b in zip(out[0][0], out[1][0])) and torch.equal(out[0][1], out[1][1])
+
+
+def test_a_row_without_a_token_is_an_error(monkeypatch):
+    """Logits of NaN give no token: generate says which sequence's, and leaves all as they were."""
+    emulate(monkeypatch)
+    m = _model()
+    d, ref = Decoder(m, 3, page_size=16), Decoder(m, 3, page_size=16)
+    for x in (d, ref):
+        x.append(_ids(3, 5))
+    good = d.logits.clone()
+    d.logits[1, 3] = float("nan")
+    with pytest.raises(RuntimeError, match=r"no token for sequences \[1\]"):
+        d.generate(1)
+    assert d.lens == [5] * 3 and d.lengths.tolist() == d.lens and m.training
+    d.logits = good
+    want = ref.generate(9, temperature=0)
+    assert torch.equal(d.generate(4, temperature=0), want[:, :4])
+    d.pools[0]["k_pages"], kept = torch.full_like(d.pools[0]["k_pages"], float("nan")), d.pools[0]["k_pages"]
+    with pytest.raises(RuntimeError, match=r"no token for sequences \[0, 1, 2\]"):
+        d.generate(1, temperature=0)
+    assert d.lens == [8] * 3 and d.lengths.tolist() == d.lens
+    d.pools[0]["k_pages"] = kept
+    assert torch.equal(d.generate(5, temperature=0), want[:, 4:])

@@ -91,3 +91,27 @@ def test_tokens_behind_a_sequences_own_may_be_anything(moe):
         out.append((*logits, d.generate(12, temperature=0)))
     assert all(torch.equal(a, b) for a, b in zip(*out))
     _status()
+
+
+@pytest.mark.parametrize("moe,graph", [(False, True), (True, True), (True, False)])
+def test_a_row_without_a_token_is_an_error(moe, graph):
+    """One sequence's cache holds NaN: generate says so, leaves all as they were and no error behind; the cache mended, it gives what it
+    would have given."""
+    from heiretsu_b200.models.decode import Decoder
+
+    m = _model(moe=moe)
+    d, ref = Decoder(m, 3), Decoder(m, 3)
+    for x in (d, ref):
+        x.append(_ids(3, 30))
+    want = torch.cat([ref.generate(n, temperature=0, cuda_graph=graph) for n in (6, 25)], 1)
+    assert torch.equal(d.generate(6, temperature=0, cuda_graph=graph), want[:, :6])
+    pool, page = d.pools[1]["v_pages"], d.owned[1][0]
+    kept = pool[page].clone()
+    pool[page, 2, 7, 5] = float("nan")
+    with pytest.raises(RuntimeError, match=r"no token for sequences \[1\]"):
+        d.generate(25, temperature=0, cuda_graph=graph)
+    _status()
+    assert d.lens == [35] * 3 and d.lengths.tolist() == d.lens
+    pool[page] = kept
+    assert torch.equal(d.generate(25, temperature=0, cuda_graph=graph), want[:, 6:])
+    _status()
