@@ -16,7 +16,7 @@ from __future__ import annotations
 import contextlib
 import functools
 import gc
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -26,6 +26,22 @@ from ..ops._C import check_status
 from .fused import LN_EPS, _dt, _is_moe, _vpad, fused_supported
 
 GRAPH_STEPS = 8  # a capture costs some 5 steps: fewer are run one by one
+MAX_VOCAB = 1 << 19  # of sample_tokens
+
+
+def decoder_supported(model) -> Tuple[bool, str]:
+    """Whether a ``Decoder`` takes this model, and why not (generate() on the plain modules takes any)."""
+    topo = getattr(model, "topo", None)
+    ok, why = fused_supported(model.cfg, topo)
+    if not ok:
+        return False, why
+    if topo is not None and (getattr(topo, "tp", 1) > 1 or getattr(topo, "ep", 1) > 1):
+        return False, "needs tp 1 and ep 1 (generate() on the plain modules has both)"
+    if not hasattr(model.tr.ln_f.weight, "w16"):
+        return False, "needs flattened parameters (parallel.flat.FlatParams)"
+    if model.cfg.vocab_size > MAX_VOCAB:
+        return False, f"samples from a vocabulary of at most {MAX_VOCAB}"
+    return True, ""
 
 
 def _on_its_device(method):
@@ -64,14 +80,10 @@ class Decoder:
     ``block_size`` tokens of every sequence)."""
 
     def __init__(self, model, batch: int, cache_bits: int = 16, page_size: int = 64, pages: Optional[int] = None):
-        cfg, topo = model.cfg, getattr(model, "topo", None)
-        ok, why = fused_supported(cfg, topo)
+        cfg = model.cfg
+        ok, why = decoder_supported(model)
         if not ok:
             raise ValueError(f"decoding on the fused engine: {why}")
-        if topo is not None and (getattr(topo, "tp", 1) > 1 or getattr(topo, "ep", 1) > 1):
-            raise ValueError("decoding on the fused engine needs tp 1 and ep 1 (generate() on the plain modules has both)")
-        if not hasattr(model.tr.ln_f.weight, "w16"):
-            raise ValueError("decoding on the fused engine needs flattened parameters (parallel.flat.FlatParams)")
         if cache_bits not in (8, 16):
             raise ValueError(f"a cache has 16 or 8 bits, got {cache_bits}")
         if batch < 1:

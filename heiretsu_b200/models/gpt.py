@@ -320,10 +320,12 @@ class GPT(nn.Module):
         return preference_loss(self, idx, targets, ref_logp, beta, label_smoothing)
 
     def generate(self, idx: torch.Tensor, max_new_tokens: int, **kw) -> torch.Tensor:
-        """``idx`` [B, T] extended by sampled tokens (models/generate.py), by the native kernels where the model is fused
-        (and ``kv_cache`` is not False)."""
+        """``idx`` [B, T] extended by sampled tokens (models/generate.py), by the native kernels where the model is fused,
+        a ``Decoder`` takes it and ``kv_cache`` is not False."""
+        from .decode import decoder_supported
         from .generate import generate
-        kw.setdefault("engine", "fused" if self.fused and idx.is_cuda and kw.get("kv_cache", True) else "plain")
+        fused = self.fused and idx.is_cuda and kw.get("kv_cache", True) and decoder_supported(self)[0]
+        kw.setdefault("engine", "fused" if fused else "plain")
         return generate(self, idx, max_new_tokens, **kw)
 
     def num_params(self) -> int:

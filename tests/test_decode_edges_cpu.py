@@ -142,3 +142,38 @@ def test_a_row_without_a_token_is_an_error(monkeypatch):
     assert d.lens == [8] * 3 and d.lengths.tolist() == d.lens
     d.pools[0]["k_pages"] = kept
     assert torch.equal(d.generate(5, temperature=0), want[:, 4:])
+
+
+def test_a_model_that_a_decoder_does_not_take_generates_on_the_plain_modules(monkeypatch):
+    """GPT.generate's own choice of engine: the fused one where it has what that needs, and only there."""
+    from heiretsu_b200.models import generate as gen
+
+    emulate(monkeypatch)
+    engines = []
+    monkeypatch.setattr(gen, "generate", lambda model, idx, n, engine="plain", **kw: engines.append(engine))
+    idx = SimpleNamespace(is_cuda=True)
+
+    def engine(model, **kw):
+        model.fused = True
+        engines.clear()
+        model.generate(idx, 4, **kw)
+        return engines[0]
+
+    assert engine(_model()) == "fused" and engine(_model(), kv_cache=False) == "plain"
+    assert engine(_model(), engine="plain") == "plain" and engine(_model(), cache_bits=8) == "fused"
+    for topo in (SimpleNamespace(tp=2), SimpleNamespace(ep=2)):
+        m = _model()
+        m.topo = topo
+        assert engine(m) == "plain" and engine(m, engine="fused") == "fused"  # asked for, the decoder refuses
+        with pytest.raises(ValueError, match="tp 1 and ep 1"):
+            Decoder(m, 1)
+    m = GPT(GPTConfig(**CFG))
+    assert engine(m) == "plain"
+    monkeypatch.setattr(decode, "MAX_VOCAB", 100)
+    assert engine(_model()) == "plain"
+    with pytest.raises(ValueError, match="vocabulary"):
+        Decoder(_model(), 1)
+    m = _model()
+    m.fused = False
+    m.generate(idx, 4)
+    assert engines[-1] == "plain"
