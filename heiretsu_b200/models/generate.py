@@ -83,7 +83,7 @@ def _pick(logits: torch.Tensor, temperature: float, top_k: Optional[int], genera
     if temperature <= 0:
         return logits.argmax(dim=-1, keepdim=True)
     logits = logits.float() / temperature
-    if top_k is not None and top_k < logits.size(-1):
+    if top_k is not None and 0 < top_k < logits.size(-1):
         kth = torch.topk(logits, top_k, dim=-1).values[:, -1:]
         logits = logits.masked_fill(logits < kth, float("-inf"))
     if top_p < 1 or min_p > 0:
@@ -98,7 +98,7 @@ def generate(model, idx: torch.Tensor, max_new_tokens: int, temperature: float =
              engine: str = "plain", cache_bits: int = 16) -> torch.Tensor:
     """Extend ``idx`` [B, T0] by ``max_new_tokens`` sampled tokens; returns [B, T0 + new].
 
-    ``temperature <= 0`` picks the most likely token; ``top_k``, ``top_p`` and ``min_p`` cut the distribution. With
+    ``temperature <= 0`` picks the most likely token; ``top_k`` (0 or less: all), ``top_p`` and ``min_p`` cut the distribution. With
     ``kv_cache`` the total length must fit in ``block_size``; without it the context is cropped to the
     last ``block_size`` tokens, as training saw them. ``engine`` "fused" decodes with the native kernels
     (models/decode.py; flattened parameters on a GPU): 16-bit weights, a cache of 16 or 8 bits, a CUDA graph per token.

@@ -39,7 +39,7 @@ def main(argv=None) -> None:
     ap.add_argument("--num_samples", type=int, default=1)
     ap.add_argument("--max_new_tokens", type=int, default=64)
     ap.add_argument("--temperature", type=float, default=0.8, help="<= 0: always the most likely token")
-    ap.add_argument("--top_k", type=int, default=200)
+    ap.add_argument("--top_k", type=int, default=200, help="keep this many of the likeliest tokens; 0: all")
     ap.add_argument("--top_p", type=float, default=1.0, help="keep the likeliest tokens that have this share of the probability")
     ap.add_argument("--min_p", type=float, default=0.0, help="keep tokens with this share of the likeliest one's probability")
     ap.add_argument("--engine", choices=("plain", "fused"), default="plain",

@@ -177,3 +177,20 @@ def test_a_model_that_a_decoder_does_not_take_generates_on_the_plain_modules(mon
     m.fused = False
     m.generate(idx, 4)
     assert engines[-1] == "plain"
+
+
+@pytest.mark.parametrize("top_k", [0, -1, 200, 10 ** 6])
+@pytest.mark.parametrize("top_p,min_p", [(1.0, 0.0), (0.6, 0.05)])
+def test_a_top_k_of_0_or_of_the_vocabulary_keeps_all(monkeypatch, top_k, top_p, min_p):
+    """On either engine; the plain sampler draws what it draws without a top_k."""
+    from heiretsu_b200.models.generate import _pick, generate
+
+    x = 3 * torch.randn(64, 200, generator=torch.Generator().manual_seed(2))
+    draw = lambda k: _pick(x, 0.8, k, torch.Generator().manual_seed(5), top_p, min_p)  # noqa: E731
+    assert torch.equal(draw(top_k), draw(None))
+    emulate(monkeypatch)
+    m = _model()
+    for engine in ("plain", "fused"):
+        out = [generate(m, _ids(2, 4), 6, 0.9, k, torch.Generator().manual_seed(3), engine=engine, top_p=top_p, min_p=min_p)
+               for k in (top_k, None)]
+        assert torch.equal(*out)
