@@ -9,6 +9,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <functional>
 #include <limits>
 #include <string>
 
@@ -48,22 +50,51 @@ std::string dims(const at::Tensor& t) {
   return s + "]";
 }
 
-// No two elements at one address: sorted by stride, each dimension steps over all that lies within the ones before.
-bool disjoint(const at::Tensor& t) {
-  int64_t stride[4], size[4];
+// Dimensions of more than one element, by stride.
+struct Layout {
+  int64_t stride[4], size[4], dim[4];
   int n = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) {
-    if (t.size(i) <= 1) continue;
-    int j = n++;
-    for (; j > 0 && stride[j - 1] > t.stride(i); --j) stride[j] = stride[j - 1], size[j] = size[j - 1];
-    stride[j] = t.stride(i), size[j] = t.size(i);
+  explicit Layout(const at::Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      if (t.size(i) <= 1) continue;
+      int j = n++;
+      for (; j > 0 && stride[j - 1] > t.stride(i); --j)
+        stride[j] = stride[j - 1], size[j] = size[j - 1], dim[j] = dim[j - 1];
+      stride[j] = t.stride(i), size[j] = t.size(i), dim[j] = i;
+    }
   }
-  int64_t reach = 1;
-  for (int j = 0; j < n; ++j) {
-    if (stride[j] < reach) return false;
-    reach = stride[j] * size[j];
+  int64_t reach(int inner) const {  // elements from the first to behind the last, of the first `inner` dimensions
+    int64_t r = 1;
+    for (int j = 0; j < inner; ++j) r += (size[j] - 1) * stride[j];
+    return r;
   }
+};
+// No two elements at one address: each dimension steps over all that lies within the ones before.
+bool disjoint(const at::Tensor& t) {
+  const Layout x(t);
+  for (int j = 0; j < x.n; ++j)
+    if (x.stride[j] < (j > 0 ? x.stride[j - 1] * x.size[j - 1] : 1)) return false;
   return true;
+}
+// Whether two tensors of one type and the same sizes, each disjoint, reach into each other. The outer dimensions that both have
+// with the same strides are told apart exactly, such as pages that hold K and V; what lies within them counts as a whole,
+// so with the same strides throughout they do if they share an element.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0) return false;
+  const Layout x(a), y(b);
+  int inner = x.n;
+  while (inner > 0 && x.dim[inner - 1] == y.dim[inner - 1] && x.stride[inner - 1] == y.stride[inner - 1]) --inner;
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr()), es = a.element_size();
+  if (bytes % es != 0) return true;
+  // the inner parts of two elements are less than a step of the next dimension apart: its share is the quotient or one more
+  const std::function<bool(int64_t, int)> meet = [&](int64_t apart, int j) {
+    if (j == inner) return apart < x.reach(inner) && -apart < y.reach(inner);
+    const int64_t s = x.stride[j - 1], q = apart >= 0 ? apart / s : -((-apart + s - 1) / s);
+    for (const int64_t i : {q, q + 1})
+      if (std::abs(i) < x.size[j - 1] && meet(apart - i * s, j - 1)) return true;
+    return false;
+  };
+  return meet(bytes / es, x.n);
 }
 
 void check_same_device(const at::Tensor& t, const at::Device& dev, const char* op, const char* name) {
@@ -150,6 +181,8 @@ void kv_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
   const char* op = "kv_write";
   TORCH_CHECK(half_type(k.scalar_type()) && v.scalar_type() == k.scalar_type(), op, ": k and v must both be bf16 or fp16");
   const KvPool p = check_pool(k_pages, v_pages, k_exp, v_exp, k.scalar_type(), op);
+  TORCH_CHECK(!overlap(k_pages, v_pages) && (p.type != kKvCodes || !overlap(*k_exp, *v_exp)), op,
+              ": the cache's K and V must not overlap");
   check_slots(slots, op);
   TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == slots.size(0) && k.size(1) == p.heads &&
                   k.size(2) == p.dim,

@@ -1,6 +1,7 @@
 """Calls of the decoder and of the decoding operators that are easy to get wrong: other devices, padded batches, broken rows,
 settings at their ends. The host code, on emulated kernels (``decode_emulation``)."""
 import contextlib
+import itertools
 from types import SimpleNamespace
 
 import pytest
@@ -12,6 +13,8 @@ from heiretsu_b200.config import GPTConfig
 from heiretsu_b200.models import decode
 from heiretsu_b200.models.decode import Decoder
 from heiretsu_b200.models.gpt import GPT
+from heiretsu_b200.ops import _C
+from heiretsu_b200.ops import kernels as K
 
 CFG = dict(block_size=64, vocab_size=200, n_layer=2, n_head=2, n_embed=128)
 
@@ -194,3 +197,52 @@ def test_a_top_k_of_0_or_of_the_vocabulary_keeps_all(monkeypatch, top_k, top_p, 
         out = [generate(m, _ids(2, 4), 6, 0.9, k, torch.Generator().manual_seed(3), engine=engine, top_p=top_p, min_p=min_p)
                for k in (top_k, None)]
         assert torch.equal(*out)
+
+
+needs_extension = pytest.mark.skipif(not _C.available(), reason="the extension is not built")
+
+
+@needs_extension
+def test_writes_to_pools_that_overlap_are_refused():
+    """K and V pools that share elements, not only those that begin at one address; pools that lie in each other's gaps are fine."""
+    k, slots = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.arange(3)
+
+    def write(match, k_pages, v_pages, **exps):
+        with pytest.raises(RuntimeError, match=match):
+            K.kv_write(k, k, slots, k_pages, v_pages, **exps)
+
+    buf = torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16)
+    write("overlap", buf[:4], buf[3:7])
+    write("overlap", buf[3:7], buf[:4])
+    write("overlap", buf[::2][:3], buf[4:7])
+    write("CUDA", buf[:4], buf[4:])
+    write("CUDA", buf[::2], buf[1::2])
+    native = torch.zeros(4, 16, 2, 2, 64, dtype=torch.bfloat16)  # [pages, slots, K or V, heads, channels]
+    write("CUDA", native[:, :, 0].transpose(1, 2), native[:, :, 1].transpose(1, 2))
+    mixed = torch.zeros(4, 2, 2 * 16 * 64, dtype=torch.bfloat16)  # pages of K by heads and V by slots
+    write("CUDA", mixed[:, 0].view(4, 2, 16, 64), mixed[:, 1].view(4, 16, 2, 64).transpose(1, 2))
+    write("overlap", mixed[:, 0].view(4, 2, 16, 64), mixed[:, 0, 8:].as_strided((4, 2, 16, 64), (4096, 64, 128, 1), 8))
+    heads = torch.zeros(4, 5, 16, 64, dtype=torch.bfloat16)
+    write("CUDA", heads[:, :2], heads[:, 2:4])
+    write("overlap", heads[:, :2], heads[:, 1:3])
+    codes, exps = torch.zeros(8, 2, 16, 64, dtype=torch.int8), torch.zeros(8, 2, 16, dtype=torch.uint8)
+    write("overlap", codes[:4], codes[4:], k_exp=exps[:4], v_exp=exps[2:6])
+    write("overlap", codes[:4], codes[2:6], k_exp=exps[:4], v_exp=exps[4:])
+    write("CUDA", codes[:4], codes[4:], k_exp=exps[:4], v_exp=exps[4:])
+
+
+@needs_extension
+def test_what_overlaps_is_what_shares_an_element():
+    """Every shift of one small view against another, by listing their elements."""
+    k, slots = torch.zeros(1, 2, 16, dtype=torch.bfloat16), torch.arange(1)
+    buf = torch.zeros(20000, dtype=torch.bfloat16)
+    for sizes, strides in [((2, 2, 16, 16), (1100, 528, 32)), ((3, 2, 16, 16), (512, 16, 32)), ((2, 2, 16, 16), (16, 32, 64)), ((1, 2, 16, 16), (7, 520, 32))]:
+        strides = tuple(s // 8 * 8 for s in strides) + (1,)
+        at = {sum(i * s for i, s in zip(ix, strides)) for ix in itertools.product(*map(range, sizes))}
+        for shift in range(-2400, 2401, 8):
+            a, b = buf.as_strided(sizes, strides, 4800), buf.as_strided(sizes, strides, 4800 + shift)
+            shared = any(x + shift in at for x in at)
+            with pytest.raises(RuntimeError) as e:
+                K.kv_write(k, k, slots, a, b)
+            told = "overlap" in str(e.value) or "one buffer" in str(e.value)
+            assert told == shared, (sizes, strides, shift, str(e.value)[:100])
