@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import contextlib
 import functools
-import gc
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -60,7 +59,6 @@ def _capture(device: torch.device, fn):
     kernels for another device run at once then, and its graph is empty."""
     stream, g = torch.cuda.Stream(device), torch.cuda.CUDAGraph()
     torch.cuda.synchronize(device)
-    gc.collect()  # nothing that owns device memory may go during a capture
     torch.cuda.empty_cache()
     with torch.cuda.stream(stream):
         g.capture_begin()
