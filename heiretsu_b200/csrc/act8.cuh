@@ -35,7 +35,8 @@ __device__ __forceinline__ float act8_scale(uint32_t byte) {
   return byte == kAct8Nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
 }
 // Four codes, the first in the low byte. Rounding by adding 1.5 * 2^23: the sum's low byte is the code in two's
-// complement (|x 2^-e| <= 127; the product is exact, or too small to count). Blocks with byte 255 get codes 0 (an infinity or NaN times 0 is NaN).
+// complement (|x 2^-e| <= 127; the product is exact, or too small to count). Blocks with byte 255 get codes 0 (an infinity or
+// NaN times 0 is NaN).
 __device__ __forceinline__ uint32_t act8_codes(const float (&x)[4], uint32_t byte) {
   const float inv = act8_inv_scale(byte);
   uint32_t c[4];

@@ -6,15 +6,18 @@
 // Every K and V is read once and takes part in 4 operations a query head that shares it: bound by memory. So the tiles lie where
 // copies put them, and the products take the small matrix instructions (8 query heads are a column each; those of 128 rows
 // would be all but empty). Device times on a B200, and what the bytes alone take at a copy's 6.5 TB/s:
-//   64 sequences of up to 8192 tokens, 8 K/V heads of 128 with 4 query heads each, bf16    174 us    169
-//   1 of 100003, the same heads, fp16                                                       71       63
-//   61 of up to 1024, 12 heads of 64, bf16                                                  25.1     14.6
-//   256 of up to 1024, 20 heads of 64, in codes                                             96       54
-//   1 of 57, 12 heads of 64                                                                  5.7      0.03
+//   64 sequences of up to 8192 tokens, 8 K/V heads of 128 with 4 query heads each, bf16    173 us    169
+//   the same in codes                                                                      112       85
+//   64 of up to 8192, 2 K/V heads of 64 with 16 query heads each (K and V read twice)       43.5     21.2
+//   1 of 100003, 8 K/V heads of 128 with 4 query heads each, fp16                           71       63
+//   61 of up to 1024, 12 heads of 64, bf16                                                  25.3     14.6
+//   61 of up to 1024, 8 heads of 32 / 16, bf16                                              14.1 / 11.6    4.9 / 2.4
+//   256 of up to 1024, 20 heads of 64, in codes                                             96.4     54
+//   1 of 57, 12 heads of 64                                                                  5.9      0.03
 // Long sequences are near their bytes. Short ones pay the start, the joins and the second kernel (about 3 us each); codes
 // pay their widening, 5 to 7 instructions for 4 codes.
-// Tried and slower: tiles loaded into registers (64 x 8192 227 us instead of 191), every warp copying for itself (256 in
-// codes 109 instead of 95), stages of K and of V apart (64 x 8192 184 instead of 174).
+// Tried and slower, each beside the kernel of its time: tiles loaded into registers (64 x 8192 227 us instead of 191), every
+// warp copying for itself (256 in codes 109 instead of 95), stages of K and of V apart (64 x 8192 184 instead of 174).
 #include <algorithm>
 #include <atomic>
 
@@ -134,11 +137,12 @@ struct Shape {
   static constexpr int kRow = D * kSize;                 // bytes of a token
   static constexpr int kBoxes = kRow <= 128 ? 1 : kRow / 128;  // along the channels
   static constexpr int kGroup = 16 * kRow;               // bytes of 16 tokens
-  // What a warp takes at a time: 8 KB of K and V (head dim 16, and 32 in codes: 4, 16 in codes: 2). 61 x up to 1024 tokens of 12
-  // heads of 64 take 26.9 us in bf16, with 4 KB 28.2. In codes the registers for that are there with one CTA an SM: 256 x up to
-  // 1024 tokens of 20 heads of 64 96.5 us, 1 x 60000 of 2 heads 15.3; with 4 KB and two CTAs 99 and 19.1 (but 16 x up to 384
-  // of 12 heads 9.1 instead of 10.0), with 2 KB 129. Head dim 128 in codes, 64 x up to 8192 tokens of 8 heads: 115 us; 4 KB and
-  // two CTAs, which have to spill, 141.
+  // What a warp takes at a time: 8 KB of K and V (head dim 16, and 32 in codes: 4, 16 in codes: 2). When this was chosen, 61 x up
+  // to 1024 tokens of 12 heads of 64 took 26.9 us in bf16, with 4 KB 28.2 (its one stage a warp then has a second; later steps
+  // brought 25.3). In codes the registers for that are there with one CTA an SM: 256 x up to 1024 tokens of 20 heads of 64
+  // 96.5 us, 1 x 60000 of 2 heads 15.3; with 4 KB and two CTAs 99 and 19.1 (but 16 x up to 384 of 12 heads 9.1 instead
+  // of 10.0), with 2 KB 129. Head dim 128 in codes, 64 x up to 8192 tokens of 8 heads: 115 us; 4 KB and two CTAs, which
+  // have to spill, 141.
   static constexpr int KT = kGroup == 4096 ? 1 : kGroup == 2048 ? 2 : 4;
   static constexpr int kTokens = 16 * KT;
   static constexpr int kKv = KT * kGroup;                // bytes of K of a tile
@@ -246,7 +250,9 @@ struct Join {
     uint16_t* dst = static_cast<uint16_t*>(a.out) + row * D + lane * E;
     const float inv = rcp(sum);
     if (lane * E < D) {
-      if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
+      if constexpr (E == 4)
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv));
       else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = pack16<F16>(acc[0] * inv, acc[1] * inv);
       else *dst = from_f32<F16>(acc[0] * inv);
     }
@@ -286,9 +292,10 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
   // Codes of K are widened to fp16, in fewer instructions than to bf16, and bf16 q is scaled by a power of two for it. Codes of V
   // are widened to bf16: a weight takes the scale of its head of a token with it, and these may lie further apart than fp16 goes.
   constexpr bool V16 = F16 && !CODES;
-  // The scores' reference is raised only where one passes it by more than 2^kSlack: maxima across lanes cost more than the
-  // rest of a tile's softmax (64 x 8192: 180.6 us instead of 181.2). fp16 weights are lifted by 2^kLift, which keeps them
-  // below 2^15 and what is 2^-31 of the largest; bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
+  // The scores' reference is raised only where one passes it by more than 2^kSlack: that saves the maxima across lanes of most
+  // tiles (when it was brought in: 1 x 100003 73 us instead of 75, 256 x 1024 in codes 92.7 instead of 94.7, 64 x 8192
+  // 180.6 instead of 181.2). fp16 weights are lifted by 2^kLift, which keeps them below 2^15 and what is 2^-31 of the largest;
+  // bf16 ones are lowered to 1 at most, so that no sum of V is out of range that would not be with the largest as reference.
   constexpr float kSlack = 8.f, kLift = V16 ? 7.f : -kSlack;
   extern __shared__ uint8_t smem_raw[];  // the warps' rings, exponent bytes, a part for each warp
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -363,7 +370,8 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
   }
   // number 2 w: where the run of warp w begins; 2 w + 1: where it ends, in its ring
   const auto part = [&](int i) {
-    return reinterpret_cast<float*>(smem + (i & 1 ? (i >> 1) * stages * S::kStage : kWarps * stages * (S::kStage + S::kExps) + (i >> 1) * (part_head(n.cols) + n.cols * D) * 4));
+    const int w = i >> 1, behind = kWarps * stages * (S::kStage + S::kExps);  // behind the rings and exponent bytes
+    return reinterpret_cast<float*>(smem + (i & 1 ? w * stages * S::kStage : behind + w * (part_head(n.cols) + n.cols * D) * 4));
   };
   // A unit on the way through a run.
   struct Walk {
@@ -398,8 +406,9 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
 
   uint8_t* const exps_at = smem + kWarps * stages * S::kStage;
   if (warp >= kWarps) {
-    // Lane i of the first such warp keeps the ring of warp i filled, of the next one that of warp kEach + i: the copies of a tile are issued when its stage has been read, in the order of the
-    // warp's run and across its units. The places of the next tile are on their way meanwhile.
+    // Lane i of the first such warp keeps the ring of warp i filled, of the next one that of warp kEach + i: the copies of a tile
+    // are issued when its stage has been read, in the order of the warp's run and across its units. The places of the next tile
+    // are on their way meanwhile.
     const int run = (warp - kWarps) * kEach + min(lane, kEach - 1), w0 = c0 + share(c1 - c0, run, kWarps);
     int left = lane < kEach ? c0 + share(c1 - c0, run + 1, kWarps) - w0 : 0;
     Walk nx{};
@@ -496,7 +505,8 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
     }
     __syncwarp();
   }
-  const int w0 = warp < kWarps ? c0 + share(c1 - c0, warp, kWarps) : 0, w1 = warp < kWarps ? c0 + share(c1 - c0, warp + 1, kWarps) : 0;
+  const int w0 = warp < kWarps ? c0 + share(c1 - c0, warp, kWarps) : 0;
+  const int w1 = warp < kWarps ? c0 + share(c1 - c0, warp + 1, kWarps) : 0;
   uint8_t* const ring = smem + warp * stages * S::kStage;
   uint8_t* const exps = exps_at + warp * stages * S::kExps;
   const uint32_t ring0 = smem_u32(ring);
@@ -521,7 +531,7 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
       for (int i = 0; i < 2; ++i) {
         const uint16_t* s = src + 16 * x + (CODES ? 2 : 8) * i;
         q_ahead[x][i] = 0;
-        if (g < kCols && head < n.G) {
+        if (head < n.G) {
           if (a.q_vec) q_ahead[x][i] = *reinterpret_cast<const uint32_t*>(s);
           else q_ahead[x][i] = s[0] | (static_cast<uint32_t>(s[1]) << 16);
         }
@@ -686,7 +696,8 @@ __global__ void __launch_bounds__((Shape<D, CODES>::kThreads), (Shape<D, CODES>:
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // a word: channels 2g and 2g + 1 of two tokens
               if (i + x >= D / 16) break;
-              const uint32_t y[4] = {widen_bf16(r[2 * x]), widen_bf16(r[2 * x] >> 8), widen_bf16(r[2 * x + 1]), widen_bf16(r[2 * x + 1] >> 8)};
+              const uint32_t y[4] = {widen_bf16(r[2 * x]), widen_bf16(r[2 * x] >> 8), widen_bf16(r[2 * x + 1]),
+                                     widen_bf16(r[2 * x + 1] >> 8)};
               mma<V16>(o[i + x], y[0], y[1], y[2], y[3], hi[0], hi[1]);
               mma<V16>(o[i + x], y[0], y[1], y[2], y[3], rest[0], rest[1]);
             }
@@ -929,10 +940,12 @@ void launch_dim(const DecodeArgs& a, int ctas, cudaStream_t s) {
 }
 
 // Tables of at most this many tokens, and of at most three times as many for each CTA that fits: CTAs take whole units, which
-// saves the second kernel. 12 heads of 64, bf16: 8 sequences of up to 256 tokens 6.4 us instead of 8.4, 64 of them 12.9
-// instead of 13.9 (664 tokens a CTA); but 128 of up to 200 19.2 instead of 18.1 (1038), 512 of up to 256 53 instead of 45; and 8 of up
-// to 512 8.0 instead of 9.4, but 1 of up to 512 8.3 instead of 7.3. (8 heads of 128, 4 query heads each, would gain beyond
-// that: 128 of up to 200 19.7 instead of 22.3; 20 heads of 64 in codes would lose, 25 instead of 21.)
+// saves the second kernel. When this was set, 12 heads of 64, bf16: 8 sequences of up to 256 tokens 6.4 us instead of 8.4,
+// 64 of them 12.9 instead of 13.9 (664 tokens a CTA); but 128 of up to 200 19.2 instead of 18.1 (1038), 512 of up to 256 53
+// instead of 45; and 8 of up to 512 8.0 instead of 9.4, but 1 of up to 512 8.3 instead of 7.3. (8 heads of 128, 4 query heads
+// each, would gain beyond that: 128 of up to 200 19.7 instead of 22.3; 20 heads of 64 in codes would lose, 25 instead of
+// 21.) The rule goes by the table's width, as the lengths are on the device: 8 sequences of 57 tokens take 6.0 us with a table of
+// 64, 8.4 with one of 1024.
 constexpr int kWholeTokens = 256;
 
 // CTAs on an SM, and tokens of a tile.
@@ -950,7 +963,10 @@ Fit fit_dim(bool codes) {
 // As many CTAs as the SMs hold, or fewer where the table cannot hold a tile for each of their warps.
 DecodePlan decode_attention_plan(const KvPool& p, int seqs, int units, int longest) {
   const bool codes = p.type == kKvCodes;
-  const Fit f = p.dim == 16 ? fit_dim<16>(codes) : p.dim == 32 ? fit_dim<32>(codes) : p.dim == 64 ? fit_dim<64>(codes) : fit_dim<128>(codes);
+  const Fit f = p.dim == 16   ? fit_dim<16>(codes)
+                : p.dim == 32 ? fit_dim<32>(codes)
+                : p.dim == 64 ? fit_dim<64>(codes)
+                              : fit_dim<128>(codes);
   DecodePlan d;
   const long tiles = (longest + f.tokens - 1) / f.tokens, most = (1l << 31) - 1;
   d.seqs = static_cast<int>(std::min<long>(std::min(seqs, kMaxSeqs), most / std::max(1l, units * tiles)));

@@ -275,7 +275,8 @@ std::tuple<at::Tensor, at::Tensor> decode_attention(const at::Tensor& q, const a
     a.lengths = lengths.data_ptr<int>() + b;
     a.out = static_cast<uint16_t*>(out.data_ptr()) + b * out.stride(0);
     a.lse = lse.data_ptr<float>() + b * a.heads_q;
-    // two parts and their records for each CTA; each launch its own, as the next may begin before the last has joined its
+    // Two parts and their records for each CTA. The next launch may be given the same memory: it begins when the join behind
+    // this one has ended (only the join itself is launched early, beside the kernel that it waits for).
     at::Tensor part;
     a.record = nullptr;
     if (plan.split) {

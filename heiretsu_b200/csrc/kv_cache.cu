@@ -2,8 +2,8 @@
 // written (the format of act8.cuh with a block per head of a token), and back:
 //   byte = e + 127, e >= -126 the least with max |x| <= 127 * 2^e over a head of a token;  code = rint(x / 2^e);  x' = code * 2^e
 // Bound by memory (one pass, 16 bytes a load), and for a step's few tokens by the launch. B200, write and read together:
-// 8192 tokens of 20 heads of 64 into 8 bits and back 26.2 us (126 MB, 4.8 TB/s), 4099 of 12 heads in 16 bits 8.6 us,
-// 16 tokens into 8 bits 3.9 us.
+// 8192 tokens of 20 heads of 64 into 8 bits and back 27.0 us (126 MB, 4.7 TB/s), 4099 of 12 heads in 16 bits 9.5 us,
+// 16 tokens into 8 bits 4.2 us.
 #include "act8.cuh"
 #include "common.cuh"
 #include "decode_args.h"

@@ -13,8 +13,13 @@
 //
 // The row is read once, and its passes are made in shared memory: bound by the arithmetic of the weights (10 instructions
 // in 64 bits and about 20 others each) and, for few rows, by the chain of barriers. Device times on a B200, and what the
-// bytes alone take: rows of 50257, 1 by top_k 15.0 us (0.02), 64 whole ones in 32 bits 17.0 us (2.0), 256 by top_p 53.5 us
-// (3.9); 101 of 32003 with settings of their own 28.7 us (1.0).
+// bytes alone take: rows of 50257, 1 by top_k 15.9 us (0.02), 64 whole ones in 32 bits 17.2 us (2.0), 256 by top_p 53.7 us
+// (3.9), 256 greedy 8.9 us, 256 by min_p 17.5 us; 101 of 32003 with settings of their own 30.0 us (1.0); 64 of 130000 in 32 bits,
+// which shared memory does not hold, whole 37.5 us, by top_k 38 us, by top_p 79 us (5.1).
+// The lists hold 2048 tokens (1024 where two rows share an SM), and a bound on the top_k-th logit comes from the threads' own
+// maxima. Where that is not enough the cuts are searched for over the whole row, a pass for each bit of a key: 64 rows of 50257 by
+// top_p of 0.99, whose border lies among thousands of alike tokens, 217 us (0.9: 34), by top_k 1000 54 us (800: 19.5), 256
+// by top_k 500 86 us (400: 25), 64 of 1000 by top_k 200 (125 threads have a piece) 21 us (100: 15).
 // Tried and slower: searches by one warp (1 row 22.5 us) or of two bits a step (17.7), tables of 256 exponentials.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -227,7 +232,8 @@ struct Sums {
   int used = 0;
   __device__ __forceinline__ u64 operator()(u64 v) {
     uint32_t* s = slots[used++];
-    const uint32_t part[3] = {static_cast<uint32_t>(v & 0x3FFFFF), static_cast<uint32_t>(v >> 22 & 0x3FFFFF), static_cast<uint32_t>(v >> 44)};
+    const uint32_t part[3] = {static_cast<uint32_t>(v & 0x3FFFFF), static_cast<uint32_t>(v >> 22 & 0x3FFFFF),
+                              static_cast<uint32_t>(v >> 44)};
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
       const uint32_t x = __reduce_add_sync(kFull, part[i]);
@@ -560,7 +566,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(const S
       __syncthreads();
       equal = lane == 0 ? warp_ties[warp] : 0;
       kept = mine_above;
-      if (lane == 0) kept += warp_parts[warp][0] + (static_cast<u64>(warp_parts[warp][1]) << 20) + (static_cast<u64>(warp_parts[warp][2]) << 40);
+      if (lane == 0)
+        kept += warp_parts[warp][0] + (static_cast<u64>(warp_parts[warp][1]) << 20) +
+                (static_cast<u64>(warp_parts[warp][2]) << 40);
     } else {
       const float above_ties = !limited ? low : t >= kmax ? kInf : P::logit(t + 1);
       if (t == 0) x.pieces_of([&](const uint4& r, int) { kept += x.template weigh<true>(r, weight); });  // nothing is cut

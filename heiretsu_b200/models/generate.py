@@ -102,7 +102,8 @@ def generate(model, idx: torch.Tensor, max_new_tokens: int, temperature: float =
     ``kv_cache`` the total length must fit in ``block_size``; without it the context is cropped to the
     last ``block_size`` tokens, as training saw them. ``engine`` "fused" decodes with the native kernels
     (models/decode.py; flattened parameters on a GPU): 16-bit weights, a cache of 16 or 8 bits, a CUDA graph per token.
-    Its random numbers are used differently: the same generator gives other samples of the same distribution."""
+    Its random numbers are used differently: the same generator gives other samples. Of logits that equal the ``top_k``-th it keeps
+    the first ``top_k`` by index, the plain engine all."""
     cfg = model.cfg
     if engine not in ("plain", "fused"):
         raise ValueError(f"engine must be plain or fused, got {engine!r}")
